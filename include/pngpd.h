@@ -369,6 +369,77 @@ int pngpd_adam_step(float* params_dev, const float* grads_dev, float* exp_avg_de
                     float* exp_avg_sq_dev, int64_t n, float lr, float beta1, float beta2, float eps,
                     int step, float grad_scale, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Operators of a classification head of the caller's own making, next to the fixed one of the model
+ * (model/pointnet.py:174-190, loss main_1v.py:270): a linear layer with its epilogue, dropout, and the cross entropy
+ * of a linear layer over any number of classes, each with its gradients.  No counterpart in the reference beyond those
+ * lines.
+ *
+ * Matrices are row-major; ld* is the distance of two rows in elements (at least the row's length), and a matrix
+ * without an ld argument is dense.  `type` is the element type of every matrix and bias; sums and statistics are
+ * 32-bit (64-bit over a batch's losses).  Outputs must not overlap inputs or each other.  Sizes: 0 <= rows, 1 <= the
+ * others, each below 2^31.  A call with no rows launches what the outputs that do not depend on rows need (zero
+ * gradients).  All calls are stream-ordered, allocate nothing and can be captured into a graph; two calls that may
+ * run at the same time need workspaces of their own.
+ * ------------------------------------------------------------------------------------------ */
+enum { PNGPD_TYPE_F32 = 0, PNGPD_TYPE_BF16 = 1, PNGPD_TYPE_F16 = 2 };
+enum { PNGPD_ACT_NONE = 0, PNGPD_ACT_RELU = 1, PNGPD_ACT_GELU = 2, PNGPD_ACT_GELU_TANH = 3, PNGPD_ACT_SILU = 4 };
+enum { PNGPD_REDUCE_NONE = 0, PNGPD_REDUCE_MEAN = 1, PNGPD_REDUCE_SUM = 2 };
+
+/*
+ * y[M,N] = act(x[M,K] weight[N,K]^T + bias[N]) + residual[M,N].  bias_dev, residual_dev: optional.
+ * z_dev [M,N], optional: x weight^T + bias rounded to `type`, which pngpd_linear_backward takes (a ReLU's tiny positive
+ * sums keep their sign there).  Needed for the backward pass of every activation but NONE.
+ */
+size_t pngpd_linear_workspace_bytes(int type, int64_t M, int64_t N, int64_t K, int backward);
+int pngpd_linear_forward(int type, int64_t M, int64_t N, int64_t K, const void* x_dev, int64_t ldx, const void* weight_dev,
+                         int64_t ldw, const void* bias_dev, int act, const void* residual_dev, int64_t ldr, void* y_dev,
+                         void* z_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of pngpd_linear_forward from dy_dev [M,N]: dz = dy act'(z), dx_dev [M,K] = dz weight, dweight_dev [N,K] =
+ * dz^T x, dbias_dev [N] = column sums of dz; each output is optional.  (The residual's gradient is dy itself.)
+ * For 16-bit types dz is rounded to `type` between the two products, as the operands of the matrix unit are.
+ */
+int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void* dy_dev, int64_t ld_dy, const void* z_dev,
+                          const void* x_dev, int64_t ldx, const void* weight_dev, int64_t ldw, int act, void* dx_dev,
+                          void* dweight_dev, void* dbias_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/*
+ * y[i] = residual[i] + (draw(i) >= round(p 2^32) ? x[i] / (1 - p) : 0) for the rows x cols elements i in row-major
+ * order.  draw(i): the lower (i even) or upper 32 bits of mix64(key + i / 2), key = mix64(seed ^ mix64(offset)), mix64
+ * = splitmix64's step.  The mask depends on seed, offset and position alone and is never stored; the backward pass is
+ * the same call on dy without the residual.  rng_dev, optional: int64 [2] = {seed, offset} read on the device when the
+ * kernel runs, in place of the two arguments (a captured graph draws a new mask whenever they change).
+ */
+int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64_t ldx, const void* residual_dev, int64_t ldr,
+                  void* y_dev, double p, uint64_t seed, uint64_t offset, const int64_t* rng_dev, void* stream);
+
+/*
+ * Cross entropy of softmax(x[T,D] weight[V,D]^T + bias[V]) without the [T,V] logits ever being stored whole: they are
+ * formed in pieces of the vocabulary, and every row keeps its running maximum and sum.
+ *   loss_t = lse_t - (1 - label_smoothing) z[t, target_t] - label_smoothing / V * sum_v z[t, v]
+ * Rows whose target is ignore_index have loss 0 and no gradient, whatever they hold.  Any other target outside [0, V)
+ * is not used as an index: its loss is NaN and its row contributes no gradient (as pngpd_nll_loss does).
+ * loss_dev: float [T] for PNGPD_REDUCE_NONE, else float [1] (the mean is over the rows that are not ignored: NaN when
+ * there are none).  lse_dev float [T]: log sum exp of every row's logits, what the backward pass needs.
+ */
+size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V, int64_t D, int backward);
+int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D, const void* x_dev, int64_t ldx,
+                                       const void* weight_dev, int64_t ldw, const void* bias_dev, const int64_t* target_dev,
+                                       int64_t ignore_index, float label_smoothing, int reduction, float* loss_dev,
+                                       float* lse_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of the forward call with the same arguments: dloss_dev float [T] (PNGPD_REDUCE_NONE) or [1] -> dx_dev
+ * [T,D], dweight_dev [V,D], dbias_dev [V], each optional.  The logits are formed again piece by piece.
+ */
+int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t D, const void* x_dev, int64_t ldx,
+                                        const void* weight_dev, int64_t ldw, const void* bias_dev, const int64_t* target_dev,
+                                        int64_t ignore_index, float label_smoothing, int reduction, const float* lse_dev,
+                                        const float* dloss_dev, void* dx_dev, void* dweight_dev, void* dbias_dev,
+                                        void* workspace_dev, size_t workspace_bytes, void* stream);
+
 /*
  * Diagnostic: pngpd_forward_infer with the two conv-stack launches of the step bracketed by HIP
  * events recorded on `stream`; waits for the trunk launch to finish and returns the two kernel

@@ -1,0 +1,195 @@
+"""64-bit restatement of the classification-head operators (pointnetgpd_amd/head.py), with bounds on the error a kernel may
+make.  Everything runs on the CPU in float64 on the operands as they are (rounded to their type already).
+
+Bounds, element by element.  u = 2^-24 (half a step of 32 bits), h = finfo(type).eps / 2.
+* A sum of n products in 32 bits, in any order: n u sum |a b| (plus 8 u for operands taken in pieces).
+* A rounding to the type: h relative, and `tiny` absolute where the type flushes (half precision: 2^-25).
+* A function evaluated in 32 bits: FN u relative to the size of its parts.
+* 32 bits end at 2^-126: a probability, weight or product below that may come out as 0, so each carries FLUSH = 2^-126
+  besides its relative error.  (exp(-88) is 2^-127: a class 88 below the row's largest logit has such a probability, and
+  a bound that is only relative would ask for digits the type does not hold.)
+"""
+import math
+
+import numpy as np
+import torch
+
+U = 2.0 ** -24
+FLUSH = 2.0 ** -126
+FN = 16.0                      # units of U an activation, exp or log may be off by, relative to its terms
+CURVE = {None: 0.0, "relu": 0.0, "gelu": 0.8, "gelu_tanh": 0.85, "silu": 0.5}      # max |act''|
+TOP_SLOPE = 1.13               # max |act'|
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    return 2.0 ** -25 if dtype == torch.float16 else 0.0
+
+
+def act(z, name):
+    """(act(z), act'(z)) in 64 bits."""
+    if name is None:
+        return z, torch.ones_like(z)
+    if name == "relu":
+        return torch.relu(z), (z > 0).double()
+    if name == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s + z * s * (1 - s)
+    if name == "gelu":
+        c = torch.special.ndtr(z)
+        return z * c, c + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    u = math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)
+    t = torch.tanh(u)
+    return 0.5 * z * (1 + t), 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * math.sqrt(2 / math.pi) * (1 + 3 * 0.044715 * z * z)
+
+
+def linear(x, w, b, name, r, dy):
+    """{output: (value, bound)} for y, dx, dw, db of 2-D operands on the CPU."""
+    dt = x.dtype
+    h, tn = half_step(dt), tiny(dt)
+    X, W = x.double(), w.double()
+    M, K = X.shape
+    N = W.shape[0]
+    z = X @ W.t()
+    az = X.abs() @ W.abs().t()
+    if b is not None:
+        z = z + b.double()
+        az = az + b.double().abs()
+    ez = (K + 10) * U * az
+    y, slope = act(z, name)
+    ey = TOP_SLOPE * ez + FN * U * (y.abs() + z.abs() * (name is not None))
+    if r is not None:
+        ey = ey + U * (y.abs() + r.double().abs())
+        y = y + r.double()
+    out = {"y": (y, ey + h * (y.abs() + ey) + tn)}
+    if dy is None:
+        return out
+    g = dy.double()
+    dz = g * slope
+    kept = 0.0 if name in (None, "relu") else 1.0       # a ReLU's kept sum matters by its sign alone
+    ed = g.abs() * (CURVE[name] * (kept * (ez + h * z.abs() + tn)) + FN * U * (1 + z.abs()) * (name not in (None, "relu")))
+    if name is not None:
+        ed = ed + h * dz.abs() + tn
+    adz = dz.abs() + ed
+
+    def product(a, ea, b_, n):
+        v = a @ b_
+        e = ea @ b_.abs() + (n + 10) * U * ((a.abs() + ea) @ b_.abs())
+        return v, e + h * (v.abs() + e) + tn
+
+    out["dx"] = product(dz, ed, W, N)
+    out["dw"] = product(dz.t(), ed.t(), X, M)
+    v = dz.sum(0)
+    e = ed.sum(0) + (M + 4) * U * adz.sum(0)
+    out["db"] = (v, e + h * (v.abs() + e) + tn)
+    return out
+
+
+def mix64(v):
+    with np.errstate(over="ignore"):
+        v = np.asarray(v, dtype=np.uint64) + np.uint64(0x9E3779B97F4A7C15)
+        v = (v ^ (v >> np.uint64(30))) * np.uint64(0xBF58476D1CE4E5B9)
+        v = (v ^ (v >> np.uint64(27))) * np.uint64(0x94D049BB133111EB)
+        return v ^ (v >> np.uint64(31))
+
+
+def keep_mask(n, p, seed, offset):
+    """Which of n elements dropout keeps (bool, numpy)."""
+    with np.errstate(over="ignore"):
+        key = mix64(np.uint64(seed % 2 ** 64) ^ mix64(np.uint64(offset % 2 ** 64)))
+        word = mix64(key + np.arange((n + 1) // 2, dtype=np.uint64))
+    draw = np.stack([word & np.uint64(0xFFFFFFFF), word >> np.uint64(32)], axis=1).reshape(-1)[:n]
+    return draw >= np.uint64(int(round(p * 2 ** 32)))
+
+
+def dropout(x, p, seed, offset, r):
+    """(value, bound); the mask itself has no tolerance."""
+    keep = torch.from_numpy(keep_mask(x.numel(), p, seed, offset)).view(x.shape)
+    v = torch.where(keep, x.double() / (1 - p) if p < 1 else torch.zeros(()).double(), torch.zeros(()).double())
+    e = 2 * U * v.abs()
+    if r is not None:
+        v = v + r.double()
+        e = e + U * (v.abs() + e)
+    return v, e + half_step(x.dtype) * (v.abs() + e) + tiny(x.dtype)
+
+
+def cross_entropy(x, w, target, b, ignore, eps, reduction, dloss):
+    """{output: (value, bound)} for loss, dx, dw, db."""
+    dt = x.dtype
+    h, tn = half_step(dt), tiny(dt)
+    X, W = x.double(), w.double()
+    T, D = X.shape
+    V = W.shape[0]
+    live = (target != ignore) & (target >= 0) & (target < V)
+    counted = target != ignore
+    X = torch.where(live[:, None], X, torch.zeros_like(X))
+    z = X @ W.t()
+    az = X.abs() @ W.abs().t()
+    if b is not None:
+        z = z + b.double()
+        az = az + b.double().abs().nan_to_num(posinf=0.0)
+    ez = (D + 10) * U * az
+    lse = torch.logsumexp(z, dim=1)
+    zf = torch.where(z == -math.inf, torch.zeros_like(z), z)
+    el = ez.max(dim=1).values + (V / 32 + 128) * U + FN * U * (lse.abs() + zf.abs().max(dim=1).values)
+    idx = target.clamp(0, V - 1)
+    zy = z.gather(1, idx[:, None])[:, 0]
+    loss = lse - (1 - eps) * zy
+    e = 2 * el + FN * U * (lse.abs() + zy.abs())
+    if eps > 0:
+        loss = loss - eps / V * z.sum(1)
+        e = e + eps * (ez.sum(1) / V + (V / 32 + 32) * U * zf.abs().sum(1) / V)
+    loss = torch.where(counted, torch.where(live, loss, torch.full_like(loss, math.nan)), torch.zeros_like(loss))
+    e = torch.where(counted, e, torch.zeros_like(e))
+    count = counted.sum().double()
+    if reduction == "none":
+        out = {"loss": (loss, e)}
+    else:
+        d = count if reduction == "mean" else 1.0
+        out = {"loss": (loss.sum() / d, e.sum() / d + 4 * U * loss.abs().sum() / d)}
+    if dloss is None:
+        return out
+    g = dloss.double().expand(T) / (count if reduction == "mean" else 1.0)
+    g = torch.where(live, g, torch.zeros_like(g))[:, None]
+    p = torch.exp(z - lse[:, None])
+    wanted = torch.full_like(z, eps / V)
+    wanted.scatter_add_(1, idx[:, None], torch.full_like(zy, 1 - eps)[:, None])
+    part = p - wanted
+    dz = torch.where(g == 0, torch.zeros_like(z), part * g)
+    ed = g.abs() * (p * (ez + el[:, None] + FN * U * (1 + zf.abs() + lse.abs()[:, None])) + FN * U * (p + wanted))
+    ed = torch.where(g == 0, torch.zeros_like(ed), ed + (g.abs() + 1) * FLUSH)
+    ed = ed + h * (dz.abs() + ed) + (g.abs().max() * 2.0 ** -37 if dt == torch.float16 else 0.0)
+
+    def product(a, ea, b_, n):
+        v = a @ b_
+        er = ea @ b_.abs() + (n + 10) * U * ((a.abs() + ea) @ b_.abs()) + n * FLUSH
+        return v, er + h * (v.abs() + er) + tn
+
+    out["dx"] = product(dz, ed, W, V)
+    out["dw"] = product(dz.t(), ed.t(), X, T)
+    v = dz.sum(0)
+    er = ed.sum(0) + (T + 4) * U * (dz.abs() + ed).sum(0)
+    out["db"] = (v, er + h * (v.abs() + er) + tn)
+    return out
+
+
+def worst(got, value, bound):
+    """Largest |got - value| / bound (NaN and infinities have to agree); at most 1 passes."""
+    got, value = got.detach().cpu().double(), value.double()
+    if got.shape != value.shape:
+        raise AssertionError(f"shape {tuple(got.shape)} instead of {tuple(value.shape)}")
+    odd = ~torch.isfinite(value)
+    if not torch.equal(torch.isnan(got), torch.isnan(value)):
+        return math.inf
+    inf = torch.isinf(value)
+    if not torch.equal(got[inf], value[inf]):
+        return math.inf
+    d, lim = (got - value).abs()[~odd], bound.expand(value.shape)[~odd]
+    if d.numel() == 0:
+        return 0.0
+    if not bool((d <= lim).all()):
+        return float((d / lim.clamp(min=1e-300)).max())
+    return float((d / lim.clamp(min=1e-300)).max())

@@ -35,6 +35,10 @@ LIB_SOURCES = [
     "train_bwd2.hip",
     "tall_gemm.hip",
     "train_api.cpp",
+    "head_product.hip",
+    "head_dropout.hip",
+    "head_loss.hip",
+    "head_api.cpp",
 ]
 
 

@@ -1,0 +1,79 @@
+// Element types, activations and reductions shared by the classification-head kernels.
+#pragma once
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include "pngpd.h"
+
+namespace pngpd {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) { return (float)v; }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) { return (T)v; }      // rounds to nearest even
+
+// act(z) and act'(z).  gelu: z Phi(z); gelu_tanh: z sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3), which is
+// 0.5 z (1 + tanh u) without tanh's cancellation for large negative z; silu: z sigmoid(z).  z = -inf gives 0 and slope
+// 0 in all of them (the limits; the plain formulas give -inf * 0), NaN stays NaN.
+__device__ __forceinline__ float sigmoid_f(float v) { return 1.f / (1.f + __expf(-v)); }
+
+constexpr float GELU_C = 0.7978845608028654f;      // sqrt(2 / pi)
+
+template <int ACT>
+__device__ __forceinline__ float act_f(float z) {
+    if constexpr (ACT == PNGPD_ACT_RELU) return z < 0.f ? 0.f : z;
+    if constexpr (ACT == PNGPD_ACT_GELU) return z == -__builtin_inff() ? 0.f : 0.5f * z * erfcf(-z * 0.70710678118654752f);
+    if constexpr (ACT == PNGPD_ACT_GELU_TANH)
+        return z == -__builtin_inff() ? 0.f : z * sigmoid_f(2.f * GELU_C * (z + 0.044715f * z * z * z));
+    if constexpr (ACT == PNGPD_ACT_SILU) return z == -__builtin_inff() ? 0.f : z * sigmoid_f(z);
+    return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z) {
+    if constexpr (ACT == PNGPD_ACT_RELU) return z > 0.f ? 1.f : z == z ? 0.f : z;
+    if constexpr (ACT == PNGPD_ACT_GELU) {
+        if (__builtin_fabsf(z) > 16.f) return z > 0.f ? 1.f : 0.f;      // the bell is below 1e-55
+        return 0.5f * erfcf(-z * 0.70710678118654752f) + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+    }
+    if constexpr (ACT == PNGPD_ACT_GELU_TANH) {
+        if (__builtin_fabsf(z) > 16.f) return z > 0.f ? 1.f : 0.f;
+        const float s = sigmoid_f(2.f * GELU_C * (z + 0.044715f * z * z * z));
+        return s + z * s * (1.f - s) * 2.f * GELU_C * (1.f + 0.134145f * z * z);
+    }
+    if constexpr (ACT == PNGPD_ACT_SILU) {
+        if (__builtin_fabsf(z) > 100.f) return z > 0.f ? 1.f : 0.f;
+        const float s = sigmoid_f(z);
+        return s + z * s * (1.f - s);
+    }
+    return z == z ? 1.f : z;
+}
+
+// The pre-activation kept for the backward pass, rounded to the operands' type.  A ReLU's slope is its sign, so a sum
+// that the type would round to zero keeps it: it becomes the type's smallest number.
+template <typename T, int ACT>
+__device__ __forceinline__ T keep_z(float z) {
+    T r = (T)z;
+    if constexpr (ACT == PNGPD_ACT_RELU && sizeof(T) == 2) {
+        if (z > 0.f && (float)r == 0.f) r = __builtin_bit_cast(T, (unsigned short)1);
+    }
+    return r;
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+// fmaxf drops NaN; a row that holds one has to come out NaN, which the sum of exponentials sees to
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+
+}  // namespace pngpd

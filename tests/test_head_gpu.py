@@ -1,0 +1,542 @@
+"""GPU parity of the classification-head operators (pointnetgpd_amd/head.py) against their 64-bit restatement, within the
+bounds that oracle/head_oracle.py derives element by element."""
+import math
+
+import pytest
+import torch
+
+from oracle import head_oracle as ho
+from pointnetgpd_amd import head
+
+pytestmark = pytest.mark.gpu
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def make(seed, *shapes, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(*s, generator=g) * scale for s in shapes]
+
+
+def grid(t, step):
+    """On a grid whose sums are exact in 32 bits: a ReLU's border is then on the same side for every order of the sum."""
+    return torch.round(t / step) * step
+
+
+def check(outputs, want):
+    bad = {k: r for k, r in ((k, ho.worst(outputs[k], *want[k])) for k in outputs) if not r <= 1.0}
+    assert not bad, bad
+
+
+def linear_case(seed, M, N, K, dt, act, bias, residual):
+    x, w, b, r, dy = make(seed, (M, K), (N, K), (N,), (M, N), (M, N))
+    w = w / math.sqrt(K)
+    if act == "relu":
+        x, w, b = grid(x, 2.0 ** -6), grid(w, 2.0 ** -10), grid(b, 2.0 ** -10)
+    x, w, b, r, dy = (t.to(dt) for t in (x, w, b, r, dy))
+    return x, w, b if bias else None, r if residual else None, dy
+
+
+def run_linear(x, w, b, r, act, dy):
+    leaves = [t.cuda().requires_grad_() if t is not None else None for t in (x, w, b, r)]
+    y = head.linear(*leaves[:3], activation=act, residual=leaves[3])
+    used = [t for t in leaves if t is not None]
+    grads = dict(zip([n for n, t in zip(("dx", "dw", "db", "dr"), leaves) if t is not None],
+                     torch.autograd.grad(y, used, dy.cuda())))
+    return {"y": y, **grads}
+
+
+SIZES = [(1, 1, 1), (1, 16, 8), (2, 3, 5), (1, 512, 4096), (3, 1030, 200), (16, 200, 1030), (64, 64, 64), (65, 130, 67),
+         (128, 256, 64), (200, 7, 1024), (257, 513, 129), (300, 777, 1001), (1023, 40, 24), (512, 384, 640)]
+
+
+@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_linear_and_its_gradients(kind, M, N, K):
+    i = SIZES.index((M, N, K))
+    act = (None, "relu", "gelu", "gelu_tanh", "silu")[i % 5]
+    x, w, b, r, dy = linear_case(M + N + K, M, N, K, TYPES[kind], act, bias=i % 3 != 2, residual=i % 2 == 0)
+    got = run_linear(x, w, b, r, act, dy)
+    want = ho.linear(x, w, b, act, r, dy)
+    if "dr" in got:
+        assert torch.equal(got.pop("dr").cpu(), dy)
+    assert got["y"].dtype == x.dtype
+    check(got, want)
+
+
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_every_activation_with_bias_and_residual(kind, act):
+    x, w, b, r, dy = linear_case(5, 70, 96, 80, TYPES[kind], act, True, True)
+    got = run_linear(x, w, b, r, act, dy)
+    got.pop("dr")
+    check(got, ho.linear(x, w, b, act, r, dy))
+
+
+@pytest.mark.parametrize("M,N,K", [(2048, 1024, 512), (1500, 1100, 1300), (4096, 256, 128)])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_linear_over_many_tiles(kind, M, N, K):
+    x, w, b, r, dy = linear_case(17, M, N, K, TYPES[kind], "gelu", True, True)
+    got = run_linear(x, w, b, r, "gelu", dy)
+    got.pop("dr")
+    check(got, ho.linear(x, w, b, "gelu", r, dy))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_linear_takes_any_strides_and_alignment(kind):
+    dt = TYPES[kind]
+    M, N, K = 130, 72, 88
+    x, w, b, r, dy = linear_case(23, M, N, K, dt, "silu", True, True)
+    want = ho.linear(x, w, b, "silu", r, dy)
+
+    def odd_start(t):                       # a view that starts one element into its storage
+        s = torch.full((t.numel() + 1,), float("nan"), dtype=dt, device="cuda")
+        s[1:] = t.reshape(-1).cuda()
+        return s[1:].view(t.shape)
+
+    def wide(t):                            # rows further apart than they are long, NaN between them
+        s = torch.full((t.shape[0], t.shape[1] + 9), float("nan"), dtype=dt, device="cuda")
+        s[:, 3:3 + t.shape[1]] = t.cuda()
+        return s[:, 3:3 + t.shape[1]]
+
+    def lying(t):                           # columns dense instead of rows
+        return t.t().contiguous().cuda().t()
+
+    for lay in (odd_start, wide, lying):
+        xs, ws, rs, ds = (lay(t).detach().requires_grad_() for t in (x, w, r, dy))
+        bs = b.cuda().requires_grad_()
+        y = head.linear(xs, ws, bs, activation="silu", residual=rs)
+        dx, dw, db = torch.autograd.grad(y, (xs, ws, bs), ds.detach())
+        check({"y": y, "dx": dx, "dw": dw, "db": db}, want)
+    # one residual row for all, one gradient value for all, and more than two dimensions
+    row = r[:1].expand(M, N)
+    y = head.linear(x.cuda().view(2, 65, K), w.cuda(), b.cuda(), activation="silu",
+                    residual=r[:1].cuda().expand(M, N).view(2, 65, N))
+    assert y.shape == (2, 65, N)
+    check({"y": y.reshape(M, N)}, ho.linear(x, w, b, "silu", row, None))
+    xs = x.cuda().requires_grad_()
+    dx, = torch.autograd.grad(head.linear(xs, w.cuda()).float().sum(), xs)
+    check({"dx": dx}, {"dx": ho.linear(x, w, None, None, None, torch.ones(M, N, dtype=dt))["dx"]})
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_no_rows(kind):
+    dt = TYPES[kind]
+    x = torch.empty(0, 24, dtype=dt, device="cuda", requires_grad=True)
+    w = torch.randn(16, 24, device="cuda").to(dt).requires_grad_()
+    b = torch.randn(16, device="cuda").to(dt).requires_grad_()
+    y = head.linear(x, w, b, activation="relu")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+    assert y.shape == (0, 16) and dx.shape == (0, 24) and not dw.any() and not db.any()
+    t = torch.empty(0, dtype=torch.int64, device="cuda")
+    loss = head.linear_cross_entropy(x, w, t, b, reduction="sum")
+    dx, dw, db = torch.autograd.grad(loss, (x, w, b))
+    assert loss.item() == 0 and not dw.any() and not db.any()
+    assert math.isnan(head.linear_cross_entropy(x, w, t).item())
+    assert head.linear_cross_entropy(x, w, t, reduction="none").shape == (0,)
+    assert head.dropout(x, 0.5, 3).shape == (0, 24)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "gelu_tanh", "silu"])
+def test_linear_carries_infinities_and_nan_in_their_rows_only(kind, act):
+    dt = TYPES[kind]
+    x, w, b, _, _ = linear_case(3, 70, 40, 48, dt, act, True, False)
+    x, w = x.abs() + 0.125, w.abs() + 0.125                     # one sign: an infinity stays one in every sum
+    x[3, 5], x[40, 7], x[66, 0] = math.inf, -math.inf, math.nan
+    y = head.linear(x.cuda(), w.cuda(), b.cuda(), activation=act).cpu()
+    assert torch.isnan(y[66]).all() and (y[3] == math.inf).all()
+    assert (y[40] == (-math.inf if act is None else 0.0)).all()
+    rest = [i for i in range(70) if i not in (3, 40, 66)]
+    want = ho.linear(x[rest], w, b, act, None, None)["y"]
+    assert ho.worst(y[rest], *want) <= 1.0
+
+
+def test_float32_products_keep_the_types_range():
+    """Operands near both ends of float32's range, whose products lie inside it."""
+    x, w = make(2, (130, 64), (130, 64))
+    big, small = (x * 2.0 ** 100), (w * 2.0 ** -100)
+    for a, b in ((big, small), (small, big), (x * 2.0 ** -60, w * 2.0 ** -60), (x * 2.0 ** 126 / 8, w * 2.0 ** -20)):
+        y = head.linear(a.cuda(), b.cuda())
+        want, bound = ho.linear(a, b, None, None, None, None)["y"]
+        assert ho.worst(y, want, bound + 2.0 ** -149 * 64) <= 1.0
+    top = torch.full((1, 8), torch.finfo(torch.float32).max)
+    one = torch.zeros(1, 8)
+    one[0, 0] = 1.0
+    assert head.linear(top.cuda(), one.cuda()).item() == top[0, 0].item()
+
+
+# ---- dropout --------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("shape", [(1,), (1, 1), (3, 5), (7, 1), (256, 512), (33, 1001), (5, 6, 7), (1, 100003)])
+@pytest.mark.parametrize("p", [0.0, 0.3, 1.0])
+def test_dropout_is_exact_in_its_mask(kind, shape, p):
+    dt = TYPES[kind]
+    x, r, dy = (t.to(dt) for t in make(sum(shape), shape, shape, shape))
+    seed, offset = 0x123456789ABCDEF, 77
+    for res in (None, r):
+        xs = x.cuda().requires_grad_()
+        rs = res.cuda().requires_grad_() if res is not None else None
+        y = head.dropout(xs, p, seed, offset, residual=rs)
+        assert ho.worst(y, *ho.dropout(x, p, seed, offset, res)) <= 1.0
+        grads = torch.autograd.grad(y, (xs,) if res is None else (xs, rs), dy.cuda())
+        assert ho.worst(grads[0], *ho.dropout(dy, p, seed, offset, None)) <= 1.0
+        if res is not None:
+            assert torch.equal(grads[1].cpu(), dy)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_dropout_depends_on_the_position_not_on_the_strides(kind):
+    dt = TYPES[kind]
+    x, r = (t.to(dt) for t in make(4, (67, 50), (67, 50)))
+    want = head.dropout(x.cuda(), 0.4, 9, 2, residual=r.cuda())
+    pad = torch.full((67, 61), float("nan"), dtype=dt, device="cuda")
+    pad[:, 5:55] = x.cuda()
+    odd = torch.empty(67 * 50 + 1, dtype=dt, device="cuda")
+    odd[1:] = r.reshape(-1).cuda()
+    for xs in (pad[:, 5:55], x.t().contiguous().cuda().t()):
+        for rs in (r.cuda(), odd[1:].view(67, 50), r.t().contiguous().cuda().t()):
+            assert torch.equal(head.dropout(xs, 0.4, 9, 2, residual=rs), want)
+    row = head.dropout(x[:1].cuda().expand(67, 50), 0.4, 9, 2)
+    assert ho.worst(row, *ho.dropout(x[:1].expand(67, 50).contiguous(), 0.4, 9, 2, None)) <= 1.0
+
+
+def test_dropout_keeps_infinities_and_nan_of_dropped_places_out():
+    x = torch.full((64, 64), math.nan)
+    y = head.dropout(x.cuda(), 0.5, 1, 0).cpu()
+    keep = torch.from_numpy(ho.keep_mask(4096, 0.5, 1, 0)).view(64, 64)
+    assert torch.isnan(y[keep]).all() and (y[~keep] == 0).all()
+    assert (head.dropout(x.cuda(), 1.0, 1, 0) == 0).all()
+
+
+def test_dropout_takes_its_seed_from_the_device():
+    x, = make(6, (100, 30))
+    xs = x.cuda().requires_grad_()
+    rng = torch.tensor([-5, 12], dtype=torch.int64, device="cuda")
+    y = head.dropout(xs, 0.25, rng)
+    assert torch.equal(y, head.dropout(xs, 0.25, -5, 12))
+    dx, = torch.autograd.grad(y, xs, torch.ones_like(y))
+    assert torch.equal(dx != 0, torch.from_numpy(ho.keep_mask(3000, 0.25, -5, 12)).view(100, 30).cuda())
+    y = head.dropout(xs, 0.25, rng)
+    rng += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, xs, torch.ones_like(y))
+
+
+# ---- linear + cross entropy ------------------------------------------------------------------------------------------------
+
+def loss_case(seed, T, V, D, dt, bias, pad=True):
+    g = torch.Generator().manual_seed(seed)
+    x, w, b = (torch.randn(*s, generator=g) for s in ((T, D), (V, D), (V,)))
+    target = torch.randint(0, V, (T,), generator=g)
+    if pad and T > 2:
+        target[torch.rand(T, generator=g) < 0.2] = -100
+    return x.to(dt), (w * 2 / math.sqrt(D)).to(dt), b.to(dt) if bias else None, target
+
+
+def run_loss(x, w, target, b, eps, reduction, dloss, ignore=-100):
+    leaves = [t.cuda().requires_grad_() if t is not None else None for t in (x, w, b)]
+    loss = head.linear_cross_entropy(leaves[0], leaves[1], target.cuda(), leaves[2], ignore_index=ignore, label_smoothing=eps,
+                                     reduction=reduction)
+    grads = torch.autograd.grad(loss, [t for t in leaves if t is not None], dloss.cuda())
+    return {"loss": loss, **dict(zip(("dx", "dw", "db"), grads))}
+
+
+LOSS_SIZES = [(1, 1, 1), (1, 2, 8), (2, 3, 5), (256, 3, 256), (1, 5000, 64), (16, 1031, 200), (17, 4100, 96), (64, 64, 64),
+              (65, 130, 67), (130, 257, 72), (300, 777, 101), (513, 1024, 128)]
+
+
+@pytest.mark.parametrize("T,V,D", LOSS_SIZES)
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_linear_cross_entropy_and_its_gradients(kind, T, V, D):
+    i = LOSS_SIZES.index((T, V, D))
+    reduction = ("mean", "sum", "none")[i % 3]
+    eps = 0.1 if i % 2 else 0.0
+    x, w, b, target = loss_case(T + V + D, T, V, D, TYPES[kind], bias=i % 4 != 3)
+    scale = 256.0 if kind == "f16" else 1.0              # half precision trains with a scaled loss
+    dloss = torch.rand(T, generator=torch.Generator().manual_seed(i)) * scale / T if reduction == "none" else \
+        torch.tensor(scale if reduction == "mean" else scale / T)
+    got = run_loss(x, w, target, b, eps, reduction, dloss)
+    assert got["loss"].dtype == torch.float32
+    check(got, ho.cross_entropy(x, w, target, b, -100, eps, reduction, dloss))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_linear_cross_entropy_over_several_pieces_of_the_vocabulary(kind):
+    """Sizes at which the [T, V] logits pass the largest piece: 2100 x 70000 in 32 bits are 588 MB."""
+    T, V, D = 2100, 70000, 16
+    dt = TYPES[kind]
+    x, w, b, target = loss_case(1, T, V, D, dt, True)
+    dloss = torch.tensor(1024.0 if kind == "f16" else 1.0)
+    got = run_loss(x, w, target, b, 0.1, "mean", dloss)
+    rows = [0, 1, 63, 64, 1000, 2098, 2099]
+    count = (target != -100).sum().item()
+    part = ho.cross_entropy(x[rows], w, target[rows], b, -100, 0.1, "sum", dloss / count)
+    check({"dx": got["dx"][rows]}, {"dx": part["dx"]})
+    # everything else against plain 64-bit products on the device
+    X, W = x.cuda().double(), w.cuda().double()
+    z = X @ W.t() + b.cuda().double()
+    live = (target != -100).cuda()
+    logp = torch.log_softmax(z, 1)
+    wanted = torch.full_like(z, 0.1 / V)
+    wanted[torch.arange(T, device="cuda")[live], target.cuda()[live]] += 0.9
+    wanted[~live] = 0
+    loss = -(wanted * logp).sum() / count
+    assert abs(got["loss"].item() - loss.item()) < 2e-3        # (V / 32 + ...) units of 2^-24, the bound of a row's loss
+    dz = (logp.exp() * live[:, None] - wanted) * (dloss.item() / count)
+    u = ho.half_step(dt) + 2.0 ** -9 * (kind == "bf16")
+    for name, ref, mag in (("dw", dz.t() @ X, dz.abs().t() @ X.abs()), ("db", dz.sum(0), dz.abs().sum(0))):
+        err = (got[name].double() - ref).abs()
+        # dz rounded once (h), its probability off by the logits' and lse's errors (below 2e-3), the result rounded (h)
+        assert bool((err <= (2 * u + 2e-3) * mag + ho.tiny(dt)).all()), name
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_ignored_rows_and_bad_labels(kind, reduction):
+    dt = TYPES[kind]
+    x, w, b, target = loss_case(12, 70, 50, 24, dt, True, pad=False)
+    target[5:9] = 7                                       # the ignored label may be a class
+    x[5], x[6], x[7] = math.nan, math.inf, torch.finfo(dt).max
+    dloss = torch.rand(70) if reduction == "none" else torch.tensor(1.0)
+    got = run_loss(x, w, target, b, 0.0, reduction, dloss, ignore=7)
+    check(got, ho.cross_entropy(x, w, target, b, 7, 0.0, reduction, dloss))
+    assert (got["dx"][target == 7] == 0).all()
+    target[20], target[21] = 50, -1                       # not a class, not ignored: NaN, and no gradient
+    got = run_loss(x, w, target, b, 0.0, reduction, dloss, ignore=7)
+    check(got, ho.cross_entropy(x, w, target, b, 7, 0.0, reduction, dloss))
+    assert (got["dx"][20:22] == 0).all()
+
+
+def test_a_batch_of_ignored_rows():
+    x, w, b, target = loss_case(12, 9, 50, 24, torch.float32, True)
+    target[:] = -100
+    got = run_loss(x, w, target, b, 0.0, "mean", torch.tensor(1.0))
+    assert math.isnan(got["loss"].item()) and not got["dx"].any() and not got["dw"].any() and not got["db"].any()
+    got = run_loss(x, w, target, b, 0.0, "none", torch.ones(9))
+    assert not got["loss"].any() and not got["dw"].any()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_masked_classes(kind):
+    """A bias of -inf takes a class out; the type's lowest value nearly does; a label on a masked class costs inf."""
+    dt = TYPES[kind]
+    V = 600
+    x, w, b, target = loss_case(15, 40, V, 32, dt, True, pad=False)
+    b[:256], b[300:302], b[V - 1] = -math.inf, torch.finfo(dt).min, -math.inf
+    target = 256 + target % 40
+    dloss = torch.ones(40) * (64.0 if kind == "f16" else 1.0)
+    got = run_loss(x, w, target, b, 0.0, "none", dloss)
+    want = ho.cross_entropy(x, w, target, b, -100, 0.0, "none", dloss)
+    # a logit at the type's lowest value is exact enough to be nothing: its own magnitude is no error of the row
+    b2 = b.clone()
+    b2[300:302] = -1000.0 if kind != "f16" else -60000.0
+    want2 = ho.cross_entropy(x, w, target, b.masked_fill(b == torch.finfo(dt).min, -math.inf), -100, 0.0, "none", dloss)
+    for k in want:
+        want[k] = (want2[k][0], want2[k][1])
+    check(got, want)
+    assert (got["db"][:256] == 0).all() and (got["dw"][:256] == 0).all()
+    target[3] = 0
+    got = run_loss(x, w, target, b, 0.0, "none", dloss)
+    assert got["loss"][3].item() == math.inf and torch.isfinite(got["loss"][4:]).all()
+    b[:] = -math.inf                                      # nothing left at all
+    assert torch.isnan(head.linear_cross_entropy(x.cuda(), w.cuda(), target.cuda(), b.cuda(), reduction="none")).all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_large_logits_and_a_sure_row(kind):
+    x, w, b, target = loss_case(19, 33, 300, 16, TYPES[kind], False, pad=False)
+    x = x * 40
+    dloss = torch.tensor(1.0)
+    check(run_loss(x, w, target, b, 0.0, "mean", dloss), ho.cross_entropy(x, w, target, b, -100, 0.0, "mean", dloss))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_linear_cross_entropy_takes_any_strides(kind):
+    dt = TYPES[kind]
+    x, w, b, target = loss_case(31, 60, 90, 40, dt, True)
+    want = ho.cross_entropy(x, w, target, b, -100, 0.0, "none", torch.ones(60))
+    xs = torch.full((60, 47), math.nan, dtype=dt, device="cuda")
+    xs[:, 1:41] = x.cuda()
+    xs = xs[:, 1:41].detach().requires_grad_()
+    ws = w.t().contiguous().cuda().t().requires_grad_()
+    bs = torch.stack([b, b]).t().contiguous().cuda()[:, 0].detach().requires_grad_()
+    ts = torch.stack([target, target]).t().contiguous().cuda()[:, 0]
+    loss = head.linear_cross_entropy(xs, ws, ts.int(), bs, reduction="none")
+    dx, dw, db = torch.autograd.grad(loss, (xs, ws, bs), torch.ones((), device="cuda").expand(60))
+    check({"loss": loss, "dx": dx, "dw": dw, "db": db}, want)
+    loss = head.linear_cross_entropy(x.cuda().view(3, 20, 40), w.cuda(), target.cuda().view(3, 20), b.cuda(), reduction="none")
+    assert loss.shape == (3, 20)
+    check({"loss": loss.reshape(-1)}, {"loss": want["loss"]})
+
+
+# ---- against differences, together, captured --------------------------------------------------------------------------------
+
+def test_gradients_against_differences():
+    """Directional derivatives by central differences of step 2^-6 in float32.  The loss is a mean of rows whose logits move
+    by at most 1 per unit of the direction: the third derivative is at most 4, the truncation h^2 / 6 * 4 = 1.7e-4; the two
+    losses (below 8) are off by at most 40 units of 2^-24 each: 40 * 8 * 2^-24 / 2^-6 = 1.3e-3 at worst."""
+    x, w, b, target = loss_case(41, 48, 37, 20, torch.float32, True)
+    x, w, b, target = x.cuda(), w.cuda(), b.cuda(), target.cuda()
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    loss = head.linear_cross_entropy(leaves[0], leaves[1], target, leaves[2], label_smoothing=0.1)
+    grads = torch.autograd.grad(loss, leaves)
+    h = 2.0 ** -6
+    for i in range(3):
+        d = torch.randn_like(leaves[i])
+        moved = d @ w.t() if i == 0 else x @ d.t() if i == 1 else d.expand(48, 37)
+        d = d / moved.abs().max()
+        at = []
+        for s in (h, -h):
+            args = [x, w, b]
+            args[i] = args[i] + s * d
+            at.append(head.linear_cross_entropy(args[0], args[1], target, args[2], label_smoothing=0.1).item())
+        slope = (grads[i].double() * d.double()).sum().item()
+        assert abs((at[0] - at[1]) / (2 * h) - slope) < 1.5e-3, i
+    # the smooth activations: sum of y over a direction of the output; |act'''| <= 3, moved by at most 1 a unit: truncation
+    # 48 * 30 * h^2 / 6 * 3 spread over random signs - a tenth of it - against slopes of some tens
+    x, w, b, r, dy = (t.cuda() if t is not None else None for t in linear_case(43, 48, 30, 20, torch.float32, None, True, False))
+    for act in ("gelu", "gelu_tanh", "silu"):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        grads = torch.autograd.grad(head.linear(*leaves, activation=act), leaves, dy)
+        for i in range(3):
+            d = torch.randn_like(leaves[i])
+            moved = d @ w.t() if i == 0 else x @ d.t() if i == 1 else d.expand(48, 30)
+            d = d / moved.abs().max()
+            at = []
+            for s in (h, -h):
+                args = [x, w, b]
+                args[i] = args[i] + s * d
+                at.append((head.linear(*args, activation=act).double() * dy.double()).sum().item())
+            slope = (grads[i].double() * d.double()).sum().item()
+            assert abs((at[0] - at[1]) / (2 * h) - slope) < 0.02 + 1e-3 * abs(slope), (act, i)
+
+
+def head_step(x, params, target, rng):
+    """linear -> dropout with its residual -> linear_cross_entropy, as a training step uses them."""
+    w1, b1, w2, b2, w3, b3 = params
+    h1 = head.linear(x, w1, b1, activation="relu")
+    h2 = head.linear(h1, w2, b2, activation="gelu")
+    h3 = head.dropout(h2, 0.3, rng, residual=h1)
+    loss = head.linear_cross_entropy(h3, w3, target, b3, label_smoothing=0.05)
+    return loss, torch.autograd.grad(loss, params)
+
+
+def head_params(dt, D, H, V, seed):
+    p = make(seed, (H, D), (H,), (H, H), (H,), (V, H), (V,))
+    return [(t / math.sqrt(t.shape[-1]) if t.dim() == 2 else 0.1 * t).to(dt).cuda().requires_grad_() for t in p]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_the_operators_together(kind):
+    """A head's step against the same step in 64 bits.  Three layers of rounding, each of h relative to its values and
+    amplified by norms near 1: 16 h of a tensor's norm (and what float32 sums leave, 1e-5) bounds it."""
+    dt = TYPES[kind]
+    params = head_params(dt, 96, 128, 333, 51)
+    x, = make(52, (200, 96))
+    x = x.to(dt).cuda()
+    target = torch.randint(0, 333, (200,), generator=torch.Generator().manual_seed(1)).cuda()
+    target[::9] = -100
+    rng = torch.tensor([77, 3], dtype=torch.int64, device="cuda")
+    loss, grads = head_step(x, params, target, rng)
+    P = [p.detach().cpu().double().requires_grad_() for p in params]
+    keep = torch.from_numpy(ho.keep_mask(200 * 128, 0.3, 77, 3)).view(200, 128).double()
+    X = x.cpu().double()
+    h1 = torch.relu(X @ P[0].t() + P[1])
+    h2 = torch.nn.functional.gelu(h1 @ P[2].t() + P[3])
+    h3 = h1 + keep * h2 / 0.7
+    want = torch.nn.functional.cross_entropy(h3 @ P[4].t() + P[5], target.cpu(), label_smoothing=0.05)
+    wg = torch.autograd.grad(want, P)
+    tol = 16 * ho.half_step(dt) + 1e-5
+    assert abs(loss.item() - want.item()) <= tol * abs(want.item())
+    for g, v in zip(grads, wg):
+        assert (g.cpu().double() - v).norm() <= tol * v.norm()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_results_do_not_change_from_run_to_run(kind):
+    dt = TYPES[kind]
+    params = head_params(dt, 96, 128, 333, 61)
+    x = make(62, (300, 96))[0].to(dt).cuda()
+    target = torch.randint(0, 333, (300,), generator=torch.Generator().manual_seed(2)).cuda()
+    rng = torch.tensor([5, 5], dtype=torch.int64, device="cuda")
+    loss, grads = head_step(x, params, target, rng)
+    for _ in range(3):
+        again, more = head_step(x, params, target, rng)
+        assert torch.equal(loss, again) and all(torch.equal(a, b) for a, b in zip(grads, more))
+
+
+def test_two_captured_steps_replayed_between_eager_work():
+    """Two graphs of the same step on different inputs, replayed in turn, with a new mask each time and eager work and
+    synchronizations in between; every replay against the eager result."""
+    dt = torch.bfloat16
+    params = head_params(dt, 64, 128, 200, 71)
+    target = torch.randint(0, 200, (96,), generator=torch.Generator().manual_seed(3)).cuda()
+    xs = [make(s, (96, 64))[0].to(dt).cuda() for s in (72, 73)]
+    rngs = [torch.tensor([7, i], dtype=torch.int64, device="cuda") for i in range(2)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        head_step(xs[0], params, target, rngs[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for x, rng in zip(xs, rngs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            loss, grads = head_step(x, params, target, rng)
+        graphs.append(g)
+        outs.append((loss, grads))
+    for step in range(4):
+        for i in range(2):
+            xs[i].copy_(make(100 + 2 * step + i, (96, 64))[0].to(dt))
+            rngs[i].add_(11)
+        for i in range(2):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            loss, grads = head_step(xs[i], params, target, rngs[i])
+            assert torch.equal(loss, outs[i][0]), (step, i)
+            assert all(torch.equal(a, b) for a, b in zip(grads, outs[i][1])), (step, i)
+
+
+def test_calls_on_two_streams_at_once():
+    dt = torch.bfloat16
+    params = head_params(dt, 256, 512, 3000, 81)
+    target = torch.randint(0, 3000, (512,), generator=torch.Generator().manual_seed(4)).cuda()
+    xs = [make(s, (512, 256))[0].to(dt).cuda() for s in (82, 83)]
+    rng = torch.tensor([1, 2], dtype=torch.int64, device="cuda")
+    want = [head_step(x, params, target, rng) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = []
+    for _ in range(3):
+        for x, s in zip(xs, streams):
+            with torch.cuda.stream(s):
+                got.append(head_step(x, params, target, rng))
+    torch.cuda.synchronize()
+    for i, (loss, grads) in enumerate(got):
+        assert torch.equal(loss, want[i % 2][0])
+        assert all(torch.equal(a, b) for a, b in zip(grads, want[i % 2][1]))
+
+
+def test_refusals_on_the_device():
+    x, w = torch.zeros(4, 8, device="cuda"), torch.zeros(6, 8, device="cuda")
+    t = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for bad, err in ((lambda: head.linear(x, w.bfloat16()), TypeError), (lambda: head.linear(x, w[:, :5]), ValueError),
+                     (lambda: head.linear(x.double(), w.double()), TypeError), (lambda: head.linear(x, w.cpu()), RuntimeError),
+                     (lambda: head.linear(x, w, torch.zeros(5, device="cuda")), ValueError),
+                     (lambda: head.linear(x, w, residual=torch.zeros(4, 5, device="cuda")), ValueError),
+                     (lambda: head.dropout(x, 1.5, 0), ValueError), (lambda: head.dropout(x, float("nan"), 0), ValueError),
+                     (lambda: head.dropout(x, 0.5, torch.zeros(2, device="cuda")), ValueError),
+                     (lambda: head.dropout(x, 0.5, torch.zeros(2, dtype=torch.int64, device="cuda"), 1), ValueError),
+                     (lambda: head.dropout(x, 0.5, 0, residual=x[:2]), ValueError),
+                     (lambda: head.linear_cross_entropy(x, w, t[:3]), ValueError),
+                     (lambda: head.linear_cross_entropy(x, w, t.float()), TypeError),
+                     (lambda: head.linear_cross_entropy(x, w, t.cpu()), RuntimeError),
+                     (lambda: head.linear_cross_entropy(x, w, t, label_smoothing=2.0), ValueError)):
+        with pytest.raises(err):
+            bad()
+    y = head.linear(x.requires_grad_(), w)
+    dx, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):                     # differentiable once
+        torch.autograd.grad(dx.sum() + 0 * y.sum(), w.requires_grad_())
