@@ -377,10 +377,14 @@ int pngpd_adam_step(float* params_dev, const float* grads_dev, float* exp_avg_de
  *
  * Matrices are row-major; ld* is the distance of two rows in elements (at least the row's length), and a matrix
  * without an ld argument is dense.  `type` is the element type of every matrix and bias; sums and statistics are
- * 32-bit (64-bit over a batch's losses).  Outputs must not overlap inputs or each other.  Sizes: 0 <= rows, 1 <= the
- * others, each below 2^31.  A call with no rows launches what the outputs that do not depend on rows need (zero
- * gradients).  All calls are stream-ordered, allocate nothing and can be captured into a graph; two calls that may
- * run at the same time need workspaces of their own.
+ * 32-bit (64-bit over a batch's losses).  Outputs must not overlap inputs or each other.  Sizes: 0 <= rows < 2^31,
+ * 1 <= N, K, D <= 2^21, 1 <= V < 2^31, T V <= 2^44.  A call with no rows still writes the outputs that do not depend on
+ * rows (zero gradients).  All calls are stream-ordered, allocate nothing and can be captured into a graph; two calls
+ * that may run at the same time need workspaces of their own.
+ *
+ * Matrices may start anywhere and have any ld, but rows that are not whole 16-byte chunks are copied into the workspace
+ * first.  pngpd_*_workspace_bytes(..., aligned): aligned != 0 if x, weight and dy start at 16-byte addresses and their
+ * ld is a multiple of 16 bytes up to 2^23 bytes, 0 if not (more workspace, whatever the call is given).
  * ------------------------------------------------------------------------------------------ */
 enum { PNGPD_TYPE_F32 = 0, PNGPD_TYPE_BF16 = 1, PNGPD_TYPE_F16 = 2 };
 enum { PNGPD_ACT_NONE = 0, PNGPD_ACT_RELU = 1, PNGPD_ACT_GELU = 2, PNGPD_ACT_GELU_TANH = 3, PNGPD_ACT_SILU = 4 };
@@ -391,7 +395,7 @@ enum { PNGPD_REDUCE_NONE = 0, PNGPD_REDUCE_MEAN = 1, PNGPD_REDUCE_SUM = 2 };
  * z_dev [M,N], optional: x weight^T + bias rounded to `type`, which pngpd_linear_backward takes (a ReLU's tiny positive
  * sums keep their sign there).  Needed for the backward pass of every activation but NONE.
  */
-size_t pngpd_linear_workspace_bytes(int type, int64_t M, int64_t N, int64_t K, int backward);
+size_t pngpd_linear_workspace_bytes(int type, int64_t M, int64_t N, int64_t K, int backward, int aligned);
 int pngpd_linear_forward(int type, int64_t M, int64_t N, int64_t K, const void* x_dev, int64_t ldx, const void* weight_dev,
                          int64_t ldw, const void* bias_dev, int act, const void* residual_dev, int64_t ldr, void* y_dev,
                          void* z_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
@@ -424,7 +428,7 @@ int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64
  * loss_dev: float [T] for PNGPD_REDUCE_NONE, else float [1] (the mean is over the rows that are not ignored: NaN when
  * there are none).  lse_dev float [T]: log sum exp of every row's logits, what the backward pass needs.
  */
-size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V, int64_t D, int backward);
+size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V, int64_t D, int backward, int aligned);
 int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D, const void* x_dev, int64_t ldx,
                                        const void* weight_dev, int64_t ldw, const void* bias_dev, const int64_t* target_dev,
                                        int64_t ignore_index, float label_smoothing, int reduction, float* loss_dev,

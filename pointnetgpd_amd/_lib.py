@@ -79,14 +79,14 @@ SIGNATURES = {
     "pngpd_nll_loss": (c_int, [c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "pngpd_adam_step": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_float, c_float, c_float, c_float,
                                 c_int, c_float, c_void_p]),
-    "pngpd_linear_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int]),
+    "pngpd_linear_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int, c_int]),
     "pngpd_linear_forward": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int,
                                      c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "pngpd_linear_backward": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
                                       c_void_p, c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "pngpd_dropout": (c_int, [c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_double, c_uint64,
                               c_uint64, c_void_p, c_void_p]),
-    "pngpd_linear_cross_entropy_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int]),
+    "pngpd_linear_cross_entropy_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int, c_int]),
     "pngpd_linear_cross_entropy_forward": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                                    c_void_p, c_void_p, c_int64, c_float, c_int, c_void_p, c_void_p, c_void_p,
                                                    c_size_t, c_void_p]),

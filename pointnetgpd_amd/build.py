@@ -36,6 +36,9 @@ LIB_SOURCES = [
     "tall_gemm.hip",
     "train_api.cpp",
     "head_product.hip",
+    "head_tile_f32.hip",
+    "head_tile_bf16.hip",
+    "head_tile_f16.hip",
     "head_dropout.hip",
     "head_loss.hip",
     "head_api.cpp",

@@ -6,45 +6,74 @@
 
 namespace pngpd {
 
-// One operand of a product out[m][n] = sum_k A(m,k) B(n,k).  Rows (m or n) are `rows`, the contraction index is k.
+constexpr int64_t HEAD_MAX_LD = (int64_t)1 << 23;            // bytes between rows: 256 rows stay below 2^31
+constexpr int64_t HEAD_MAX_EXTENT = HEAD_MAX_LD / 4;         // elements of a dense row
+
+// One operand of a product out[m][n] = sum_k A(m,k) B(n,k).
 // k_contiguous: element (r, k) sits at p[r * ld + k]; otherwise at p[k * ld + r] (the operand lies transposed).
+// Both take rows as head_direct() describes them; head_lay_out() makes such rows of others.
 struct HeadOperand {
     const void* p;
     int64_t ld;
     bool k_contiguous;
 };
+// 16-byte aligned rows whose dense extent is whole 16-byte chunks (or has zeros behind it up to one), and distances that
+// keep a tile's offsets below 2^31
+inline bool head_direct(const void* p, int64_t ld, int64_t extent, size_t size) {
+    const int64_t c = 16 / (int64_t)size;
+    return ((uintptr_t)p & 15) == 0 && ld % c == 0 && extent % c == 0 && ld <= HEAD_MAX_LD / (int64_t)size;
+}
 
 // What becomes of a product's 32-bit sums.
-enum { HEAD_EPI_LINEAR = 0, HEAD_EPI_DZ = 1, HEAD_EPI_SCALED = 2 };
+enum { HEAD_EPI_LINEAR = 0, HEAD_EPI_DZ = 1, HEAD_EPI_SCALED = 2, HEAD_EPI_STATS = 3 };
 struct HeadEpilogue {
     int kind = HEAD_EPI_SCALED;
-    // LINEAR: out = act(acc + bias[n]) + residual[m][n]; z (may be NULL) receives acc + bias, rows ld_out_z = N
+    // LINEAR: out = act(acc + bias[n]) + residual[m][n]; z (may be NULL, dense [M][N]) receives acc + bias
     const void* bias = nullptr;
     const void* residual = nullptr;
     int64_t ld_residual = 0;
     int act = 0;
     void* z = nullptr;
-    // DZ: out = (exp(acc + bias[n] - lse[m]) - smooth - (target[m] == n + first_n ? 1 - eps : 0)) * row_weight[m]
+    // DZ: out = (exp(acc + bias[n] - lse[m]) - smooth - (target[m] == n + first_n ? 1 - eps : 0)) * row_weight[m]; rows of
+    // ld_out, zeros behind column N
     const float* lse = nullptr;
     const float* row_weight = nullptr;
     const int64_t* target = nullptr;
     int64_t first_n = 0;
     float smooth = 0.f, one_minus_eps = 1.f;
-    // SCALED: out = scale[0] * (acc + add[m][n]); scale NULL: 1; add NULL: 0 (32-bit, rows of N)
+    // SCALED: out = scale[0] * (acc + add[m][n]); scale NULL: 1; add NULL: 0 (32-bit, dense [M][N])
     const float* scale = nullptr;
     const float* add = nullptr;
-    // the output: `type` as the operands, or 32-bit floats when out_f32
+    // STATS: stats[i][m] = maximum, sum of exp(z - maximum) and sum of row m's logits z = acc + bias in the i-th block of
+    // columns; target_logit[m] = z[m][target[m]] where that is a column
+    float4* stats = nullptr;
+    float* target_logit = nullptr;
+    // the output (all but STATS): of the operands' type, or 32-bit floats when out_f32
     void* out = nullptr;
     int64_t ld_out = 0;
     bool out_f32 = false;
 };
 
-hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b,
-                        const HeadEpilogue& e, hipStream_t s);
+// How a product is cut: tile shape, cuts of the contraction (joined by a second kernel from 32-bit partial sums).
+struct HeadPlan {
+    int shape, splits, tiles_m, tiles_n;
+    int64_t k_split;
+    size_t partial_bytes;
+    int stats_blocks;           // blocks of columns a STATS epilogue writes
+};
+HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind);
 
-// dz[m][n] = dy[m][n] * act'(z[m][n]) (rows of N)
-hipError_t head_act_backward(int type, int64_t M, int64_t N, const void* dy, int64_t ld_dy, const void* z, int act,
-                             void* dz, hipStream_t s);
+// partial: head_plan(...).partial_bytes
+hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b,
+                        const HeadEpilogue& e, float* partial, hipStream_t s);
+
+// dst[r][0 .. ld) = src[r][0 .. cols) and zeros behind them; rows with row_weight[r] == 0 (row_weight may be NULL) become
+// zeros whatever they hold.  dst is 16-byte aligned, ld whole chunks.
+hipError_t head_lay_out(int type, int64_t rows, int64_t cols, const void* src, int64_t ld_src, const float* row_weight, void* dst,
+                        int64_t ld, hipStream_t s);
+// dz[m][n] = dy[m][n] * act'(z[m][n]); z dense, dz rows of ld_dz (whole chunks) with zeros behind column N
+hipError_t head_act_backward(int type, int64_t M, int64_t N, const void* dy, int64_t ld_dy, const void* z, int act, void* dz,
+                             int64_t ld_dz, hipStream_t s);
 // out[n] = scale * sum_m a[m][n]; part: 32-bit [head_col_sum_parts(M)][N]
 int64_t head_col_sum_parts(int64_t M);
 hipError_t head_col_sum(int type, int64_t M, int64_t N, const void* a, int64_t ld, float* part, const float* scale,
@@ -57,20 +86,13 @@ hipError_t head_dropout(int type, int64_t rows, int64_t cols, const void* x, int
                         int64_t ldr, void* y, double p, uint64_t seed, uint64_t offset, const int64_t* rng_dev,
                         hipStream_t s);
 
-// Running statistics of a row of logits over the pieces of the vocabulary.
-struct HeadRowStats {
-    float *max, *sum, *target_logit, *logit_sum;      // [T] each
-};
-hipError_t head_stats_piece(int64_t T, int64_t n, const float* logits, int64_t ld, int64_t first_n,
-                            const int64_t* target, const HeadRowStats& st, bool first, hipStream_t s);
-hipError_t head_loss_finish(int64_t T, int64_t V, const int64_t* target, int64_t ignore_index, float eps, int reduction,
-                            const HeadRowStats& st, float* loss, float* lse, hipStream_t s);
+// lse[t] and the loss of every row from its statistics; the batch's loss into `loss` (row_loss then is scratch), or the
+// rows' (reduction none: row_loss == loss)
+hipError_t head_loss_finish(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit,
+                            const int64_t* target, int64_t ignore_index, float eps, int reduction, float* row_loss, float* loss,
+                            float* lse, hipStream_t s);
 // row_weight[t] = weight of row t in the gradient divided by 2^e, out_scale[0] = 2^e (type f16 only, else 2^e = 1)
 hipError_t head_row_weights(int type, int64_t T, int64_t V, const int64_t* target, int64_t ignore_index, int reduction,
                             const float* dloss, float* row_weight, float* out_scale, hipStream_t s);
-
-// out[t] = x[t] where row_weight[t] != 0, zeros elsewhere (rows of D): what a padding row holds stays out of sums
-hipError_t head_live_rows(int type, int64_t T, int64_t D, const void* x, int64_t ldx, const float* row_weight, void* out,
-                          hipStream_t s);
 
 }  // namespace pngpd

@@ -10,10 +10,9 @@ namespace {
 using pngpd::fail;
 using pngpd::HeadEpilogue;
 using pngpd::HeadOperand;
-using pngpd::HeadRowStats;
 
 constexpr int64_t MAX_SIZE = 2147483647;
-constexpr size_t PIECE_BYTES = (size_t)256 << 20;      // of logits (forward) or their gradients (backward) at a time
+constexpr size_t PIECE_BYTES = (size_t)256 << 20;      // of the logits' gradients at a time
 
 inline size_t esize(int type) { return type == PNGPD_TYPE_F32 ? 4 : 2; }
 inline bool type_ok(int type) { return type >= PNGPD_TYPE_F32 && type <= PNGPD_TYPE_F16; }
@@ -36,6 +35,15 @@ int check_sizes(const char* who, int type, int64_t rows, int64_t a, int64_t b) {
     return PNGPD_OK;
 }
 
+int check_linear(const char* who, int type, int64_t M, int64_t N, int64_t K, int act) {
+    int rc = check_sizes(who, type, M, N, K);
+    if (rc) return rc;
+    if (N > pngpd::HEAD_MAX_EXTENT || K > pngpd::HEAD_MAX_EXTENT)
+        return fail(PNGPD_ERR_SHAPE, "%s: N = %lld, K = %lld, at most %lld", who, (long long)N, (long long)K, (long long)pngpd::HEAD_MAX_EXTENT);
+    if (act < PNGPD_ACT_NONE || act > PNGPD_ACT_SILU) return fail(PNGPD_ERR_INVALID, "%s: unknown activation %d", who, act);
+    return PNGPD_OK;
+}
+
 int check_ld(const char* who, const char* name, int64_t ld, int64_t least) {
     if (ld < least || ld > ((int64_t)1 << 40)) return fail(PNGPD_ERR_SHAPE, "%s: %s = %lld for rows of %lld", who, name, (long long)ld, (long long)least);
     return PNGPD_OK;
@@ -49,50 +57,95 @@ int check_ws(const char* who, const void* ws, size_t have, size_t need) {
     return PNGPD_OK;
 }
 
+// rows of `extent` elements as the products take them: whole 16-byte chunks
+inline int64_t padded(int64_t extent, int type) {
+    const int64_t c = 16 / (int64_t)esize(type);
+    return (extent + c - 1) / c * c;
+}
+
+// An operand as the products take it: itself, or a copy in `room` (rows of padded(extent)).
+struct Rows {
+    const void* p;
+    int64_t ld;
+};
+inline bool direct(const void* p, int64_t ld, int64_t extent, int type) { return pngpd::head_direct(p, ld, extent, esize(type)); }
+hipError_t direct_rows(int type, int64_t rows, int64_t extent, const void* p, int64_t ld, void* room, hipStream_t s, Rows* out) {
+    if (direct(p, ld, extent, type)) {
+        *out = Rows{p, ld};
+        return hipSuccess;
+    }
+    *out = Rows{room, padded(extent, type)};
+    return pngpd::head_lay_out(type, rows, extent, p, ld, nullptr, room, out->ld, s);
+}
+
+inline size_t max2(size_t a, size_t b) { return a > b ? a : b; }
+
 struct LinearWs {
-    void* dz;
-    float* part;
+    void *x, *w, *dz;           // laid out, if they have to be
+    float *part, *partial;
     size_t bytes;
-    LinearWs(void* base, int type, int64_t M, int64_t N, int64_t K, bool backward) {
+    // copy_*: x, weight or dz (dy where there is no activation) is not as the products take it
+    LinearWs(void* base, int type, int64_t M, int64_t N, int64_t K, bool backward, bool copy_x, bool copy_w, bool copy_dz) {
         Bump b(base);
         dz = nullptr;
-        part = nullptr;
-        if (backward && M > 0) {
-            dz = b.take((size_t)M * N * esize(type));
-            part = (float*)b.take((size_t)pngpd::head_col_sum_parts(M) * N * 4);
+        part = partial = nullptr;
+        x = w = nullptr;
+        if (M > 0) {
+            if (copy_x) x = b.take((size_t)M * padded(K, type) * esize(type));
+            if (copy_w) w = b.take((size_t)N * padded(K, type) * esize(type));
+            size_t cut = pngpd::head_plan(type, M, N, K, pngpd::HEAD_EPI_LINEAR).partial_bytes;
+            if (backward) {
+                if (copy_dz) dz = b.take((size_t)M * padded(N, type) * esize(type));
+                part = (float*)b.take((size_t)pngpd::head_col_sum_parts(M) * N * 4);
+                cut = max2(pngpd::head_plan(type, M, K, N, pngpd::HEAD_EPI_SCALED).partial_bytes,
+                           pngpd::head_plan(type, N, K, M, pngpd::HEAD_EPI_SCALED).partial_bytes);
+            }
+            partial = (float*)b.take(cut);
         }
-        (void)K;
         bytes = b.off;
     }
 };
 
 struct LossWs {
-    int64_t piece;             // columns of the vocabulary at a time
-    void* tile;                // logits (32-bit, forward) or their gradients (of the type, backward): [T, piece]
-    HeadRowStats st;
-    float *row_weight, *scale, *part, *dx_sum;
-    void* x;
+    int64_t piece;             // columns of the vocabulary whose gradients are formed at a time
+    void *x, *w, *tile;        // laid out; gradients of a piece's logits, [T][padded(piece)]
+    float4* stats;
+    float *target_logit, *row_loss, *row_weight, *scale, *part, *dx_sum, *partial;
     size_t bytes;
-    LossWs(void* base, int type, int64_t T, int64_t V, int64_t D, bool backward) {
+    LossWs(void* base, int type, int64_t T, int64_t V, int64_t D, bool backward, bool copy_x, bool copy_w) {
         Bump b(base);
-        const int64_t rows = T > 0 ? T : 1;
-        const size_t e = backward ? esize(type) : 4;
-        piece = (int64_t)(PIECE_BYTES / ((size_t)rows * e)) / 256 * 256;
-        if (piece < 256) piece = 256;
-        if (piece > V) piece = V;
-        tile = b.take((size_t)rows * piece * e);
-        st = HeadRowStats{};
-        row_weight = scale = part = dx_sum = nullptr;
-        x = nullptr;
+        const int64_t rows = T > 0 ? T : 1, dp = padded(D, type);
+        const size_t e = esize(type);
+        x = copy_x || backward ? b.take((size_t)rows * dp * e) : nullptr;      // the gradients take a copy without padding rows
+        w = copy_w ? b.take((size_t)V * dp * e) : nullptr;
+        tile = nullptr;
+        stats = nullptr;
+        target_logit = row_loss = row_weight = scale = part = dx_sum = partial = nullptr;
+        piece = V;
         if (!backward) {
-            float* p = (float*)b.take((size_t)rows * 4 * 4);
-            st = HeadRowStats{p, p + rows, p + 2 * rows, p + 3 * rows};
+            const pngpd::HeadPlan p = pngpd::head_plan(type, rows, V, D, pngpd::HEAD_EPI_STATS);
+            stats = (float4*)b.take((size_t)p.stats_blocks * rows * sizeof(float4));
+            target_logit = (float*)b.take((size_t)rows * 4);
+            row_loss = (float*)b.take((size_t)rows * 4);
+            partial = (float*)b.take(p.partial_bytes);
         } else {
+            piece = (int64_t)(PIECE_BYTES / ((size_t)rows * e)) / 256 * 256;
+            if (piece < 256) piece = 256;
+            if (piece > pngpd::HEAD_MAX_EXTENT) piece = pngpd::HEAD_MAX_EXTENT;
+            if (piece > V) piece = V;
+            tile = b.take((size_t)rows * padded(piece, type) * e);
             row_weight = (float*)b.take((size_t)rows * 4);
             scale = (float*)b.take(4);
-            x = b.take((size_t)rows * D * esize(type));
             part = (float*)b.take((size_t)pngpd::head_col_sum_parts(T) * piece * 4);
             if (piece < V) dx_sum = (float*)b.take((size_t)rows * D * 4);
+            size_t cut = 0;
+            const int64_t last = V % piece ? V % piece : piece;
+            for (int64_t n : {piece, last}) {
+                cut = max2(cut, pngpd::head_plan(type, rows, n, D, pngpd::HEAD_EPI_DZ).partial_bytes);
+                cut = max2(cut, pngpd::head_plan(type, n, D, rows, pngpd::HEAD_EPI_SCALED).partial_bytes);
+                cut = max2(cut, pngpd::head_plan(type, rows, D, n, pngpd::HEAD_EPI_SCALED).partial_bytes);
+            }
+            partial = (float*)b.take(cut);
         }
         bytes = b.off;
     }
@@ -102,6 +155,8 @@ int check_loss(const char* who, int type, int64_t T, int64_t V, int64_t D, const
                const int64_t* target, float eps, int reduction) {
     int rc = check_sizes(who, type, T, V, D);
     if (rc) return rc;
+    if (D > pngpd::HEAD_MAX_EXTENT) return fail(PNGPD_ERR_SHAPE, "%s: D = %lld, at most %lld", who, (long long)D, (long long)pngpd::HEAD_MAX_EXTENT);
+    if ((double)T * (double)V > 17592186044416.0) return fail(PNGPD_ERR_SHAPE, "%s: T x V beyond 2^44", who);
     if (!w || (T > 0 && (!x || !target))) return fail(PNGPD_ERR_INVALID, "%s: NULL argument", who);
     if ((rc = check_ld(who, "ldx", ldx, D)) || (rc = check_ld(who, "ldw", ldw, D))) return rc;
     if (!(eps >= 0.f && eps <= 1.f)) return fail(PNGPD_ERR_INVALID, "%s: label_smoothing %g", who, (double)eps);
@@ -116,23 +171,23 @@ inline void* at(void* p, int64_t elements, int type) { return p ? (char*)p + (si
 
 extern "C" {
 
-size_t pngpd_linear_workspace_bytes(int type, int64_t M, int64_t N, int64_t K, int backward) {
-    if (check_sizes("pngpd_linear_workspace_bytes", type, M, N, K)) return 0;
-    return LinearWs(nullptr, type, M, N, K, backward != 0).bytes;
+size_t pngpd_linear_workspace_bytes(int type, int64_t M, int64_t N, int64_t K, int backward, int aligned) {
+    if (check_linear("pngpd_linear_workspace_bytes", type, M, N, K, PNGPD_ACT_NONE)) return 0;
+    const bool k = !aligned || padded(K, type) != K;
+    return LinearWs(nullptr, type, M, N, K, backward != 0, k, k, true).bytes;
 }
 
 int pngpd_linear_forward(int type, int64_t M, int64_t N, int64_t K, const void* x_dev, int64_t ldx, const void* weight_dev,
                          int64_t ldw, const void* bias_dev, int act, const void* residual_dev, int64_t ldr, void* y_dev,
                          void* z_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
     const char* who = "pngpd_linear_forward";
-    int rc = check_sizes(who, type, M, N, K);
+    int rc = check_linear(who, type, M, N, K, act);
     if (rc) return rc;
-    if (act < PNGPD_ACT_NONE || act > PNGPD_ACT_SILU) return fail(PNGPD_ERR_INVALID, "%s: unknown activation %d", who, act);
     if (M == 0) return PNGPD_OK;
     if (!x_dev || !weight_dev || !y_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL argument", who);
     if ((rc = check_ld(who, "ldx", ldx, K)) || (rc = check_ld(who, "ldw", ldw, K))) return rc;
     if (residual_dev && (rc = check_ld(who, "ldr", ldr, N))) return rc;
-    LinearWs ws(workspace_dev, type, M, N, K, false);
+    LinearWs ws(workspace_dev, type, M, N, K, false, !direct(x_dev, ldx, K, type), !direct(weight_dev, ldw, K, type), false);
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
     HeadEpilogue e;
     e.kind = pngpd::HEAD_EPI_LINEAR;
@@ -143,7 +198,11 @@ int pngpd_linear_forward(int type, int64_t M, int64_t N, int64_t K, const void* 
     e.z = z_dev;
     e.out = y_dev;
     e.ld_out = N;
-    HIP_TRY(pngpd::head_product(type, M, N, K, HeadOperand{x_dev, ldx, true}, HeadOperand{weight_dev, ldw, true}, e, (hipStream_t)stream));
+    hipStream_t s = (hipStream_t)stream;
+    Rows x, w;
+    HIP_TRY(direct_rows(type, M, K, x_dev, ldx, ws.x, s, &x));
+    HIP_TRY(direct_rows(type, N, K, weight_dev, ldw, ws.w, s, &w));
+    HIP_TRY(pngpd::head_product(type, M, N, K, HeadOperand{x.p, x.ld, true}, HeadOperand{w.p, w.ld, true}, e, ws.partial, s));
     return PNGPD_OK;
 }
 
@@ -151,9 +210,8 @@ int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void*
                           const void* x_dev, int64_t ldx, const void* weight_dev, int64_t ldw, int act, void* dx_dev,
                           void* dweight_dev, void* dbias_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
     const char* who = "pngpd_linear_backward";
-    int rc = check_sizes(who, type, M, N, K);
+    int rc = check_linear(who, type, M, N, K, act);
     if (rc) return rc;
-    if (act < PNGPD_ACT_NONE || act > PNGPD_ACT_SILU) return fail(PNGPD_ERR_INVALID, "%s: unknown activation %d", who, act);
     hipStream_t s = (hipStream_t)stream;
     if (M == 0) {
         if (dweight_dev) HIP_TRY(pngpd::head_zero(dweight_dev, (size_t)N * K * esize(type), s));
@@ -165,26 +223,27 @@ int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void*
     if ((rc = check_ld(who, "ld_dy", ld_dy, N))) return rc;
     if (dweight_dev && (rc = check_ld(who, "ldx", ldx, K))) return rc;
     if (dx_dev && (rc = check_ld(who, "ldw", ldw, K))) return rc;
-    LinearWs ws(workspace_dev, type, M, N, K, true);
+    LinearWs ws(workspace_dev, type, M, N, K, true, dweight_dev && !direct(x_dev, ldx, K, type),
+                dx_dev && !direct(weight_dev, ldw, K, type), act != PNGPD_ACT_NONE || !direct(dy_dev, ld_dy, N, type));
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
-    const void* dz = dy_dev;
-    int64_t ld_dz = ld_dy;
-    if (act != PNGPD_ACT_NONE) {
-        HIP_TRY(pngpd::head_act_backward(type, M, N, dy_dev, ld_dy, z_dev, act, ws.dz, s));
-        dz = ws.dz;
-        ld_dz = N;
-    }
-    if (dbias_dev) HIP_TRY(pngpd::head_col_sum(type, M, N, dz, ld_dz, ws.part, nullptr, dbias_dev, s));
+    Rows dz{ws.dz, padded(N, type)};
+    if (act != PNGPD_ACT_NONE) HIP_TRY(pngpd::head_act_backward(type, M, N, dy_dev, ld_dy, z_dev, act, ws.dz, dz.ld, s));
+    else HIP_TRY(direct_rows(type, M, N, dy_dev, ld_dy, ws.dz, s, &dz));
+    if (dbias_dev) HIP_TRY(pngpd::head_col_sum(type, M, N, dz.p, dz.ld, ws.part, nullptr, dbias_dev, s));
     HeadEpilogue e;
     e.kind = pngpd::HEAD_EPI_SCALED;
     e.ld_out = K;
     if (dx_dev) {
+        Rows w;
+        HIP_TRY(direct_rows(type, N, K, weight_dev, ldw, ws.w, s, &w));
         e.out = dx_dev;
-        HIP_TRY(pngpd::head_product(type, M, K, N, HeadOperand{dz, ld_dz, true}, HeadOperand{weight_dev, ldw, false}, e, s));
+        HIP_TRY(pngpd::head_product(type, M, K, N, HeadOperand{dz.p, dz.ld, true}, HeadOperand{w.p, w.ld, false}, e, ws.partial, s));
     }
     if (dweight_dev) {
+        Rows x;
+        HIP_TRY(direct_rows(type, M, K, x_dev, ldx, ws.x, s, &x));
         e.out = dweight_dev;
-        HIP_TRY(pngpd::head_product(type, N, K, M, HeadOperand{dz, ld_dz, false}, HeadOperand{x_dev, ldx, false}, e, s));
+        HIP_TRY(pngpd::head_product(type, N, K, M, HeadOperand{dz.p, dz.ld, false}, HeadOperand{x.p, x.ld, false}, e, ws.partial, s));
     }
     return PNGPD_OK;
 }
@@ -203,9 +262,11 @@ int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64
     return PNGPD_OK;
 }
 
-size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V, int64_t D, int backward) {
-    if (check_sizes("pngpd_linear_cross_entropy_workspace_bytes", type, T, V, D)) return 0;
-    return LossWs(nullptr, type, T, V, D, backward != 0).bytes;
+size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V, int64_t D, int backward, int aligned) {
+    const void* some = &type;      // the sizes alone are checked
+    if (check_loss("pngpd_linear_cross_entropy_workspace_bytes", type, T, V, D, some, D, some, D, (const int64_t*)some, 0.f, 0)) return 0;
+    const bool d = !aligned || padded(D, type) != D;
+    return LossWs(nullptr, type, T, V, D, backward != 0, d, d).bytes;
 }
 
 int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D, const void* x_dev, int64_t ldx,
@@ -218,24 +279,25 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
     if ((T > 0 || reduction != PNGPD_REDUCE_NONE) && !loss_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL loss", who);
     if (T > 0 && !lse_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL lse", who);
     hipStream_t s = (hipStream_t)stream;
-    LossWs ws(workspace_dev, type, T, V, D, false);
+    LossWs ws(workspace_dev, type, T, V, D, false, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
     if (T > 0) {
         if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
-        for (int64_t v = 0; v < V; v += ws.piece) {
-            const int64_t n = V - v < ws.piece ? V - v : ws.piece;
-            HeadEpilogue e;
-            e.kind = pngpd::HEAD_EPI_LINEAR;
-            e.bias = at(bias_dev, v, type);
-            e.out = ws.tile;
-            e.ld_out = n;
-            e.out_f32 = true;
-            HIP_TRY(pngpd::head_product(type, T, n, D, HeadOperand{x_dev, ldx, true}, HeadOperand{at(weight_dev, v * ldw, type), ldw, true}, e, s));
-            HIP_TRY(pngpd::head_stats_piece(T, n, (const float*)ws.tile, n, v, target_dev, ws.st, v == 0, s));
-        }
+        Rows x, w;
+        HIP_TRY(direct_rows(type, T, D, x_dev, ldx, ws.x, s, &x));
+        HIP_TRY(direct_rows(type, V, D, weight_dev, ldw, ws.w, s, &w));
+        HeadEpilogue e;
+        e.kind = pngpd::HEAD_EPI_STATS;
+        e.bias = bias_dev;
+        e.target = target_dev;
+        e.stats = ws.stats;
+        e.target_logit = ws.target_logit;
+        HIP_TRY(pngpd::head_product(type, T, V, D, HeadOperand{x.p, x.ld, true}, HeadOperand{w.p, w.ld, true}, e, ws.partial, s));
     } else if (reduction == PNGPD_REDUCE_NONE) {
         return PNGPD_OK;
     }
-    HIP_TRY(pngpd::head_loss_finish(T, V, target_dev, ignore_index, label_smoothing, reduction, ws.st, loss_dev, lse_dev, s));
+    const int blocks = T > 0 ? pngpd::head_plan(type, T, V, D, pngpd::HEAD_EPI_STATS).stats_blocks : 0;
+    HIP_TRY(pngpd::head_loss_finish(T, V, blocks, ws.stats, ws.target_logit, target_dev, ignore_index, label_smoothing, reduction,
+                                    reduction == PNGPD_REDUCE_NONE ? loss_dev : ws.row_loss, loss_dev, lse_dev, s));
     return PNGPD_OK;
 }
 
@@ -254,14 +316,16 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         return PNGPD_OK;
     }
     if (!lse_dev || !dloss_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL argument", who);
-    LossWs ws(workspace_dev, type, T, V, D, true);
+    LossWs ws(workspace_dev, type, T, V, D, true, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
     HIP_TRY(pngpd::head_row_weights(type, T, V, target_dev, ignore_index, reduction, dloss_dev, ws.row_weight, ws.scale, s));
-    HIP_TRY(pngpd::head_live_rows(type, T, D, x_dev, ldx, ws.row_weight, ws.x, s));
-    const HeadOperand x{ws.x, D, true};
+    const HeadOperand x{ws.x, padded(D, type), true}, xt{ws.x, padded(D, type), false};
+    HIP_TRY(pngpd::head_lay_out(type, T, D, x_dev, ldx, ws.row_weight, ws.x, x.ld, s));
+    Rows whole;
+    HIP_TRY(direct_rows(type, V, D, weight_dev, ldw, ws.w, s, &whole));
     for (int64_t v = 0; v < V; v += ws.piece) {
-        const int64_t n = V - v < ws.piece ? V - v : ws.piece;
-        const void* w = at(weight_dev, v * ldw, type);
+        const int64_t n = V - v < ws.piece ? V - v : ws.piece, np = padded(n, type);
+        const void* w = at(whole.p, v * whole.ld, type);
         HeadEpilogue e;
         e.kind = pngpd::HEAD_EPI_DZ;
         e.bias = at(bias_dev, v, type);
@@ -272,16 +336,16 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         e.smooth = label_smoothing / (float)V;
         e.one_minus_eps = 1.f - label_smoothing;
         e.out = ws.tile;
-        e.ld_out = n;
-        HIP_TRY(pngpd::head_product(type, T, n, D, x, HeadOperand{w, ldw, true}, e, s));
-        if (dbias_dev) HIP_TRY(pngpd::head_col_sum(type, T, n, ws.tile, n, ws.part, ws.scale, at(dbias_dev, v, type), s));
+        e.ld_out = np;
+        HIP_TRY(pngpd::head_product(type, T, n, D, x, HeadOperand{w, whole.ld, true}, e, ws.partial, s));
+        if (dbias_dev) HIP_TRY(pngpd::head_col_sum(type, T, n, ws.tile, np, ws.part, ws.scale, at(dbias_dev, v, type), s));
         HeadEpilogue g;
         g.kind = pngpd::HEAD_EPI_SCALED;
         g.ld_out = D;
         if (dweight_dev) {
             g.out = at(dweight_dev, v * D, type);
             g.scale = ws.scale;
-            HIP_TRY(pngpd::head_product(type, n, D, T, HeadOperand{ws.tile, n, false}, HeadOperand{ws.x, D, false}, g, s));
+            HIP_TRY(pngpd::head_product(type, n, D, T, HeadOperand{ws.tile, np, false}, xt, g, ws.partial, s));
         }
         if (dx_dev) {
             const bool last = v + n == V;
@@ -289,7 +353,7 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
             g.out_f32 = !last;
             g.scale = last ? ws.scale : nullptr;
             g.out = last ? dx_dev : (void*)ws.dx_sum;
-            HIP_TRY(pngpd::head_product(type, T, D, n, HeadOperand{ws.tile, n, true}, HeadOperand{w, ldw, false}, g, s));
+            HIP_TRY(pngpd::head_product(type, T, D, n, HeadOperand{ws.tile, np, true}, HeadOperand{w, whole.ld, false}, g, ws.partial, s));
         }
     }
     return PNGPD_OK;

@@ -1,68 +1,53 @@
-// Row statistics, loss and gradient weights of linear_cross_entropy (the products are head_product.hip's).
+// Loss and gradient weights of linear_cross_entropy from the rows' statistics (the products are head_product.hip's).
 //
-// A row's statistics run over the pieces of the vocabulary: maximum m, sum s of exp(z - m), the target's logit and, for
-// label smoothing, the sum of the logits.  A piece joins them with  s <- s exp(m - m') + s_piece exp(m_piece - m').
+// A block of columns leaves a row's maximum m, sum s of exp(z - m) and sum of z; blocks join by
+// s = s1 exp(m1 - m) + s2 exp(m2 - m) under m = max(m1, m2).
 #include "head.h"
 #include "head_math.h"
 
 namespace pngpd {
 namespace {
 
-// exp(v - m) for a running maximum that may be -inf (nothing finite seen yet): -inf - -inf counts as "no term"
-__device__ __forceinline__ float exp_under(float v, float m) { return v == -__builtin_inff() ? 0.f : expf(v - m); }
-
-// one wave a row
-__global__ __launch_bounds__(256) void stats_piece_kernel(int64_t T, int64_t n, const float* logits, int64_t ld, int64_t first_n,
-                                                          const int64_t* target, HeadRowStats st, bool first) {
-    const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (t >= T) return;
-    const int lane = threadIdx.x & 63;
-    const float* z = logits + t * ld;
-    float m = -__builtin_inff(), zs = 0.f;
-    for (int64_t i = lane; i < n; i += 64) {
-        m = __builtin_fmaxf(m, z[i]);
-        zs += z[i];
-    }
-    m = wave_max(m);
-    zs = wave_sum(zs);
-    float s = 0.f;
-    for (int64_t i = lane; i < n; i += 64) s += exp_under(z[i], m);
-    s = wave_sum(s);
-    if (lane == 0) {
-        const int64_t y = target[t] - first_n;
-        if (y >= 0 && y < n) st.target_logit[t] = z[y];
-        else if (first) st.target_logit[t] = __builtin_nanf("");      // stays so if no piece holds the label
-        if (first) {
-            st.max[t] = m;
-            st.sum[t] = s;
-            st.logit_sum[t] = zs;
-        } else {
-            const float m0 = st.max[t], m1 = __builtin_fmaxf(m0, m);
-            st.sum[t] = st.sum[t] * (m0 == m1 ? 1.f : exp_under(m0, m1)) + s * (m == m1 ? 1.f : exp_under(m, m1));
-            st.max[t] = m1;
-            st.logit_sum[t] += zs;
-        }
-    }
+__device__ __forceinline__ void join_stats(float4& v, const float4& u) {
+    const float m = __builtin_fmaxf(v.x, u.x);
+    v.y = v.y * (v.x == m ? 1.f : __expf(v.x - m)) + u.y * (u.x == m ? 1.f : __expf(u.x - m));
+    v.x = m;
+    v.z += u.z;
 }
 
-// loss of every row, and of the batch: one workgroup, sums over the rows in 64 bits
-__global__ __launch_bounds__(1024) void loss_finish_kernel(int64_t T, int64_t V, const int64_t* target, int64_t ignore, float eps,
-                                                           int reduction, HeadRowStats st, float* loss, float* lse) {
+// 32 rows a workgroup, 8 threads a row, each over its share of the blocks; then the threads of a row in order
+__global__ __launch_bounds__(256) void row_loss_kernel(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit,
+                                                       const int64_t* target, int64_t ignore, float eps, float* loss, float* lse) {
+    __shared__ float4 share[8][32];
+    const int r = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const int64_t t = (int64_t)blockIdx.x * 32 + r;
+    float4 v = make_float4(-__builtin_inff(), 0.f, 0.f, 0.f);
+    if (t < T)
+        for (int i = part; i < blocks; i += 8) join_stats(v, stats[(int64_t)i * T + t]);
+    share[part][r] = v;
+    __syncthreads();
+    if (part || t >= T) return;
+    for (int i = 1; i < 8; ++i) join_stats(v, share[i][r]);
+    const float l = v.x + logf(v.y);
+    lse[t] = l;
+    const int64_t y = target[t];
+    float x = 0.f;
+    if (y != ignore) {
+        x = y >= 0 && y < V ? l - (1.f - eps) * target_logit[t] : __builtin_nanf("");
+        if (eps > 0.f) x -= eps / (float)V * v.z;
+    }
+    loss[t] = x;
+}
+
+// the batch's loss: one workgroup, sums over the rows in 64 bits
+__global__ __launch_bounds__(1024) void batch_loss_kernel(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore,
+                                                          int reduction, float* loss) {
     __shared__ double part[16], count[16];
     double sum = 0, used = 0;
     for (int64_t t = threadIdx.x; t < T; t += 1024) {
-        const float l = st.max[t] + logf(st.sum[t]);
-        lse[t] = l;
-        float v = 0.f;
-        if (target[t] != ignore) {
-            v = l - (1.f - eps) * st.target_logit[t];
-            if (eps > 0.f) v -= eps / (float)V * st.logit_sum[t];
-            used += 1;
-        }
-        if (reduction == PNGPD_REDUCE_NONE) loss[t] = v;
-        sum += v;
+        sum += row_loss[t];
+        used += target[t] != ignore;
     }
-    if (reduction == PNGPD_REDUCE_NONE) return;
     for (int o = 32; o; o >>= 1) {
         sum += __shfl_xor(sum, o);
         used += __shfl_xor(used, o);
@@ -119,16 +104,6 @@ __global__ __launch_bounds__(1024) void row_weights_kernel(bool scaled, int64_t 
     if (threadIdx.x == 0) out_scale[0] = scale;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void live_rows_kernel(int64_t rows, int64_t D, const T* x, int64_t ldx, const float* weight,
-                                                        T* out) {
-    const int64_t total = rows * D;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t t = i / D, d = i - t * D;
-        out[i] = weight[t] != 0.f ? x[t * ldx + d] : (T)0.f;
-    }
-}
-
 // bytes: an even number (every element type has at least two)
 __global__ __launch_bounds__(256) void zero_kernel(unsigned short* p, size_t n) {
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0;
@@ -142,24 +117,14 @@ hipError_t head_zero(void* p, size_t bytes, hipStream_t s) {
     return hipGetLastError();
 }
 
-hipError_t head_live_rows(int type, int64_t T, int64_t D, const void* x, int64_t ldx, const float* weight, void* out,
-                          hipStream_t s) {
-    const int64_t blocks = (T * D + 255) / 256;
-    const unsigned grid = (unsigned)(blocks < 16384 ? blocks : 16384);
-    if (type == PNGPD_TYPE_F32) live_rows_kernel<float><<<grid, 256, 0, s>>>(T, D, (const float*)x, ldx, weight, (float*)out);
-    else live_rows_kernel<bf16_t><<<grid, 256, 0, s>>>(T, D, (const bf16_t*)x, ldx, weight, (bf16_t*)out);      // 16-bit copies
-    return hipGetLastError();
-}
-
-hipError_t head_stats_piece(int64_t T, int64_t n, const float* logits, int64_t ld, int64_t first_n, const int64_t* target,
-                            const HeadRowStats& st, bool first, hipStream_t s) {
-    stats_piece_kernel<<<(unsigned)((T + 3) / 4), 256, 0, s>>>(T, n, logits, ld, first_n, target, st, first);
-    return hipGetLastError();
-}
-
-hipError_t head_loss_finish(int64_t T, int64_t V, const int64_t* target, int64_t ignore, float eps, int reduction,
-                            const HeadRowStats& st, float* loss, float* lse, hipStream_t s) {
-    loss_finish_kernel<<<1, 1024, 0, s>>>(T, V, target, ignore, eps, reduction, st, loss, lse);
+hipError_t head_loss_finish(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit, const int64_t* target,
+                            int64_t ignore, float eps, int reduction, float* row_loss, float* loss, float* lse, hipStream_t s) {
+    if (T > 0) {
+        row_loss_kernel<<<(unsigned)((T + 31) / 32), 256, 0, s>>>(T, V, blocks, stats, target_logit, target, ignore, eps, row_loss, lse);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || reduction == PNGPD_REDUCE_NONE) return e;
+    }
+    batch_loss_kernel<<<1, 1024, 0, s>>>(T, row_loss, target, ignore, reduction, loss);
     return hipGetLastError();
 }
 

@@ -1,117 +1,182 @@
-// Products of the classification head: out[m][n] = epilogue(sum_k A(m,k) B(n,k)).
-//
-// One tile of 64 x 64 outputs per workgroup of 256 threads, 4 x 4 outputs a thread, the contraction in steps of 16
-// through LDS, sums as 32-bit fma chains.  Any stride, any alignment, both operand orders.
+// Products of the classification head: the choice of a tile shape, the joining of split contractions, and the passes that
+// lay operands out.
 #include "head.h"
 #include "head_math.h"
+#include "head_tile.h"
 
 namespace pngpd {
 namespace {
 
-constexpr int TM = 64, TN = 64, TK = 16;
+// ---- joining partial sums --------------------------------------------------------------------------------------------------------
 
-template <typename T, int ACT>
-__device__ __forceinline__ void store_out(const HeadEpilogue& e, int64_t N, int64_t m, int64_t n, float acc) {
-    float v;
-    if (e.kind == HEAD_EPI_LINEAR) {
-        const float z = acc + (e.bias ? to_f32(((const T*)e.bias)[n]) : 0.f);
-        if (e.z) ((T*)e.z)[m * N + n] = keep_z<T, ACT>(z);
-        v = act_f<ACT>(z);
-        if (e.residual) v += to_f32(((const T*)e.residual)[m * e.ld_residual + n]);
-    } else if (e.kind == HEAD_EPI_DZ) {
-        const float w = e.row_weight[m];
-        const float z = acc + (e.bias ? to_f32(((const T*)e.bias)[n]) : 0.f);
-        const float p = expf(z - e.lse[m]) - e.smooth;
-        v = w == 0.f ? 0.f : (p - (e.target[m] == n + e.first_n ? e.one_minus_eps : 0.f)) * w;
-    } else {
-        v = (acc + (e.add ? e.add[m * N + n] : 0.f)) * (e.scale ? e.scale[0] : 1.f);
-    }
-    if (e.out_f32) ((float*)e.out)[m * e.ld_out + n] = e.kind == HEAD_EPI_SCALED ? v : acc + (e.bias ? to_f32(((const T*)e.bias)[n]) : 0.f);
-    else ((T*)e.out)[m * e.ld_out + n] = from_f32<T>(v);
-}
-
-template <typename T, int ACT>
-__global__ __launch_bounds__(256) void product_simple_kernel(int64_t M, int64_t N, int64_t K, HeadOperand a, HeadOperand b,
-                                                             HeadEpilogue e) {
-    __shared__ float sa[TK][TM + 1], sb[TK][TN + 1];
-    const int64_t m0 = (int64_t)blockIdx.y * TM, n0 = (int64_t)blockIdx.x * TN;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < K; k0 += TK) {
-        for (int i = threadIdx.x; i < TM * TK; i += 256) {
-            int r = a.k_contiguous ? i / TK : i % TM, k = a.k_contiguous ? i % TK : i / TM;
-            const int64_t gm = m0 + r, gk = k0 + k;
-            sa[k][r] = gm < M && gk < K ? to_f32(((const T*)a.p)[a.k_contiguous ? gm * a.ld + gk : gk * a.ld + gm]) : 0.f;
-            r = b.k_contiguous ? i / TK : i % TN, k = b.k_contiguous ? i % TK : i / TN;
-            const int64_t gn = n0 + r, hk = k0 + k;
-            sb[k][r] = gn < N && hk < K ? to_f32(((const T*)b.p)[b.k_contiguous ? gn * b.ld + hk : hk * b.ld + gn]) : 0.f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < TK; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_fmaf(sa[k][ty + 16 * i], sb[k][tx + 16 * j], acc[i][j]);
-        __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-            if (m < M && n < N) store_out<T, ACT>(e, N, m, n, acc[i][j]);
-        }
-}
-
-template <typename T>
-hipError_t launch(int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b, const HeadEpilogue& e,
-                  hipStream_t s) {
-    // at most 65535 tiles of rows in one launch
-    const int64_t rows = (int64_t)65535 * TM;
-    for (int64_t m = 0; m < M; m += rows) {
-        const int64_t part = M - m < rows ? M - m : rows;
-        HeadOperand ap = a;
-        ap.p = (const T*)a.p + (a.k_contiguous ? m * a.ld : m);
-        HeadEpilogue ep = e;
-        ep.out = e.out_f32 ? (void*)((float*)e.out + m * e.ld_out) : (void*)((T*)e.out + m * e.ld_out);
-        if (e.residual) ep.residual = (const T*)e.residual + m * e.ld_residual;
-        if (e.z) ep.z = (T*)e.z + m * N;
-        if (e.lse) ep.lse = e.lse + m;
-        if (e.row_weight) ep.row_weight = e.row_weight + m;
-        if (e.target) ep.target = e.target + m;
-        if (e.add) ep.add = e.add + m * N;
-        const dim3 grid((unsigned)((N + TN - 1) / TN), (unsigned)((part + TM - 1) / TM));
-        switch (e.kind == HEAD_EPI_LINEAR ? e.act : PNGPD_ACT_NONE) {
-            case PNGPD_ACT_RELU: product_simple_kernel<T, PNGPD_ACT_RELU><<<grid, 256, 0, s>>>(part, N, K, ap, b, ep); break;
-            case PNGPD_ACT_GELU: product_simple_kernel<T, PNGPD_ACT_GELU><<<grid, 256, 0, s>>>(part, N, K, ap, b, ep); break;
-            case PNGPD_ACT_GELU_TANH:
-                product_simple_kernel<T, PNGPD_ACT_GELU_TANH><<<grid, 256, 0, s>>>(part, N, K, ap, b, ep);
-                break;
-            case PNGPD_ACT_SILU: product_simple_kernel<T, PNGPD_ACT_SILU><<<grid, 256, 0, s>>>(part, N, K, ap, b, ep); break;
-            default: product_simple_kernel<T, PNGPD_ACT_NONE><<<grid, 256, 0, s>>>(part, N, K, ap, b, ep);
-        }
-        hipError_t err = hipGetLastError();
-        if (err != hipSuccess) return err;
-    }
-    return hipSuccess;
-}
-
-template <typename T, int ACT>
-__global__ __launch_bounds__(256) void act_backward_kernel(int64_t M, int64_t N, const T* dy, int64_t ld, const T* z, T* dz) {
-    const int64_t total = M * N;
+// 4 neighbouring columns of a row a thread: the cuts of the contraction added in order, then the epilogue
+template <typename E, int KIND>
+__global__ __launch_bounds__(256) void join_kernel(int64_t M, int64_t N, int64_t quads, int splits, const float* partial, HeadEpilogue e,
+                                                   bool vec) {
+    const int64_t total = M * quads;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t m = i / N, n = i - m * N;
-        dz[i] = from_f32<T>(to_f32(dy[m * ld + n]) * act_slope<ACT>(to_f32(z[i])));
+        const int64_t m = i / quads, n = (i - m * quads) * 4;
+        const int64_t have = N - n;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (have > 0) {
+            const int valid = (int)(have < 4 ? have : 4);
+            for (int s = 0; s < splits; ++s) v += load4(partial + ((int64_t)s * M + m) * N + n, valid, vec);
+        }
+        const int64_t room = (KIND == TILE_DZ ? e.ld_out : N) - n;
+        finish4<E, KIND>(e, N, m, n, (int)(room < 4 ? room : 4), vec, v);
     }
 }
 
+// a row a workgroup: statistics of its logits, formed from the cuts of the contraction
+template <typename E>
+__global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, int splits, const float* partial, HeadEpilogue e) {
+    __shared__ float4 share[4];
+    const int64_t m = blockIdx.x;
+    const int64_t y = e.target[m];
+    const E* bias = (const E*)e.bias;
+    float mx = -__builtin_inff(), sum = 0.f, zs = 0.f;
+    for (int64_t n = threadIdx.x; n < N; n += 256) {
+        float z = 0.f;
+        for (int s = 0; s < splits; ++s) z += partial[((int64_t)s * M + m) * N + n];
+        if (bias) z += to_f32(bias[n]);
+        if (n == y) e.target_logit[m] = z;
+        zs += z;
+        const float top = __builtin_fmaxf(mx, z);
+        sum = sum * (mx == top ? 1.f : __expf(mx - top)) + (z == -__builtin_inff() ? 0.f : __expf(z - top));
+        mx = top;
+    }
+    const float top = wave_max(mx);
+    sum = wave_sum(sum * (mx == top ? 1.f : __expf(mx - top)));
+    zs = wave_sum(zs);
+    if ((threadIdx.x & 63) == 0) share[threadIdx.x >> 6] = make_float4(top, sum, zs, 0.f);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float4 v = share[0];
+        for (int w = 1; w < 4; ++w) {
+            const float4 u = share[w];
+            const float t = __builtin_fmaxf(v.x, u.x);
+            v.y = v.y * (v.x == t ? 1.f : __expf(v.x - t)) + u.y * (u.x == t ? 1.f : __expf(u.x - t));
+            v.x = t;
+            v.z += u.z;
+        }
+        e.stats[m] = v;
+    }
+}
+
+template <typename E>
+hipError_t join(int64_t M, int64_t N, int splits, const float* partial, const HeadEpilogue& e, hipStream_t s) {
+    const bool vec = epilogue_vec(e, N, sizeof(E)) && N % 4 == 0;
+    const int64_t quads = ((e.kind == HEAD_EPI_DZ ? e.ld_out : N) + 3) / 4;
+    const int64_t blocks = (M * quads + 255) / 256;
+    const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
+    switch (e.kind) {
+        case HEAD_EPI_LINEAR: join_kernel<E, TILE_LINEAR><<<grid, 256, 0, s>>>(M, N, quads, splits, partial, e, vec); break;
+        case HEAD_EPI_DZ: join_kernel<E, TILE_DZ><<<grid, 256, 0, s>>>(M, N, quads, splits, partial, e, vec); break;
+        case HEAD_EPI_SCALED: join_kernel<E, TILE_SCALED><<<grid, 256, 0, s>>>(M, N, quads, splits, partial, e, vec); break;
+        default: join_stats_kernel<E><<<(unsigned)M, 256, 0, s>>>(M, N, splits, partial, e);
+    }
+    return hipGetLastError();
+}
+
+template <typename E>
+hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b, const HeadEpilogue& e,
+                   float* partial, hipStream_t s) {
+    const HeadPlan p = head_plan(type, M, N, K, e.kind);
+    TileArgs g{};
+    g.M = M;
+    g.N = N;
+    g.K = K;
+    g.a = (const char*)a.p;
+    g.b = (const char*)b.p;
+    g.lda = a.ld * (int64_t)sizeof(E);
+    g.ldb = b.ld * (int64_t)sizeof(E);
+    g.tiles_m = p.tiles_m;
+    g.tiles_n = p.tiles_n;
+    g.splits = p.splits;
+    g.k_split = p.k_split;
+    g.partial = partial;
+    g.e = e;
+    const int kind = p.splits > 1 ? TILE_PARTIAL
+                     : e.kind == HEAD_EPI_LINEAR ? TILE_LINEAR
+                     : e.kind == HEAD_EPI_DZ     ? TILE_DZ
+                     : e.kind == HEAD_EPI_STATS  ? TILE_STATS
+                                                 : TILE_SCALED;
+    const bool vec = p.splits > 1 ? N % 4 == 0 : epilogue_vec(e, N, sizeof(E));
+    hipError_t err;
+    if constexpr (__is_same(E, float)) err = launch_tile_f32(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
+    else if constexpr (__is_same(E, bf16_t)) err = launch_tile_bf16(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
+    else err = launch_tile_f16(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
+    if (err != hipSuccess || p.splits == 1) return err;
+    return join<E>(M, N, p.splits, partial, e, s);
+}
+
+// ---- passes over whole matrices -----------------------------------------------------------------------------------------------------
+
+// A thread's chunk (16 bytes of the destination): row and first column, rows of `per_row` chunks
+__device__ __forceinline__ bool chunk_of(int64_t rows, int64_t per_row, int64_t* r, int64_t* c) {
+    const int64_t first = (int64_t)blockIdx.x * 256;
+    const int64_t r0 = first / per_row;                      // uniform
+    const unsigned off = (unsigned)(first - r0 * per_row) + threadIdx.x;      // per_row <= HEAD_MAX_LD / 16
+    const unsigned d = off / (unsigned)per_row;
+    *r = r0 + d;
+    *c = off - d * (unsigned)per_row;
+    return *r < rows;
+}
+
 template <typename T>
-hipError_t act_backward(int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz, hipStream_t s) {
-    const int64_t blocks = (M * N + 255) / 256;
-    const unsigned grid = (unsigned)(blocks < 16384 ? blocks : 16384);
+struct Chunk {
+    static constexpr int C = 16 / sizeof(T);
+    typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T V;
+    // up to C values from p, `valid` of them there, zeros behind
+    __device__ static __forceinline__ V load(const T* p, int64_t valid, bool aligned) {
+        V v;
+        if (aligned && valid >= C) return *(const V*)p;
+#pragma unroll
+        for (int i = 0; i < C; ++i) v[i] = i < valid ? p[i] : (T)0.f;
+        return v;
+    }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void lay_out_kernel(int64_t rows, int64_t cols, const T* src, int64_t ld_src, const float* weight,
+                                                      T* dst, int64_t ld, bool aligned) {
+    constexpr int C = Chunk<T>::C;
+    int64_t r, c;
+    if (!chunk_of(rows, ld / C, &r, &c)) return;
+    typename Chunk<T>::V v = {};
+    if (!weight || weight[r] != 0.f) v = Chunk<T>::load(src + r * ld_src + c * C, cols - c * C, aligned);
+    *(typename Chunk<T>::V*)(dst + r * ld + c * C) = v;
+}
+
+template <typename T>
+hipError_t lay_out(int64_t rows, int64_t cols, const void* src, int64_t ld_src, const float* weight, void* dst, int64_t ld, hipStream_t s) {
+    const bool aligned = ((uintptr_t)src & 15) == 0 && ld_src % Chunk<T>::C == 0;
+    const int64_t chunks = rows * (ld / Chunk<T>::C);
+    lay_out_kernel<T><<<(unsigned)((chunks + 255) / 256), 256, 0, s>>>(rows, cols, (const T*)src, ld_src, weight, (T*)dst, ld, aligned);
+    return hipGetLastError();
+}
+
+template <typename T, int ACT>
+__global__ __launch_bounds__(256) void act_backward_kernel(int64_t M, int64_t N, const T* dy, int64_t ld, bool dy_aligned, const T* z,
+                                                           bool z_aligned, T* dz, int64_t ld_dz) {
+    constexpr int C = Chunk<T>::C;
+    int64_t r, c;
+    if (!chunk_of(M, ld_dz / C, &r, &c)) return;
+    const typename Chunk<T>::V g = Chunk<T>::load(dy + r * ld + c * C, N - c * C, dy_aligned);
+    const typename Chunk<T>::V v = Chunk<T>::load(z + r * N + c * C, N - c * C, z_aligned);
+    typename Chunk<T>::V o;
+#pragma unroll
+    for (int i = 0; i < C; ++i) o[i] = (T)((float)g[i] * act_slope<ACT>((float)v[i]));
+    *(typename Chunk<T>::V*)(dz + r * ld_dz + c * C) = o;
+}
+
+template <typename T>
+hipError_t act_backward(int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz, int64_t ld_dz, hipStream_t s) {
+    constexpr int C = Chunk<T>::C;
+    const unsigned grid = (unsigned)((M * (ld_dz / C) + 255) / 256);
+    const bool da = ((uintptr_t)dy & 15) == 0 && ld % C == 0, za = ((uintptr_t)z & 15) == 0 && N % C == 0;
 #define PNGPD_ACT_CASE(A) \
-    case A: act_backward_kernel<T, A><<<grid, 256, 0, s>>>(M, N, (const T*)dy, ld, (const T*)z, (T*)dz); break;
+    case A: act_backward_kernel<T, A><<<grid, 256, 0, s>>>(M, N, (const T*)dy, ld, da, (const T*)z, za, (T*)dz, ld_dz); break;
     switch (act) {
         PNGPD_ACT_CASE(PNGPD_ACT_RELU)
         PNGPD_ACT_CASE(PNGPD_ACT_GELU)
@@ -123,14 +188,23 @@ hipError_t act_backward(int64_t M, int64_t N, const void* dy, int64_t ld, const 
     return hipGetLastError();
 }
 
+// 64 columns of 4 values (256 columns) by 4 rows at a time a workgroup
 template <typename T>
-__global__ __launch_bounds__(256) void col_sum_part_kernel(int64_t M, int64_t N, const T* a, int64_t ld, int64_t rows, float* part) {
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
+__global__ __launch_bounds__(256) void col_sum_part_kernel(int64_t M, int64_t N, const T* a, int64_t ld, bool vec, int64_t rows, float* part) {
+    __shared__ f32x4 share[3][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t n = (int64_t)blockIdx.x * 256 + lane * 4;
     const int64_t m0 = (int64_t)blockIdx.y * rows, m1 = m0 + rows < M ? m0 + rows : M;
-    float s = 0.f;
-    for (int64_t m = m0; m < m1; ++m) s += to_f32(a[m * ld + n]);
-    part[(int64_t)blockIdx.y * N + n] = s;
+    const int valid = (int)(N - n < 0 ? 0 : N - n < 4 ? N - n : 4);
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (valid > 0)
+        for (int64_t m = m0 + w; m < m1; m += 4) s += load4(a + m * ld + n, valid, vec);
+    if (w) share[w - 1][lane] = s;
+    __syncthreads();
+    if (w == 0) {
+        for (int i = 0; i < 3; ++i) s += share[i][lane];
+        for (int i = 0; i < valid; ++i) part[(int64_t)blockIdx.y * N + n + i] = s[i];
+    }
 }
 
 template <typename T>
@@ -146,7 +220,8 @@ template <typename T>
 hipError_t col_sum(int64_t M, int64_t N, const void* a, int64_t ld, float* part, const float* scale, void* out, hipStream_t s) {
     const int64_t parts = head_col_sum_parts(M), rows = (M + parts - 1) / parts;
     const unsigned gx = (unsigned)((N + 255) / 256);
-    col_sum_part_kernel<T><<<dim3(gx, (unsigned)parts), 256, 0, s>>>(M, N, (const T*)a, ld, rows, part);
+    const bool vec = ((uintptr_t)a & (4 * sizeof(T) - 1)) == 0 && ld % 4 == 0;
+    col_sum_part_kernel<T><<<dim3(gx, (unsigned)parts), 256, 0, s>>>(M, N, (const T*)a, ld, vec, rows, part);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     col_sum_join_kernel<T><<<gx, 256, 0, s>>>((int)parts, N, part, scale, (T*)out);
@@ -156,25 +231,57 @@ hipError_t col_sum(int64_t M, int64_t N, const void* a, int64_t ld, float* part,
 }  // namespace
 
 int64_t head_col_sum_parts(int64_t M) {
-    const int64_t p = (M + 63) / 64;
+    const int64_t p = (M + 31) / 32;
     return p < 1 ? 1 : p > 64 ? 64 : p;
 }
 
-#define PNGPD_BY_TYPE(call)                                  \
-    switch (type) {                                          \
+HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
+    const int64_t step = type == PNGPD_TYPE_F32 ? 32 : 64, steps = (K + step - 1) / step;
+    auto tiles = [&](int shape) {
+        int bm, bn;
+        shape_size(shape, &bm, &bn);
+        return ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+    };
+    HeadPlan p;
+    p.shape = M <= 32 ? SHAPE_FEW_ROWS : N <= 32 ? SHAPE_FEW_COLS : tiles(SHAPE_256) >= 192 ? SHAPE_256 : SHAPE_128;
+    int bm, bn;
+    shape_size(p.shape, &bm, &bn);
+    p.tiles_m = (int)((M + bm - 1) / bm);
+    p.tiles_n = (int)((N + bn - 1) / bn);
+    const int64_t t = tiles(p.shape);
+    int64_t splits = 1;
+    if (t < 256) {
+        splits = 512 / t;
+        if (splits > steps / 4) splits = steps / 4;
+        if (splits < 1) splits = 1;
+    }
+    const int64_t per = (steps + splits - 1) / splits;
+    p.k_split = per * step;
+    p.splits = (int)((steps + per - 1) / per);
+    p.stats_blocks = p.splits > 1 ? 1 : p.tiles_n;
+    p.partial_bytes = p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
+    return p;
+}
+
+#define PNGPD_BY_TYPE(call)                                      \
+    switch (type) {                                              \
         case PNGPD_TYPE_F32: { typedef float T; return call; }   \
         case PNGPD_TYPE_BF16: { typedef bf16_t T; return call; } \
         case PNGPD_TYPE_F16: { typedef f16_t T; return call; }   \
-        default: return hipErrorInvalidValue;                \
+        default: return hipErrorInvalidValue;                    \
     }
 
 hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b,
-                        const HeadEpilogue& e, hipStream_t s) {
-    PNGPD_BY_TYPE((launch<T>(M, N, K, a, b, e, s)))
+                        const HeadEpilogue& e, float* partial, hipStream_t s) {
+    PNGPD_BY_TYPE((product<T>(type, M, N, K, a, b, e, partial, s)))
+}
+hipError_t head_lay_out(int type, int64_t rows, int64_t cols, const void* src, int64_t ld_src, const float* weight, void* dst,
+                        int64_t ld, hipStream_t s) {
+    PNGPD_BY_TYPE((lay_out<T>(rows, cols, src, ld_src, weight, dst, ld, s)))
 }
 hipError_t head_act_backward(int type, int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz,
-                             hipStream_t s) {
-    PNGPD_BY_TYPE((act_backward<T>(M, N, dy, ld, z, act, dz, s)))
+                             int64_t ld_dz, hipStream_t s) {
+    PNGPD_BY_TYPE((act_backward<T>(M, N, dy, ld, z, act, dz, ld_dz, s)))
 }
 hipError_t head_col_sum(int type, int64_t M, int64_t N, const void* a, int64_t ld, float* part, const float* scale, void* out,
                         hipStream_t s) {

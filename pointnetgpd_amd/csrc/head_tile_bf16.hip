@@ -1,0 +1,8 @@
+// The tile kernels of head_tile.h for bf16 operands.
+#include "head_tile.h"
+
+namespace pngpd {
+hipError_t launch_tile_bf16(int shape, int kind, bool ak, bool bk, const TileArgs& g, bool vec, hipStream_t s) {
+    return launch_tile<bf16_t>(shape, kind, ak, bk, g, vec, s);
+}
+}  // namespace pngpd

@@ -1,0 +1,8 @@
+// The tile kernels of head_tile.h for f16 operands.
+#include "head_tile.h"
+
+namespace pngpd {
+hipError_t launch_tile_f16(int shape, int kind, bool ak, bool bk, const TileArgs& g, bool vec, hipStream_t s) {
+    return launch_tile<f16_t>(shape, kind, ak, bk, g, vec, s);
+}
+}  // namespace pngpd

@@ -15,7 +15,7 @@ struct AttrSlot {
     std::atomic<const void*> kern{nullptr};
     std::atomic<unsigned long long> devices{0};     // bit d: the attribute is set on device d
 };
-constexpr int MAX_KERNELS = 64;
+constexpr int MAX_KERNELS = 128;
 AttrSlot g_attr[MAX_KERNELS];
 }  // namespace
 

@@ -59,6 +59,11 @@ def _rows(t, cols):
     return t2.contiguous(), cols
 
 
+def _aligned(size, *matrices):
+    """Whether all (tensor, distance of rows) start at 16-byte addresses with rows of whole 16-byte chunks apart."""
+    return int(all(t.data_ptr() % 16 == 0 and ld * size % 16 == 0 and ld * size <= 1 << 23 for t, ld in matrices))
+
+
 def _vector(t):
     return t if t is None or t.is_contiguous() else t.contiguous()
 
@@ -96,7 +101,7 @@ def _linear_forward(x, weight, bias, residual, act, keep):
     z = torch.empty((M, N), dtype=x.dtype, device=dev) if keep and act else None
     r2, ldr = _rows(residual, N) if residual is not None else (None, N)
     b = _vector(bias)
-    nbytes = lib.pngpd_linear_workspace_bytes(kind, M, N, K, 0)
+    nbytes = lib.pngpd_linear_workspace_bytes(kind, M, N, K, 0, _aligned(x.element_size(), (x2, ldx), (w2, ldw)))
     with torch.cuda.device(dev):
         ws = _workspace(nbytes, dev)
         _lib.check(lib.pngpd_linear_forward(kind, M, N, K, _ptr(x2), ldx, _ptr(w2), ldw, _ptr(b), act, _ptr(r2), ldr, _ptr(y),
@@ -132,7 +137,8 @@ class LinearFunction(torch.autograd.Function):
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
         dw = torch.empty((N, K), dtype=x.dtype, device=dev) if need_w else None
         db = torch.empty(N, dtype=x.dtype, device=dev) if need_b else None
-        nbytes = lib.pngpd_linear_workspace_bytes(kind, M, N, K, 1)
+        nbytes = lib.pngpd_linear_workspace_bytes(kind, M, N, K, 1,
+                                                  _aligned(x.element_size(), (x2, ldx), (w2, ldw), (d2, ld_dy)))
         with torch.cuda.device(dev):
             ws = _workspace(nbytes, dev)
             _lib.check(lib.pngpd_linear_backward(kind, M, N, K, _ptr(d2), ld_dy, _ptr(z), _ptr(x2), ldx, _ptr(w2), ldw, ctx.act,
@@ -259,7 +265,8 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
         dw = torch.empty((V, D), dtype=x.dtype, device=dev) if need_w else None
         db = torch.empty(V, dtype=x.dtype, device=dev) if need_b else None
-        nbytes = lib.pngpd_linear_cross_entropy_workspace_bytes(kind, T, V, D, 1)
+        nbytes = lib.pngpd_linear_cross_entropy_workspace_bytes(
+            kind, T, V, D, 1, _aligned(x.element_size(), (x2, ldx), (w2, ldw)))
         b = _vector(bias)
         with torch.cuda.device(dev):
             ws = _workspace(nbytes, dev)
@@ -278,7 +285,8 @@ def _loss_forward(x, weight, bias, target, ignore_index, label_smoothing, reduct
     T = x2.shape[0]
     loss = torch.empty(x.shape[:-1] if reduction == 0 else (), dtype=torch.float32, device=dev)
     lse = torch.empty(T, dtype=torch.float32, device=dev)
-    nbytes = lib.pngpd_linear_cross_entropy_workspace_bytes(kind, T, V, D, 0)
+    nbytes = lib.pngpd_linear_cross_entropy_workspace_bytes(
+        kind, T, V, D, 0, _aligned(x.element_size(), (x2, ldx), (w2, ldw)))
     b = _vector(bias)
     with torch.cuda.device(dev):
         ws = _workspace(nbytes, dev)

@@ -41,7 +41,8 @@ def _linear(lib, type=0, M=2, N=3, K=4, x=16, ldx=4, w=16, ldw=4, act=0, r=0, ld
     (dict(type=3), ERR_INVALID), (dict(type=-1), ERR_INVALID), (dict(M=-1), ERR_SHAPE), (dict(N=0), ERR_SHAPE),
     (dict(K=0), ERR_SHAPE), (dict(M=2 ** 31), ERR_SHAPE), (dict(x=None), ERR_INVALID), (dict(w=None), ERR_INVALID),
     (dict(y=None), ERR_INVALID), (dict(act=5), ERR_INVALID), (dict(ldx=3), ERR_SHAPE), (dict(ldw=3), ERR_SHAPE),
-    (dict(r=16, ldr=2), ERR_SHAPE)])
+    (dict(r=16, ldr=2), ERR_SHAPE), (dict(K=2 ** 21 + 1, ldx=2 ** 22, ldw=2 ** 22), ERR_SHAPE), (dict(N=2 ** 21 + 1), ERR_SHAPE),
+    (dict(K=5, ldx=5, ldw=5), ERR_INVALID)])      # rows that have to be copied, and no workspace
 def test_linear_forward_refuses(change, code):
     lib = _lib.load()
     assert _linear(lib, **change) == code
@@ -77,7 +78,7 @@ def test_dropout_refuses(change, code):
     (dict(type=-2), ERR_INVALID), (dict(T=-1), ERR_SHAPE), (dict(V=0), ERR_SHAPE), (dict(D=0), ERR_SHAPE),
     (dict(x=None), ERR_INVALID), (dict(w=None), ERR_INVALID), (dict(target=None), ERR_INVALID), (dict(eps=1.5), ERR_INVALID),
     (dict(eps=float("nan")), ERR_INVALID), (dict(reduction=3), ERR_INVALID), (dict(ldw=3), ERR_SHAPE),
-    (dict(lse=None), ERR_INVALID), (dict(out=None), ERR_INVALID), (dict(ws=None), ERR_INVALID), (dict(nbytes=64), ERR_WORKSPACE)])
+    (dict(lse=None), ERR_INVALID), (dict(out=None), ERR_INVALID), (dict(T=2 ** 24, V=2 ** 24), ERR_SHAPE), (dict(D=2 ** 21 + 1, ldw=2 ** 22), ERR_SHAPE), (dict(ws=None), ERR_INVALID), (dict(nbytes=64), ERR_WORKSPACE)])
 def test_linear_cross_entropy_refuses(change, code):
     lib = _lib.load()
     a = dict(type=0, T=2, V=5, D=4, x=16, w=16, ldw=4, target=16, eps=0.0, reduction=1, lse=16, out=16, ws=4096, nbytes=1 << 20)
@@ -92,9 +93,9 @@ def test_linear_cross_entropy_refuses(change, code):
 def test_workspace_sizes_are_bounded_and_grow_with_no_logits():
     lib = _lib.load()
     whole = 8192 * 131072 * 4
-    assert 0 < lib.pngpd_linear_cross_entropy_workspace_bytes(1, 8192, 131072, 1024, 0) < whole // 8
-    assert 0 < lib.pngpd_linear_cross_entropy_workspace_bytes(1, 8192, 131072, 1024, 1) < whole // 8
-    assert lib.pngpd_linear_workspace_bytes(5, 1, 1, 1, 0) == 0
+    assert 0 < lib.pngpd_linear_cross_entropy_workspace_bytes(1, 8192, 131072, 1024, 0, 1) < whole // 8
+    assert 0 < lib.pngpd_linear_cross_entropy_workspace_bytes(1, 8192, 131072, 1024, 1, 1) < whole // 8
+    assert lib.pngpd_linear_workspace_bytes(5, 1, 1, 1, 0, 1) == 0
 
 
 # ---- the restatement itself -----------------------------------------------------------------------------------------------
