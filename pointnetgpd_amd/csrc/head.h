@@ -48,6 +48,7 @@ struct HeadEpilogue {
     // columns; target_logit[m] = z[m][target[m]] where that is a column
     float4* stats = nullptr;
     float* target_logit = nullptr;
+    bool want_logit_sum = false;
     // the output (all but STATS): of the operands' type, or 32-bit floats when out_f32
     void* out = nullptr;
     int64_t ld_out = 0;

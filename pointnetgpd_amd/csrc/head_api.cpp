@@ -291,6 +291,7 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
         e.target = target_dev;
         e.stats = ws.stats;
         e.target_logit = ws.target_logit;
+        e.want_logit_sum = label_smoothing > 0.f;
         HIP_TRY(pngpd::head_product(type, T, V, D, HeadOperand{x.p, x.ld, true}, HeadOperand{w.p, w.ld, true}, e, ws.partial, s));
     } else if (reduction == PNGPD_REDUCE_NONE) {
         return PNGPD_OK;

@@ -88,18 +88,25 @@ __global__ __launch_bounds__(1024) void row_weights_kernel(bool scaled, int64_t 
         used += count[i];
         g = __builtin_fmaxf(g, top[i]);
     }
-    const float share = reduction == PNGPD_REDUCE_MEAN ? 1.f / used : 1.f;
+    // half precision: the largest weight becomes 2^13 .. 2^14, |dz| <= 2 times that is inside its range, and a probability of
+    // 2^-37 still is a number
+    if (reduction != PNGPD_REDUCE_NONE) {
+        // One weight for all rows stays out of dz and goes into the products' 32-bit sums: p - 1 of the labels would be rounded
+        // the same way in every row otherwise (off by up to 2^-9 in one direction in bfloat16).
+        const float unit = scaled ? 16384.f : 1.f;
+        for (int64_t t = threadIdx.x; t < T; t += 1024) weight[t] = target[t] != ignore && target[t] >= 0 && target[t] < V ? unit : 0.f;
+        if (threadIdx.x == 0) out_scale[0] = dloss[0] * (reduction == PNGPD_REDUCE_MEAN ? 1.f / __builtin_fmaxf(used, 1.f) : 1.f) / unit;
+        return;
+    }
     float scale = 1.f;
-    if (scaled && g * share > 0.f && g * share < __builtin_inff()) {
-        // the largest weight becomes 2^13 .. 2^14: |dz| <= 2 times that, inside half precision's range, and a
-        // probability of 2^-37 still is a number
+    if (scaled && g > 0.f && g < __builtin_inff()) {
         int e;
-        (void)frexpf(g * share, &e);
+        (void)frexpf(g, &e);
         scale = ldexpf(1.f, e - 14);
     }
     for (int64_t t = threadIdx.x; t < T; t += 1024) {
         const bool live = target[t] != ignore && target[t] >= 0 && target[t] < V;
-        weight[t] = live ? dloss[reduction == PNGPD_REDUCE_NONE ? t : 0] * share / scale : 0.f;
+        weight[t] = live ? dloss[t] / scale : 0.f;
     }
     if (threadIdx.x == 0) out_scale[0] = scale;
 }

@@ -19,14 +19,38 @@ __device__ __forceinline__ T from_f32(float v) { return (T)v; }      // rounds t
 // act(z) and act'(z).  gelu: z Phi(z); gelu_tanh: z sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3), which is
 // 0.5 z (1 + tanh u) without tanh's cancellation for large negative z; silu: z sigmoid(z).  z = -inf gives 0 and slope
 // 0 in all of them (the limits; the plain formulas give -inf * 0), NaN stays NaN.
-__device__ __forceinline__ float sigmoid_f(float v) { return 1.f / (1.f + __expf(-v)); }
+__device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
 constexpr float GELU_C = 0.7978845608028654f;      // sqrt(2 / pi)
+
+// Phi(z), and exp(-z^2 / 2) on the way.  Phi(-|z|) = exp(-z^2 / 2) Q(t), t = 1 / (1 + 0.297 |z|): Q is a least-squares fit of
+// erfcx's scaled form in t, reweighted towards equal relative error over |z| <= 14 (4e-8 in exact arithmetic, 2.7e-7 in
+// 32 bits); one exponential and one reciprocal, where the library's erfcf takes some 60 instructions.
+__device__ __forceinline__ float normal_cdf(float z, float* bell) {
+    const float e = __expf(-0.5f * z * z);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.2969848480983499f, __builtin_fabsf(z), 1.f));
+    float q = 0.0391947381f;
+    q = __builtin_fmaf(q, t, -0.178475707f);
+    q = __builtin_fmaf(q, t, 0.255165062f);
+    q = __builtin_fmaf(q, t, -0.101603871f);
+    q = __builtin_fmaf(q, t, 0.157105486f);
+    q = __builtin_fmaf(q, t, 0.0886519629f);
+    q = __builtin_fmaf(q, t, 0.121786028f);
+    q = __builtin_fmaf(q, t, 0.118163349f);
+    q = __builtin_fmaf(q, t, 1.29719759e-05f);
+    q *= e;
+    *bell = e;
+    return z < 0.f ? q : 1.f - q;
+}
 
 template <int ACT>
 __device__ __forceinline__ float act_f(float z) {
     if constexpr (ACT == PNGPD_ACT_RELU) return z < 0.f ? 0.f : z;
-    if constexpr (ACT == PNGPD_ACT_GELU) return z == -__builtin_inff() ? 0.f : 0.5f * z * erfcf(-z * 0.70710678118654752f);
+    if constexpr (ACT == PNGPD_ACT_GELU) {
+        float bell;
+        const float y = z * normal_cdf(z, &bell);
+        return z == -__builtin_inff() ? 0.f : y;
+    }
     if constexpr (ACT == PNGPD_ACT_GELU_TANH)
         return z == -__builtin_inff() ? 0.f : z * sigmoid_f(2.f * GELU_C * (z + 0.044715f * z * z * z));
     if constexpr (ACT == PNGPD_ACT_SILU) return z == -__builtin_inff() ? 0.f : z * sigmoid_f(z);
@@ -37,18 +61,20 @@ template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
     if constexpr (ACT == PNGPD_ACT_RELU) return z > 0.f ? 1.f : z == z ? 0.f : z;
     if constexpr (ACT == PNGPD_ACT_GELU) {
-        if (__builtin_fabsf(z) > 16.f) return z > 0.f ? 1.f : 0.f;      // the bell is below 1e-55
-        return 0.5f * erfcf(-z * 0.70710678118654752f) + z * 0.3989422804014327f * __expf(-0.5f * z * z);
+        float bell;
+        const float s = normal_cdf(z, &bell);
+        // beyond 16 the bell is below 1e-55 (and an infinite z would make 0 * inf of it)
+        return __builtin_fabsf(z) > 16.f ? (z > 0.f ? 1.f : 0.f) : __builtin_fmaf(z * 0.3989422804014327f, bell, s);
     }
     if constexpr (ACT == PNGPD_ACT_GELU_TANH) {
-        if (__builtin_fabsf(z) > 16.f) return z > 0.f ? 1.f : 0.f;
         const float s = sigmoid_f(2.f * GELU_C * (z + 0.044715f * z * z * z));
-        return s + z * s * (1.f - s) * 2.f * GELU_C * (1.f + 0.134145f * z * z);
+        const float v = s + z * s * (1.f - s) * 2.f * GELU_C * (1.f + 0.134145f * z * z);
+        return __builtin_fabsf(z) > 16.f ? (z > 0.f ? 1.f : 0.f) : v;
     }
     if constexpr (ACT == PNGPD_ACT_SILU) {
-        if (__builtin_fabsf(z) > 100.f) return z > 0.f ? 1.f : 0.f;
         const float s = sigmoid_f(z);
-        return s + z * s * (1.f - s);
+        const float v = s + z * s * (1.f - s);
+        return __builtin_fabsf(z) > 100.f ? (z > 0.f ? 1.f : 0.f) : v;
     }
     return z == z ? 1.f : z;
 }

@@ -9,21 +9,19 @@ namespace {
 
 // ---- joining partial sums --------------------------------------------------------------------------------------------------------
 
-// 4 neighbouring columns of a row a thread: the cuts of the contraction added in order, then the epilogue
+// 8 neighbouring columns of a row a thread: the cuts of the contraction added in order, then the epilogue
 template <typename E, int KIND>
-__global__ __launch_bounds__(256) void join_kernel(int64_t M, int64_t N, int64_t quads, int splits, const float* partial, HeadEpilogue e,
-                                                   bool vec) {
-    const int64_t total = M * quads;
+__global__ __launch_bounds__(256) void join_kernel(int64_t M, int64_t N, int64_t groups, int splits, const float* partial, HeadEpilogue e,
+                                                   bool vec, bool partial_vec) {
+    const int64_t total = M * groups;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t m = i / quads, n = (i - m * quads) * 4;
+        const int64_t m = i / groups, n = (i - m * groups) * 8;
         const int64_t have = N - n;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (have > 0) {
-            const int valid = (int)(have < 4 ? have : 4);
-            for (int s = 0; s < splits; ++s) v += load4(partial + ((int64_t)s * M + m) * N + n, valid, vec);
-        }
+        const int valid = (int)(have < 0 ? 0 : have < 8 ? have : 8);
+        Eight v = {};
+        for (int s = 0; s < splits; ++s) add8(v, load8(partial + ((int64_t)s * M + m) * N + n, valid, partial_vec));
         const int64_t room = (KIND == TILE_DZ ? e.ld_out : N) - n;
-        finish4<E, KIND>(e, N, m, n, (int)(room < 4 ? room : 4), vec, v);
+        finish8<E, KIND>(e, N, m, n, (int)(room < 8 ? room : 8), vec, v);
     }
 }
 
@@ -65,14 +63,14 @@ __global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, i
 
 template <typename E>
 hipError_t join(int64_t M, int64_t N, int splits, const float* partial, const HeadEpilogue& e, hipStream_t s) {
-    const bool vec = epilogue_vec(e, N, sizeof(E)) && N % 4 == 0;
-    const int64_t quads = ((e.kind == HEAD_EPI_DZ ? e.ld_out : N) + 3) / 4;
-    const int64_t blocks = (M * quads + 255) / 256;
+    const bool vec = epilogue_vec(e, N, sizeof(E)), pv = N % 4 == 0;
+    const int64_t groups = ((e.kind == HEAD_EPI_DZ ? e.ld_out : N) + 7) / 8;
+    const int64_t blocks = (M * groups + 255) / 256;
     const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
     switch (e.kind) {
-        case HEAD_EPI_LINEAR: join_kernel<E, TILE_LINEAR><<<grid, 256, 0, s>>>(M, N, quads, splits, partial, e, vec); break;
-        case HEAD_EPI_DZ: join_kernel<E, TILE_DZ><<<grid, 256, 0, s>>>(M, N, quads, splits, partial, e, vec); break;
-        case HEAD_EPI_SCALED: join_kernel<E, TILE_SCALED><<<grid, 256, 0, s>>>(M, N, quads, splits, partial, e, vec); break;
+        case HEAD_EPI_LINEAR: join_kernel<E, TILE_LINEAR><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e, vec, pv); break;
+        case HEAD_EPI_DZ: join_kernel<E, TILE_DZ><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e, vec, pv); break;
+        case HEAD_EPI_SCALED: join_kernel<E, TILE_SCALED><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e, vec, pv); break;
         default: join_stats_kernel<E><<<(unsigned)M, 256, 0, s>>>(M, N, splits, partial, e);
     }
     return hipGetLastError();
@@ -186,6 +184,21 @@ hipError_t act_backward(int64_t M, int64_t N, const void* dy, int64_t ld, const 
     }
 #undef PNGPD_ACT_CASE
     return hipGetLastError();
+}
+
+template <typename T>
+__device__ __forceinline__ f32x4 load4(const T* p, int valid, bool vec) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (vec && valid >= 4) {
+        typedef __attribute__((ext_vector_type(4))) T t4;
+        const t4 r = *(const t4*)p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (float)r[i];
+    } else {
+        for (int i = 0; i < 4; ++i)
+            if (i < valid) v[i] = (float)p[i];
+    }
+    return v;
 }
 
 // 64 columns of 4 values (256 columns) by 4 rows at a time a workgroup

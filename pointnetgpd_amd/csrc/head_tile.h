@@ -158,86 +158,107 @@ struct TileOperand {
     }
 };
 
-__device__ __forceinline__ float act_any(float z, int act) {
-    switch (act) {
-        case PNGPD_ACT_RELU: return act_f<PNGPD_ACT_RELU>(z);
-        case PNGPD_ACT_GELU: return act_f<PNGPD_ACT_GELU>(z);
-        case PNGPD_ACT_GELU_TANH: return act_f<PNGPD_ACT_GELU_TANH>(z);
-        case PNGPD_ACT_SILU: return act_f<PNGPD_ACT_SILU>(z);
-        default: return z;
-    }
-}
-
-// Four neighbouring values of a row, as one access where `vec` says that every row starts suitably aligned.
+// Eight neighbouring values of a row, as 16-byte accesses where `vec` says that every row starts suitably aligned.
+struct Eight {
+    float v[8];
+};
 template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* p, int valid, bool vec) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (vec && valid >= 4) {
-        typedef __attribute__((ext_vector_type(4))) T t4;
-        const t4 r = *(const t4*)p;
+__device__ __forceinline__ Eight load8(const T* p, int valid, bool vec) {
+    constexpr int C = 16 / sizeof(T);
+    typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T chunk;
+    Eight r;
+    if (vec && valid >= 8) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (float)r[i];
+        for (int k = 0; k < 8 / C; ++k) {
+            const chunk c = ((const chunk*)p)[k];
+#pragma unroll
+            for (int i = 0; i < C; ++i) r.v[k * C + i] = (float)c[i];
+        }
     } else {
-        for (int i = 0; i < 4; ++i)
-            if (i < valid) v[i] = (float)p[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.v[i] = i < valid ? (float)p[i] : 0.f;
     }
-    return v;
+    return r;
 }
 template <typename T>
-__device__ __forceinline__ void store4(T* p, const f32x4& v, int valid, bool vec) {
-    if (vec && valid >= 4) {
-        typedef __attribute__((ext_vector_type(4))) T t4;
-        t4 r;
+__device__ __forceinline__ void store8(T* p, const Eight& r, int valid, bool vec) {
+    constexpr int C = 16 / sizeof(T);
+    typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T chunk;
+    if (vec && valid >= 8) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = (T)v[i];
-        *(t4*)p = r;
+        for (int k = 0; k < 8 / C; ++k) {
+            chunk c;
+#pragma unroll
+            for (int i = 0; i < C; ++i) c[i] = (T)r.v[k * C + i];
+            ((chunk*)p)[k] = c;
+        }
     } else {
-        for (int i = 0; i < 4; ++i)
-            if (i < valid) p[i] = (T)v[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < valid) p[i] = (T)r.v[i];
     }
 }
+__device__ __forceinline__ void add8(Eight& a, const Eight& b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a.v[i] += b.v[i];
+}
+template <int ACT>
+__device__ __forceinline__ void act8(Eight& a) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a.v[i] = act_f<ACT>(a.v[i]);
+}
 
-// What becomes of 4 neighbouring sums of row m, from column n on (valid of them exist).
+// What becomes of 8 neighbouring sums of row m, from column n on (valid of them exist).
 template <typename E, int KIND>
-__device__ __forceinline__ void finish4(const HeadEpilogue& e, int64_t N, int64_t m, int64_t n, int valid, bool vec, f32x4 acc) {
+__device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_t m, int64_t n, int valid, bool vec, Eight& a) {
     if constexpr (KIND == TILE_LINEAR) {
-        if (e.bias) acc += load4((const E*)e.bias + n, valid, vec);
+        if (e.bias) add8(a, load8((const E*)e.bias + n, valid, vec));
         if (e.z) {
-            if (e.act == PNGPD_ACT_RELU) {
-                E* z = (E*)e.z + m * N + n;
-                for (int i = 0; i < 4; ++i)
-                    if (i < valid) z[i] = keep_z<E, PNGPD_ACT_RELU>(acc[i]);
+            E* z = (E*)e.z + m * N + n;
+            if (sizeof(E) == 2 && e.act == PNGPD_ACT_RELU) {
+                Eight k;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) k.v[i] = (float)keep_z<E, PNGPD_ACT_RELU>(a.v[i]);
+                store8(z, k, valid, vec);
             } else {
-                store4((E*)e.z + m * N + n, acc, valid, vec);
+                store8(z, a, valid, vec);
             }
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] = act_any(acc[i], e.act);
-        if (e.residual) acc += load4((const E*)e.residual + m * e.ld_residual + n, valid, vec);
-        store4((E*)e.out + m * e.ld_out + n, acc, valid, vec);
+        switch (e.act) {
+            case PNGPD_ACT_RELU: act8<PNGPD_ACT_RELU>(a); break;
+            case PNGPD_ACT_GELU: act8<PNGPD_ACT_GELU>(a); break;
+            case PNGPD_ACT_GELU_TANH: act8<PNGPD_ACT_GELU_TANH>(a); break;
+            case PNGPD_ACT_SILU: act8<PNGPD_ACT_SILU>(a); break;
+        }
+        if (e.residual) add8(a, load8((const E*)e.residual + m * e.ld_residual + n, valid, vec));
+        store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
     } else if constexpr (KIND == TILE_DZ) {
-        const float w = e.row_weight[m], lse = e.lse[m];
         // the columns between N and the row's end are the zeros behind a dense extent; the bias ends at N
-        const int real = (int)(N - n < 4 ? N - n : 4);
-        if (e.bias) acc += load4((const E*)e.bias + n, real, vec);
+        const float w = e.row_weight[m], lse = e.lse[m];
+        const int real = (int)(N - n < 8 ? N - n : 8);
+        if (e.bias) add8(a, load8((const E*)e.bias + n, real, vec));
         const int64_t y = e.target[m] - e.first_n - n;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float p = __expf(acc[i] - lse) - e.smooth - (y == i ? e.one_minus_eps : 0.f);
-            acc[i] = w == 0.f || i >= real ? 0.f : p * w;
+        for (int i = 0; i < 8; ++i) {
+            const float p = __expf(a.v[i] - lse) - e.smooth - (y == i ? e.one_minus_eps : 0.f);
+            a.v[i] = w == 0.f || i >= real ? 0.f : p * w;
         }
-        store4((E*)e.out + m * e.ld_out + n, acc, valid, vec);
+        store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
     } else {
-        if (e.add) acc += load4(e.add + m * N + n, valid, vec);
-        if (e.scale) acc *= e.scale[0];
-        if (e.out_f32) store4((float*)e.out + m * e.ld_out + n, acc, valid, vec);
-        else store4((E*)e.out + m * e.ld_out + n, acc, valid, vec);
+        if (e.add) add8(a, load8(e.add + m * N + n, valid, vec));
+        if (e.scale) {
+            const float s = e.scale[0];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a.v[i] *= s;
+        }
+        if (e.out_f32) store8((float*)e.out + m * e.ld_out + n, a, valid, vec);
+        else store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
     }
 }
 
-// rows of every matrix the epilogue touches start at a multiple of 4 elements
+// rows of every matrix the epilogue touches start at 16-byte addresses, so does every eighth of their columns
 inline bool epilogue_vec(const HeadEpilogue& e, int64_t N, size_t sz) {
-    auto ok = [](const void* p, int64_t ld, size_t size) { return !p || (((uintptr_t)p & (4 * size - 1)) == 0 && ld % 4 == 0); };
+    auto ok = [](const void* p, int64_t ld, size_t size) { return !p || (((uintptr_t)p & 15) == 0 && ld % (16 / (int64_t)size) == 0); };
     return ok(e.out, e.ld_out, e.out_f32 ? 4 : sz) && ok(e.bias, 0, sz) && ok(e.residual, e.ld_residual, sz) && ok(e.z, N, sz) && ok(e.add, N, 4);
 }
 
@@ -332,41 +353,64 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
         // a row's maximum, sum and target over this tile's columns: lane, then the 4 lanes of the row, then the waves
         __syncthreads();
         float4* share = (float4*)smem;      // [WN][BM]
+        const int first_n = wn * FN * 16 + 4 * q;
+        if (g.e.bias) {
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                const int64_t n = n0 + first_n + i * 16;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const float b = n + c < g.N ? (float)((const E*)g.e.bias)[n + c] : 0.f;
+#pragma unroll
+                    for (int j = 0; j < FM; ++j) acc[i][j][c] += b;
+                }
+            }
+        }
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
             const int r = (wm * FM + j) * 16 + t;
             const int64_t m = m0 + r;
-            const int64_t y = m < g.M ? g.e.target[m] : -1;
-            float mx = -__builtin_inff(), zs = 0.f;
+            float zs = 0.f;
+            if (g.e.want_logit_sum) {
 #pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                const int64_t n = n0 + (wn * FN + i) * 16 + 4 * q;
-                const int64_t have = g.N - n;
-                const int valid = (int)(have < 0 ? 0 : have < 4 ? have : 4);
-                if (g.e.bias) acc[i][j] += load4((const E*)g.e.bias + n, valid, vec);
+                for (int i = 0; i < FN; ++i)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c >= valid) {
-                        acc[i][j][c] = -__builtin_inff();
-                        continue;
-                    }
-                    const float z = acc[i][j][c];
-                    mx = __builtin_fmaxf(mx, z);
-                    zs += z;
-                    if (n + c == y) g.e.target_logit[m] = z;
-                }
+                    for (int c = 0; c < 4; ++c) zs += first_n + i * 16 + c < rows_n ? acc[i][j][c] : 0.f;
+                zs += __shfl_xor(zs, 16);
+                zs += __shfl_xor(zs, 32);
             }
+            // the label's logit: one lane of the row holds it, if this tile does
+            const int64_t y = m < g.M ? g.e.target[m] - n0 - first_n : -1;
+            if (y >= 0 && y < FN * 16 && (y & 15) < 4 && first_n + y < rows_n) {
+                float z = 0.f;
+#pragma unroll
+                for (int i = 0; i < FN; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) z = y == i * 16 + c ? acc[i][j][c] : z;
+                g.e.target_logit[m] = z;
+            }
+            if (rows_n < BN) {
+#pragma unroll
+                for (int i = 0; i < FN; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) acc[i][j][c] = first_n + i * 16 + c < rows_n ? acc[i][j][c] : -__builtin_inff();
+            }
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < FN; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) mx = __builtin_fmaxf(mx, acc[i][j][c]);
             mx = __builtin_fmaxf(mx, __shfl_xor(mx, 16));
             mx = __builtin_fmaxf(mx, __shfl_xor(mx, 32));
+            // exp(z - mx); where nothing is finite the terms are exp(-inf) = 0, not exp(-inf + inf)
+            const float base = mx == -__builtin_inff() ? 0.f : mx;
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < FN; ++i)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s += acc[i][j][c] == -__builtin_inff() ? 0.f : __expf(acc[i][j][c] - mx);
+                for (int c = 0; c < 4; ++c) s += __expf(acc[i][j][c] - base);
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
-            zs += __shfl_xor(zs, 16);
-            zs += __shfl_xor(zs, 32);
             if (q == 0) share[wn * BM + r] = make_float4(mx, s, zs, 0.f);
         }
         __syncthreads();
@@ -382,18 +426,37 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
             g.e.stats[(int64_t)tn * g.M + m0 + r] = v;
         }
     } else {
+        // The sums go through LDS, as many rows as it holds at a time, and come back as 8 neighbouring columns a thread: whole
+        // lines of memory for the epilogue's loads and stores.  16-byte chunk c of staged row r at slot c ^ (r & 15).
+        constexpr int HOLD = 2 * STAGE / (BN * 4), ROWS = HOLD < BM ? HOLD : BM, PASSES = BM / ROWS, JP = FM / PASSES;
+        constexpr int MIX = (BN / 4 < 16 ? BN / 4 : 16) - 1, GROUPS = BN / 8;
+        static_assert(ROWS * PASSES == BM && JP * PASSES == FM, "rows of a pass");
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const int64_t m = m0 + (wm * FM + j) * 16 + t;
-            if (m >= g.M) continue;
+        for (int pass = 0; pass < PASSES; ++pass) {
+            __syncthreads();
 #pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                const int64_t n = n0 + (wn * FN + i) * 16 + 4 * q;
+            for (int j = 0; j < JP; ++j) {
+                const int r = (wm * JP + j) * 16 + t;
+#pragma unroll
+                for (int i = 0; i < FN; ++i) {
+                    const int c = (wn * FN + i) * 4 + q;
+                    *(f32x4*)(smem + r * (BN * 4) + (c ^ (r & MIX)) * 16) = acc[i][pass * JP + j];
+                }
+            }
+            __syncthreads();
+#pragma unroll 1
+            for (int item = threadIdx.x; item < ROWS * GROUPS; item += WAVES * 64) {
+                const int r = item / GROUPS, c = (item % GROUPS) * 2;
+                const int in = r / (JP * 16);                      // which wave row staged it
+                const int64_t m = m0 + (in * FM + pass * JP) * 16 + (r - in * JP * 16), n = n0 + c * 4;
                 const int64_t have = (KIND == TILE_DZ ? g.e.ld_out : g.N) - n;
-                if (have <= 0) continue;
-                const int valid = (int)(have < 4 ? have : 4);
-                if constexpr (KIND == TILE_PARTIAL) store4(g.partial + ((int64_t)split * g.M + m) * g.N + n, acc[i][j], valid, vec);
-                else finish4<E, KIND>(g.e, g.N, m, n, valid, vec, acc[i][j]);
+                if (m >= g.M || have <= 0) continue;
+                const int valid = (int)(have < 8 ? have : 8);
+                const f32x4 lo = *(const f32x4*)(smem + r * (BN * 4) + (c ^ (r & MIX)) * 16);
+                const f32x4 hi = *(const f32x4*)(smem + r * (BN * 4) + ((c + 1) ^ (r & MIX)) * 16);
+                Eight a = {{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
+                if constexpr (KIND == TILE_PARTIAL) store8(g.partial + ((int64_t)split * g.M + m) * g.N + n, a, valid, vec);
+                else finish8<E, KIND>(g.e, g.N, m, n, valid, vec, a);
             }
         }
     }
