@@ -21,7 +21,8 @@ __global__ __launch_bounds__(256) void join_kernel(int64_t M, int64_t N, int64_t
         Eight v = {};
         for (int s = 0; s < splits; ++s) add8(v, load8(partial + ((int64_t)s * M + m) * N + n, valid, partial_vec));
         const int64_t room = (KIND == TILE_DZ ? e.ld_out : N) - n;
-        finish8<E, KIND>(e, N, m, n, (int)(room < 8 ? room : 8), vec, v);
+        const int real = (int)(room < 8 ? room : 8);
+        finish8<E, KIND>(e, N, m, n, real, vec, load_columns<E, KIND>(e, N, n, vec), load_ahead<E, KIND>(e, N, m, n, real, vec), v);
     }
 }
 

@@ -208,11 +208,49 @@ __device__ __forceinline__ void act8(Eight& a) {
     for (int i = 0; i < 8; ++i) a.v[i] = act_f<ACT>(a.v[i]);
 }
 
-// What becomes of 8 neighbouring sums of row m, from column n on (valid of them exist).
+// The epilogue of 8 neighbouring sums of a row, in the order a latency-bound loop wants it: what depends on the columns is
+// loaded once (Columns), what depends on the row for several rows ahead (Ahead), then the sums are finished.
+struct Columns {
+    Eight bias;
+    float scale;
+};
 template <typename E, int KIND>
-__device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_t m, int64_t n, int valid, bool vec, Eight& a) {
+__device__ __forceinline__ Columns load_columns(const HeadEpilogue& e, int64_t N, int64_t n, bool vec) {
+    Columns c = {};
+    c.scale = 1.f;
+    if constexpr (KIND == TILE_LINEAR || KIND == TILE_DZ) {
+        if (e.bias) c.bias = load8((const E*)e.bias + n, (int)(N - n < 0 ? 0 : N - n < 8 ? N - n : 8), vec);
+    }
+    if constexpr (KIND == TILE_SCALED) {
+        if (e.scale) c.scale = e.scale[0];
+    }
+    return c;
+}
+struct Ahead {
+    Eight more;             // LINEAR: residual; SCALED: what is added
+    float weight, lse;      // DZ
+    int label;
+};
+template <typename E, int KIND>
+__device__ __forceinline__ Ahead load_ahead(const HeadEpilogue& e, int64_t N, int64_t m, int64_t n, int valid, bool vec) {
+    Ahead h = {};
     if constexpr (KIND == TILE_LINEAR) {
-        if (e.bias) add8(a, load8((const E*)e.bias + n, valid, vec));
+        if (e.residual) h.more = load8((const E*)e.residual + m * e.ld_residual + n, valid, vec);
+    } else if constexpr (KIND == TILE_DZ) {
+        h.weight = e.row_weight[m];
+        h.lse = e.lse[m];
+        const int64_t y = e.target[m] - e.first_n - n;
+        h.label = y >= 0 && y < 8 ? (int)y : -1;
+    } else if constexpr (KIND == TILE_SCALED) {
+        if (e.add) h.more = load8(e.add + m * N + n, valid, vec);
+    }
+    return h;
+}
+template <typename E, int KIND>
+__device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_t m, int64_t n, int valid, bool vec, const Columns& col,
+                                        const Ahead& h, Eight& a) {
+    if constexpr (KIND == TILE_LINEAR) {
+        add8(a, col.bias);
         if (e.z) {
             E* z = (E*)e.z + m * N + n;
             if (sizeof(E) == 2 && e.act == PNGPD_ACT_RELU) {
@@ -230,27 +268,22 @@ __device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_
             case PNGPD_ACT_GELU_TANH: act8<PNGPD_ACT_GELU_TANH>(a); break;
             case PNGPD_ACT_SILU: act8<PNGPD_ACT_SILU>(a); break;
         }
-        if (e.residual) add8(a, load8((const E*)e.residual + m * e.ld_residual + n, valid, vec));
+        if (e.residual) add8(a, h.more);
         store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
     } else if constexpr (KIND == TILE_DZ) {
-        // the columns between N and the row's end are the zeros behind a dense extent; the bias ends at N
-        const float w = e.row_weight[m], lse = e.lse[m];
+        // the columns between N and the row's end are the zeros behind a dense extent
         const int real = (int)(N - n < 8 ? N - n : 8);
-        if (e.bias) add8(a, load8((const E*)e.bias + n, real, vec));
-        const int64_t y = e.target[m] - e.first_n - n;
+        add8(a, col.bias);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float p = __expf(a.v[i] - lse) - e.smooth - (y == i ? e.one_minus_eps : 0.f);
-            a.v[i] = w == 0.f || i >= real ? 0.f : p * w;
+            const float p = __expf(a.v[i] - h.lse) - e.smooth - (h.label == i ? e.one_minus_eps : 0.f);
+            a.v[i] = h.weight == 0.f || i >= real ? 0.f : p * h.weight;
         }
         store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
     } else {
-        if (e.add) add8(a, load8(e.add + m * N + n, valid, vec));
-        if (e.scale) {
-            const float s = e.scale[0];
+        if (e.add) add8(a, h.more);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) a.v[i] *= s;
-        }
+        for (int i = 0; i < 8; ++i) a.v[i] *= col.scale;
         if (e.out_f32) store8((float*)e.out + m * e.ld_out + n, a, valid, vec);
         else store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
     }
@@ -430,7 +463,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
         // lines of memory for the epilogue's loads and stores.  16-byte chunk c of staged row r at slot c ^ (r & 15).
         constexpr int HOLD = 2 * STAGE / (BN * 4), ROWS = HOLD < BM ? HOLD : BM, PASSES = BM / ROWS, JP = FM / PASSES;
         constexpr int MIX = (BN / 4 < 16 ? BN / 4 : 16) - 1, GROUPS = BN / 8;
-        static_assert(ROWS * PASSES == BM && JP * PASSES == FM, "rows of a pass");
+        constexpr int RSTEP = WAVES * 64 / GROUPS, BATCH = ROWS / RSTEP < 4 ? ROWS / RSTEP : 4;
+        static_assert(ROWS * PASSES == BM && JP * PASSES == FM && (WAVES * 64) % GROUPS == 0 && ROWS % (RSTEP * BATCH) == 0, "rows of a pass");
+        const int c = (threadIdx.x % GROUPS) * 2;
+        const int64_t n = n0 + c * 4, have = (KIND == TILE_DZ ? g.e.ld_out : g.N) - n;
+        const int valid = (int)(have < 0 ? 0 : have < 8 ? have : 8);
+        const Columns col = load_columns<E, KIND>(g.e, g.N, n, vec);
 #pragma unroll
         for (int pass = 0; pass < PASSES; ++pass) {
             __syncthreads();
@@ -444,19 +482,27 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
                 }
             }
             __syncthreads();
+            // a thread keeps its columns; its rows are THREADS / GROUPS apart
 #pragma unroll 1
-            for (int item = threadIdx.x; item < ROWS * GROUPS; item += WAVES * 64) {
-                const int r = item / GROUPS, c = (item % GROUPS) * 2;
-                const int in = r / (JP * 16);                      // which wave row staged it
-                const int64_t m = m0 + (in * FM + pass * JP) * 16 + (r - in * JP * 16), n = n0 + c * 4;
-                const int64_t have = (KIND == TILE_DZ ? g.e.ld_out : g.N) - n;
-                if (m >= g.M || have <= 0) continue;
-                const int valid = (int)(have < 8 ? have : 8);
-                const f32x4 lo = *(const f32x4*)(smem + r * (BN * 4) + (c ^ (r & MIX)) * 16);
-                const f32x4 hi = *(const f32x4*)(smem + r * (BN * 4) + ((c + 1) ^ (r & MIX)) * 16);
-                Eight a = {{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
-                if constexpr (KIND == TILE_PARTIAL) store8(g.partial + ((int64_t)split * g.M + m) * g.N + n, a, valid, vec);
-                else finish8<E, KIND>(g.e, g.N, m, n, valid, vec, a);
+            for (int r0 = threadIdx.x / GROUPS; r0 < ROWS; r0 += RSTEP * BATCH) {
+                Ahead ahead[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    const int r = r0 + k * RSTEP, in = r / (JP * 16);      // which wave row staged it
+                    const int64_t m = m0 + (in * FM + pass * JP) * 16 + (r - in * JP * 16);
+                    if (r < ROWS && m < g.M && valid > 0) ahead[k] = load_ahead<E, KIND>(g.e, g.N, m, n, valid, vec);
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    const int r = r0 + k * RSTEP, in = r / (JP * 16);
+                    const int64_t m = m0 + (in * FM + pass * JP) * 16 + (r - in * JP * 16);
+                    if (r >= ROWS || m >= g.M || valid <= 0) continue;
+                    const f32x4 lo = *(const f32x4*)(smem + r * (BN * 4) + (c ^ (r & MIX)) * 16);
+                    const f32x4 hi = *(const f32x4*)(smem + r * (BN * 4) + ((c + 1) ^ (r & MIX)) * 16);
+                    Eight a = {{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
+                    if constexpr (KIND == TILE_PARTIAL) store8(g.partial + ((int64_t)split * g.M + m) * g.N + n, a, valid, vec);
+                    else finish8<E, KIND>(g.e, g.N, m, n, valid, vec, col, ahead[k], a);
+                }
             }
         }
     }
