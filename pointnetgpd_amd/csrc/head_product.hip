@@ -257,7 +257,7 @@ HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
         return ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
     };
     HeadPlan p;
-    p.shape = M <= 32 ? SHAPE_FEW_ROWS : N <= 32 ? SHAPE_FEW_COLS : tiles(SHAPE_256) >= 192 ? SHAPE_256 : SHAPE_128;
+    p.shape = M <= 32 ? SHAPE_FEW_ROWS : N <= 32 ? SHAPE_FEW_COLS : type != PNGPD_TYPE_F32 && tiles(SHAPE_256) >= 192 ? SHAPE_256 : SHAPE_128;
     int bm, bn;
     shape_size(p.shape, &bm, &bn);
     p.tiles_m = (int)((M + bm - 1) / bm);

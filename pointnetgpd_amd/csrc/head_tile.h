@@ -64,15 +64,18 @@ __device__ __forceinline__ void stage_load(unsigned lds, unsigned voff, const i3
 }
 __device__ __forceinline__ void stage_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
-__device__ __forceinline__ i32x4 make_rsrc(const char* p, int64_t bytes) {
+__device__ __forceinline__ i32x4 make_rsrc(const char* p, int bytes) {
     const unsigned long long v = (unsigned long long)p;
     i32x4 r;
     r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)v);
     r[1] = __builtin_amdgcn_readfirstlane((int)((unsigned)(v >> 32) & 0xffffu));
-    r[2] = __builtin_amdgcn_readfirstlane((int)(bytes < 0 ? 0 : bytes));
+    r[2] = __builtin_amdgcn_readfirstlane(bytes);
     r[3] = 0x00020000;
     return r;
 }
+
+// Nothing is scheduled across a part's border: the compiler would otherwise keep more fragments alive than fit.
+__device__ __forceinline__ void part_begins() { __builtin_amdgcn_sched_barrier(0); }
 
 // One operand of a tile: R rows, its loads and its fragment reads.  WAVES waves share the loads.
 template <typename E, int R, bool KC, int WAVES>
@@ -80,8 +83,13 @@ struct TileOperand {
     static constexpr int SZ = sizeof(E), STEP = 128 / SZ, BYTES = R * 128, PIECES = BYTES / 1024;
     static constexpr int PER_WAVE = (PIECES + WAVES - 1) / WAVES;
     static constexpr int ROW_BYTES = R * SZ;             // of one contraction step, rows dense
-    unsigned voff[PER_WAVE];
-    unsigned beyond;                                     // bit i: piece i's chunk lies beyond the contraction in the last step
+    // A wave's pieces are WAVES apart.  Where that distance leaves the permutation as it is, they differ by a uniform number
+    // of bytes, which goes into the descriptor: one offset register instead of one a piece.
+    static constexpr int APART = KC ? WAVES * 8 : WAVES * 1024 / ROW_BYTES;      // rows, or contraction steps
+    static constexpr bool UNIFORM = KC || (SZ == 2 && APART % 16 == 0);
+    static constexpr int OFFSETS = UNIFORM ? 1 : PER_WAVE;
+    unsigned voff[OFFSETS];
+    unsigned beyond;                                     // bit 31: the lane's chunk lies beyond the contraction in the last step
 
     // permutation of the chunk index of contraction step k (rows dense): in units of the columns one read takes, 2 chunks
     // (16 columns of 16 bits) or 4 (16 floats)
@@ -93,9 +101,8 @@ struct TileOperand {
     __device__ __forceinline__ void init(int wave, int lane, int64_t ld) {
         beyond = 0;
 #pragma unroll
-        for (int i = 0; i < PER_WAVE; ++i) {
-            const int p = wave + i * WAVES;
-            const int o = p * 1024 + lane * 16;
+        for (int i = 0; i < OFFSETS; ++i) {
+            const int o = (wave + i * WAVES) * 1024 + lane * 16;
             if constexpr (KC) {
                 const int row = o / 128, c = ((o / 16) & 7) ^ (row & 7);
                 voff[i] = (unsigned)(row * ld) + c * 16;
@@ -108,30 +115,27 @@ struct TileOperand {
         }
     }
     // marks the chunks of the last step that lie beyond the contraction (`left` elements are left in it)
-    __device__ __forceinline__ void init_tail(int wave, int lane, int left) {
+    __device__ __forceinline__ void init_tail(int lane, int left) {
         if constexpr (KC) {
-#pragma unroll
-            for (int i = 0; i < PER_WAVE; ++i) {
-                const int o = (wave + i * WAVES) * 1024 + lane * 16;
-                const int c = ((o / 16) & 7) ^ ((o / 128) & 7);
-                if (c * (16 / SZ) >= left) beyond |= 1u << i;
-            }
+            const int c = (lane & 7) ^ (lane >> 3);
+            beyond = c * (16 / SZ) >= left ? 0x80000000u : 0u;
         }
     }
-    // base: the tile's first element of this step; left: contraction elements from here on; rows: valid rows of the tile
-    __device__ __forceinline__ void load(const char* base, int64_t ld, int64_t left, int rows, unsigned lds, int wave) {
-        i32x4 rsrc;
-        // an operand's dense extent is whole chunks, in itself or with zeros behind it (head_direct)
+    // base: the tile's first element of this step; left: contraction elements from here on (none: zeros arrive); rows: valid
+    // rows of the tile.  An operand's dense extent is whole chunks, in itself or with zeros behind it (head_direct).
+    __device__ __forceinline__ void load(const char* base, unsigned ld, int left, int rows, unsigned lds, int wave) {
         constexpr int C = 16 / SZ;
-        if constexpr (KC) rsrc = make_rsrc(base, (rows - 1) * ld + (left + C - 1) / C * 16);
-        else rsrc = make_rsrc(base, ((left < STEP ? left : STEP) - 1) * ld + (rows + C - 1) / C * 16);
-        const bool tail = KC && left < STEP;
+        const int here = left < STEP ? left : STEP;
+        const int bytes = KC ? (int)((rows - 1) * ld) + (here + C - 1) / C * 16 : (int)((here - 1) * ld) + (rows + C - 1) / C * 16;
+        const unsigned last = KC && left < STEP ? 0x80000000u : 0u;
 #pragma unroll
         for (int i = 0; i < PER_WAVE; ++i) {
             if (PIECES % WAVES != 0 && wave + i * WAVES >= PIECES) break;
-            unsigned v = voff[i];
-            if (tail) v |= (beyond >> i & 1u) << 31;
-            stage_load(lds + (wave + i * WAVES) * 1024, v, rsrc);
+            const unsigned skip = UNIFORM ? i * APART * ld : 0;
+            unsigned v = voff[UNIFORM ? 0 : i];
+            if constexpr (KC) v |= beyond & last;
+            const int rest = left > 0 ? bytes - (int)skip : 0;
+            stage_load(lds + (wave + i * WAVES) * 1024, v, make_rsrc(base + skip, rest > 0 ? rest : 0));
         }
     }
     // fragment of 16 rows from row0 (a multiple of 16), part ks (0 or 1) of the step
@@ -333,8 +337,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
     ob.init(wave, lane, g.ldb);
     const int tail = (int)((k_end - k_begin) % STEP);
     if (tail) {
-        oa.init_tail(wave, lane, tail);
-        ob.init_tail(wave, lane, tail);
+        oa.init_tail(lane, tail);
+        ob.init_tail(lane, tail);
     }
     const char* pa = g.a + (AK ? m0 * g.lda + k_begin * (int)sizeof(E) : k_begin * g.lda + m0 * (int)sizeof(E));
     const char* pb = g.b + (BK ? n0 * g.ldb + k_begin * (int)sizeof(E) : k_begin * g.ldb + n0 * (int)sizeof(E));
@@ -347,39 +351,64 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    int64_t left = k_end - k_begin;
-    int cur = 0;
-    if (left > 0) {
-        oa.load(pa, g.lda, left, rows_m, lds0, wave);
-        ob.load(pb, g.ldb, left, rows_n, lds0 + BM * 128, wave);
-    }
-    while (left > 0) {
-        stage_wait();      // this step's tiles are in LDS, and every wave is done reading the other half
-        const int64_t next = left - STEP;
-        if (next > 0) {
-            pa += step_a;
-            pb += step_b;
-            const unsigned dst = lds0 + (cur ^ 1) * STAGE;
-            oa.load(pa, g.lda, next, rows_m, dst, wave);
-            ob.load(pb, g.ldb, next, rows_n, dst + BM * 128, wave);
-        }
-        const char* sa = smem + cur * STAGE;
-        const char* sb = sa + BM * 128;
+    // Four parts a step: the two halves of the step's contraction, and of the wave's m fragments in each.  While the matrix
+    // unit works on one part, the fragments of the next one come out of LDS.  The last part is carried over the barrier: its
+    // fragments are in registers by then, so the matrix unit has work while the next step's first ones arrive, and the loads
+    // after next go into the half of LDS that nobody reads any more.
+    constexpr int H = FM / 2;
+    static_assert(FM % 2 == 0, "two halves of the m fragments");
+    int left = (int)(k_end - k_begin);
+    i32x4 fa[2][H], fb[2][FN];
+    const auto read_a = [&](const char* base, int ks, int half, i32x4* f) {
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            i32x4 fa[FM], fb[FN];
+        for (int j = 0; j < H; ++j) f[j] = OpA::frag(base, (wm * FM + half * H + j) * 16, ks, lane);
+    };
+    const auto read_b = [&](const char* base, int ks, i32x4* f) {
 #pragma unroll
-            for (int j = 0; j < FM; ++j) fa[j] = OpA::frag(sa, (wm * FM + j) * 16, ks, lane);
+        for (int i = 0; i < FN; ++i) f[i] = OpB::frag(base + BM * 128, (wn * FN + i) * 16, ks, lane);
+    };
+    const auto multiply = [&](int half, const i32x4* a, const i32x4* b) {
 #pragma unroll
-            for (int i = 0; i < FN; ++i) fb[i] = OpB::frag(sb, (wn * FN + i) * 16, ks, lane);
+        for (int i = 0; i < FN; ++i)
 #pragma unroll
-            for (int i = 0; i < FN; ++i)
+            for (int j = 0; j < H; ++j) acc[i][half * H + j] = mma16<E>(b[i], a[j], acc[i][half * H + j]);
+    };
+    const unsigned lda = (unsigned)g.lda, ldb = (unsigned)g.ldb;
+    oa.load(pa, lda, left, rows_m, lds0, wave);
+    ob.load(pb, ldb, left, rows_n, lds0 + BM * 128, wave);
+    // before the first step the carried part is zeros
 #pragma unroll
-                for (int j = 0; j < FM; ++j) acc[i][j] = mma16<E>(fb[i], fa[j], acc[i][j]);
-        }
-        cur ^= 1;
-        left = next;
-    }
+    for (int j = 0; j < H; ++j) fa[1][j] = i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < FN; ++i) fb[1][i] = i32x4{0, 0, 0, 0};
+    unsigned cur = 0;
+    stage_wait();
+    do {
+        // this step's tiles are in LDS, and every wave is done reading the other half
+        const char* sa = smem + cur;
+        cur = STAGE - cur;
+        left -= STEP;
+        pa += step_a;
+        pb += step_b;
+        read_b(sa, 0, fb[0]);
+        read_a(sa, 0, 0, fa[0]);
+        oa.load(pa, lda, left, rows_m, lds0 + cur, wave);
+        ob.load(pb, ldb, left, rows_n, lds0 + cur + BM * 128, wave);
+        multiply(1, fa[1], fb[1]);
+        part_begins();
+        read_a(sa, 0, 1, fa[1]);
+        multiply(0, fa[0], fb[0]);
+        part_begins();
+        read_b(sa, 1, fb[1]);
+        read_a(sa, 1, 0, fa[0]);
+        multiply(1, fa[1], fb[0]);
+        part_begins();
+        read_a(sa, 1, 1, fa[1]);
+        multiply(0, fa[0], fb[1]);
+        part_begins();
+        stage_wait();
+    } while (left > 0);
+    multiply(1, fa[1], fb[1]);
 
     const int t = lane & 15, q = lane >> 4;
     if constexpr (KIND == TILE_STATS) {
@@ -532,7 +561,10 @@ hipError_t launch_one(const TileArgs& g, bool vec, hipStream_t s) {
 template <typename E, bool AK, bool BK, int KIND>
 hipError_t launch_shape(int shape, const TileArgs& g, bool vec, hipStream_t s) {
     switch (shape) {
-        case SHAPE_256: return launch_one<E, 256, 256, 2, 4, AK, BK, KIND>(g, vec, s);
+        case SHAPE_256:
+            // floats need no larger tile than 128: their matrix instructions take eight times as long over what LDS delivers
+            if constexpr (sizeof(E) == 2) return launch_one<E, 256, 256, 2, 4, AK, BK, KIND>(g, vec, s);
+            return hipErrorInvalidValue;
         case SHAPE_128: return launch_one<E, 128, 128, 2, 2, AK, BK, KIND>(g, vec, s);
         case SHAPE_FEW_ROWS: return launch_one<E, 32, 128, 1, 4, AK, BK, KIND>(g, vec, s);
         default: return launch_one<E, 128, 32, 4, 1, AK, BK, KIND>(g, vec, s);
