@@ -72,13 +72,13 @@ hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOpe
 // zeros whatever they hold.  dst is 16-byte aligned, ld whole chunks.
 hipError_t head_lay_out(int type, int64_t rows, int64_t cols, const void* src, int64_t ld_src, const float* row_weight, void* dst,
                         int64_t ld, hipStream_t s);
-// dz[m][n] = dy[m][n] * act'(z[m][n]); z dense, dz rows of ld_dz (whole chunks) with zeros behind column N
-hipError_t head_act_backward(int type, int64_t M, int64_t N, const void* dy, int64_t ld_dy, const void* z, int act, void* dz,
-                             int64_t ld_dz, hipStream_t s);
-// out[n] = scale * sum_m a[m][n]; part: 32-bit [head_col_sum_parts(M)][N]
-int64_t head_col_sum_parts(int64_t M);
-hipError_t head_col_sum(int type, int64_t M, int64_t N, const void* a, int64_t ld, float* part, const float* scale,
-                        void* out, hipStream_t s);
+// dz[m][n] = dy[m][n] * act'(z[m][n]) (z dense; act NONE: dy itself) into dz (may be NULL; rows of ld_dz, whole chunks, zeros
+// behind column N), and the columns' sums over blocks of rows into part (may be NULL; 32-bit [head_col_parts][N])
+size_t head_col_parts(int type, int64_t M, int64_t N);
+hipError_t head_grad_rows(int type, int64_t M, int64_t N, const void* dy, int64_t ld_dy, const void* z, int act, void* dz,
+                          int64_t ld_dz, float* part, hipStream_t s);
+// out[n] = scale[0] (NULL: 1) times the sum of column n's parts
+hipError_t head_col_join(int type, int64_t M, int64_t N, const float* part, const float* scale, void* out, hipStream_t s);
 
 // a fill kernel, not a memset: the call may be captured
 hipError_t head_zero(void* p, size_t bytes, hipStream_t s);

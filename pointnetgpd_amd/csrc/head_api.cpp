@@ -96,7 +96,7 @@ struct LinearWs {
             size_t cut = pngpd::head_plan(type, M, N, K, pngpd::HEAD_EPI_LINEAR).partial_bytes;
             if (backward) {
                 if (copy_dz) dz = b.take((size_t)M * padded(N, type) * esize(type));
-                part = (float*)b.take((size_t)pngpd::head_col_sum_parts(M) * N * 4);
+                part = (float*)b.take((size_t)pngpd::head_col_parts(type, M, N) * N * 4);
                 cut = max2(pngpd::head_plan(type, M, K, N, pngpd::HEAD_EPI_SCALED).partial_bytes,
                            pngpd::head_plan(type, N, K, M, pngpd::HEAD_EPI_SCALED).partial_bytes);
             }
@@ -133,13 +133,13 @@ struct LossWs {
             if (piece < 256) piece = 256;
             if (piece > pngpd::HEAD_MAX_EXTENT) piece = pngpd::HEAD_MAX_EXTENT;
             if (piece > V) piece = V;
+            const int64_t last = V % piece ? V % piece : piece;
             tile = b.take((size_t)rows * padded(piece, type) * e);
             row_weight = (float*)b.take((size_t)rows * 4);
             scale = (float*)b.take(4);
-            part = (float*)b.take((size_t)pngpd::head_col_sum_parts(T) * piece * 4);
+            part = (float*)b.take((size_t)max2(pngpd::head_col_parts(type, rows, piece) * piece, pngpd::head_col_parts(type, rows, last) * last) * 4);
             if (piece < V) dx_sum = (float*)b.take((size_t)rows * D * 4);
             size_t cut = 0;
-            const int64_t last = V % piece ? V % piece : piece;
             for (int64_t n : {piece, last}) {
                 cut = max2(cut, pngpd::head_plan(type, rows, n, D, pngpd::HEAD_EPI_DZ).partial_bytes);
                 cut = max2(cut, pngpd::head_plan(type, n, D, rows, pngpd::HEAD_EPI_SCALED).partial_bytes);
@@ -226,10 +226,13 @@ int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void*
     LinearWs ws(workspace_dev, type, M, N, K, true, dweight_dev && !direct(x_dev, ldx, K, type),
                 dx_dev && !direct(weight_dev, ldw, K, type), act != PNGPD_ACT_NONE || !direct(dy_dev, ld_dy, N, type));
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
-    Rows dz{ws.dz, padded(N, type)};
-    if (act != PNGPD_ACT_NONE) HIP_TRY(pngpd::head_act_backward(type, M, N, dy_dev, ld_dy, z_dev, act, ws.dz, dz.ld, s));
-    else HIP_TRY(direct_rows(type, M, N, dy_dev, ld_dy, ws.dz, s, &dz));
-    if (dbias_dev) HIP_TRY(pngpd::head_col_sum(type, M, N, dz.p, dz.ld, ws.part, nullptr, dbias_dev, s));
+    // one pass over dy (and z): dz where it is not dy as it lies, and the bias gradient's partial sums
+    const bool same = act == PNGPD_ACT_NONE && direct(dy_dev, ld_dy, N, type);
+    const Rows dz = same ? Rows{dy_dev, ld_dy} : Rows{ws.dz, padded(N, type)};
+    if (!same || dbias_dev)
+        HIP_TRY(pngpd::head_grad_rows(type, M, N, dy_dev, ld_dy, z_dev, act, same ? nullptr : ws.dz, dz.ld,
+                                      dbias_dev ? ws.part : nullptr, s));
+    if (dbias_dev) HIP_TRY(pngpd::head_col_join(type, M, N, ws.part, nullptr, dbias_dev, s));
     HeadEpilogue e;
     e.kind = pngpd::HEAD_EPI_SCALED;
     e.ld_out = K;
@@ -253,6 +256,7 @@ int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64
     const char* who = "pngpd_dropout";
     int rc = check_sizes(who, type, rows, cols, 1);
     if (rc) return rc;
+    if ((double)rows * (double)cols > 4398046511104.0) return fail(PNGPD_ERR_SHAPE, "%s: more than 2^42 elements", who);
     if (!(p >= 0.0 && p <= 1.0)) return fail(PNGPD_ERR_INVALID, "%s: p = %g", who, p);
     if (rows == 0) return PNGPD_OK;
     if (!x_dev || !y_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL argument", who);
@@ -339,7 +343,10 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         e.out = ws.tile;
         e.ld_out = np;
         HIP_TRY(pngpd::head_product(type, T, n, D, x, HeadOperand{w, whole.ld, true}, e, ws.partial, s));
-        if (dbias_dev) HIP_TRY(pngpd::head_col_sum(type, T, n, ws.tile, np, ws.part, ws.scale, at(dbias_dev, v, type), s));
+        if (dbias_dev) {
+            HIP_TRY(pngpd::head_grad_rows(type, T, n, ws.tile, np, nullptr, PNGPD_ACT_NONE, nullptr, 0, ws.part, s));
+            HIP_TRY(pngpd::head_col_join(type, T, n, ws.part, ws.scale, at(dbias_dev, v, type), s));
+        }
         HeadEpilogue g;
         g.kind = pngpd::HEAD_EPI_SCALED;
         g.ld_out = D;

@@ -12,38 +12,98 @@
 namespace pngpd {
 namespace {
 
+constexpr int PER_THREAD = 8;      // neighbouring elements: 4 hashes, 16 bytes of a 16-bit type
+
 template <typename T>
-__global__ __launch_bounds__(256) void dropout_kernel(int64_t rows, int64_t cols, const T* x, int64_t ldx, const T* r, int64_t ldr,
+struct Eight {
+    static constexpr int C = 16 / sizeof(T);
+    typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T chunk;
+    T v[PER_THREAD];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int k = 0; k < PER_THREAD / C; ++k) {
+            const chunk c = ((const chunk*)p)[k];
+#pragma unroll
+            for (int i = 0; i < C; ++i) v[k * C + i] = c[i];
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+        for (int k = 0; k < PER_THREAD / C; ++k) {
+            chunk c;
+#pragma unroll
+            for (int i = 0; i < C; ++i) c[i] = v[k * C + i];
+            ((chunk*)p)[k] = c;
+        }
+    }
+};
+
+// DENSE: x and the residual are one run of memory as y is, all 16-byte aligned
+template <typename T, bool DENSE, bool RESIDUAL>
+__global__ __launch_bounds__(256) void dropout_kernel(int64_t total, int64_t cols, const T* x, int64_t ldx, const T* r, int64_t ldr,
                                                       T* y, unsigned long long border, float scale, unsigned long long seed,
-                                                      unsigned long long offset, const int64_t* rng) {
+                                                      unsigned long long offset, const int64_t* rng, bool y_aligned) {
+    const int64_t i0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * PER_THREAD;
+    if (i0 >= total) return;
+    Eight<T> a, b;
+    const bool whole = DENSE && i0 + PER_THREAD <= total;
+    if (whole) {
+        a.load(x + i0);
+        if (RESIDUAL) b.load(r + i0);
+    } else {
+        int64_t m = DENSE ? 0 : i0 / cols, n = i0 - m * cols;
+#pragma unroll
+        for (int k = 0; k < PER_THREAD; ++k) {
+            const bool there = i0 + k < total;
+            a.v[k] = there ? x[DENSE ? i0 + k : m * ldx + n] : (T)0.f;
+            if (RESIDUAL) b.v[k] = there ? r[DENSE ? i0 + k : m * ldr + n] : (T)0.f;
+            if (++n == cols && !DENSE) {
+                n = 0;
+                ++m;
+            }
+        }
+    }
     if (rng) {
         seed = (unsigned long long)rng[0];
         offset = (unsigned long long)rng[1];
     }
-    const unsigned long long key = mix64(seed ^ mix64(offset));
-    const int64_t total = rows * cols, pairs = (total + 1) / 2;
-    for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < pairs; j += (int64_t)gridDim.x * 256) {
-        const unsigned long long w = mix64(key + (unsigned long long)j);
+    const unsigned long long first = mix64(seed ^ mix64(offset)) + (unsigned long long)(i0 >> 1);
+#pragma unroll
+    for (int k = 0; k < PER_THREAD; k += 2) {
+        const unsigned long long w = mix64(first + (k >> 1));
+#pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int64_t i = 2 * j + h;
-            if (i >= total) break;
-            const int64_t m = i / cols, n = i - m * cols;
-            const bool keep = (h ? w >> 32 : w & 0xffffffffull) >= border;
-            float v = keep ? to_f32(x[m * ldx + n]) * scale : 0.f;
-            if (r) v += to_f32(r[m * ldr + n]);
-            y[i] = from_f32<T>(v);
+            const unsigned draw = h ? (unsigned)(w >> 32) : (unsigned)w;
+            float v = (unsigned long long)draw >= border ? to_f32(a.v[k + h]) * scale : 0.f;
+            if (RESIDUAL) v += to_f32(b.v[k + h]);
+            a.v[k + h] = from_f32<T>(v);
         }
+    }
+    if (y_aligned && i0 + PER_THREAD <= total) {
+        a.store(y + i0);
+    } else {
+#pragma unroll
+        for (int k = 0; k < PER_THREAD; ++k)
+            if (i0 + k < total) y[i0 + k] = a.v[k];
     }
 }
 
 template <typename T>
 hipError_t launch(int64_t rows, int64_t cols, const void* x, int64_t ldx, const void* r, int64_t ldr, void* y, double p,
                   uint64_t seed, uint64_t offset, const int64_t* rng, hipStream_t s) {
-    const int64_t blocks = (rows * cols + 511) / 512;
-    const unsigned grid = (unsigned)(blocks < 16384 ? blocks : 16384);
+    const int64_t total = rows * cols;
+    const unsigned grid = (unsigned)((total + 256 * PER_THREAD - 1) / (256 * PER_THREAD));
     const unsigned long long border = (unsigned long long)__builtin_rint(p * 4294967296.0);
     const float scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
-    dropout_kernel<T><<<grid, 256, 0, s>>>(rows, cols, (const T*)x, ldx, (const T*)r, ldr, (T*)y, border, scale, seed, offset, rng);
+    auto run_of = [&](const void* q, int64_t ld) { return ((uintptr_t)q & 15) == 0 && (ld == cols || rows == 1); };
+    const bool dense = run_of(x, ldx) && (!r || run_of(r, ldr));
+#define PNGPD_DROPOUT(D, R) \
+    dropout_kernel<T, D, R><<<grid, 256, 0, s>>>(total, cols, (const T*)x, ldx, (const T*)r, ldr, (T*)y, border, scale, seed, offset, rng, ((uintptr_t)y & 15) == 0)
+    if (dense && r) PNGPD_DROPOUT(true, true);
+    else if (dense) PNGPD_DROPOUT(true, false);
+    else if (r) PNGPD_DROPOUT(false, true);
+    else PNGPD_DROPOUT(false, false);
+#undef PNGPD_DROPOUT
     return hipGetLastError();
 }
 

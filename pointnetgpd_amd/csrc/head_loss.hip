@@ -15,19 +15,23 @@ __device__ __forceinline__ void join_stats(float4& v, const float4& u) {
     v.z += u.z;
 }
 
-// 32 rows a workgroup, 8 threads a row, each over its share of the blocks; then the threads of a row in order
+// 2^lanes rows a workgroup, the other threads side by side over a row's blocks; then the threads of a row in order
 __global__ __launch_bounds__(256) void row_loss_kernel(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit,
-                                                       const int64_t* target, int64_t ignore, float eps, float* loss, float* lse) {
-    __shared__ float4 share[8][32];
-    const int r = threadIdx.x & 31, part = threadIdx.x >> 5;
-    const int64_t t = (int64_t)blockIdx.x * 32 + r;
+                                                       const int64_t* target, int64_t ignore, float eps, int lanes, float* loss, float* lse) {
+    __shared__ float4 share[256];
+    const int rows = 1 << lanes, r = threadIdx.x & (rows - 1), part = threadIdx.x >> lanes, shares = 256 >> lanes;
+    const int64_t t = (int64_t)blockIdx.x * rows + r;
     float4 v = make_float4(-__builtin_inff(), 0.f, 0.f, 0.f);
     if (t < T)
-        for (int i = part; i < blocks; i += 8) join_stats(v, stats[(int64_t)i * T + t]);
-    share[part][r] = v;
+        for (int i = part; i < blocks; i += shares) join_stats(v, stats[(int64_t)i * T + t]);
+    share[threadIdx.x] = v;
     __syncthreads();
+    for (int step = shares / 2; step; step >>= 1) {
+        if (part < step) join_stats(share[threadIdx.x], share[threadIdx.x + (step << lanes)]);
+        __syncthreads();
+    }
     if (part || t >= T) return;
-    for (int i = 1; i < 8; ++i) join_stats(v, share[i][r]);
+    v = share[r];
     const float l = v.x + logf(v.y);
     lse[t] = l;
     const int64_t y = target[t];
@@ -127,7 +131,11 @@ hipError_t head_zero(void* p, size_t bytes, hipStream_t s) {
 hipError_t head_loss_finish(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit, const int64_t* target,
                             int64_t ignore, float eps, int reduction, float* row_loss, float* loss, float* lse, hipStream_t s) {
     if (T > 0) {
-        row_loss_kernel<<<(unsigned)((T + 31) / 32), 256, 0, s>>>(T, V, blocks, stats, target_logit, target, ignore, eps, row_loss, lse);
+        int lanes = 5;                                       // few rows: more threads a row
+        while (lanes > 0 && (T >> lanes) < 64 && (256 >> lanes) < blocks) --lanes;
+        const int rows = 1 << lanes;
+        row_loss_kernel<<<(unsigned)((T + rows - 1) / rows), 256, 0, s>>>(T, V, blocks, stats, target_logit, target, ignore, eps, lanes,
+                                                                           row_loss, lse);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || reduction == PNGPD_REDUCE_NONE) return e;
     }

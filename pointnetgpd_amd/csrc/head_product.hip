@@ -155,99 +155,125 @@ hipError_t lay_out(int64_t rows, int64_t cols, const void* src, int64_t ld_src, 
     return hipGetLastError();
 }
 
-template <typename T, int ACT>
-__global__ __launch_bounds__(256) void act_backward_kernel(int64_t M, int64_t N, const T* dy, int64_t ld, bool dy_aligned, const T* z,
-                                                           bool z_aligned, T* dz, int64_t ld_dz) {
+// How a pass over [M, N] is cut when it also sums columns: 2^lanes threads of a workgroup side by side over chunks of
+// columns, the others over rows, `parts` blocks of `rows` rows.
+struct ColumnCut {
+    int lanes;
+    unsigned blocks;
+    int64_t parts, rows;
+};
+ColumnCut column_cut(int64_t M, int64_t N, int chunk) {
+    if (M < 1) M = 1;
+    ColumnCut c;
+    const int64_t chunks = (N + chunk - 1) / chunk;
+    c.lanes = 0;
+    while (c.lanes < 6 && (1 << c.lanes) < chunks) ++c.lanes;
+    c.blocks = (unsigned)((chunks + (1 << c.lanes) - 1) >> c.lanes);
+    const int64_t side = 256 >> c.lanes;                        // rows at a time
+    int64_t parts = 2048 / c.blocks;                            // enough workgroups to fill the chip
+    const int64_t most = (M + 4 * side - 1) / (4 * side);       // but four turns of each at least
+    if (parts > most) parts = most;
+    if (parts > 256) parts = 256;
+    if (parts < 1) parts = 1;
+    c.rows = ((M + parts - 1) / parts + side - 1) / side * side;
+    c.parts = (M + c.rows - 1) / c.rows;
+    return c;
+}
+
+// One pass over dy and z: bound by memory, so the sums of the columns ride along.
+template <typename T, int ACT, bool WRITE>
+__global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, const T* dy, int64_t ld, bool dy_aligned, const T* z,
+                                                        bool z_aligned, T* dz, int64_t ld_dz, float* part, int lanes, int64_t rows) {
     constexpr int C = Chunk<T>::C;
-    int64_t r, c;
-    if (!chunk_of(M, ld_dz / C, &r, &c)) return;
-    const typename Chunk<T>::V g = Chunk<T>::load(dy + r * ld + c * C, N - c * C, dy_aligned);
-    const typename Chunk<T>::V v = Chunk<T>::load(z + r * N + c * C, N - c * C, z_aligned);
-    typename Chunk<T>::V o;
+    __shared__ float share[256][C + 1];
+    const int wide = 1 << lanes, side = 256 >> lanes;
+    const int64_t col = ((int64_t)blockIdx.x * wide + (threadIdx.x & (wide - 1))) * C;
+    const int row = threadIdx.x >> lanes;
+    const int64_t m0 = (int64_t)blockIdx.y * rows, m1 = m0 + rows < M ? m0 + rows : M;
+    float sum[C] = {};
+    if (col < N) {
+#pragma unroll 2
+        for (int64_t m = m0 + row; m < m1; m += side) {
+            const typename Chunk<T>::V g = Chunk<T>::load(dy + m * ld + col, N - col, dy_aligned);
+            typename Chunk<T>::V o = g;
+            if constexpr (ACT != PNGPD_ACT_NONE) {
+                const typename Chunk<T>::V v = Chunk<T>::load(z + m * N + col, N - col, z_aligned);
 #pragma unroll
-    for (int i = 0; i < C; ++i) o[i] = (T)((float)g[i] * act_slope<ACT>((float)v[i]));
-    *(typename Chunk<T>::V*)(dz + r * ld_dz + c * C) = o;
+                for (int i = 0; i < C; ++i) o[i] = (T)((float)g[i] * act_slope<ACT>((float)v[i]));
+            }
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                if (ACT != PNGPD_ACT_NONE && col + i >= N) o[i] = (T)0.f;
+                sum[i] += (float)o[i];
+            }
+            if constexpr (WRITE) *(typename Chunk<T>::V*)(dz + m * ld_dz + col) = o;
+        }
+    }
+    if (!part) return;
+#pragma unroll
+    for (int i = 0; i < C; ++i) share[threadIdx.x][i] = sum[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < wide * C; c += 256) {
+        const int64_t n = (int64_t)blockIdx.x * wide * C + c;
+        if (n >= N) continue;
+        float s = 0.f;
+        for (int r = 0; r < side; ++r) s += share[(r << lanes) + c / C][c % C];
+        part[(int64_t)blockIdx.y * N + n] = s;
+    }
 }
 
 template <typename T>
-hipError_t act_backward(int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz, int64_t ld_dz, hipStream_t s) {
+hipError_t grad_rows(int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz, int64_t ld_dz, float* part,
+                     hipStream_t s) {
     constexpr int C = Chunk<T>::C;
-    const unsigned grid = (unsigned)((M * (ld_dz / C) + 255) / 256);
+    const ColumnCut c = column_cut(M, N, C);
+    const dim3 grid(c.blocks, (unsigned)c.parts);
     const bool da = ((uintptr_t)dy & 15) == 0 && ld % C == 0, za = ((uintptr_t)z & 15) == 0 && N % C == 0;
-#define PNGPD_ACT_CASE(A) \
-    case A: act_backward_kernel<T, A><<<grid, 256, 0, s>>>(M, N, (const T*)dy, ld, da, (const T*)z, za, (T*)dz, ld_dz); break;
+#define PNGPD_GRAD_ROWS(A, W) \
+    grad_rows_kernel<T, A, W><<<grid, 256, 0, s>>>(M, N, (const T*)dy, ld, da, (const T*)z, za, (T*)dz, ld_dz, part, c.lanes, c.rows)
     switch (act) {
-        PNGPD_ACT_CASE(PNGPD_ACT_RELU)
-        PNGPD_ACT_CASE(PNGPD_ACT_GELU)
-        PNGPD_ACT_CASE(PNGPD_ACT_GELU_TANH)
-        PNGPD_ACT_CASE(PNGPD_ACT_SILU)
+        case PNGPD_ACT_NONE:
+            if (dz) PNGPD_GRAD_ROWS(PNGPD_ACT_NONE, true);
+            else PNGPD_GRAD_ROWS(PNGPD_ACT_NONE, false);
+            break;
+        case PNGPD_ACT_RELU: PNGPD_GRAD_ROWS(PNGPD_ACT_RELU, true); break;
+        case PNGPD_ACT_GELU: PNGPD_GRAD_ROWS(PNGPD_ACT_GELU, true); break;
+        case PNGPD_ACT_GELU_TANH: PNGPD_GRAD_ROWS(PNGPD_ACT_GELU_TANH, true); break;
+        case PNGPD_ACT_SILU: PNGPD_GRAD_ROWS(PNGPD_ACT_SILU, true); break;
         default: return hipErrorInvalidValue;
     }
-#undef PNGPD_ACT_CASE
+#undef PNGPD_GRAD_ROWS
     return hipGetLastError();
 }
 
+// 32 columns by 8 shares of the parts a workgroup
 template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* p, int valid, bool vec) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (vec && valid >= 4) {
-        typedef __attribute__((ext_vector_type(4))) T t4;
-        const t4 r = *(const t4*)p;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (float)r[i];
-    } else {
-        for (int i = 0; i < 4; ++i)
-            if (i < valid) v[i] = (float)p[i];
-    }
-    return v;
-}
-
-// 64 columns of 4 values (256 columns) by 4 rows at a time a workgroup
-template <typename T>
-__global__ __launch_bounds__(256) void col_sum_part_kernel(int64_t M, int64_t N, const T* a, int64_t ld, bool vec, int64_t rows, float* part) {
-    __shared__ f32x4 share[3][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t n = (int64_t)blockIdx.x * 256 + lane * 4;
-    const int64_t m0 = (int64_t)blockIdx.y * rows, m1 = m0 + rows < M ? m0 + rows : M;
-    const int valid = (int)(N - n < 0 ? 0 : N - n < 4 ? N - n : 4);
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    if (valid > 0)
-        for (int64_t m = m0 + w; m < m1; m += 4) s += load4(a + m * ld + n, valid, vec);
-    if (w) share[w - 1][lane] = s;
-    __syncthreads();
-    if (w == 0) {
-        for (int i = 0; i < 3; ++i) s += share[i][lane];
-        for (int i = 0; i < valid; ++i) part[(int64_t)blockIdx.y * N + n + i] = s[i];
-    }
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void col_sum_join_kernel(int parts, int64_t N, const float* part, const float* scale, T* out) {
-    const int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
+__global__ __launch_bounds__(256) void col_join_kernel(int parts, int64_t N, const float* part, const float* scale, T* out) {
+    __shared__ float share[8][32];
+    const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t n = (int64_t)blockIdx.x * 32 + c;
     float s = 0.f;
-    for (int i = 0; i < parts; ++i) s += part[(int64_t)i * N + n];
+    if (n < N) {
+#pragma unroll 8
+        for (int i = w; i < parts; i += 8) s += part[(int64_t)i * N + n];
+    }
+    share[w][c] = s;
+    __syncthreads();
+    if (w || n >= N) return;
+    for (int i = 1; i < 8; ++i) s += share[i][c];
     out[n] = from_f32<T>(scale ? s * scale[0] : s);
 }
 
 template <typename T>
-hipError_t col_sum(int64_t M, int64_t N, const void* a, int64_t ld, float* part, const float* scale, void* out, hipStream_t s) {
-    const int64_t parts = head_col_sum_parts(M), rows = (M + parts - 1) / parts;
-    const unsigned gx = (unsigned)((N + 255) / 256);
-    const bool vec = ((uintptr_t)a & (4 * sizeof(T) - 1)) == 0 && ld % 4 == 0;
-    col_sum_part_kernel<T><<<dim3(gx, (unsigned)parts), 256, 0, s>>>(M, N, (const T*)a, ld, vec, rows, part);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    col_sum_join_kernel<T><<<gx, 256, 0, s>>>((int)parts, N, part, scale, (T*)out);
+hipError_t col_join(int64_t M, int64_t N, const float* part, const float* scale, void* out, hipStream_t s) {
+    const int parts = (int)column_cut(M, N, Chunk<T>::C).parts;
+    col_join_kernel<T><<<(unsigned)((N + 31) / 32), 256, 0, s>>>(parts, N, part, scale, (T*)out);
     return hipGetLastError();
 }
 
 }  // namespace
 
-int64_t head_col_sum_parts(int64_t M) {
-    const int64_t p = (M + 31) / 32;
-    return p < 1 ? 1 : p > 64 ? 64 : p;
-}
+size_t head_col_parts(int type, int64_t M, int64_t N) { return (size_t)column_cut(M, N, type == PNGPD_TYPE_F32 ? 4 : 8).parts; }
 
 HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
     const int64_t step = type == PNGPD_TYPE_F32 ? 32 : 64, steps = (K + step - 1) / step;
@@ -264,10 +290,11 @@ HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
     p.tiles_n = (int)((N + bn - 1) / bn);
     const int64_t t = tiles(p.shape);
     int64_t splits = 1;
-    if (t < 256) {
+    // A tile of its own takes half a microsecond a step, the joining kernel three to four: cut only what has 12 steps or more,
+    // into cuts of 4 at least.
+    if (t < 256 && steps >= 12) {
         splits = 512 / t;
         if (splits > steps / 4) splits = steps / 4;
-        if (splits < 1) splits = 1;
     }
     const int64_t per = (steps + splits - 1) / splits;
     p.k_split = per * step;
@@ -293,13 +320,12 @@ hipError_t head_lay_out(int type, int64_t rows, int64_t cols, const void* src, i
                         int64_t ld, hipStream_t s) {
     PNGPD_BY_TYPE((lay_out<T>(rows, cols, src, ld_src, weight, dst, ld, s)))
 }
-hipError_t head_act_backward(int type, int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz,
-                             int64_t ld_dz, hipStream_t s) {
-    PNGPD_BY_TYPE((act_backward<T>(M, N, dy, ld, z, act, dz, ld_dz, s)))
+hipError_t head_grad_rows(int type, int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz,
+                          int64_t ld_dz, float* part, hipStream_t s) {
+    PNGPD_BY_TYPE((grad_rows<T>(M, N, dy, ld, z, act, dz, ld_dz, part, s)))
 }
-hipError_t head_col_sum(int type, int64_t M, int64_t N, const void* a, int64_t ld, float* part, const float* scale, void* out,
-                        hipStream_t s) {
-    PNGPD_BY_TYPE((col_sum<T>(M, N, a, ld, part, scale, out, s)))
+hipError_t head_col_join(int type, int64_t M, int64_t N, const float* part, const float* scale, void* out, hipStream_t s) {
+    PNGPD_BY_TYPE((col_join<T>(M, N, part, scale, out, s)))
 }
 
 }  // namespace pngpd

@@ -16,7 +16,7 @@ of the capture.
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -48,15 +48,21 @@ def _require(x, name, like=None, shape=None):
 
 
 def _rows(t, cols):
-    """(tensor [rows, cols] whose rows are dense, distance of two rows): a view where the strides allow it, else a copy."""
+    """(tensor whose memory is rows of `cols` dense elements, distance of two rows): a view where the strides allow it, else
+    a copy."""
+    if t.is_contiguous():
+        return t, cols
     t2 = t.reshape(-1, cols)
-    rows = t2.shape[0]
-    if rows <= 1 or cols == 1 and t2.stride(0) >= 1:
-        if cols == 1 or t2.stride(1) == 1:
-            return t2, max(cols, t2.stride(0))
-    elif t2.stride(1) == 1 and t2.stride(0) >= cols:
-        return t2, t2.stride(0)
+    if cols == 1 or t2.stride(1) == 1:
+        if t2.shape[0] <= 1:
+            return t2, cols
+        if t2.stride(0) >= cols:
+            return t2, t2.stride(0)
     return t2.contiguous(), cols
+
+
+def _count(t, cols):
+    return t.numel() // cols
 
 
 def _aligned(size, *matrices):
@@ -76,8 +82,38 @@ def _workspace(nbytes, dev):
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
-def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+# the stream's handle without a Stream object around it; torch.cuda.device / current_stream cost more than a small kernel's
+# launch, above all when the forward pass (the caller's thread) and the backward pass (autograd's) take turns in them
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+class _OnDevice:
+    """Makes a device the current one for the calls inside, if it is not."""
+    __slots__ = ("index", "before")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return _raw_stream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(*sizes):
+    return _lib.load().pngpd_linear_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=4096)
+def _loss_bytes(*sizes):
+    return _lib.load().pngpd_linear_cross_entropy_workspace_bytes(*sizes)
 
 
 def _wants_grad(*tensors):
@@ -95,17 +131,17 @@ def _linear_forward(x, weight, bias, residual, act, keep):
     N, K = weight.shape
     x2, ldx = _rows(x, K)
     w2, ldw = _rows(weight, K)
-    M = x2.shape[0]
+    M = _count(x, K)
     dev, kind = x.device, _TYPES[x.dtype]
     y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=dev)
     z = torch.empty((M, N), dtype=x.dtype, device=dev) if keep and act else None
     r2, ldr = _rows(residual, N) if residual is not None else (None, N)
     b = _vector(bias)
-    nbytes = lib.pngpd_linear_workspace_bytes(kind, M, N, K, 0, _aligned(x.element_size(), (x2, ldx), (w2, ldw)))
-    with torch.cuda.device(dev):
+    nbytes = _linear_bytes(kind, M, N, K, 0, _aligned(x.element_size(), (x2, ldx), (w2, ldw)))
+    with _OnDevice(dev.index) as stream:
         ws = _workspace(nbytes, dev)
         _lib.check(lib.pngpd_linear_forward(kind, M, N, K, _ptr(x2), ldx, _ptr(w2), ldw, _ptr(b), act, _ptr(r2), ldr, _ptr(y),
-                                            _ptr(z), _ptr(ws), nbytes, _stream(dev)))
+                                            _ptr(z), _ptr(ws), nbytes, stream))
     return y, z
 
 
@@ -133,16 +169,16 @@ class LinearFunction(torch.autograd.Function):
         x2, ldx = _rows(x, K)
         w2, ldw = _rows(weight, K)
         d2, ld_dy = _rows(dy, N)
-        M = x2.shape[0]
+        M = _count(x, K)
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
         dw = torch.empty((N, K), dtype=x.dtype, device=dev) if need_w else None
         db = torch.empty(N, dtype=x.dtype, device=dev) if need_b else None
-        nbytes = lib.pngpd_linear_workspace_bytes(kind, M, N, K, 1,
+        nbytes = _linear_bytes(kind, M, N, K, 1,
                                                   _aligned(x.element_size(), (x2, ldx), (w2, ldw), (d2, ld_dy)))
-        with torch.cuda.device(dev):
+        with _OnDevice(dev.index) as stream:
             ws = _workspace(nbytes, dev)
             _lib.check(lib.pngpd_linear_backward(kind, M, N, K, _ptr(d2), ld_dy, _ptr(z), _ptr(x2), ldx, _ptr(w2), ldw, ctx.act,
-                                                 _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(dev)))
+                                                 _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, stream))
         return dx, dw, db, dy if need_r else None, None
 
 
@@ -186,9 +222,9 @@ def _dropout_call(x, residual, p, seed, offset, rng):
     else:
         x2, ldx = _rows(x, cols)
         r2, ldr = _rows(residual, cols) if residual is not None else (None, cols)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev.index) as stream:
         _lib.check(lib.pngpd_dropout(_TYPES[x.dtype], x.numel() // cols, cols, _ptr(x2), ldx, _ptr(r2), ldr, _ptr(y), p, seed,
-                                     offset, _ptr(rng), _stream(dev)))
+                                     offset, _ptr(rng), stream))
     return y
 
 
@@ -260,19 +296,19 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
         dev, kind = x.device, _TYPES[x.dtype]
         x2, ldx = _rows(x, D)
         w2, ldw = _rows(weight, D)
-        T = x2.shape[0]
+        T = _count(x, D)
         dloss = _conj_free(dloss)[0].to(torch.float32).contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
         dw = torch.empty((V, D), dtype=x.dtype, device=dev) if need_w else None
         db = torch.empty(V, dtype=x.dtype, device=dev) if need_b else None
-        nbytes = lib.pngpd_linear_cross_entropy_workspace_bytes(
+        nbytes = _loss_bytes(
             kind, T, V, D, 1, _aligned(x.element_size(), (x2, ldx), (w2, ldw)))
         b = _vector(bias)
-        with torch.cuda.device(dev):
+        with _OnDevice(dev.index) as stream:
             ws = _workspace(nbytes, dev)
             _lib.check(lib.pngpd_linear_cross_entropy_backward(
                 kind, T, V, D, _ptr(x2), ldx, _ptr(w2), ldw, _ptr(b), _ptr(target), ignore_index, label_smoothing, reduction,
-                _ptr(lse), _ptr(dloss), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(dev)))
+                _ptr(lse), _ptr(dloss), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, stream))
         return dx, dw, db, None, None, None, None
 
 
@@ -282,17 +318,17 @@ def _loss_forward(x, weight, bias, target, ignore_index, label_smoothing, reduct
     dev, kind = x.device, _TYPES[x.dtype]
     x2, ldx = _rows(x, D)
     w2, ldw = _rows(weight, D)
-    T = x2.shape[0]
+    T = _count(x, D)
     loss = torch.empty(x.shape[:-1] if reduction == 0 else (), dtype=torch.float32, device=dev)
     lse = torch.empty(T, dtype=torch.float32, device=dev)
-    nbytes = lib.pngpd_linear_cross_entropy_workspace_bytes(
+    nbytes = _loss_bytes(
         kind, T, V, D, 0, _aligned(x.element_size(), (x2, ldx), (w2, ldw)))
     b = _vector(bias)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev.index) as stream:
         ws = _workspace(nbytes, dev)
         _lib.check(lib.pngpd_linear_cross_entropy_forward(kind, T, V, D, _ptr(x2), ldx, _ptr(w2), ldw, _ptr(b), _ptr(target),
                                                           ignore_index, label_smoothing, reduction, _ptr(loss), _ptr(lse),
-                                                          _ptr(ws), nbytes, _stream(dev)))
+                                                          _ptr(ws), nbytes, stream))
     return loss, lse
 
 
