@@ -275,30 +275,59 @@ hipError_t col_join(int64_t M, int64_t N, const float* part, const float* scale,
 
 size_t head_col_parts(int type, int64_t M, int64_t N) { return (size_t)column_cut(M, N, type == PNGPD_TYPE_F32 ? 4 : 8).parts; }
 
+namespace {
+
+// What a step of 128 bytes a row takes, in microseconds, with k tiles of a shape on every compute unit (measured over 32 to
+// 96 steps on 256 units, operands of normal numbers; 1.2 to 1.4 PFLOP/s for 256 x 256 tiles of 16-bit elements, 1.1 for
+// 128 x 128, 0.65 for the small ones, 0.14 for floats).
+double step_us(bool f32, int shape, int64_t k) {
+    const double n = (double)k;
+    if (f32) {
+        if (shape == SHAPE_128) return 1.9 * n;
+        return k <= 1 ? 0.6 : 0.49 * n;
+    }
+    switch (shape) {
+        case SHAPE_256: return k <= 1 ? 1.75 : 1.6 * n;
+        case SHAPE_128: return k <= 1 ? 0.65 : 1.02 * (double)((k + 1) / 2);
+        case SHAPE_64: return k <= 1 ? 0.29 : 0.205 * n;
+        default: return k <= 1 ? 0.33 : 0.25 * n;
+    }
+}
+// What a tile takes besides: its first loads and its epilogue.
+double tile_us(int shape) { return shape == SHAPE_256 ? 11.0 : shape == SHAPE_128 ? 9.0 : 4.0; }
+
+}  // namespace
+
+// The shape, and the number of cuts of the contraction, that should take the least time.  A cut contraction costs the
+// joining kernel's 4 us and its traffic (32-bit sums written and read, at some 4 TB/s).
 HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
-    const int64_t step = type == PNGPD_TYPE_F32 ? 32 : 64, steps = (K + step - 1) / step;
-    auto tiles = [&](int shape) {
+    (void)kind;
+    const bool f32 = type == PNGPD_TYPE_F32;
+    const int64_t step = f32 ? 32 : 64, steps = (K + step - 1) / step;
+    HeadPlan p{};
+    double best = 1e300;
+    for (int shape = SHAPE_256; shape <= SHAPE_FEW_COLS; ++shape) {
+        if (f32 && shape == SHAPE_256) continue;
         int bm, bn;
         shape_size(shape, &bm, &bn);
-        return ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
-    };
-    HeadPlan p;
-    p.shape = M <= 32 ? SHAPE_FEW_ROWS : N <= 32 ? SHAPE_FEW_COLS : type != PNGPD_TYPE_F32 && tiles(SHAPE_256) >= 192 ? SHAPE_256 : SHAPE_128;
-    int bm, bn;
-    shape_size(p.shape, &bm, &bn);
-    p.tiles_m = (int)((M + bm - 1) / bm);
-    p.tiles_n = (int)((N + bn - 1) / bn);
-    const int64_t t = tiles(p.shape);
-    int64_t splits = 1;
-    // A tile of its own takes half a microsecond a step, the joining kernel three to four: cut only what has 12 steps or more,
-    // into cuts of 4 at least.
-    if (t < 256 && steps >= 12) {
-        splits = 512 / t;
-        if (splits > steps / 4) splits = steps / 4;
+        const int64_t tm = (M + bm - 1) / bm, tn = (N + bn - 1) / bn, tiles = tm * tn;
+        for (int64_t cuts = 1; cuts <= 32; ++cuts) {
+            const int64_t per = (steps + cuts - 1) / cuts;
+            if (cuts > 1 && (per < 4 || tiles >= 512)) break;
+            if ((steps + per - 1) / per != cuts) continue;
+            const int64_t k = (tiles * cuts + 255) / 256;
+            double us = (double)per * step_us(f32, shape, k) + tile_us(shape) * (shape == SHAPE_256 ? (double)k : 1.0);
+            if (cuts > 1) us += 4.0 + (double)cuts * (double)M * (double)N * 8e-6 / 4.0;
+            if (us < best * 0.999) {
+                best = us;
+                p.shape = shape;
+                p.splits = (int)cuts;
+                p.tiles_m = (int)tm;
+                p.tiles_n = (int)tn;
+                p.k_split = per * step;
+            }
+        }
     }
-    const int64_t per = (steps + splits - 1) / splits;
-    p.k_split = per * step;
-    p.splits = (int)((steps + per - 1) / per);
     p.stats_blocks = p.splits > 1 ? 1 : p.tiles_n;
     p.partial_bytes = p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
     return p;

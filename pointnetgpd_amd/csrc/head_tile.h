@@ -62,7 +62,11 @@ __device__ __forceinline__ f32x4 mma16(const i32x4& a, const i32x4& b, f32x4 c) 
 __device__ __forceinline__ void stage_load(unsigned lds, unsigned voff, const i32x4& rsrc) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rsrc) : "memory");
 }
-__device__ __forceinline__ void stage_wait() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
+// All but the wave's last AHEAD loads have landed, and its LDS reads; then the barrier.
+template <int AHEAD>
+__device__ __forceinline__ void stage_wait() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(AHEAD) : "memory");
+}
 
 __device__ __forceinline__ i32x4 make_rsrc(const char* p, int bytes) {
     const unsigned long long v = (unsigned long long)p;
@@ -81,7 +85,8 @@ __device__ __forceinline__ void part_begins() { __builtin_amdgcn_sched_barrier(0
 template <typename E, int R, bool KC, int WAVES>
 struct TileOperand {
     static constexpr int SZ = sizeof(E), STEP = 128 / SZ, BYTES = R * 128, PIECES = BYTES / 1024;
-    static constexpr int PER_WAVE = (PIECES + WAVES - 1) / WAVES;
+    static constexpr int PER_WAVE = PIECES / WAVES;
+    static_assert(PIECES % WAVES == 0, "every wave issues as many loads");
     static constexpr int ROW_BYTES = R * SZ;             // of one contraction step, rows dense
     // A wave's pieces are WAVES apart.  Where that distance leaves the permutation as it is, they differ by a uniform number
     // of bytes, which goes into the descriptor: one offset register instead of one a piece.
@@ -130,7 +135,6 @@ struct TileOperand {
         const unsigned last = KC && left < STEP ? 0x80000000u : 0u;
 #pragma unroll
         for (int i = 0; i < PER_WAVE; ++i) {
-            if (PIECES % WAVES != 0 && wave + i * WAVES >= PIECES) break;
             const unsigned skip = UNIFORM ? i * APART * ld : 0;
             unsigned v = voff[UNIFORM ? 0 : i];
             if constexpr (KC) v |= beyond & last;
@@ -302,7 +306,7 @@ inline bool epilogue_vec(const HeadEpilogue& e, int64_t N, size_t sz) {
 // ---- the kernel -------------------------------------------------------------------------------------------------------------
 
 // BM x BN outputs by WM x WN waves; AK / BK: the contraction is dense in the m / n operand
-template <typename E, int BM, int BN, int WM, int WN, bool AK, bool BK, int KIND>
+template <typename E, int BM, int BN, int WM, int WN, bool AK, bool BK, int KIND, int RING>
 __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs g, bool vec) {
     constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, STEP = 128 / (int)sizeof(E);
     constexpr int STAGE = (BM + BN) * 128;
@@ -374,26 +378,33 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
             for (int j = 0; j < H; ++j) acc[i][half * H + j] = mma16<E>(b[i], a[j], acc[i][half * H + j]);
     };
     const unsigned lda = (unsigned)g.lda, ldb = (unsigned)g.ldb;
-    oa.load(pa, lda, left, rows_m, lds0, wave);
-    ob.load(pb, ldb, left, rows_n, lds0 + BM * 128, wave);
+    constexpr int AHEAD = (RING - 2) * (OpA::PER_WAVE + OpB::PER_WAVE);
+    int ahead = left;                      // what is left of the contraction where the next load starts
+    unsigned into = 0, from = 0;           // stages the next load fills and the next step reads
+    const auto load_next = [&]() {
+        oa.load(pa, lda, ahead, rows_m, lds0 + into, wave);
+        ob.load(pb, ldb, ahead, rows_n, lds0 + into + BM * 128, wave);
+        ahead -= STEP;
+        pa += step_a;
+        pb += step_b;
+        into = into == (RING - 1) * STAGE ? 0 : into + STAGE;
+    };
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i) load_next();
     // before the first step the carried part is zeros
 #pragma unroll
     for (int j = 0; j < H; ++j) fa[1][j] = i32x4{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < FN; ++i) fb[1][i] = i32x4{0, 0, 0, 0};
-    unsigned cur = 0;
-    stage_wait();
+    stage_wait<AHEAD>();
     do {
-        // this step's tiles are in LDS, and every wave is done reading the other half
-        const char* sa = smem + cur;
-        cur = STAGE - cur;
+        // this step's tiles are in LDS, and every wave is done reading the stage before it, which the next load fills
+        const char* sa = smem + from;
+        from = from == (RING - 1) * STAGE ? 0 : from + STAGE;
         left -= STEP;
-        pa += step_a;
-        pb += step_b;
         read_b(sa, 0, fb[0]);
         read_a(sa, 0, 0, fa[0]);
-        oa.load(pa, lda, left, rows_m, lds0 + cur, wave);
-        ob.load(pb, ldb, left, rows_n, lds0 + cur + BM * 128, wave);
+        load_next();
         multiply(1, fa[1], fb[1]);
         part_begins();
         read_a(sa, 0, 1, fa[1]);
@@ -406,9 +417,11 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
         read_a(sa, 1, 1, fa[1]);
         multiply(0, fa[0], fb[1]);
         part_begins();
-        stage_wait();
+        stage_wait<AHEAD>();
     } while (left > 0);
     multiply(1, fa[1], fb[1]);
+    // zeros still on their way into LDS must not meet what the epilogue puts there
+    if (AHEAD > 0) asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
 
     const int t = lane & 15, q = lane >> 4;
     if constexpr (KIND == TILE_STATS) {
@@ -490,7 +503,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
     } else {
         // The sums go through LDS, as many rows as it holds at a time, and come back as 8 neighbouring columns a thread: whole
         // lines of memory for the epilogue's loads and stores.  16-byte chunk c of staged row r at slot c ^ (r & 15).
-        constexpr int HOLD = 2 * STAGE / (BN * 4), ROWS = HOLD < BM ? HOLD : BM, PASSES = BM / ROWS, JP = FM / PASSES;
+        constexpr int HOLD = RING * STAGE / (BN * 4), ROWS = HOLD < BM ? HOLD : BM, PASSES = BM / ROWS, JP = FM / PASSES;
         constexpr int MIX = (BN / 4 < 16 ? BN / 4 : 16) - 1, GROUPS = BN / 8;
         constexpr int RSTEP = WAVES * 64 / GROUPS, BATCH = ROWS / RSTEP < 4 ? ROWS / RSTEP : 4;
         static_assert(ROWS * PASSES == BM && JP * PASSES == FM && (WAVES * 64) % GROUPS == 0 && ROWS % (RSTEP * BATCH) == 0, "rows of a pass");
@@ -539,17 +552,17 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------
 
-// tile shapes: 256 x 256 by 8 waves, 128 x 128, 32 x 128 (few rows) and 128 x 32 (few columns) by 4
-enum { SHAPE_256 = 0, SHAPE_128 = 1, SHAPE_FEW_ROWS = 2, SHAPE_FEW_COLS = 3 };
+// tile shapes: 256 x 256 by 8 waves, 128 x 128, 64 x 64, 32 x 128 (few rows) and 128 x 32 (few columns) by 4
+enum { SHAPE_256 = 0, SHAPE_128 = 1, SHAPE_64 = 2, SHAPE_FEW_ROWS = 3, SHAPE_FEW_COLS = 4 };
 inline void shape_size(int shape, int* bm, int* bn) {
-    *bm = shape == SHAPE_256 ? 256 : shape == SHAPE_FEW_ROWS ? 32 : 128;
-    *bn = shape == SHAPE_256 ? 256 : shape == SHAPE_FEW_COLS ? 32 : 128;
+    *bm = shape == SHAPE_256 ? 256 : shape == SHAPE_64 ? 64 : shape == SHAPE_FEW_ROWS ? 32 : 128;
+    *bn = shape == SHAPE_256 ? 256 : shape == SHAPE_64 ? 64 : shape == SHAPE_FEW_COLS ? 32 : 128;
 }
 
-template <typename E, int BM, int BN, int WM, int WN, bool AK, bool BK, int KIND>
+template <typename E, int BM, int BN, int WM, int WN, bool AK, bool BK, int KIND, int RING>
 hipError_t launch_one(const TileArgs& g, bool vec, hipStream_t s) {
-    constexpr int lds = 2 * (BM + BN) * 128;
-    const auto kern = product_tile_kernel<E, BM, BN, WM, WN, AK, BK, KIND>;
+    constexpr int lds = RING * (BM + BN) * 128;
+    const auto kern = product_tile_kernel<E, BM, BN, WM, WN, AK, BK, KIND, RING>;
     if (lds > 65536) {
         const hipError_t e = set_max_lds_once((const void*)kern, lds);
         if (e != hipSuccess) return e;
@@ -563,11 +576,16 @@ hipError_t launch_shape(int shape, const TileArgs& g, bool vec, hipStream_t s) {
     switch (shape) {
         case SHAPE_256:
             // floats need no larger tile than 128: their matrix instructions take eight times as long over what LDS delivers
-            if constexpr (sizeof(E) == 2) return launch_one<E, 256, 256, 2, 4, AK, BK, KIND>(g, vec, s);
+            if constexpr (sizeof(E) == 2) return launch_one<E, 256, 256, 2, 4, AK, BK, KIND, 2>(g, vec, s);
             return hipErrorInvalidValue;
-        case SHAPE_128: return launch_one<E, 128, 128, 2, 2, AK, BK, KIND>(g, vec, s);
-        case SHAPE_FEW_ROWS: return launch_one<E, 32, 128, 1, 4, AK, BK, KIND>(g, vec, s);
-        default: return launch_one<E, 128, 32, 4, 1, AK, BK, KIND>(g, vec, s);
+        case SHAPE_128:
+            // alone on its compute unit a tile waits for its loads: one more stage (0.65 instead of 0.90 us a step); two to a
+            // unit cover each other and would not fit with three stages
+            if (sizeof(E) == 2 && g.tiles_m * g.tiles_n * g.splits <= 256) return launch_one<E, 128, 128, 2, 2, AK, BK, KIND, 3>(g, vec, s);
+            return launch_one<E, 128, 128, 2, 2, AK, BK, KIND, 2>(g, vec, s);
+        case SHAPE_64: return launch_one<E, 64, 64, 2, 2, AK, BK, KIND, 3>(g, vec, s);
+        case SHAPE_FEW_ROWS: return launch_one<E, 32, 128, 1, 4, AK, BK, KIND, 3>(g, vec, s);
+        default: return launch_one<E, 128, 32, 4, 1, AK, BK, KIND, 3>(g, vec, s);
     }
 }
 
