@@ -28,23 +28,31 @@ _ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
-def _require(x, name, like=None, shape=None):
+def _refuse(x, name, like, shape):
+    """Raises what is wrong with an argument that `_fits` does not take."""
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name}: expected a tensor, got {type(x).__name__}")
     if not x.is_cuda:
         raise RuntimeError(f"{name} is on {x.device}: pointnetgpd_amd runs on MI355X only (there is no CPU path)")
     if x.layout != torch.strided:
         raise TypeError(f"{name}: expected a dense tensor, got layout {x.layout}")
-    if like is None:
-        if x.dtype not in _TYPES:
-            raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {x.dtype}")
-    else:
-        if x.device != like.device:
-            raise RuntimeError(f"{name} is on {x.device}, the input on {like.device}")
-        if x.dtype != like.dtype:
-            raise TypeError(f"{name} is {x.dtype}, the input {like.dtype}")
-    if shape is not None and tuple(x.shape) != tuple(shape):
-        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(x.shape)}")
+    if x.dtype not in _TYPES:
+        raise TypeError(f"{name}: expected float32, bfloat16 or float16, got {x.dtype}")
+    if like is not None and x.device != like.device:
+        raise RuntimeError(f"{name} is on {x.device}, the input on {like.device}")
+    if like is not None and x.dtype != like.dtype:
+        raise TypeError(f"{name} is {x.dtype}, the input {like.dtype}")
+    raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(x.shape)}")
+
+
+def _fits(x, like=None, shape=None):
+    return isinstance(x, torch.Tensor) and x.is_cuda and x.layout == torch.strided and x.dtype in _TYPES and \
+        (like is None or (x.dtype == like.dtype and x.device == like.device)) and (shape is None or x.shape == shape)
+
+
+def _require(x, name, like=None, shape=None):
+    if not _fits(x, like, shape):
+        _refuse(x, name, like, shape)
 
 
 def _rows(t, cols):
@@ -61,13 +69,9 @@ def _rows(t, cols):
     return t2.contiguous(), cols
 
 
-def _count(t, cols):
-    return t.numel() // cols
-
-
-def _aligned(size, *matrices):
-    """Whether all (tensor, distance of rows) start at 16-byte addresses with rows of whole 16-byte chunks apart."""
-    return int(all(t.data_ptr() % 16 == 0 and ld * size % 16 == 0 and ld * size <= 1 << 23 for t, ld in matrices))
+def _aligned(t, ld, size):
+    """Whether rows start at 16-byte addresses, whole 16-byte chunks and at most 2^23 bytes apart."""
+    return t.data_ptr() % 16 == 0 and ld * size % 16 == 0 and ld * size <= 1 << 23
 
 
 def _vector(t):
@@ -78,50 +82,56 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(nbytes, dev):
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-
-
-# the stream's handle without a Stream object around it; torch.cuda.device / current_stream cost more than a small kernel's
-# launch, above all when the forward pass (the caller's thread) and the backward pass (autograd's) take turns in them
+# Handles without Python objects around them: torch.cuda.device / current_stream cost more than a small kernel's launch, above
+# all when the forward pass (the caller's thread) and the backward pass (autograd's) take turns in them.
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-class _OnDevice:
-    """Makes a device the current one for the calls inside, if it is not."""
-    __slots__ = ("index", "before")
-
-    def __init__(self, index):
-        self.index = index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return _raw_stream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _call(fn, t, *args):
+    """fn(*args, stream) on t's device and its current stream."""
+    index = t.get_device()
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc)
 
 
 @functools.lru_cache(maxsize=4096)
-def _linear_bytes(*sizes):
-    return _lib.load().pngpd_linear_workspace_bytes(*sizes)
+def _linear_bytes(kind, M, N, K, backward, aligned):
+    return _lib.load().pngpd_linear_workspace_bytes(kind, M, N, K, backward, aligned)
 
 
 @functools.lru_cache(maxsize=4096)
-def _loss_bytes(*sizes):
-    return _lib.load().pngpd_linear_cross_entropy_workspace_bytes(*sizes)
+def _loss_bytes(kind, T, V, D, backward, aligned):
+    return _lib.load().pngpd_linear_cross_entropy_workspace_bytes(kind, T, V, D, backward, aligned)
+
+
+def _workspace(nbytes, like):
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def _conj_free(*tensors):
-    return [t.resolve_neg() if t is not None and t.is_neg() else t for t in tensors]
+def _plain(t):
+    """Without a pending negation (a lazy view of a complex tensor's part)."""
+    return t.resolve_neg() if t is not None and t.is_neg() else t
+
+
+def _once(backward):
+    """once_differentiable, whose wrapper is skipped where no graph of the gradient is asked for."""
+    wrapped = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return wrapped(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
 
 
 # ---- linear ---------------------------------------------------------------------------------------------------------------
@@ -131,17 +141,16 @@ def _linear_forward(x, weight, bias, residual, act, keep):
     N, K = weight.shape
     x2, ldx = _rows(x, K)
     w2, ldw = _rows(weight, K)
-    M = _count(x, K)
-    dev, kind = x.device, _TYPES[x.dtype]
-    y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=dev)
-    z = torch.empty((M, N), dtype=x.dtype, device=dev) if keep and act else None
-    r2, ldr = _rows(residual, N) if residual is not None else (None, N)
+    M = x.numel() // K
+    kind, size = _TYPES[x.dtype], x.element_size()
+    y = x.new_empty(x.shape[:-1] + (N,))
+    z = x.new_empty((M, N)) if keep and act else None
+    r2, ldr = (None, N) if residual is None else _rows(residual, N)
     b = _vector(bias)
-    nbytes = _linear_bytes(kind, M, N, K, 0, _aligned(x.element_size(), (x2, ldx), (w2, ldw)))
-    with _OnDevice(dev.index) as stream:
-        ws = _workspace(nbytes, dev)
-        _lib.check(lib.pngpd_linear_forward(kind, M, N, K, _ptr(x2), ldx, _ptr(w2), ldw, _ptr(b), act, _ptr(r2), ldr, _ptr(y),
-                                            _ptr(z), _ptr(ws), nbytes, stream))
+    nbytes = _linear_bytes(kind, M, N, K, 0, _aligned(x2, ldx, size) and _aligned(w2, ldw, size))
+    ws = _workspace(nbytes, x)
+    _call(lib.pngpd_linear_forward, x, kind, M, N, K, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b), act, _ptr(r2), ldr,
+          y.data_ptr(), _ptr(z), _ptr(ws), nbytes)
     return y, z
 
 
@@ -150,35 +159,34 @@ class LinearFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        y, z = _linear_forward(x, weight, bias, residual, act, any(ctx.needs_input_grad[:3]))
+        need = ctx.needs_input_grad
+        y, z = _linear_forward(x, weight, bias, residual, act, need[0] or need[1] or need[2])
         ctx.act = act
         ctx.save_for_backward(x, weight, z)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         lib = _lib.load()
         x, weight, z = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dy, = _conj_free(dy)
+        dy = _plain(dy)
         if not (need_x or need_w or need_b):
             return None, None, None, dy if need_r else None, None
         N, K = weight.shape
-        dev, kind = x.device, _TYPES[x.dtype]
         x2, ldx = _rows(x, K)
         w2, ldw = _rows(weight, K)
         d2, ld_dy = _rows(dy, N)
-        M = _count(x, K)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty((N, K), dtype=x.dtype, device=dev) if need_w else None
-        db = torch.empty(N, dtype=x.dtype, device=dev) if need_b else None
-        nbytes = _linear_bytes(kind, M, N, K, 1,
-                                                  _aligned(x.element_size(), (x2, ldx), (w2, ldw), (d2, ld_dy)))
-        with _OnDevice(dev.index) as stream:
-            ws = _workspace(nbytes, dev)
-            _lib.check(lib.pngpd_linear_backward(kind, M, N, K, _ptr(d2), ld_dy, _ptr(z), _ptr(x2), ldx, _ptr(w2), ldw, ctx.act,
-                                                 _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, stream))
+        M = x.numel() // K
+        kind, size = _TYPES[x.dtype], x.element_size()
+        dx = x.new_empty(x.shape) if need_x else None
+        dw = x.new_empty((N, K)) if need_w else None
+        db = x.new_empty(N) if need_b else None
+        nbytes = _linear_bytes(kind, M, N, K, 1, _aligned(x2, ldx, size) and _aligned(w2, ldw, size) and _aligned(d2, ld_dy, size))
+        ws = _workspace(nbytes, x)
+        _call(lib.pngpd_linear_backward, x, kind, M, N, K, d2.data_ptr(), ld_dy, _ptr(z), x2.data_ptr(), ldx, w2.data_ptr(), ldw,
+              ctx.act, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
         return dx, dw, db, dy if need_r else None, None
 
 
@@ -200,7 +208,7 @@ def linear(x, weight, bias=None, activation=None, residual=None):
         _require(bias, "bias", x, (N,))
     if residual is not None:
         _require(residual, "residual", x, x.shape[:-1] + (N,))
-    x, weight, bias, residual = _conj_free(x, weight, bias, residual)
+    x, weight, bias, residual = _plain(x), _plain(weight), _plain(bias), _plain(residual)
     act = _ACTIVATIONS[activation]
     if _wants_grad(x, weight, bias, residual):
         return LinearFunction.apply(x, weight, bias, residual, act)
@@ -211,20 +219,17 @@ def linear(x, weight, bias=None, activation=None, residual=None):
 
 def _dropout_call(x, residual, p, seed, offset, rng):
     lib = _lib.load()
-    dev = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    if x.numel() == 0:
-        return y
+    n = x.numel()
     cols = x.shape[-1] if x.dim() else 1
     if x.is_contiguous() and (residual is None or residual.is_contiguous()):
-        # one long row would pass the size limit: the rows stay those of the tensor
         x2, ldx, r2, ldr = x, cols, residual, cols
     else:
         x2, ldx = _rows(x, cols)
-        r2, ldr = _rows(residual, cols) if residual is not None else (None, cols)
-    with _OnDevice(dev.index) as stream:
-        _lib.check(lib.pngpd_dropout(_TYPES[x.dtype], x.numel() // cols, cols, _ptr(x2), ldx, _ptr(r2), ldr, _ptr(y), p, seed,
-                                     offset, _ptr(rng), stream))
+        r2, ldr = (None, cols) if residual is None else _rows(residual, cols)
+    y = x.new_empty(x.shape)
+    if n:
+        _call(lib.pngpd_dropout, x, _TYPES[x.dtype], n // cols, cols, x2.data_ptr(), ldx, _ptr(r2), ldr, y.data_ptr(), p, seed,
+              offset, _ptr(rng))
     return y
 
 
@@ -234,16 +239,18 @@ class DropoutFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, offset, rng):
         ctx.args = (p, seed, offset)
-        ctx.save_for_backward(rng)
+        if rng is not None:
+            ctx.save_for_backward(rng)
         return _dropout_call(x, residual, p, seed, offset, rng)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        rng, = ctx.saved_tensors
-        dy, = _conj_free(dy)
-        dx = _dropout_call(dy, None, *ctx.args, rng) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None
+        saved = ctx.saved_tensors
+        dy = _plain(dy)
+        need_x, need_r = ctx.needs_input_grad[:2]
+        dx = _dropout_call(dy, None, *ctx.args, saved[0] if saved else None) if need_x else None
+        return dx, dy if need_r else None, None, None, None, None
 
 
 def dropout(x, p, seed, offset=0, residual=None):
@@ -267,13 +274,30 @@ def dropout(x, p, seed, offset=0, residual=None):
             raise ValueError("offset: the seed tensor holds it")
         rng, seed = seed, 0
     seed, offset = int(seed) & (2 ** 64 - 1), int(offset) & (2 ** 64 - 1)
-    x, residual = _conj_free(x, residual)
+    x, residual = _plain(x), _plain(residual)
     if _wants_grad(x, residual):
         return DropoutFunction.apply(x, residual, p, seed, offset, rng)
     return _dropout_call(x, residual, p, seed, offset, rng)
 
 
 # ---- linear + cross entropy -----------------------------------------------------------------------------------------------
+
+def _loss_forward(x, weight, bias, target, ignore_index, label_smoothing, reduction):
+    lib = _lib.load()
+    V, D = weight.shape
+    x2, ldx = _rows(x, D)
+    w2, ldw = _rows(weight, D)
+    T = x.numel() // D
+    kind, size = _TYPES[x.dtype], x.element_size()
+    loss = torch.empty(x.shape[:-1] if reduction == 0 else (), dtype=torch.float32, device=x.device)
+    lse = torch.empty(T, dtype=torch.float32, device=x.device)
+    b = _vector(bias)
+    nbytes = _loss_bytes(kind, T, V, D, 0, _aligned(x2, ldx, size) and _aligned(w2, ldw, size))
+    ws = _workspace(nbytes, x)
+    _call(lib.pngpd_linear_cross_entropy_forward, x, kind, T, V, D, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b),
+          target.data_ptr(), ignore_index, label_smoothing, reduction, loss.data_ptr(), lse.data_ptr(), _ptr(ws), nbytes)
+    return loss, lse
+
 
 class LinearCrossEntropyFunction(torch.autograd.Function):
     """autograd bridge of `linear_cross_entropy`: pngpd_linear_cross_entropy_forward / _backward."""
@@ -286,50 +310,26 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dloss):
         lib = _lib.load()
         x, weight, bias, target, lse = ctx.saved_tensors
-        ignore_index, label_smoothing, reduction = ctx.args
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         V, D = weight.shape
-        dev, kind = x.device, _TYPES[x.dtype]
         x2, ldx = _rows(x, D)
         w2, ldw = _rows(weight, D)
-        T = _count(x, D)
-        dloss = _conj_free(dloss)[0].to(torch.float32).contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty((V, D), dtype=x.dtype, device=dev) if need_w else None
-        db = torch.empty(V, dtype=x.dtype, device=dev) if need_b else None
-        nbytes = _loss_bytes(
-            kind, T, V, D, 1, _aligned(x.element_size(), (x2, ldx), (w2, ldw)))
+        T = x.numel() // D
+        kind, size = _TYPES[x.dtype], x.element_size()
+        dloss = _plain(dloss).contiguous()
+        dx = x.new_empty(x.shape) if need_x else None
+        dw = x.new_empty((V, D)) if need_w else None
+        db = x.new_empty(V) if need_b else None
         b = _vector(bias)
-        with _OnDevice(dev.index) as stream:
-            ws = _workspace(nbytes, dev)
-            _lib.check(lib.pngpd_linear_cross_entropy_backward(
-                kind, T, V, D, _ptr(x2), ldx, _ptr(w2), ldw, _ptr(b), _ptr(target), ignore_index, label_smoothing, reduction,
-                _ptr(lse), _ptr(dloss), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, stream))
+        nbytes = _loss_bytes(kind, T, V, D, 1, _aligned(x2, ldx, size) and _aligned(w2, ldw, size))
+        ws = _workspace(nbytes, x)
+        _call(lib.pngpd_linear_cross_entropy_backward, x, kind, T, V, D, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _ptr(b),
+              target.data_ptr(), *ctx.args, lse.data_ptr(), dloss.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
         return dx, dw, db, None, None, None, None
-
-
-def _loss_forward(x, weight, bias, target, ignore_index, label_smoothing, reduction):
-    lib = _lib.load()
-    V, D = weight.shape
-    dev, kind = x.device, _TYPES[x.dtype]
-    x2, ldx = _rows(x, D)
-    w2, ldw = _rows(weight, D)
-    T = _count(x, D)
-    loss = torch.empty(x.shape[:-1] if reduction == 0 else (), dtype=torch.float32, device=dev)
-    lse = torch.empty(T, dtype=torch.float32, device=dev)
-    nbytes = _loss_bytes(
-        kind, T, V, D, 0, _aligned(x.element_size(), (x2, ldx), (w2, ldw)))
-    b = _vector(bias)
-    with _OnDevice(dev.index) as stream:
-        ws = _workspace(nbytes, dev)
-        _lib.check(lib.pngpd_linear_cross_entropy_forward(kind, T, V, D, _ptr(x2), ldx, _ptr(w2), ldw, _ptr(b), _ptr(target),
-                                                          ignore_index, label_smoothing, reduction, _ptr(loss), _ptr(lse),
-                                                          _ptr(ws), nbytes, stream))
-    return loss, lse
 
 
 def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
@@ -355,13 +355,15 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, label_
         raise TypeError("target: expected a tensor of whole numbers")
     if target.device != x.device:
         raise RuntimeError(f"target is on {target.device}, the input on {x.device}")
-    if tuple(target.shape) != tuple(x.shape[:-1]):
+    if target.shape != x.shape[:-1]:
         raise ValueError(f"target: expected shape {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
     label_smoothing = float(label_smoothing)
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"label_smoothing: expected a number in [0, 1], got {label_smoothing}")
-    target = target.detach().to(torch.int64).contiguous()
-    x, weight, bias = _conj_free(x, weight, bias)
+    if target.dtype != torch.int64:
+        target = target.to(torch.int64)
+    target = _vector(target)
+    x, weight, bias = _plain(x), _plain(weight), _plain(bias)
     args = (int(ignore_index), label_smoothing, _REDUCTIONS[reduction])
     if _wants_grad(x, weight, bias):
         return LinearCrossEntropyFunction.apply(x, weight, bias, target, *args)
