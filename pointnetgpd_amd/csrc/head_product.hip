@@ -10,15 +10,16 @@ namespace {
 // ---- joining partial sums --------------------------------------------------------------------------------------------------------
 
 // 8 neighbouring columns of a row a thread: the cuts of the contraction added in order, then the epilogue
-template <typename E, int KIND>
-__global__ __launch_bounds__(256) void join_kernel(int64_t M, int64_t N, int64_t groups, int splits, const float* partial, HeadEpilogue e,
+template <typename E, int KIND, int THREADS>
+__global__ __launch_bounds__(THREADS) void join_kernel(int64_t M, int64_t N, int64_t groups, int splits, const float* partial, HeadEpilogue e,
                                                    bool vec, bool partial_vec) {
     const int64_t total = M * groups;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * THREADS) {
         const int64_t m = i / groups, n = (i - m * groups) * 8;
         const int64_t have = N - n;
         const int valid = (int)(have < 0 ? 0 : have < 8 ? have : 8);
         Eight v = {};
+#pragma unroll 4
         for (int s = 0; s < splits; ++s) add8(v, load8(partial + ((int64_t)s * M + m) * N + n, valid, partial_vec));
         const int64_t room = (KIND == TILE_DZ ? e.ld_out : N) - n;
         const int real = (int)(room < 8 ? room : 8);
@@ -66,20 +67,113 @@ template <typename E>
 hipError_t join(int64_t M, int64_t N, int splits, const float* partial, const HeadEpilogue& e, hipStream_t s) {
     const bool vec = epilogue_vec(e, N, sizeof(E)), pv = N % 4 == 0;
     const int64_t groups = ((e.kind == HEAD_EPI_DZ ? e.ld_out : N) + 7) / 8;
-    const int64_t blocks = (M * groups + 255) / 256;
+    // little to join: small workgroups, so that its loads leave from many compute units
+    const bool few = M * groups < 65536;
+    const int64_t threads = few ? 64 : 256, blocks = (M * groups + threads - 1) / threads;
     const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
+#define PNGPD_JOIN(KIND)                                                                                          \
+    if (few) join_kernel<E, KIND, 64><<<grid, 64, 0, s>>>(M, N, groups, splits, partial, e, vec, pv);              \
+    else join_kernel<E, KIND, 256><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e, vec, pv)
     switch (e.kind) {
-        case HEAD_EPI_LINEAR: join_kernel<E, TILE_LINEAR><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e, vec, pv); break;
-        case HEAD_EPI_DZ: join_kernel<E, TILE_DZ><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e, vec, pv); break;
-        case HEAD_EPI_SCALED: join_kernel<E, TILE_SCALED><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e, vec, pv); break;
+        case HEAD_EPI_LINEAR: PNGPD_JOIN(TILE_LINEAR); break;
+        case HEAD_EPI_DZ: PNGPD_JOIN(TILE_DZ); break;
+        case HEAD_EPI_SCALED: PNGPD_JOIN(TILE_SCALED); break;
         default: join_stats_kernel<E><<<(unsigned)M, 256, 0, s>>>(M, N, splits, partial, e);
     }
+#undef PNGPD_JOIN
+    return hipGetLastError();
+}
+
+// ---- one to four rows -----------------------------------------------------------------------------------------------------------
+
+// y[m][n] for up to MR rows m: a wave takes NR rows of the weight, its lanes 16-byte chunks of them side by side, and adds its
+// lanes' 32-bit fma chains at the end.  Bound by reading the weight once: 4096 x 4096 bf16 (33.5 MB) for one row.
+constexpr int FEW_M = 4;
+
+template <typename E, int MR, int NR>
+__global__ __launch_bounds__(256) void rows_kernel(int M, int64_t N, int64_t chunks, const E* x, int64_t ldx, const E* w, int64_t ldw,
+                                                   HeadEpilogue e) {
+    constexpr int C = 16 / sizeof(E), U = MR * NR > 8 ? 2 : 4;
+    typedef __attribute__((ext_vector_type(16 / sizeof(E)))) E chunk;
+    const int lane = threadIdx.x & 63;
+    const int64_t n0 = ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * NR;
+    if (n0 >= N) return;
+    const E *px[MR], *pw[NR];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) px[m] = x + (m < M ? m : 0) * ldx;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) pw[r] = w + (n0 + r < N ? n0 + r : n0) * ldw;
+    float acc[MR][NR] = {};
+    int64_t c = lane;
+    for (; c + (U - 1) * 64 < chunks; c += U * 64) {
+        chunk a[U][MR], b[U][NR];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int r = 0; r < NR; ++r) b[u][r] = ((const chunk*)pw[r])[c + u * 64];
+#pragma unroll
+            for (int m = 0; m < MR; ++m) a[u][m] = ((const chunk*)px[m])[c + u * 64];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+#pragma unroll
+                for (int m = 0; m < MR; ++m)
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) acc[m][r] = __builtin_fmaf((float)a[u][m][i], (float)b[u][r][i], acc[m][r]);
+    }
+    for (; c < chunks; c += 64) {
+        chunk a[MR], b[NR];
+#pragma unroll
+        for (int r = 0; r < NR; ++r) b[r] = ((const chunk*)pw[r])[c];
+#pragma unroll
+        for (int m = 0; m < MR; ++m) a[m] = ((const chunk*)px[m])[c];
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+#pragma unroll
+            for (int m = 0; m < MR; ++m)
+#pragma unroll
+                for (int r = 0; r < NR; ++r) acc[m][r] = __builtin_fmaf((float)a[m][i], (float)b[r][i], acc[m][r]);
+    }
+    float mine = 0.f;
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            const float v = wave_sum(acc[m][r]);
+            if (lane == m * NR + r) mine = v;
+        }
+    const int m = lane / NR;
+    const int64_t n = n0 + lane % NR;
+    if (lane >= MR * NR || m >= M || n >= N) return;
+    const Columns col = load_columns<E, TILE_LINEAR>(e, n + 1, n, false);
+    Eight v = {{mine}};
+    finish8<E, TILE_LINEAR>(e, N, m, n, 1, false, col, load_ahead<E, TILE_LINEAR>(e, N, m, n, 1, false), v);
+}
+
+template <typename E, int MR>
+hipError_t rows(int M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b, const HeadEpilogue& e, hipStream_t s) {
+    constexpr int C = 16 / sizeof(E);
+    const int64_t chunks = (K + C - 1) / C;
+    // four rows of the weight a wave once that leaves a wave for every SIMD
+#define PNGPD_ROWS(NR) \
+    rows_kernel<E, MR, NR><<<(unsigned)((N + 4 * NR - 1) / (4 * NR)), 256, 0, s>>>(M, N, chunks, (const E*)a.p, a.ld, (const E*)b.p, b.ld, e)
+    if (N >= 4096) PNGPD_ROWS(4);
+    else if (N >= 2048) PNGPD_ROWS(2);
+    else PNGPD_ROWS(1);
+#undef PNGPD_ROWS
     return hipGetLastError();
 }
 
 template <typename E>
 hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b, const HeadEpilogue& e,
                    float* partial, hipStream_t s) {
+    if (M <= FEW_M && e.kind == HEAD_EPI_LINEAR) {
+        if (M == 1) return rows<E, 1>((int)M, N, K, a, b, e, s);
+        if (M == 2) return rows<E, 2>((int)M, N, K, a, b, e, s);
+        return rows<E, 4>((int)M, N, K, a, b, e, s);
+    }
     const HeadPlan p = head_plan(type, M, N, K, e.kind);
     TileArgs g{};
     g.M = M;
@@ -301,10 +395,10 @@ double tile_us(int shape) { return shape == SHAPE_256 ? 11.0 : shape == SHAPE_12
 // The shape, and the number of cuts of the contraction, that should take the least time.  A cut contraction costs the
 // joining kernel's 4 us and its traffic (32-bit sums written and read, at some 4 TB/s).
 HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
-    (void)kind;
     const bool f32 = type == PNGPD_TYPE_F32;
     const int64_t step = f32 ? 32 : 64, steps = (K + step - 1) / step;
     HeadPlan p{};
+    if (M <= FEW_M && kind == HEAD_EPI_LINEAR) return p;      // rows_kernel, nothing to join
     double best = 1e300;
     for (int shape = SHAPE_256; shape <= SHAPE_FEW_COLS; ++shape) {
         if (f32 && shape == SHAPE_256) continue;
