@@ -378,7 +378,7 @@ int pngpd_adam_step(float* params_dev, const float* grads_dev, float* exp_avg_de
  * Matrices are row-major; ld* is the distance of two rows in elements (at least the row's length), and a matrix
  * without an ld argument is dense.  `type` is the element type of every matrix and bias; sums and statistics are
  * 32-bit (64-bit over a batch's losses).  Outputs must not overlap inputs or each other.  Sizes: 0 <= rows < 2^31,
- * 1 <= N, K, D <= 2^21, 1 <= V < 2^31, T V <= 2^44.  A call with no rows still writes the outputs that do not depend on
+ * 1 <= N, K, D <= 2^21, 1 <= V <= 2^24.  A call with no rows still writes the outputs that do not depend on
  * rows (zero gradients).  All calls are stream-ordered, allocate nothing and can be captured into a graph; two calls
  * that may run at the same time need workspaces of their own.
  *

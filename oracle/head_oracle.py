@@ -96,13 +96,17 @@ def mix64(v):
         return v ^ (v >> np.uint64(31))
 
 
-def keep_mask(n, p, seed, offset):
-    """Which of n elements dropout keeps (bool, numpy)."""
+def keep_mask_at(first, n, p, seed, offset):
+    """Which of the n elements from `first` on (an even one) dropout keeps (bool, numpy)."""
     with np.errstate(over="ignore"):
         key = mix64(np.uint64(seed % 2 ** 64) ^ mix64(np.uint64(offset % 2 ** 64)))
-        word = mix64(key + np.arange((n + 1) // 2, dtype=np.uint64))
+        word = mix64(key + np.arange(first // 2, first // 2 + (n + 1) // 2, dtype=np.uint64))
     draw = np.stack([word & np.uint64(0xFFFFFFFF), word >> np.uint64(32)], axis=1).reshape(-1)[:n]
     return draw >= np.uint64(int(round(p * 2 ** 32)))
+
+
+def keep_mask(n, p, seed, offset):
+    return keep_mask_at(0, n, p, seed, offset)
 
 
 def dropout(x, p, seed, offset, r):

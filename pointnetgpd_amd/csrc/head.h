@@ -87,11 +87,11 @@ hipError_t head_dropout(int type, int64_t rows, int64_t cols, const void* x, int
                         int64_t ldr, void* y, double p, uint64_t seed, uint64_t offset, const int64_t* rng_dev,
                         hipStream_t s);
 
-// lse[t] and the loss of every row from its statistics; the batch's loss into `loss` (row_loss then is scratch), or the
-// rows' (reduction none: row_loss == loss)
-hipError_t head_loss_finish(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit,
-                            const int64_t* target, int64_t ignore_index, float eps, int reduction, float* row_loss, float* loss,
-                            float* lse, hipStream_t s);
+// lse[t] and the loss of every row from its statistics; the batch's loss from its rows'
+hipError_t head_row_loss(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit, const int64_t* target,
+                         int64_t ignore_index, float eps, float* row_loss, float* lse, hipStream_t s);
+hipError_t head_batch_loss(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore_index, int reduction, float* loss,
+                           hipStream_t s);
 // row_weight[t] = weight of row t in the gradient divided by 2^e, out_scale[0] = 2^e (type f16 only, else 2^e = 1)
 hipError_t head_row_weights(int type, int64_t T, int64_t V, const int64_t* target, int64_t ignore_index, int reduction,
                             const float* dloss, float* row_weight, float* out_scale, hipStream_t s);

@@ -12,7 +12,9 @@ using pngpd::HeadEpilogue;
 using pngpd::HeadOperand;
 
 constexpr int64_t MAX_SIZE = 2147483647;
-constexpr size_t PIECE_BYTES = (size_t)256 << 20;      // of the logits' gradients at a time
+constexpr int64_t MAX_CLASSES = (int64_t)1 << 24;
+constexpr size_t PIECE_BYTES = (size_t)256 << 20;      // of the logits' gradients at a time, or as much as x and weight take
+constexpr size_t STATS_BYTES = (size_t)256 << 20;      // of rows' statistics at a time
 
 inline size_t esize(int type) { return type == PNGPD_TYPE_F32 ? 4 : 2; }
 inline bool type_ok(int type) { return type >= PNGPD_TYPE_F32 && type <= PNGPD_TYPE_F16; }
@@ -107,6 +109,7 @@ struct LinearWs {
 };
 
 struct LossWs {
+    int64_t rows_at_once;      // rows whose statistics are formed at a time (forward)
     int64_t piece;             // columns of the vocabulary whose gradients are formed at a time
     void *x, *w, *tile;        // laid out; gradients of a piece's logits, [T][padded(piece)]
     float4* stats;
@@ -122,14 +125,28 @@ struct LossWs {
         stats = nullptr;
         target_logit = row_loss = row_weight = scale = part = dx_sum = partial = nullptr;
         piece = V;
+        rows_at_once = rows;
         if (!backward) {
-            const pngpd::HeadPlan p = pngpd::head_plan(type, rows, V, D, pngpd::HEAD_EPI_STATS);
-            stats = (float4*)b.take((size_t)p.stats_blocks * rows * sizeof(float4));
+            // 64 columns a block at least; a product of 2^34 elements stays inside a grid
+            int64_t at_once = (int64_t)(STATS_BYTES / sizeof(float4)) / ((V + 63) / 64) / 256 * 256;
+            const int64_t most = ((int64_t)1 << 34) / V / 256 * 256;
+            if (at_once > most) at_once = most;
+            if (at_once < 256) at_once = 256;
+            rows_at_once = rows < at_once ? rows : at_once;
+            const int64_t last = rows % rows_at_once ? rows % rows_at_once : rows_at_once;
+            size_t cut = 0, blocks = 0;
+            for (int64_t n : {rows_at_once, last}) {
+                const pngpd::HeadPlan p = pngpd::head_plan(type, n, V, D, pngpd::HEAD_EPI_STATS);
+                blocks = max2(blocks, (size_t)p.stats_blocks * n);
+                cut = max2(cut, p.partial_bytes);
+            }
+            stats = (float4*)b.take(blocks * sizeof(float4));
             target_logit = (float*)b.take((size_t)rows * 4);
             row_loss = (float*)b.take((size_t)rows * 4);
-            partial = (float*)b.take(p.partial_bytes);
+            partial = (float*)b.take(cut);
         } else {
-            piece = (int64_t)(PIECE_BYTES / ((size_t)rows * e)) / 256 * 256;
+            const size_t budget = max2(PIECE_BYTES, ((size_t)rows + (size_t)V) * (size_t)D * e);
+            piece = (int64_t)(budget / ((size_t)rows * e)) / 256 * 256;
             if (piece < 256) piece = 256;
             if (piece > pngpd::HEAD_MAX_EXTENT) piece = pngpd::HEAD_MAX_EXTENT;
             if (piece > V) piece = V;
@@ -156,7 +173,7 @@ int check_loss(const char* who, int type, int64_t T, int64_t V, int64_t D, const
     int rc = check_sizes(who, type, T, V, D);
     if (rc) return rc;
     if (D > pngpd::HEAD_MAX_EXTENT) return fail(PNGPD_ERR_SHAPE, "%s: D = %lld, at most %lld", who, (long long)D, (long long)pngpd::HEAD_MAX_EXTENT);
-    if ((double)T * (double)V > 17592186044416.0) return fail(PNGPD_ERR_SHAPE, "%s: T x V beyond 2^44", who);
+    if (V > MAX_CLASSES) return fail(PNGPD_ERR_SHAPE, "%s: V = %lld, at most %lld", who, (long long)V, (long long)MAX_CLASSES);
     if (!w || (T > 0 && (!x || !target))) return fail(PNGPD_ERR_INVALID, "%s: NULL argument", who);
     if ((rc = check_ld(who, "ldx", ldx, D)) || (rc = check_ld(who, "ldw", ldw, D))) return rc;
     if (!(eps >= 0.f && eps <= 1.f)) return fail(PNGPD_ERR_INVALID, "%s: label_smoothing %g", who, (double)eps);
@@ -289,20 +306,24 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
         Rows x, w;
         HIP_TRY(direct_rows(type, T, D, x_dev, ldx, ws.x, s, &x));
         HIP_TRY(direct_rows(type, V, D, weight_dev, ldw, ws.w, s, &w));
-        HeadEpilogue e;
-        e.kind = pngpd::HEAD_EPI_STATS;
-        e.bias = bias_dev;
-        e.target = target_dev;
-        e.stats = ws.stats;
-        e.target_logit = ws.target_logit;
-        e.want_logit_sum = label_smoothing > 0.f;
-        HIP_TRY(pngpd::head_product(type, T, V, D, HeadOperand{x.p, x.ld, true}, HeadOperand{w.p, w.ld, true}, e, ws.partial, s));
-    } else if (reduction == PNGPD_REDUCE_NONE) {
-        return PNGPD_OK;
+        float* row_loss = reduction == PNGPD_REDUCE_NONE ? loss_dev : ws.row_loss;
+        for (int64_t t = 0; t < T; t += ws.rows_at_once) {
+            const int64_t n = T - t < ws.rows_at_once ? T - t : ws.rows_at_once;
+            HeadEpilogue e;
+            e.kind = pngpd::HEAD_EPI_STATS;
+            e.bias = bias_dev;
+            e.target = target_dev + t;
+            e.stats = ws.stats;
+            e.target_logit = ws.target_logit;
+            e.want_logit_sum = label_smoothing > 0.f;
+            HIP_TRY(pngpd::head_product(type, n, V, D, HeadOperand{at(x.p, t * x.ld, type), x.ld, true}, HeadOperand{w.p, w.ld, true}, e,
+                                        ws.partial, s));
+            const int blocks = pngpd::head_plan(type, n, V, D, pngpd::HEAD_EPI_STATS).stats_blocks;
+            HIP_TRY(pngpd::head_row_loss(n, V, blocks, ws.stats, ws.target_logit, target_dev + t, ignore_index, label_smoothing,
+                                         row_loss + t, lse_dev + t, s));
+        }
     }
-    const int blocks = T > 0 ? pngpd::head_plan(type, T, V, D, pngpd::HEAD_EPI_STATS).stats_blocks : 0;
-    HIP_TRY(pngpd::head_loss_finish(T, V, blocks, ws.stats, ws.target_logit, target_dev, ignore_index, label_smoothing, reduction,
-                                    reduction == PNGPD_REDUCE_NONE ? loss_dev : ws.row_loss, loss_dev, lse_dev, s));
+    if (reduction != PNGPD_REDUCE_NONE) HIP_TRY(pngpd::head_batch_loss(T, ws.row_loss, target_dev, ignore_index, reduction, loss_dev, s));
     return PNGPD_OK;
 }
 

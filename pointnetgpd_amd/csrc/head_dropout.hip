@@ -40,11 +40,8 @@ struct Eight {
 
 // DENSE: x and the residual are one run of memory as y is, all 16-byte aligned
 template <typename T, bool DENSE, bool RESIDUAL>
-__global__ __launch_bounds__(256) void dropout_kernel(int64_t total, int64_t cols, const T* x, int64_t ldx, const T* r, int64_t ldr,
-                                                      T* y, unsigned long long border, float scale, unsigned long long seed,
-                                                      unsigned long long offset, const int64_t* rng, bool y_aligned) {
-    const int64_t i0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * PER_THREAD;
-    if (i0 >= total) return;
+__device__ __forceinline__ void dropout_eight(int64_t i0, int64_t total, int64_t cols, const T* x, int64_t ldx, const T* r, int64_t ldr,
+                                              T* y, unsigned long long border, float scale, unsigned long long key, bool y_aligned) {
     Eight<T> a, b;
     const bool whole = DENSE && i0 + PER_THREAD <= total;
     if (whole) {
@@ -63,11 +60,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(int64_t total, int64_t col
             }
         }
     }
-    if (rng) {
-        seed = (unsigned long long)rng[0];
-        offset = (unsigned long long)rng[1];
-    }
-    const unsigned long long first = mix64(seed ^ mix64(offset)) + (unsigned long long)(i0 >> 1);
+    const unsigned long long first = key + (unsigned long long)(i0 >> 1);
 #pragma unroll
     for (int k = 0; k < PER_THREAD; k += 2) {
         const unsigned long long w = mix64(first + (k >> 1));
@@ -88,11 +81,27 @@ __global__ __launch_bounds__(256) void dropout_kernel(int64_t total, int64_t col
     }
 }
 
+template <typename T, bool DENSE, bool RESIDUAL>
+__global__ __launch_bounds__(256) void dropout_kernel(int64_t total, int64_t cols, const T* x, int64_t ldx, const T* r, int64_t ldr,
+                                                      T* y, unsigned long long border, float scale, unsigned long long seed,
+                                                      unsigned long long offset, const int64_t* rng, bool y_aligned) {
+    if (rng) {
+        seed = (unsigned long long)rng[0];
+        offset = (unsigned long long)rng[1];
+    }
+    const unsigned long long key = mix64(seed ^ mix64(offset));
+    // one turn, unless the grid's 2^32 threads are not enough
+    for (int64_t i0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * PER_THREAD; i0 < total;
+         i0 += (int64_t)gridDim.x * 256 * PER_THREAD)
+        dropout_eight<T, DENSE, RESIDUAL>(i0, total, cols, x, ldx, r, ldr, y, border, scale, key, y_aligned);
+}
+
 template <typename T>
 hipError_t launch(int64_t rows, int64_t cols, const void* x, int64_t ldx, const void* r, int64_t ldr, void* y, double p,
                   uint64_t seed, uint64_t offset, const int64_t* rng, hipStream_t s) {
     const int64_t total = rows * cols;
-    const unsigned grid = (unsigned)((total + 256 * PER_THREAD - 1) / (256 * PER_THREAD));
+    const int64_t blocks = (total + 256 * PER_THREAD - 1) / (256 * PER_THREAD);
+    const unsigned grid = (unsigned)(blocks < (1 << 23) ? blocks : 1 << 23);
     const unsigned long long border = (unsigned long long)__builtin_rint(p * 4294967296.0);
     const float scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
     auto run_of = [&](const void* q, int64_t ld) { return ((uintptr_t)q & 15) == 0 && (ld == cols || rows == 1); };

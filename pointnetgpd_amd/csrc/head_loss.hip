@@ -48,6 +48,7 @@ __global__ __launch_bounds__(1024) void batch_loss_kernel(int64_t T, const float
                                                           int reduction, float* loss) {
     __shared__ double part[16], count[16];
     double sum = 0, used = 0;
+#pragma unroll 8
     for (int64_t t = threadIdx.x; t < T; t += 1024) {
         sum += row_loss[t];
         used += target[t] != ignore;
@@ -74,10 +75,11 @@ __global__ __launch_bounds__(1024) void row_weights_kernel(bool scaled, int64_t 
                                                            int reduction, const float* dloss, float* weight, float* out_scale) {
     __shared__ float count[16], top[16];
     float used = 0.f, g = 0.f;
+#pragma unroll 8
     for (int64_t t = threadIdx.x; t < T; t += 1024) {
-        if (target[t] == ignore) continue;
-        used += 1.f;
-        if (target[t] >= 0 && target[t] < V) g = __builtin_fmaxf(g, __builtin_fabsf(dloss[reduction == PNGPD_REDUCE_NONE ? t : 0]));
+        const int64_t y = target[t];
+        used += y != ignore ? 1.f : 0.f;
+        if (reduction == PNGPD_REDUCE_NONE) g = __builtin_fmaxf(g, y != ignore && y >= 0 && y < V ? __builtin_fabsf(dloss[t]) : 0.f);
     }
     used = wave_sum(used);
     g = wave_max(g);
@@ -128,17 +130,18 @@ hipError_t head_zero(void* p, size_t bytes, hipStream_t s) {
     return hipGetLastError();
 }
 
-hipError_t head_loss_finish(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit, const int64_t* target,
-                            int64_t ignore, float eps, int reduction, float* row_loss, float* loss, float* lse, hipStream_t s) {
-    if (T > 0) {
-        int lanes = 5;                                       // few rows: more threads a row
-        while (lanes > 0 && (T >> lanes) < 64 && (256 >> lanes) < blocks) --lanes;
-        const int rows = 1 << lanes;
-        row_loss_kernel<<<(unsigned)((T + rows - 1) / rows), 256, 0, s>>>(T, V, blocks, stats, target_logit, target, ignore, eps, lanes,
-                                                                           row_loss, lse);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess || reduction == PNGPD_REDUCE_NONE) return e;
-    }
+hipError_t head_row_loss(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit, const int64_t* target,
+                         int64_t ignore, float eps, float* row_loss, float* lse, hipStream_t s) {
+    int lanes = 5;                                       // few rows: more threads a row
+    while (lanes > 0 && (T >> lanes) < 64 && (256 >> lanes) < blocks) --lanes;
+    const int rows = 1 << lanes;
+    row_loss_kernel<<<(unsigned)((T + rows - 1) / rows), 256, 0, s>>>(T, V, blocks, stats, target_logit, target, ignore, eps, lanes,
+                                                                       row_loss, lse);
+    return hipGetLastError();
+}
+
+hipError_t head_batch_loss(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore, int reduction, float* loss,
+                           hipStream_t s) {
     batch_loss_kernel<<<1, 1024, 0, s>>>(T, row_loss, target, ignore, reduction, loss);
     return hipGetLastError();
 }

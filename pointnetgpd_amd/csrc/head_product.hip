@@ -175,6 +175,7 @@ hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand&
         return rows<E, 4>((int)M, N, K, a, b, e, s);
     }
     const HeadPlan p = head_plan(type, M, N, K, e.kind);
+    if (p.tiles_m == 0) return hipErrorInvalidValue;
     TileArgs g{};
     g.M = M;
     g.N = N;
@@ -205,17 +206,6 @@ hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand&
 
 // ---- passes over whole matrices -----------------------------------------------------------------------------------------------------
 
-// A thread's chunk (16 bytes of the destination): row and first column, rows of `per_row` chunks
-__device__ __forceinline__ bool chunk_of(int64_t rows, int64_t per_row, int64_t* r, int64_t* c) {
-    const int64_t first = (int64_t)blockIdx.x * 256;
-    const int64_t r0 = first / per_row;                      // uniform
-    const unsigned off = (unsigned)(first - r0 * per_row) + threadIdx.x;      // per_row <= HEAD_MAX_LD / 16
-    const unsigned d = off / (unsigned)per_row;
-    *r = r0 + d;
-    *c = off - d * (unsigned)per_row;
-    return *r < rows;
-}
-
 template <typename T>
 struct Chunk {
     static constexpr int C = 16 / sizeof(T);
@@ -230,22 +220,29 @@ struct Chunk {
     }
 };
 
+// a thread a 16-byte chunk of the destination; per_row <= HEAD_MAX_LD / 16 chunks a row
 template <typename T>
 __global__ __launch_bounds__(256) void lay_out_kernel(int64_t rows, int64_t cols, const T* src, int64_t ld_src, const float* weight,
-                                                      T* dst, int64_t ld, bool aligned) {
+                                                      T* dst, int64_t ld, bool aligned, int64_t blocks) {
     constexpr int C = Chunk<T>::C;
-    int64_t r, c;
-    if (!chunk_of(rows, ld / C, &r, &c)) return;
-    typename Chunk<T>::V v = {};
-    if (!weight || weight[r] != 0.f) v = Chunk<T>::load(src + r * ld_src + c * C, cols - c * C, aligned);
-    *(typename Chunk<T>::V*)(dst + r * ld + c * C) = v;
+    const unsigned per_row = (unsigned)(ld / C);
+    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+        const int64_t first = block * 256, r0 = first / per_row;      // uniform
+        const unsigned off = (unsigned)(first - r0 * per_row) + threadIdx.x, d = off / per_row;
+        const int64_t r = r0 + d, c = (int64_t)(off - d * per_row) * C;
+        if (r >= rows) continue;
+        typename Chunk<T>::V v = {};
+        if (!weight || weight[r] != 0.f) v = Chunk<T>::load(src + r * ld_src + c, cols - c, aligned);
+        *(typename Chunk<T>::V*)(dst + r * ld + c) = v;
+    }
 }
 
 template <typename T>
 hipError_t lay_out(int64_t rows, int64_t cols, const void* src, int64_t ld_src, const float* weight, void* dst, int64_t ld, hipStream_t s) {
     const bool aligned = ((uintptr_t)src & 15) == 0 && ld_src % Chunk<T>::C == 0;
-    const int64_t chunks = rows * (ld / Chunk<T>::C);
-    lay_out_kernel<T><<<(unsigned)((chunks + 255) / 256), 256, 0, s>>>(rows, cols, (const T*)src, ld_src, weight, (T*)dst, ld, aligned);
+    const int64_t blocks = (rows * (ld / Chunk<T>::C) + 255) / 256;
+    const unsigned grid = (unsigned)(blocks < (1 << 23) ? blocks : 1 << 23);
+    lay_out_kernel<T><<<grid, 256, 0, s>>>(rows, cols, (const T*)src, ld_src, weight, (T*)dst, ld, aligned, blocks);
     return hipGetLastError();
 }
 
@@ -409,6 +406,7 @@ HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
             const int64_t per = (steps + cuts - 1) / cuts;
             if (cuts > 1 && (per < 4 || tiles >= 512)) break;
             if ((steps + per - 1) / per != cuts) continue;
+            if (tiles * cuts >= (int64_t)1 << 23) continue;      // a grid holds 2^32 threads
             const int64_t k = (tiles * cuts + 255) / 256;
             double us = (double)per * step_us(f32, shape, k) + tile_us(shape) * (shape == SHAPE_256 ? (double)k : 1.0);
             if (cuts > 1) us += 4.0 + (double)cuts * (double)M * (double)N * 8e-6 / 4.0;

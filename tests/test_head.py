@@ -78,7 +78,7 @@ def test_dropout_refuses(change, code):
     (dict(type=-2), ERR_INVALID), (dict(T=-1), ERR_SHAPE), (dict(V=0), ERR_SHAPE), (dict(D=0), ERR_SHAPE),
     (dict(x=None), ERR_INVALID), (dict(w=None), ERR_INVALID), (dict(target=None), ERR_INVALID), (dict(eps=1.5), ERR_INVALID),
     (dict(eps=float("nan")), ERR_INVALID), (dict(reduction=3), ERR_INVALID), (dict(ldw=3), ERR_SHAPE),
-    (dict(lse=None), ERR_INVALID), (dict(out=None), ERR_INVALID), (dict(T=2 ** 24, V=2 ** 24), ERR_SHAPE), (dict(D=2 ** 21 + 1, ldw=2 ** 22), ERR_SHAPE), (dict(ws=None), ERR_INVALID), (dict(nbytes=64), ERR_WORKSPACE)])
+    (dict(lse=None), ERR_INVALID), (dict(out=None), ERR_INVALID), (dict(V=2 ** 24 + 1), ERR_SHAPE), (dict(D=2 ** 21 + 1, ldw=2 ** 22), ERR_SHAPE), (dict(ws=None), ERR_INVALID), (dict(nbytes=64), ERR_WORKSPACE)])
 def test_linear_cross_entropy_refuses(change, code):
     lib = _lib.load()
     a = dict(type=0, T=2, V=5, D=4, x=16, w=16, ldw=4, target=16, eps=0.0, reduction=1, lse=16, out=16, ws=4096, nbytes=1 << 20)

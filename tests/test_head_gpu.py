@@ -81,6 +81,17 @@ def test_linear_over_many_tiles(kind, M, N, K):
     check(got, ho.linear(x, w, b, "gelu", r, dy))
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("N,K", [(1, 8), (70, 24), (2050, 1000), (4100, 513), (513, 8200)])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_linear_of_a_few_rows(kind, N, K, M):
+    act = (None, "relu", "gelu", "gelu_tanh", "silu")[M - 1]
+    x, w, b, r, dy = linear_case(N + K + M, M, N, K, TYPES[kind], act, True, True)
+    got = run_linear(x, w, b, r, act, dy)
+    got.pop("dr")
+    check(got, ho.linear(x, w, b, act, r, dy))
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_linear_takes_any_strides_and_alignment(kind):
     dt = TYPES[kind]
@@ -368,6 +379,56 @@ def test_linear_cross_entropy_takes_any_strides(kind):
     loss = head.linear_cross_entropy(x.cuda().view(3, 20, 40), w.cuda(), target.cuda().view(3, 20), b.cuda(), reduction="none")
     assert loss.shape == (3, 20)
     check({"loss": loss.reshape(-1)}, {"loss": want["loss"]})
+
+
+# ---- beyond 32 bits --------------------------------------------------------------------------------------------------------
+
+def test_dropout_beyond_32_bits_of_elements():
+    n, tail = 2 ** 32 + 4104, 5000
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    y = head.dropout(x.view(8, n // 8), 0.25, 3, 1).view(-1)
+    keep = ho.keep_mask_at(n - tail, tail, 0.25, 3, 1)
+    assert torch.equal(y[-tail:].cpu() != 0, torch.from_numpy(keep))
+    assert torch.equal(y[:tail].cpu() != 0, torch.from_numpy(ho.keep_mask(tail, 0.25, 3, 1)))
+    share = sum((c != 0).sum().item() for c in y.split(2 ** 28)) / n
+    assert abs(share - 0.75) < 5 * (0.25 * 0.75 / n) ** 0.5
+
+
+def test_linear_beyond_32_bits_of_elements():
+    """2 100 000 rows of 2056: the last ones lie behind 4 G elements, and the weight's gradient runs over all rows."""
+    M, N, K, tail = 2_100_000, 4, 2056, 300
+    dt = torch.bfloat16
+    xt, w, b, _, dyt = linear_case(77, tail, N, K, dt, None, True, False)
+    x = torch.zeros(M, K, dtype=dt, device="cuda")
+    x[-tail:] = xt.cuda()
+    dy = torch.zeros(M, N, dtype=dt, device="cuda")
+    dy[-tail:] = dyt.cuda()
+    xs, ws, bs = x.requires_grad_(), w.cuda().requires_grad_(), b.cuda().requires_grad_()
+    y = head.linear(xs, ws, bs, activation="silu")
+    dx, dw, db = torch.autograd.grad(y, (xs, ws, bs), dy)
+    want = ho.linear(xt, w, b, "silu", None, dyt)
+    check({"y": y[-tail:], "dx": dx[-tail:], "dw": dw, "db": db}, want)
+    assert not dx[:1000].any() and torch.equal(y[:1000], y[1000:2000])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_linear_cross_entropy_beyond_32_bits_of_logits(kind):
+    """40 000 rows by 131 072 classes: 5.2 G logits, in several runs of rows (forward) and pieces of the vocabulary."""
+    T, V, D = 40000, 131072, 16
+    dt = TYPES[kind]
+    x, w, b, target = loss_case(5, T, V, D, dt, True)
+    rows = [0, 1, 255, 256, 4095, 4096, 8191, 8192, 8193, 16383, 16384, 32767, 32768, T - 2, T - 1]
+    dloss = torch.zeros(T)
+    dloss[rows] = torch.rand(len(rows)) + 0.5
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+    loss = head.linear_cross_entropy(leaves[0], leaves[1], target.cuda(), leaves[2], label_smoothing=0.1, reduction="none")
+    dx, dw, db = torch.autograd.grad(loss, leaves, dloss.cuda())
+    want = ho.cross_entropy(x[rows], w, target[rows], b, -100, 0.1, "none", dloss[rows])
+    # the sums over the rows have T terms, all but those of `rows` exact zeros
+    check({"loss": loss[rows], "dx": dx[rows], "dw": dw, "db": db}, want)
+    others = torch.ones(T, dtype=torch.bool)
+    others[rows] = False
+    assert not dx[others.cuda()].any()
 
 
 # ---- against differences, together, captured --------------------------------------------------------------------------------
