@@ -11,7 +11,7 @@ constexpr int64_t HEAD_MAX_EXTENT = HEAD_MAX_LD / 4;         // elements of a de
 
 // One operand of a product out[m][n] = sum_k A(m,k) B(n,k).
 // k_contiguous: element (r, k) sits at p[r * ld + k]; otherwise at p[k * ld + r] (the operand lies transposed).
-// Both take rows as head_direct() describes them; head_lay_out() makes such rows of others.
+// Both take rows as head_direct() describes them; head_set_up() makes such rows of others.
 struct HeadOperand {
     const void* p;
     int64_t ld;
@@ -68,17 +68,32 @@ HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind);
 hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b,
                         const HeadEpilogue& e, float* partial, hipStream_t s);
 
-// dst[r][0 .. ld) = src[r][0 .. cols) and zeros behind them; rows with row_weight[r] == 0 (row_weight may be NULL) become
-// zeros whatever they hold.  dst is 16-byte aligned, ld whole chunks.
-hipError_t head_lay_out(int type, int64_t rows, int64_t cols, const void* src, int64_t ld_src, const float* row_weight, void* dst,
-                        int64_t ld, hipStream_t s);
+// dst[r][0 .. ld) = src[r][0 .. cols) and zeros behind them.  dst is 16-byte aligned, ld whole chunks.  With a target, rows
+// whose target is ignored or no class become zeros whatever they hold.
+struct HeadLayOut {
+    const void* src;
+    int64_t rows, cols, ld_src;
+    void* dst;
+    int64_t ld;
+    bool live_rows_only;
+};
+// row_weight[t] = weight of row t in the loss's gradient divided by out_scale[0], a power of two (half precision) or the one
+// weight of all rows
+struct HeadRowWeights {
+    const int64_t* target;
+    int64_t T, V, ignore_index;
+    int reduction;
+    const float* dloss;
+    float *row_weight, *out_scale;
+};
+// Up to two matrices laid out and the rows' weights, in one launch; each may be NULL, all NULL launches nothing.
+hipError_t head_set_up(int type, const HeadLayOut* a, const HeadLayOut* b, const HeadRowWeights* w, hipStream_t s);
 // dz[m][n] = dy[m][n] * act'(z[m][n]) (z dense; act NONE: dy itself) into dz (may be NULL; rows of ld_dz, whole chunks, zeros
-// behind column N), and the columns' sums over blocks of rows into part (may be NULL; 32-bit [head_col_parts][N])
+// behind column N), and into sums (may be NULL) scale[0] (NULL: 1) times the columns' sums, by way of
+// part: 32-bit [head_col_parts][N]
 size_t head_col_parts(int type, int64_t M, int64_t N);
 hipError_t head_grad_rows(int type, int64_t M, int64_t N, const void* dy, int64_t ld_dy, const void* z, int act, void* dz,
-                          int64_t ld_dz, float* part, hipStream_t s);
-// out[n] = scale[0] (NULL: 1) times the sum of column n's parts
-hipError_t head_col_join(int type, int64_t M, int64_t N, const float* part, const float* scale, void* out, hipStream_t s);
+                          int64_t ld_dz, float* part, const float* scale, void* sums, hipStream_t s);
 
 // a fill kernel, not a memset: the call may be captured
 hipError_t head_zero(void* p, size_t bytes, hipStream_t s);
@@ -88,12 +103,10 @@ hipError_t head_dropout(int type, int64_t rows, int64_t cols, const void* x, int
                         hipStream_t s);
 
 // lse[t] and the loss of every row from its statistics; the batch's loss from its rows'
+// (batch: not NULL, and one launch does both where that is as quick; head_loss_at_once() says whether it did)
+bool head_loss_at_once(int64_t T, int blocks);
 hipError_t head_row_loss(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit, const int64_t* target,
-                         int64_t ignore_index, float eps, float* row_loss, float* lse, hipStream_t s);
+                         int64_t ignore_index, float eps, float* row_loss, float* lse, int reduction, float* batch, hipStream_t s);
 hipError_t head_batch_loss(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore_index, int reduction, float* loss,
                            hipStream_t s);
-// row_weight[t] = weight of row t in the gradient divided by 2^e, out_scale[0] = 2^e (type f16 only, else 2^e = 1)
-hipError_t head_row_weights(int type, int64_t T, int64_t V, const int64_t* target, int64_t ignore_index, int reduction,
-                            const float* dloss, float* row_weight, float* out_scale, hipStream_t s);
-
 }  // namespace pngpd

@@ -71,13 +71,12 @@ struct Rows {
     int64_t ld;
 };
 inline bool direct(const void* p, int64_t ld, int64_t extent, int type) { return pngpd::head_direct(p, ld, extent, esize(type)); }
-hipError_t direct_rows(int type, int64_t rows, int64_t extent, const void* p, int64_t ld, void* room, hipStream_t s, Rows* out) {
-    if (direct(p, ld, extent, type)) {
-        *out = Rows{p, ld};
-        return hipSuccess;
-    }
-    *out = Rows{room, padded(extent, type)};
-    return pngpd::head_lay_out(type, rows, extent, p, ld, nullptr, room, out->ld, s);
+// Itself, or where head_set_up() has to lay it out first (`job` then is what it takes).
+Rows direct_rows(int type, int64_t rows, int64_t extent, const void* p, int64_t ld, void* room, pngpd::HeadLayOut* job, bool* needed) {
+    *needed = !direct(p, ld, extent, type);
+    if (!*needed) return Rows{p, ld};
+    *job = pngpd::HeadLayOut{p, rows, extent, ld, room, padded(extent, type), false};
+    return Rows{room, job->ld};
 }
 
 inline size_t max2(size_t a, size_t b) { return a > b ? a : b; }
@@ -216,9 +215,11 @@ int pngpd_linear_forward(int type, int64_t M, int64_t N, int64_t K, const void* 
     e.out = y_dev;
     e.ld_out = N;
     hipStream_t s = (hipStream_t)stream;
-    Rows x, w;
-    HIP_TRY(direct_rows(type, M, K, x_dev, ldx, ws.x, s, &x));
-    HIP_TRY(direct_rows(type, N, K, weight_dev, ldw, ws.w, s, &w));
+    pngpd::HeadLayOut job_x, job_w;
+    bool lay_x, lay_w;
+    const Rows x = direct_rows(type, M, K, x_dev, ldx, ws.x, &job_x, &lay_x);
+    const Rows w = direct_rows(type, N, K, weight_dev, ldw, ws.w, &job_w, &lay_w);
+    HIP_TRY(pngpd::head_set_up(type, lay_x ? &job_x : nullptr, lay_w ? &job_w : nullptr, nullptr, s));
     HIP_TRY(pngpd::head_product(type, M, N, K, HeadOperand{x.p, x.ld, true}, HeadOperand{w.p, w.ld, true}, e, ws.partial, s));
     return PNGPD_OK;
 }
@@ -248,20 +249,21 @@ int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void*
     const Rows dz = same ? Rows{dy_dev, ld_dy} : Rows{ws.dz, padded(N, type)};
     if (!same || dbias_dev)
         HIP_TRY(pngpd::head_grad_rows(type, M, N, dy_dev, ld_dy, z_dev, act, same ? nullptr : ws.dz, dz.ld,
-                                      dbias_dev ? ws.part : nullptr, s));
-    if (dbias_dev) HIP_TRY(pngpd::head_col_join(type, M, N, ws.part, nullptr, dbias_dev, s));
+                                      ws.part, nullptr, dbias_dev, s));
+    pngpd::HeadLayOut job_x, job_w;
+    bool lay_x = false, lay_w = false;
+    Rows x{}, w{};
+    if (dx_dev) w = direct_rows(type, N, K, weight_dev, ldw, ws.w, &job_w, &lay_w);
+    if (dweight_dev) x = direct_rows(type, M, K, x_dev, ldx, ws.x, &job_x, &lay_x);
+    HIP_TRY(pngpd::head_set_up(type, lay_x ? &job_x : nullptr, lay_w ? &job_w : nullptr, nullptr, s));
     HeadEpilogue e;
     e.kind = pngpd::HEAD_EPI_SCALED;
     e.ld_out = K;
     if (dx_dev) {
-        Rows w;
-        HIP_TRY(direct_rows(type, N, K, weight_dev, ldw, ws.w, s, &w));
         e.out = dx_dev;
         HIP_TRY(pngpd::head_product(type, M, K, N, HeadOperand{dz.p, dz.ld, true}, HeadOperand{w.p, w.ld, false}, e, ws.partial, s));
     }
     if (dweight_dev) {
-        Rows x;
-        HIP_TRY(direct_rows(type, M, K, x_dev, ldx, ws.x, s, &x));
         e.out = dweight_dev;
         HIP_TRY(pngpd::head_product(type, N, K, M, HeadOperand{dz.p, dz.ld, false}, HeadOperand{x.p, x.ld, false}, e, ws.partial, s));
     }
@@ -303,12 +305,15 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
     LossWs ws(workspace_dev, type, T, V, D, false, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
     if (T > 0) {
         if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
-        Rows x, w;
-        HIP_TRY(direct_rows(type, T, D, x_dev, ldx, ws.x, s, &x));
-        HIP_TRY(direct_rows(type, V, D, weight_dev, ldw, ws.w, s, &w));
+        pngpd::HeadLayOut job_x, job_w;
+        bool lay_x, lay_w;
+        const Rows x = direct_rows(type, T, D, x_dev, ldx, ws.x, &job_x, &lay_x);
+        const Rows w = direct_rows(type, V, D, weight_dev, ldw, ws.w, &job_w, &lay_w);
+        HIP_TRY(pngpd::head_set_up(type, lay_x ? &job_x : nullptr, lay_w ? &job_w : nullptr, nullptr, s));
         float* row_loss = reduction == PNGPD_REDUCE_NONE ? loss_dev : ws.row_loss;
         for (int64_t t = 0; t < T; t += ws.rows_at_once) {
             const int64_t n = T - t < ws.rows_at_once ? T - t : ws.rows_at_once;
+            const bool whole = n == T;
             HeadEpilogue e;
             e.kind = pngpd::HEAD_EPI_STATS;
             e.bias = bias_dev;
@@ -320,7 +325,9 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
                                         ws.partial, s));
             const int blocks = pngpd::head_plan(type, n, V, D, pngpd::HEAD_EPI_STATS).stats_blocks;
             HIP_TRY(pngpd::head_row_loss(n, V, blocks, ws.stats, ws.target_logit, target_dev + t, ignore_index, label_smoothing,
-                                         row_loss + t, lse_dev + t, s));
+                                         row_loss + t, lse_dev + t, reduction,
+                                         whole && reduction != PNGPD_REDUCE_NONE ? loss_dev : nullptr, s));
+            if (whole && reduction != PNGPD_REDUCE_NONE && pngpd::head_loss_at_once(n, blocks)) return PNGPD_OK;
         }
     }
     if (reduction != PNGPD_REDUCE_NONE) HIP_TRY(pngpd::head_batch_loss(T, ws.row_loss, target_dev, ignore_index, reduction, loss_dev, s));
@@ -344,11 +351,13 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
     if (!lse_dev || !dloss_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL argument", who);
     LossWs ws(workspace_dev, type, T, V, D, true, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
-    HIP_TRY(pngpd::head_row_weights(type, T, V, target_dev, ignore_index, reduction, dloss_dev, ws.row_weight, ws.scale, s));
     const HeadOperand x{ws.x, padded(D, type), true}, xt{ws.x, padded(D, type), false};
-    HIP_TRY(pngpd::head_lay_out(type, T, D, x_dev, ldx, ws.row_weight, ws.x, x.ld, s));
-    Rows whole;
-    HIP_TRY(direct_rows(type, V, D, weight_dev, ldw, ws.w, s, &whole));
+    const pngpd::HeadRowWeights weights{target_dev, T, V, ignore_index, reduction, dloss_dev, ws.row_weight, ws.scale};
+    const pngpd::HeadLayOut job_x{x_dev, T, D, ldx, ws.x, x.ld, true};      // what padding rows hold stays out of the sums
+    pngpd::HeadLayOut job_w;
+    bool lay_w;
+    const Rows whole = direct_rows(type, V, D, weight_dev, ldw, ws.w, &job_w, &lay_w);
+    HIP_TRY(pngpd::head_set_up(type, &job_x, lay_w ? &job_w : nullptr, &weights, s));
     for (int64_t v = 0; v < V; v += ws.piece) {
         const int64_t n = V - v < ws.piece ? V - v : ws.piece, np = padded(n, type);
         const void* w = at(whole.p, v * whole.ld, type);
@@ -364,10 +373,9 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         e.out = ws.tile;
         e.ld_out = np;
         HIP_TRY(pngpd::head_product(type, T, n, D, x, HeadOperand{w, whole.ld, true}, e, ws.partial, s));
-        if (dbias_dev) {
-            HIP_TRY(pngpd::head_grad_rows(type, T, n, ws.tile, np, nullptr, PNGPD_ACT_NONE, nullptr, 0, ws.part, s));
-            HIP_TRY(pngpd::head_col_join(type, T, n, ws.part, ws.scale, at(dbias_dev, v, type), s));
-        }
+        if (dbias_dev)
+            HIP_TRY(pngpd::head_grad_rows(type, T, n, ws.tile, np, nullptr, PNGPD_ACT_NONE, nullptr, 0, ws.part, ws.scale,
+                                          at(dbias_dev, v, type), s));
         HeadEpilogue g;
         g.kind = pngpd::HEAD_EPI_SCALED;
         g.ld_out = D;

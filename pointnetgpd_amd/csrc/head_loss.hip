@@ -1,4 +1,4 @@
-// Loss and gradient weights of linear_cross_entropy from the rows' statistics (the products are head_product.hip's).
+// The loss of linear_cross_entropy from the rows' statistics (the products are head_product.hip's).
 //
 // A block of columns leaves a row's maximum m, sum s of exp(z - m) and sum of z; blocks join by
 // s = s1 exp(m1 - m) + s2 exp(m2 - m) under m = max(m1, m2).
@@ -13,6 +13,17 @@ __device__ __forceinline__ void join_stats(float4& v, const float4& u) {
     v.y = v.y * (v.x == m ? 1.f : __expf(v.x - m)) + u.y * (u.x == m ? 1.f : __expf(u.x - m));
     v.x = m;
     v.z += u.z;
+}
+
+__device__ __forceinline__ float loss_of_row(const float4& v, int64_t t, int64_t V, const float* target_logit, const int64_t* target,
+                                             int64_t ignore, float eps, float* lse) {
+    const float l = v.x + logf(v.y);
+    lse[t] = l;
+    const int64_t y = target[t];
+    if (y == ignore) return 0.f;
+    float x = y >= 0 && y < V ? l - (1.f - eps) * target_logit[t] : __builtin_nanf("");
+    if (eps > 0.f) x -= eps / (float)V * v.z;
+    return x;
 }
 
 // 2^lanes rows a workgroup, the other threads side by side over a row's blocks; then the threads of a row in order
@@ -31,28 +42,12 @@ __global__ __launch_bounds__(256) void row_loss_kernel(int64_t T, int64_t V, int
         __syncthreads();
     }
     if (part || t >= T) return;
-    v = share[r];
-    const float l = v.x + logf(v.y);
-    lse[t] = l;
-    const int64_t y = target[t];
-    float x = 0.f;
-    if (y != ignore) {
-        x = y >= 0 && y < V ? l - (1.f - eps) * target_logit[t] : __builtin_nanf("");
-        if (eps > 0.f) x -= eps / (float)V * v.z;
-    }
-    loss[t] = x;
+    loss[t] = loss_of_row(share[r], t, V, target_logit, target, ignore, eps, lse);
 }
 
 // the batch's loss: one workgroup, sums over the rows in 64 bits
-__global__ __launch_bounds__(1024) void batch_loss_kernel(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore,
-                                                          int reduction, float* loss) {
+__device__ __forceinline__ void batch_sum(double sum, double used, int reduction, float* loss) {
     __shared__ double part[16], count[16];
-    double sum = 0, used = 0;
-#pragma unroll 8
-    for (int64_t t = threadIdx.x; t < T; t += 1024) {
-        sum += row_loss[t];
-        used += target[t] != ignore;
-    }
     for (int o = 32; o; o >>= 1) {
         sum += __shfl_xor(sum, o);
         used += __shfl_xor(used, o);
@@ -71,50 +66,30 @@ __global__ __launch_bounds__(1024) void batch_loss_kernel(int64_t T, const float
     }
 }
 
-__global__ __launch_bounds__(1024) void row_weights_kernel(bool scaled, int64_t T, int64_t V, const int64_t* target, int64_t ignore,
-                                                           int reduction, const float* dloss, float* weight, float* out_scale) {
-    __shared__ float count[16], top[16];
-    float used = 0.f, g = 0.f;
+__global__ __launch_bounds__(1024) void batch_loss_kernel(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore,
+                                                          int reduction, float* loss) {
+    double sum = 0, used = 0;
 #pragma unroll 8
     for (int64_t t = threadIdx.x; t < T; t += 1024) {
-        const int64_t y = target[t];
-        used += y != ignore ? 1.f : 0.f;
-        if (reduction == PNGPD_REDUCE_NONE) g = __builtin_fmaxf(g, y != ignore && y >= 0 && y < V ? __builtin_fabsf(dloss[t]) : 0.f);
+        sum += row_loss[t];
+        used += target[t] != ignore;
     }
-    used = wave_sum(used);
-    g = wave_max(g);
-    if ((threadIdx.x & 63) == 0) {
-        count[threadIdx.x >> 6] = used;
-        top[threadIdx.x >> 6] = g;
+    batch_sum(sum, used, reduction, loss);
+}
+
+// rows' losses and the batch's for a small batch: a thread a row
+__global__ __launch_bounds__(1024) void small_loss_kernel(int T, int64_t V, int blocks, const float4* stats, const float* target_logit,
+                                                          const int64_t* target, int64_t ignore, float eps, int reduction, float* loss,
+                                                          float* lse) {
+    const int t = threadIdx.x;
+    double sum = 0, used = 0;
+    if (t < T) {
+        float4 v = stats[t];
+        for (int i = 1; i < blocks; ++i) join_stats(v, stats[(int64_t)i * T + t]);
+        sum = loss_of_row(v, t, V, target_logit, target, ignore, eps, lse);
+        used = target[t] != ignore;
     }
-    __syncthreads();
-    used = 0.f;
-    g = 0.f;
-    for (int i = 0; i < 16; ++i) {
-        used += count[i];
-        g = __builtin_fmaxf(g, top[i]);
-    }
-    // half precision: the largest weight becomes 2^13 .. 2^14, |dz| <= 2 times that is inside its range, and a probability of
-    // 2^-37 still is a number
-    if (reduction != PNGPD_REDUCE_NONE) {
-        // One weight for all rows stays out of dz and goes into the products' 32-bit sums: p - 1 of the labels would be rounded
-        // the same way in every row otherwise (off by up to 2^-9 in one direction in bfloat16).
-        const float unit = scaled ? 16384.f : 1.f;
-        for (int64_t t = threadIdx.x; t < T; t += 1024) weight[t] = target[t] != ignore && target[t] >= 0 && target[t] < V ? unit : 0.f;
-        if (threadIdx.x == 0) out_scale[0] = dloss[0] * (reduction == PNGPD_REDUCE_MEAN ? 1.f / __builtin_fmaxf(used, 1.f) : 1.f) / unit;
-        return;
-    }
-    float scale = 1.f;
-    if (scaled && g > 0.f && g < __builtin_inff()) {
-        int e;
-        (void)frexpf(g, &e);
-        scale = ldexpf(1.f, e - 14);
-    }
-    for (int64_t t = threadIdx.x; t < T; t += 1024) {
-        const bool live = target[t] != ignore && target[t] >= 0 && target[t] < V;
-        weight[t] = live ? dloss[t] / scale : 0.f;
-    }
-    if (threadIdx.x == 0) out_scale[0] = scale;
+    batch_sum(sum, used, reduction, loss);
 }
 
 // bytes: an even number (every element type has at least two)
@@ -130,8 +105,14 @@ hipError_t head_zero(void* p, size_t bytes, hipStream_t s) {
     return hipGetLastError();
 }
 
+bool head_loss_at_once(int64_t T, int blocks) { return T <= 1024 && blocks <= 8; }
+
 hipError_t head_row_loss(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit, const int64_t* target,
-                         int64_t ignore, float eps, float* row_loss, float* lse, hipStream_t s) {
+                         int64_t ignore, float eps, float* row_loss, float* lse, int reduction, float* batch, hipStream_t s) {
+    if (batch && head_loss_at_once(T, blocks)) {
+        small_loss_kernel<<<1, 1024, 0, s>>>((int)T, V, blocks, stats, target_logit, target, ignore, eps, reduction, batch, lse);
+        return hipGetLastError();
+    }
     int lanes = 5;                                       // few rows: more threads a row
     while (lanes > 0 && (T >> lanes) < 64 && (256 >> lanes) < blocks) --lanes;
     const int rows = 1 << lanes;
@@ -143,12 +124,6 @@ hipError_t head_row_loss(int64_t T, int64_t V, int blocks, const float4* stats, 
 hipError_t head_batch_loss(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore, int reduction, float* loss,
                            hipStream_t s) {
     batch_loss_kernel<<<1, 1024, 0, s>>>(T, row_loss, target, ignore, reduction, loss);
-    return hipGetLastError();
-}
-
-hipError_t head_row_weights(int type, int64_t T, int64_t V, const int64_t* target, int64_t ignore, int reduction,
-                            const float* dloss, float* weight, float* out_scale, hipStream_t s) {
-    row_weights_kernel<<<1, 1024, 0, s>>>(type == PNGPD_TYPE_F16, T, V, target, ignore, reduction, dloss, weight, out_scale);
     return hipGetLastError();
 }
 

@@ -220,29 +220,100 @@ struct Chunk {
     }
 };
 
-// a thread a 16-byte chunk of the destination; per_row <= HEAD_MAX_LD / 16 chunks a row
+// Gradient weights of the loss's rows, by one workgroup of 256.
+__device__ __forceinline__ void row_weights(const HeadRowWeights& w, bool scaled) {
+    __shared__ float count[4], top[4];
+    float used = 0.f, g = 0.f;
+#pragma unroll 8
+    for (int64_t t = threadIdx.x; t < w.T; t += 256) {
+        const int64_t y = w.target[t];
+        used += y != w.ignore_index ? 1.f : 0.f;
+        if (w.reduction == PNGPD_REDUCE_NONE)
+            g = __builtin_fmaxf(g, y != w.ignore_index && y >= 0 && y < w.V ? __builtin_fabsf(w.dloss[t]) : 0.f);
+    }
+    used = wave_sum(used);
+    g = wave_max(g);
+    if ((threadIdx.x & 63) == 0) {
+        count[threadIdx.x >> 6] = used;
+        top[threadIdx.x >> 6] = g;
+    }
+    __syncthreads();
+    used = count[0] + count[1] + count[2] + count[3];
+    g = __builtin_fmaxf(__builtin_fmaxf(top[0], top[1]), __builtin_fmaxf(top[2], top[3]));
+    // Half precision: the largest weight becomes 2^13 .. 2^14, |dz| <= 2 times that is inside its range, and a probability of
+    // 2^-37 still is a number.
+    // One weight for all rows stays out of dz and goes into the products' 32-bit sums: p - 1 of the labels would be rounded
+    // the same way in every row otherwise (off by up to 2^-9 in one direction in bfloat16).
+    const bool one = w.reduction != PNGPD_REDUCE_NONE;
+    float scale = 1.f;
+    if (one) {
+        scale = scaled ? 16384.f : 1.f;
+    } else if (scaled && g > 0.f && g < __builtin_inff()) {
+        int e;
+        (void)frexpf(g, &e);
+        scale = ldexpf(1.f, e - 14);
+    }
+#pragma unroll 8
+    for (int64_t t = threadIdx.x; t < w.T; t += 256) {
+        const int64_t y = w.target[t];
+        const bool live = y != w.ignore_index && y >= 0 && y < w.V;
+        w.row_weight[t] = !live ? 0.f : one ? scale : w.dloss[t] / scale;
+    }
+    if (threadIdx.x == 0)
+        w.out_scale[0] = one ? w.dloss[0] * (w.reduction == PNGPD_REDUCE_MEAN ? 1.f / __builtin_fmaxf(used, 1.f) : 1.f) / scale : scale;
+}
+
+struct LayOutRun {
+    HeadLayOut m;
+    bool aligned;
+    int64_t blocks;        // of 256 chunks
+    unsigned grid;
+};
+
+// Workgroups 0 .. a.grid lay out a, the next b.grid b, the last one the rows' weights: a thread a 16-byte chunk of the
+// destination; at most HEAD_MAX_LD / 16 chunks a row.
 template <typename T>
-__global__ __launch_bounds__(256) void lay_out_kernel(int64_t rows, int64_t cols, const T* src, int64_t ld_src, const float* weight,
-                                                      T* dst, int64_t ld, bool aligned, int64_t blocks) {
+__global__ __launch_bounds__(256) void set_up_kernel(LayOutRun a, LayOutRun b, HeadRowWeights w) {
     constexpr int C = Chunk<T>::C;
-    const unsigned per_row = (unsigned)(ld / C);
-    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    if (blockIdx.x >= a.grid + b.grid) {
+        row_weights(w, __is_same(T, f16_t));
+        return;
+    }
+    const bool second = blockIdx.x >= a.grid;
+    const LayOutRun& u = second ? b : a;
+    const unsigned per_row = (unsigned)(u.m.ld / C);
+    for (int64_t block = second ? blockIdx.x - a.grid : blockIdx.x; block < u.blocks; block += u.grid) {
         const int64_t first = block * 256, r0 = first / per_row;      // uniform
         const unsigned off = (unsigned)(first - r0 * per_row) + threadIdx.x, d = off / per_row;
         const int64_t r = r0 + d, c = (int64_t)(off - d * per_row) * C;
-        if (r >= rows) continue;
+        if (r >= u.m.rows) continue;
+        bool live = true;
+        if (u.m.live_rows_only) {
+            const int64_t y = w.target[r];
+            live = y != w.ignore_index && y >= 0 && y < w.V;
+        }
         typename Chunk<T>::V v = {};
-        if (!weight || weight[r] != 0.f) v = Chunk<T>::load(src + r * ld_src + c, cols - c, aligned);
-        *(typename Chunk<T>::V*)(dst + r * ld + c) = v;
+        if (live) v = Chunk<T>::load((const T*)u.m.src + r * u.m.ld_src + c, u.m.cols - c, u.aligned);
+        *(typename Chunk<T>::V*)((T*)u.m.dst + r * u.m.ld + c) = v;
     }
 }
 
 template <typename T>
-hipError_t lay_out(int64_t rows, int64_t cols, const void* src, int64_t ld_src, const float* weight, void* dst, int64_t ld, hipStream_t s) {
-    const bool aligned = ((uintptr_t)src & 15) == 0 && ld_src % Chunk<T>::C == 0;
-    const int64_t blocks = (rows * (ld / Chunk<T>::C) + 255) / 256;
-    const unsigned grid = (unsigned)(blocks < (1 << 23) ? blocks : 1 << 23);
-    lay_out_kernel<T><<<grid, 256, 0, s>>>(rows, cols, (const T*)src, ld_src, weight, (T*)dst, ld, aligned, blocks);
+hipError_t set_up(const HeadLayOut* a, const HeadLayOut* b, const HeadRowWeights* w, hipStream_t s) {
+    constexpr int C = Chunk<T>::C;
+    auto run = [](const HeadLayOut* m) {
+        LayOutRun r{};
+        if (!m) return r;
+        r.m = *m;
+        r.aligned = ((uintptr_t)m->src & 15) == 0 && m->ld_src % C == 0;
+        r.blocks = (m->rows * (m->ld / C) + 255) / 256;
+        r.grid = (unsigned)(r.blocks < (1 << 22) ? r.blocks : 1 << 22);
+        return r;
+    };
+    const LayOutRun ra = run(a), rb = run(b);
+    const unsigned grid = ra.grid + rb.grid + (w ? 1 : 0);
+    if (grid == 0) return hipSuccess;
+    set_up_kernel<T><<<grid, 256, 0, s>>>(ra, rb, w ? *w : HeadRowWeights{});
     return hipGetLastError();
 }
 
@@ -274,7 +345,8 @@ ColumnCut column_cut(int64_t M, int64_t N, int chunk) {
 // One pass over dy and z: bound by memory, so the sums of the columns ride along.
 template <typename T, int ACT, bool WRITE>
 __global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, const T* dy, int64_t ld, bool dy_aligned, const T* z,
-                                                        bool z_aligned, T* dz, int64_t ld_dz, float* part, int lanes, int64_t rows) {
+                                                        bool z_aligned, T* dz, int64_t ld_dz, float* part, int lanes, int64_t rows,
+                                                        const float* scale, T* sums) {
     constexpr int C = Chunk<T>::C;
     __shared__ float share[256][C + 1];
     const int wide = 1 << lanes, side = 256 >> lanes;
@@ -300,7 +372,7 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, co
             if constexpr (WRITE) *(typename Chunk<T>::V*)(dz + m * ld_dz + col) = o;
         }
     }
-    if (!part) return;
+    if (!sums) return;
 #pragma unroll
     for (int i = 0; i < C; ++i) share[threadIdx.x][i] = sum[i];
     __syncthreads();
@@ -309,32 +381,9 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, co
         if (n >= N) continue;
         float s = 0.f;
         for (int r = 0; r < side; ++r) s += share[(r << lanes) + c / C][c % C];
-        part[(int64_t)blockIdx.y * N + n] = s;
+        if (gridDim.y == 1) sums[n] = from_f32<T>(scale ? s * scale[0] : s);
+        else part[(int64_t)blockIdx.y * N + n] = s;
     }
-}
-
-template <typename T>
-hipError_t grad_rows(int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz, int64_t ld_dz, float* part,
-                     hipStream_t s) {
-    constexpr int C = Chunk<T>::C;
-    const ColumnCut c = column_cut(M, N, C);
-    const dim3 grid(c.blocks, (unsigned)c.parts);
-    const bool da = ((uintptr_t)dy & 15) == 0 && ld % C == 0, za = ((uintptr_t)z & 15) == 0 && N % C == 0;
-#define PNGPD_GRAD_ROWS(A, W) \
-    grad_rows_kernel<T, A, W><<<grid, 256, 0, s>>>(M, N, (const T*)dy, ld, da, (const T*)z, za, (T*)dz, ld_dz, part, c.lanes, c.rows)
-    switch (act) {
-        case PNGPD_ACT_NONE:
-            if (dz) PNGPD_GRAD_ROWS(PNGPD_ACT_NONE, true);
-            else PNGPD_GRAD_ROWS(PNGPD_ACT_NONE, false);
-            break;
-        case PNGPD_ACT_RELU: PNGPD_GRAD_ROWS(PNGPD_ACT_RELU, true); break;
-        case PNGPD_ACT_GELU: PNGPD_GRAD_ROWS(PNGPD_ACT_GELU, true); break;
-        case PNGPD_ACT_GELU_TANH: PNGPD_GRAD_ROWS(PNGPD_ACT_GELU_TANH, true); break;
-        case PNGPD_ACT_SILU: PNGPD_GRAD_ROWS(PNGPD_ACT_SILU, true); break;
-        default: return hipErrorInvalidValue;
-    }
-#undef PNGPD_GRAD_ROWS
-    return hipGetLastError();
 }
 
 // 32 columns by 8 shares of the parts a workgroup
@@ -356,9 +405,29 @@ __global__ __launch_bounds__(256) void col_join_kernel(int parts, int64_t N, con
 }
 
 template <typename T>
-hipError_t col_join(int64_t M, int64_t N, const float* part, const float* scale, void* out, hipStream_t s) {
-    const int parts = (int)column_cut(M, N, Chunk<T>::C).parts;
-    col_join_kernel<T><<<(unsigned)((N + 31) / 32), 256, 0, s>>>(parts, N, part, scale, (T*)out);
+hipError_t grad_rows(int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz, int64_t ld_dz, float* part,
+                     const float* scale, void* sums, hipStream_t s) {
+    constexpr int C = Chunk<T>::C;
+    const ColumnCut c = column_cut(M, N, C);
+    const dim3 grid(c.blocks, (unsigned)c.parts);
+    const bool da = ((uintptr_t)dy & 15) == 0 && ld % C == 0, za = ((uintptr_t)z & 15) == 0 && N % C == 0;
+#define PNGPD_GRAD_ROWS(A, W) \
+    grad_rows_kernel<T, A, W><<<grid, 256, 0, s>>>(M, N, (const T*)dy, ld, da, (const T*)z, za, (T*)dz, ld_dz, part, c.lanes, c.rows, scale, (T*)sums)
+    switch (act) {
+        case PNGPD_ACT_NONE:
+            if (dz) PNGPD_GRAD_ROWS(PNGPD_ACT_NONE, true);
+            else PNGPD_GRAD_ROWS(PNGPD_ACT_NONE, false);
+            break;
+        case PNGPD_ACT_RELU: PNGPD_GRAD_ROWS(PNGPD_ACT_RELU, true); break;
+        case PNGPD_ACT_GELU: PNGPD_GRAD_ROWS(PNGPD_ACT_GELU, true); break;
+        case PNGPD_ACT_GELU_TANH: PNGPD_GRAD_ROWS(PNGPD_ACT_GELU_TANH, true); break;
+        case PNGPD_ACT_SILU: PNGPD_GRAD_ROWS(PNGPD_ACT_SILU, true); break;
+        default: return hipErrorInvalidValue;
+    }
+#undef PNGPD_GRAD_ROWS
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !sums || c.parts == 1) return e;
+    col_join_kernel<T><<<(unsigned)((N + 31) / 32), 256, 0, s>>>((int)c.parts, N, part, scale, (T*)sums);
     return hipGetLastError();
 }
 
@@ -437,16 +506,12 @@ hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOpe
                         const HeadEpilogue& e, float* partial, hipStream_t s) {
     PNGPD_BY_TYPE((product<T>(type, M, N, K, a, b, e, partial, s)))
 }
-hipError_t head_lay_out(int type, int64_t rows, int64_t cols, const void* src, int64_t ld_src, const float* weight, void* dst,
-                        int64_t ld, hipStream_t s) {
-    PNGPD_BY_TYPE((lay_out<T>(rows, cols, src, ld_src, weight, dst, ld, s)))
+hipError_t head_set_up(int type, const HeadLayOut* a, const HeadLayOut* b, const HeadRowWeights* w, hipStream_t s) {
+    PNGPD_BY_TYPE((set_up<T>(a, b, w, s)))
 }
 hipError_t head_grad_rows(int type, int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz,
-                          int64_t ld_dz, float* part, hipStream_t s) {
-    PNGPD_BY_TYPE((grad_rows<T>(M, N, dy, ld, z, act, dz, ld_dz, part, s)))
-}
-hipError_t head_col_join(int type, int64_t M, int64_t N, const float* part, const float* scale, void* out, hipStream_t s) {
-    PNGPD_BY_TYPE((col_join<T>(M, N, part, scale, out, s)))
+                          int64_t ld_dz, float* part, const float* scale, void* sums, hipStream_t s) {
+    PNGPD_BY_TYPE((grad_rows<T>(M, N, dy, ld, z, act, dz, ld_dz, part, scale, sums, s)))
 }
 
 }  // namespace pngpd
