@@ -19,7 +19,16 @@ __device__ __forceinline__ T from_f32(float v) { return (T)v; }      // rounds t
 // act(z) and act'(z).  gelu: z Phi(z); gelu_tanh: z sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3), which is
 // 0.5 z (1 + tanh u) without tanh's cancellation for large negative z; silu: z sigmoid(z).  z = -inf gives 0 and slope
 // 0 in all of them (the limits; the plain formulas give -inf * 0), NaN stays NaN.
-__device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_f(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + exp2_f(-LOG2E * v)); }
+// z times a gate that has reached 0 where z is -inf (NaN stays in the gate)
+__device__ __forceinline__ float gated(float z, float gate) { return __builtin_fmaxf(z, -3.0e38f) * gate; }
+// sigmoid(2u), u = sqrt(2/pi) (z + 0.044715 z^3)
+__device__ __forceinline__ float gelu_gate(float z) {
+    const float k = -2.f * LOG2E * 0.7978845608028654f;
+    return __builtin_amdgcn_rcpf(1.f + exp2_f(z * __builtin_fmaf(k * 0.044715f, z * z, k)));
+}
 
 constexpr float GELU_C = 0.7978845608028654f;      // sqrt(2 / pi)
 
@@ -27,7 +36,7 @@ constexpr float GELU_C = 0.7978845608028654f;      // sqrt(2 / pi)
 // erfcx's scaled form in t, reweighted towards equal relative error over |z| <= 14 (4e-8 in exact arithmetic, 2.7e-7 in
 // 32 bits); one exponential and one reciprocal, where the library's erfcf takes some 60 instructions.
 __device__ __forceinline__ float normal_cdf(float z, float* bell) {
-    const float e = __expf(-0.5f * z * z);
+    const float e = exp2_f(-0.5f * LOG2E * z * z);
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.2969848480983499f, __builtin_fabsf(z), 1.f));
     float q = 0.0391947381f;
     q = __builtin_fmaf(q, t, -0.178475707f);
@@ -48,12 +57,11 @@ __device__ __forceinline__ float act_f(float z) {
     if constexpr (ACT == PNGPD_ACT_RELU) return z < 0.f ? 0.f : z;
     if constexpr (ACT == PNGPD_ACT_GELU) {
         float bell;
-        const float y = z * normal_cdf(z, &bell);
-        return z == -__builtin_inff() ? 0.f : y;
+        return gated(z, normal_cdf(z, &bell));
     }
     if constexpr (ACT == PNGPD_ACT_GELU_TANH)
-        return z == -__builtin_inff() ? 0.f : z * sigmoid_f(2.f * GELU_C * (z + 0.044715f * z * z * z));
-    if constexpr (ACT == PNGPD_ACT_SILU) return z == -__builtin_inff() ? 0.f : z * sigmoid_f(z);
+        return gated(z, gelu_gate(z));
+    if constexpr (ACT == PNGPD_ACT_SILU) return gated(z, sigmoid_f(z));
     return z;
 }
 
@@ -67,7 +75,7 @@ __device__ __forceinline__ float act_slope(float z) {
         return __builtin_fabsf(z) > 16.f ? (z > 0.f ? 1.f : 0.f) : __builtin_fmaf(z * 0.3989422804014327f, bell, s);
     }
     if constexpr (ACT == PNGPD_ACT_GELU_TANH) {
-        const float s = sigmoid_f(2.f * GELU_C * (z + 0.044715f * z * z * z));
+        const float s = gelu_gate(z);
         const float v = s + z * s * (1.f - s) * 2.f * GELU_C * (1.f + 0.134145f * z * z);
         return __builtin_fabsf(z) > 16.f ? (z > 0.f ? 1.f : 0.f) : v;
     }

@@ -216,6 +216,14 @@ __device__ __forceinline__ void act8(Eight& a) {
     for (int i = 0; i < 8; ++i) a.v[i] = act_f<ACT>(a.v[i]);
 }
 
+// exp(z - base).  16-bit operands: in one fma, whose rounded LOG2E base is off by 2^-24 of itself (a relative 1e-6 of the result
+// for |base| = 10, far below the operands' 2^-9); floats: the difference first, which is exact for z near base.
+template <typename E>
+__device__ __forceinline__ float exp_of(float z, float base) {
+    if constexpr (sizeof(E) == 2) return exp2_f(__builtin_fmaf(LOG2E, z, -LOG2E * base));
+    return exp2_f(LOG2E * (z - base));
+}
+
 // The epilogue of 8 neighbouring sums of a row, in the order a latency-bound loop wants it: what depends on the columns is
 // loaded once (Columns), what depends on the row for several rows ahead (Ahead), then the sums are finished.
 struct Columns {
@@ -279,13 +287,19 @@ __device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_
         if (e.residual) add8(a, h.more);
         store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
     } else if constexpr (KIND == TILE_DZ) {
-        // the columns between N and the row's end are the zeros behind a dense extent
-        const int real = (int)(N - n < 8 ? N - n : 8);
-        add8(a, col.bias);
+        // What only some rows or columns have stands in branches of its own: an instruction on every element costs half a
+        // microsecond a tile.
+        if (e.bias) add8(a, col.bias);
+        const float gone = e.smooth * h.weight;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float p = __expf(a.v[i] - h.lse) - e.smooth - (h.label == i ? e.one_minus_eps : 0.f);
-            a.v[i] = h.weight == 0.f || i >= real ? 0.f : p * h.weight;
+        for (int i = 0; i < 8; ++i) a.v[i] = __builtin_fmaf(exp_of<E>(a.v[i], h.lse), h.weight, -gone);
+        if (h.label >= 0) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a.v[i] = h.label == i ? __builtin_fmaf(-e.one_minus_eps, h.weight, a.v[i]) : a.v[i];
+        }
+        if (h.weight == 0.f || N - n < 8) {      // ignored rows; the columns between N and the row's end are the zeros behind it
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a.v[i] = h.weight == 0.f || n + i >= N ? 0.f : a.v[i];
         }
         store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
     } else {
@@ -483,7 +497,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
 #pragma unroll
             for (int i = 0; i < FN; ++i)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s += __expf(acc[i][j][c] - base);
+                for (int c = 0; c < 4; ++c) s += exp_of<E>(acc[i][j][c], base);
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
             if (q == 0) share[wn * BM + r] = make_float4(mx, s, zs, 0.f);
