@@ -55,17 +55,36 @@ __device__ __forceinline__ f32x4 mma16(const i32x4& a, const i32x4& b, f32x4 c) 
     }
 }
 
-// 16 bytes a lane from global memory to LDS at m0 + lane * 16.  Written out because the compiler holds back transposing
-// LDS reads until every such load it knows of has landed, those into the other half of LDS included; stage_wait() is the
-// wait that the data needs.  No register receives anything; m0 holds nothing else in these kernels (the compiler sets it in
-// front of each use of its own).
-__device__ __forceinline__ void stage_load(unsigned lds, unsigned voff, const i32x4& rsrc) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rsrc) : "memory");
+// N pieces of 16 bytes a lane from global memory to LDS, the i-th at lds + i * STRIDE + lane * 16.  Written out because the
+// compiler holds back transposing LDS reads until every such load it knows of has landed, those into other stages included;
+// stage_wait() is the wait that the data needs.  No register receives anything; m0 holds nothing else in these kernels (the
+// compiler sets it in front of each use of its own).
+template <int N, int STRIDE>
+__device__ __forceinline__ void stage_load(unsigned lds, const unsigned* voff, const i32x4& rsrc) {
+#define PNGPD_FIRST "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+#define PNGPD_NEXT(v) "\n\ts_add_u32 m0, m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 " v ", %2, 0 offen lds"
+    if constexpr (N == 1) {
+        asm volatile(PNGPD_FIRST : : "s"(lds), "v"(voff[0]), "s"(rsrc) : "memory");
+    } else if constexpr (N == 2) {
+        asm volatile(PNGPD_FIRST PNGPD_NEXT("%4") : : "s"(lds), "v"(voff[0]), "s"(rsrc), "n"(STRIDE), "v"(voff[1]) : "memory", "scc");
+    } else {
+        static_assert(N == 4, "pieces of a wave");
+        asm volatile(PNGPD_FIRST PNGPD_NEXT("%4") PNGPD_NEXT("%5") PNGPD_NEXT("%6")
+                     :
+                     : "s"(lds), "v"(voff[0]), "s"(rsrc), "n"(STRIDE), "v"(voff[1]), "v"(voff[2]), "v"(voff[3])
+                     : "memory", "scc");
+    }
+#undef PNGPD_FIRST
+#undef PNGPD_NEXT
 }
-// All but the wave's last AHEAD loads have landed, and its LDS reads; then the barrier.
+// All but the wave's last AHEAD loads have landed, and its LDS reads; then the barrier.  By the builtins, so that the compiler
+// knows that nothing read from LDS is outstanding.
 template <int AHEAD>
 __device__ __forceinline__ void stage_wait() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(AHEAD) : "memory");
+    asm volatile("" : : : "memory");
+    __builtin_amdgcn_s_waitcnt((AHEAD & 15) | 7 << 4 | (AHEAD >> 4) << 14);      // vmcnt(AHEAD) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" : : : "memory");
 }
 
 __device__ __forceinline__ i32x4 make_rsrc(const char* p, int bytes) {
@@ -78,8 +97,9 @@ __device__ __forceinline__ i32x4 make_rsrc(const char* p, int bytes) {
     return r;
 }
 
-// Nothing is scheduled across a part's border: the compiler would otherwise keep more fragments alive than fit.
-__device__ __forceinline__ void part_begins() { __builtin_amdgcn_sched_barrier(0); }
+// Keeps the order of what stands before and behind: the compiler would otherwise put the reads next to their uses, to save
+// registers, and the loads together.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
 
 // One operand of a tile: R rows, its loads and its fragment reads.  WAVES waves share the loads.
 template <typename E, int R, bool KC, int WAVES>
@@ -88,13 +108,8 @@ struct TileOperand {
     static constexpr int PER_WAVE = PIECES / WAVES;
     static_assert(PIECES % WAVES == 0, "every wave issues as many loads");
     static constexpr int ROW_BYTES = R * SZ;             // of one contraction step, rows dense
-    // A wave's pieces are WAVES apart.  Where that distance leaves the permutation as it is, they differ by a uniform number
-    // of bytes, which goes into the descriptor: one offset register instead of one a piece.
-    static constexpr int APART = KC ? WAVES * 8 : WAVES * 1024 / ROW_BYTES;      // rows, or contraction steps
-    static constexpr bool UNIFORM = KC || (SZ == 2 && APART % 16 == 0);
-    static constexpr int OFFSETS = UNIFORM ? 1 : PER_WAVE;
-    unsigned voff[OFFSETS];
-    unsigned beyond;                                     // bit 31: the lane's chunk lies beyond the contraction in the last step
+    unsigned voff[PER_WAVE];                             // of the wave's pieces, WAVES apart
+    unsigned beyond;                                     // bit 31: the lane's chunk lies beyond the contraction in its last step
 
     // permutation of the chunk index of contraction step k (rows dense): in units of the columns one read takes, 2 chunks
     // (16 columns of 16 bits) or 4 (16 floats)
@@ -106,7 +121,7 @@ struct TileOperand {
     __device__ __forceinline__ void init(int wave, int lane, int64_t ld) {
         beyond = 0;
 #pragma unroll
-        for (int i = 0; i < OFFSETS; ++i) {
+        for (int i = 0; i < PER_WAVE; ++i) {
             const int o = (wave + i * WAVES) * 1024 + lane * 16;
             if constexpr (KC) {
                 const int row = o / 128, c = ((o / 16) & 7) ^ (row & 7);
@@ -132,15 +147,13 @@ struct TileOperand {
         constexpr int C = 16 / SZ;
         const int here = left < STEP ? left : STEP;
         const int bytes = KC ? (int)((rows - 1) * ld) + (here + C - 1) / C * 16 : (int)((here - 1) * ld) + (rows + C - 1) / C * 16;
-        const unsigned last = KC && left < STEP ? 0x80000000u : 0u;
+        const i32x4 rsrc = make_rsrc(base, left > 0 ? bytes : 0);
+        stage_load<PER_WAVE, WAVES * 1024>(lds + wave * 1024, voff, rsrc);
+    }
+    // From the last step on, if it is not a whole one: its chunks beyond the contraction become offsets beyond the descriptor.
+    __device__ __forceinline__ void mask_tail() {
 #pragma unroll
-        for (int i = 0; i < PER_WAVE; ++i) {
-            const unsigned skip = UNIFORM ? i * APART * ld : 0;
-            unsigned v = voff[UNIFORM ? 0 : i];
-            if constexpr (KC) v |= beyond & last;
-            const int rest = left > 0 ? bytes - (int)skip : 0;
-            stage_load(lds + (wave + i * WAVES) * 1024, v, make_rsrc(base + skip, rest > 0 ? rest : 0));
-        }
+        for (int i = 0; i < PER_WAVE; ++i) voff[i] |= beyond;
     }
     // fragment of 16 rows from row0 (a multiple of 16), part ks (0 or 1) of the step
     __device__ static __forceinline__ i32x4 frag(const char* lds, int row0, int ks, int lane) {
@@ -371,8 +384,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
 
     // Four parts a step: the two halves of the step's contraction, and of the wave's m fragments in each.  While the matrix
     // unit works on one part, the fragments of the next one come out of LDS.  The last part is carried over the barrier: its
-    // fragments are in registers by then, so the matrix unit has work while the next step's first ones arrive, and the loads
-    // after next go into the half of LDS that nobody reads any more.
+    // fragments are in registers by then, so the matrix unit has work while the next step's first ones arrive.  The step's
+    // loads stand between the matrix instructions of the first two parts: in a row at its start they keep all waves waiting
+    // for the memory unit to take them (8192 x 4096 x 2048 with 256 x 256 tiles: 125 us), behind the middle they arrive too
+    // late (136 us); so 120 us, and 170 instead of 180 us for 8192 x 8192 x 2048 on zeros, where the clock is not held back.
     constexpr int H = FM / 2;
     static_assert(FM % 2 == 0, "two halves of the m fragments");
     int left = (int)(k_end - k_begin);
@@ -385,26 +400,39 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
 #pragma unroll
         for (int i = 0; i < FN; ++i) f[i] = OpB::frag(base + BM * 128, (wn * FN + i) * 16, ks, lane);
     };
-    const auto multiply = [&](int half, const i32x4* a, const i32x4* b) {
+    // one half of the n fragments with one half of the m fragments
+    const auto multiply = [&](int half, const i32x4* a, const i32x4* b, int part) {
 #pragma unroll
-        for (int i = 0; i < FN; ++i)
+        for (int i = part * FN / 2; i < (part + 1) * FN / 2; ++i)
 #pragma unroll
             for (int j = 0; j < H; ++j) acc[i][half * H + j] = mma16<E>(b[i], a[j], acc[i][half * H + j]);
     };
     const unsigned lda = (unsigned)g.lda, ldb = (unsigned)g.ldb;
     constexpr int AHEAD = (RING - 2) * (OpA::PER_WAVE + OpB::PER_WAVE);
+    if (left < STEP) {
+        oa.mask_tail();
+        ob.mask_tail();
+    }
     int ahead = left;                      // what is left of the contraction where the next load starts
     unsigned into = 0, from = 0;           // stages the next load fills and the next step reads
-    const auto load_next = [&]() {
-        oa.load(pa, lda, ahead, rows_m, lds0 + into, wave);
-        ob.load(pb, ldb, ahead, rows_n, lds0 + into + BM * 128, wave);
+    const auto load_a = [&]() { oa.load(pa, lda, ahead, rows_m, lds0 + into, wave); };
+    const auto load_b = [&]() { ob.load(pb, ldb, ahead, rows_n, lds0 + into + BM * 128, wave); };
+    const auto advance = [&]() {
         ahead -= STEP;
         pa += step_a;
         pb += step_b;
         into = into == (RING - 1) * STAGE ? 0 : into + STAGE;
+        if (ahead < STEP) {
+            oa.mask_tail();
+            ob.mask_tail();
+        }
     };
 #pragma unroll
-    for (int i = 0; i < RING - 1; ++i) load_next();
+    for (int i = 0; i < RING - 1; ++i) {
+        load_a();
+        load_b();
+        advance();
+    }
     // before the first step the carried part is zeros
 #pragma unroll
     for (int j = 0; j < H; ++j) fa[1][j] = i32x4{0, 0, 0, 0};
@@ -418,22 +446,37 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
         left -= STEP;
         read_b(sa, 0, fb[0]);
         read_a(sa, 0, 0, fa[0]);
-        load_next();
-        multiply(1, fa[1], fb[1]);
-        part_begins();
+        fence();
+        multiply(1, fa[1], fb[1], 0);
+        fence();
+        load_a();
+        fence();
+        multiply(1, fa[1], fb[1], 1);
+        fence();
         read_a(sa, 0, 1, fa[1]);
-        multiply(0, fa[0], fb[0]);
-        part_begins();
+        fence();
+        multiply(0, fa[0], fb[0], 0);
+        fence();
+        load_b();
+        fence();
+        multiply(0, fa[0], fb[0], 1);
+        fence();
         read_b(sa, 1, fb[1]);
         read_a(sa, 1, 0, fa[0]);
-        multiply(1, fa[1], fb[0]);
-        part_begins();
+        fence();
+        multiply(1, fa[1], fb[0], 0);
+        multiply(1, fa[1], fb[0], 1);
+        fence();
         read_a(sa, 1, 1, fa[1]);
-        multiply(0, fa[0], fb[1]);
-        part_begins();
+        fence();
+        multiply(0, fa[0], fb[1], 0);
+        multiply(0, fa[0], fb[1], 1);
+        advance();
+        fence();
         stage_wait<AHEAD>();
     } while (left > 0);
-    multiply(1, fa[1], fb[1]);
+    multiply(1, fa[1], fb[1], 0);
+    multiply(1, fa[1], fb[1], 1);
     // zeros still on their way into LDS must not meet what the epilogue puts there
     if (AHEAD > 0) asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
 
