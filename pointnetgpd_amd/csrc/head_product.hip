@@ -437,20 +437,20 @@ size_t head_col_parts(int type, int64_t M, int64_t N) { return (size_t)column_cu
 
 namespace {
 
-// What a step of 128 bytes a row takes, in microseconds, with k tiles of a shape on every compute unit (measured over 32 to
-// 96 steps on 256 units, operands of normal numbers; 1.2 to 1.4 PFLOP/s for 256 x 256 tiles of 16-bit elements, 1.1 for
-// 128 x 128, 0.65 for the small ones, 0.14 for floats).
+// What a step of 128 bytes a row takes, in microseconds, with k tiles of a shape on every compute unit (measured on 256
+// units, operands of normal numbers: 1.2 PFLOP/s for 256 x 256 tiles of 16-bit elements, 0.95 for 128 x 128 over matrices
+// that the L2 does not hold - 1.28 where it does -, 0.6 to 0.7 for the small ones, 0.14 for floats).
 double step_us(bool f32, int shape, int64_t k) {
     const double n = (double)k;
     if (f32) {
-        if (shape == SHAPE_128) return 1.9 * n;
-        return k <= 1 ? 0.6 : 0.49 * n;
+        if (shape == SHAPE_128) return 1.83 * n;
+        return k <= 1 ? 0.58 : 0.48 * n;
     }
     switch (shape) {
-        case SHAPE_256: return k <= 1 ? 1.75 : 1.6 * n;
-        case SHAPE_128: return k <= 1 ? 0.65 : 1.02 * (double)((k + 1) / 2);
-        case SHAPE_64: return k <= 1 ? 0.29 : 0.205 * n;
-        default: return k <= 1 ? 0.33 : 0.25 * n;
+        case SHAPE_256: return 1.7 * n;
+        case SHAPE_128: return k <= 1 ? 0.55 : 1.1 * (double)((k + 1) / 2);
+        case SHAPE_64: return k <= 1 ? 0.27 : 0.194 * n;
+        default: return k <= 1 ? 0.31 : 0.235 * n;
     }
 }
 // What a tile takes besides: its first loads and its epilogue.
