@@ -7,6 +7,7 @@ from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpngpd.so")
+HEAD_PATH = os.path.join(_HERE, "_head.so")
 
 OK = 0
 FP32, BF16, BF16X3 = 0, 1, 2
@@ -29,6 +30,7 @@ class PngpdError(RuntimeError):
 
 
 _lib = None
+_head = None
 
 # name -> (restype, argtypes): every symbol include/pngpd.h declares
 SIGNATURES = {
@@ -114,6 +116,19 @@ def load() -> ctypes.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def load_head():
+    """The autograd nodes of the classification-head operators (csrc/head_torch.cpp), which call the library."""
+    global _head
+    if _head is None:
+        load()
+        if not os.path.exists(HEAD_PATH):
+            raise ImportError(f"{HEAD_PATH} not found: it has not been built "
+                              "(python -c 'import __graft_entry__ as g; g.build()'); there is no other path")
+        from . import _head as module
+        _head = module
+    return _head
 
 
 def check(rc: int) -> None:

@@ -86,6 +86,28 @@ def build_library(force: bool = False, verbose_resources: bool = False) -> str:
     return LIB_PATH
 
 
+HEAD_PATH = os.path.join(ROOT, "pointnetgpd_amd", "_head.so")
+
+
+def build_head(force: bool = False) -> str:
+    """The autograd nodes of the classification-head operators: host code against torch's headers, linked to libpngpd.so."""
+    import sysconfig
+
+    import torch
+
+    src = os.path.join(CSRC, "head_torch.cpp")
+    if force or _newer(HEAD_PATH, [src, os.path.join(ROOT, "include", "pngpd.h"), os.path.abspath(__file__)]):
+        base = os.path.dirname(torch.__file__)
+        rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", os.path.join(ROOT, "include"),
+              "-isystem", os.path.join(base, "include"), "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
+              "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(rocm, "include"), src, "-o", HEAD_PATH,
+              "-L", os.path.join(base, "lib"), "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lamdhip64",
+              "-L", os.path.dirname(LIB_PATH), "-lpngpd", "-Wl,-rpath,$ORIGIN"])
+    return HEAD_PATH
+
+
 def build_probe(force: bool = False) -> str:
     src = os.path.join(ROOT, "tests", "csrc", "probe.hip")
     if force or _newer(PROBE_PATH, [src]):
@@ -123,6 +145,7 @@ def build_example(force: bool = False) -> str:
 
 def build_all(force: bool = False) -> None:
     build_library(force)
+    build_head(force)
     build_example(force)
     build_probe(force)
     build_oracle_c(force)

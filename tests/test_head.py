@@ -98,6 +98,13 @@ def test_workspace_sizes_are_bounded_and_grow_with_no_logits():
     assert lib.pngpd_linear_workspace_bytes(5, 1, 1, 1, 0, 1) == 0
 
 
+def test_a_missing_binding_is_an_error(monkeypatch, tmp_path):
+    monkeypatch.setattr(_lib, "_head", None)
+    monkeypatch.setattr(_lib, "HEAD_PATH", str(tmp_path / "_head.so"))
+    with pytest.raises(ImportError, match="not found"):
+        _lib.load_head()
+
+
 # ---- the restatement itself -----------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("name", [None, "relu", "gelu", "gelu_tanh", "silu"])

@@ -601,3 +601,83 @@ def test_refusals_on_the_device():
     dx, = torch.autograd.grad(y.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):                     # differentiable once
         torch.autograd.grad(dx.sum() + 0 * y.sum(), w.requires_grad_())
+
+
+def calls_of(x, w, b, target):
+    return (lambda: head.linear(x, w, b, activation="silu"), lambda: head.dropout(x, 0.25, 5),
+            lambda: head.linear_cross_entropy(x, w, target, b))
+
+
+def test_a_captured_backward_with_an_eager_graph_alive_raises():
+    x, w, b = (t.cuda().requires_grad_() for t in make(90, (32, 24), (40, 24), (40,)))
+    target = torch.randint(0, 40, (32,), generator=torch.Generator().manual_seed(9)).cuda()
+    for call in calls_of(x, w, b, target):
+        want, = torch.autograd.grad(call().sum(), x)                       # its graph ends here
+        kept = call()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            y = call()
+            with pytest.raises(RuntimeError, match="eager graph"):
+                torch.autograd.grad(y, x, torch.ones_like(y))
+        del kept, y, g
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            y = call()
+            dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        for _ in range(3):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(dx, want)
+        del y, g
+
+
+def test_eager_steps_on_other_streams_than_their_leaves():
+    """An eager backward pass whose leaves have a graph on another stream: the engine waits, nothing is refused."""
+    x, w, b = (t.cuda().requires_grad_() for t in make(91, (64, 24), (40, 24), (40,)))
+    target = torch.randint(0, 40, (64,), generator=torch.Generator().manual_seed(9)).cuda()
+    for call in calls_of(x, w, b, target):
+        kept = call()
+        want, = torch.autograd.grad(call().sum(), x)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got, = torch.autograd.grad(call().sum(), x)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and kept.shape == call().shape
+
+
+def test_forward_mode_is_refused():
+    x, w, b = (t.cuda() for t in make(92, (4, 24), (40, 24), (40,)))
+    target = torch.zeros(4, dtype=torch.int64, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in calls_of(dual, w, b, target):
+            with pytest.raises(RuntimeError):
+                call()
+
+
+def test_gradients_of_some_inputs_of_a_call():
+    """Each subset of the inputs that need gradients gives those inputs the same ones."""
+    x, w, b, r = (t.cuda() for t in make(93, (48, 24), (40, 24), (40,), (48, 40)))
+    target = torch.randint(0, 40, (48,), generator=torch.Generator().manual_seed(9)).cuda()
+    ops = (lambda x, w, b, r: head.linear(x, w, b, "gelu", r), lambda x, w, b, r: head.linear_cross_entropy(x, w, target, b),
+           lambda x, w, b, r: head.dropout(r, 0.25, 5, residual=x @ w.t()))
+    for op, uses in zip(ops, ("xwbr", "xwb", "xwr")):
+        full = {n: t.clone().requires_grad_() for n, t in zip("xwbr", (x, w, b, r))}
+        want = dict(zip(uses, torch.autograd.grad(op(**full).sum(), [full[n] for n in uses])))
+        for mask in range(1, 2 ** len(uses)):
+            chosen = [n for i, n in enumerate(uses) if mask >> i & 1]
+            some = {n: t.clone().requires_grad_(n in chosen) for n, t in zip("xwbr", (x, w, b, r))}
+            for n, grad in zip(chosen, torch.autograd.grad(op(**some).sum(), [some[n] for n in chosen])):
+                assert torch.equal(grad, want[n]), (uses, chosen, n)
+
+
+def test_limits_raise_the_librarys_error():
+    from pointnetgpd_amd._lib import PngpdError
+    w = torch.zeros(1, 1, device="cuda").expand(2 ** 21 + 1, 4)
+    with pytest.raises(PngpdError) as e:
+        head.linear(torch.zeros(2, 4, device="cuda"), w)
+    assert e.value.code != 0 and "pngpd_linear_forward" in str(e.value)
