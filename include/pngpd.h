@@ -420,28 +420,32 @@ int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64
                   void* y_dev, double p, uint64_t seed, uint64_t offset, const int64_t* rng_dev, void* stream);
 
 /*
- * Cross entropy of softmax(x[T,D] weight[V,D]^T + bias[V]) without the [T,V] logits ever being stored whole: they are
- * formed in pieces of the vocabulary, and every row keeps its running maximum and sum.
+ * Cross entropy of softmax(x[T,D] weight[V,D]^T + bias[V]) without the [T,V] logits having to be stored whole: they
+ * are formed in pieces of the vocabulary, and every row keeps its running maximum and sum.
  *   loss_t = lse_t - (1 - label_smoothing) z[t, target_t] - label_smoothing / V * sum_v z[t, v]
  * Rows whose target is ignore_index have loss 0 and no gradient, whatever they hold.  Any other target outside [0, V)
  * is not used as an index: its loss is NaN and its row contributes no gradient (as pngpd_nll_loss does).
  * loss_dev: float [T] for PNGPD_REDUCE_NONE, else float [1] (the mean is over the rows that are not ignored: NaN when
  * there are none).  lse_dev float [T]: log sum exp of every row's logits, what the backward pass needs.
+ * kept_dev: NULL, or pngpd_linear_cross_entropy_kept_bytes of memory (16-byte aligned) that carries what the backward
+ * pass of the same sizes would otherwise compute again: float32 logits of at most 256 MiB, or as much as x and weight
+ * take.  Its size is 0 where nothing is kept, always for 16-bit types.
  */
 size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V, int64_t D, int backward, int aligned);
+size_t pngpd_linear_cross_entropy_kept_bytes(int type, int64_t T, int64_t V, int64_t D);
 int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D, const void* x_dev, int64_t ldx,
                                        const void* weight_dev, int64_t ldw, const void* bias_dev, const int64_t* target_dev,
                                        int64_t ignore_index, float label_smoothing, int reduction, float* loss_dev,
-                                       float* lse_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
+                                       float* lse_dev, void* kept_dev, void* workspace_dev, size_t workspace_bytes, void* stream);
 
 /*
  * Gradients of the forward call with the same arguments: dloss_dev float [T] (PNGPD_REDUCE_NONE) or [1] -> dx_dev
- * [T,D], dweight_dev [V,D], dbias_dev [V], each optional.  The logits are formed again piece by piece.
+ * [T,D], dweight_dev [V,D], dbias_dev [V], each optional.  Without kept_dev the logits are formed again piece by piece.
  */
 int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t D, const void* x_dev, int64_t ldx,
                                         const void* weight_dev, int64_t ldw, const void* bias_dev, const int64_t* target_dev,
                                         int64_t ignore_index, float label_smoothing, int reduction, const float* lse_dev,
-                                        const float* dloss_dev, void* dx_dev, void* dweight_dev, void* dbias_dev,
+                                        const void* kept_dev, const float* dloss_dev, void* dx_dev, void* dweight_dev, void* dbias_dev,
                                         void* workspace_dev, size_t workspace_bytes, void* stream);
 
 /*

@@ -89,12 +89,13 @@ SIGNATURES = {
     "pngpd_dropout": (c_int, [c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_double, c_uint64,
                               c_uint64, c_void_p, c_void_p]),
     "pngpd_linear_cross_entropy_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int, c_int]),
+    "pngpd_linear_cross_entropy_kept_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
     "pngpd_linear_cross_entropy_forward": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                                    c_void_p, c_void_p, c_int64, c_float, c_int, c_void_p, c_void_p, c_void_p,
-                                                   c_size_t, c_void_p]),
+                                                   c_void_p, c_size_t, c_void_p]),
     "pngpd_linear_cross_entropy_backward": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                                     c_void_p, c_void_p, c_int64, c_float, c_int, c_void_p, c_void_p, c_void_p,
-                                                    c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+                                                    c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "pngpd_score": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p]),
 }
 

@@ -24,6 +24,9 @@ inline bool head_direct(const void* p, int64_t ld, int64_t extent, size_t size) 
     return ((uintptr_t)p & 15) == 0 && ld % c == 0 && extent % c == 0 && ld <= HEAD_MAX_LD / (int64_t)size;
 }
 
+// Partial sums lie in rows of whole 16-byte chunks.
+__host__ __device__ inline int64_t head_partial_ld(int64_t N) { return (N + 3) & ~(int64_t)3; }
+
 // What becomes of a product's 32-bit sums.
 enum { HEAD_EPI_LINEAR = 0, HEAD_EPI_DZ = 1, HEAD_EPI_SCALED = 2, HEAD_EPI_STATS = 3 };
 struct HeadEpilogue {
@@ -64,9 +67,12 @@ struct HeadPlan {
 };
 HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind);
 
-// partial: head_plan(...).partial_bytes
+// partial: head_plan(...).partial_bytes.  keep: the sums are left in partial (head_kept_bytes) and the statistics are one block
 hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b,
-                        const HeadEpilogue& e, float* partial, hipStream_t s);
+                        const HeadEpilogue& e, float* partial, bool keep, hipStream_t s);
+// Kept sums of a STATS product, and another epilogue from them.
+size_t head_kept_bytes(int type, int64_t M, int64_t N, int64_t K);
+hipError_t head_kept(int type, int64_t M, int64_t N, int64_t K, const HeadEpilogue& e, const float* kept, hipStream_t s);
 
 // dst[r][0 .. ld) = src[r][0 .. cols) and zeros behind them.  dst is 16-byte aligned, ld whole chunks.  With a target, rows
 // whose target is ignored or no class become zeros whatever they hold.

@@ -107,6 +107,8 @@ struct LinearWs {
     }
 };
 
+inline size_t loss_budget(int type, int64_t T, int64_t V, int64_t D) { return max2(PIECE_BYTES, ((size_t)T + (size_t)V) * (size_t)D * esize(type)); }
+
 struct LossWs {
     int64_t rows_at_once;      // rows whose statistics are formed at a time (forward)
     int64_t piece;             // columns of the vocabulary whose gradients are formed at a time
@@ -144,8 +146,7 @@ struct LossWs {
             row_loss = (float*)b.take((size_t)rows * 4);
             partial = (float*)b.take(cut);
         } else {
-            const size_t budget = max2(PIECE_BYTES, ((size_t)rows + (size_t)V) * (size_t)D * e);
-            piece = (int64_t)(budget / ((size_t)rows * e)) / 256 * 256;
+            piece = (int64_t)(loss_budget(type, rows, V, D) / ((size_t)rows * e)) / 256 * 256;
             if (piece < 256) piece = 256;
             if (piece > pngpd::HEAD_MAX_EXTENT) piece = pngpd::HEAD_MAX_EXTENT;
             if (piece > V) piece = V;
@@ -178,6 +179,18 @@ int check_loss(const char* who, int type, int64_t T, int64_t V, int64_t D, const
     if (!(eps >= 0.f && eps <= 1.f)) return fail(PNGPD_ERR_INVALID, "%s: label_smoothing %g", who, (double)eps);
     if (reduction < PNGPD_REDUCE_NONE || reduction > PNGPD_REDUCE_SUM) return fail(PNGPD_ERR_INVALID, "%s: unknown reduction %d", who, reduction);
     return PNGPD_OK;
+}
+
+// What the forward pass keeps for the backward pass, or 0: float32 logits (without the bias) where they are one piece of the
+// gradients' and forming them again takes longer than writing them once and reading them twice.  That is 2 D operations a
+// logit at 0.13 PFLOP/s against 12 bytes at 5 TB/s, equal at D = 160; the pass over them is a launch more, so 2^28 products
+// at least.  16-bit operands are multiplied ten times as fast and form their logits again.  Training 1023 x 1000 -> 10007
+// takes 581 us with its 41 MB kept, 684 without.
+size_t kept_bytes(int type, int64_t T, int64_t V, int64_t D) {
+    if (type != PNGPD_TYPE_F32 || T < 1 || D < 160 || (double)T * (double)V * (double)D < 268435456.0) return 0;
+    if (LossWs(nullptr, type, T, V, D, false, false, false).rows_at_once < T || LossWs(nullptr, type, T, V, D, true, false, false).piece < V) return 0;
+    const size_t bytes = pngpd::head_kept_bytes(type, T, V, D);
+    return bytes <= loss_budget(type, T, V, D) ? bytes : 0;
 }
 
 inline const void* at(const void* p, int64_t elements, int type) { return p ? (const char*)p + (size_t)elements * esize(type) : nullptr; }
@@ -220,7 +233,7 @@ int pngpd_linear_forward(int type, int64_t M, int64_t N, int64_t K, const void* 
     const Rows x = direct_rows(type, M, K, x_dev, ldx, ws.x, &job_x, &lay_x);
     const Rows w = direct_rows(type, N, K, weight_dev, ldw, ws.w, &job_w, &lay_w);
     HIP_TRY(pngpd::head_set_up(type, lay_x ? &job_x : nullptr, lay_w ? &job_w : nullptr, nullptr, s));
-    HIP_TRY(pngpd::head_product(type, M, N, K, HeadOperand{x.p, x.ld, true}, HeadOperand{w.p, w.ld, true}, e, ws.partial, s));
+    HIP_TRY(pngpd::head_product(type, M, N, K, HeadOperand{x.p, x.ld, true}, HeadOperand{w.p, w.ld, true}, e, ws.partial, false, s));
     return PNGPD_OK;
 }
 
@@ -261,11 +274,11 @@ int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void*
     e.ld_out = K;
     if (dx_dev) {
         e.out = dx_dev;
-        HIP_TRY(pngpd::head_product(type, M, K, N, HeadOperand{dz.p, dz.ld, true}, HeadOperand{w.p, w.ld, false}, e, ws.partial, s));
+        HIP_TRY(pngpd::head_product(type, M, K, N, HeadOperand{dz.p, dz.ld, true}, HeadOperand{w.p, w.ld, false}, e, ws.partial, false, s));
     }
     if (dweight_dev) {
         e.out = dweight_dev;
-        HIP_TRY(pngpd::head_product(type, N, K, M, HeadOperand{dz.p, dz.ld, false}, HeadOperand{x.p, x.ld, false}, e, ws.partial, s));
+        HIP_TRY(pngpd::head_product(type, N, K, M, HeadOperand{dz.p, dz.ld, false}, HeadOperand{x.p, x.ld, false}, e, ws.partial, false, s));
     }
     return PNGPD_OK;
 }
@@ -292,14 +305,21 @@ size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V
     return LossWs(nullptr, type, T, V, D, backward != 0, d, d).bytes;
 }
 
+size_t pngpd_linear_cross_entropy_kept_bytes(int type, int64_t T, int64_t V, int64_t D) {
+    const void* some = &type;
+    if (check_loss("pngpd_linear_cross_entropy_kept_bytes", type, T, V, D, some, D, some, D, (const int64_t*)some, 0.f, 0)) return 0;
+    return kept_bytes(type, T, V, D);
+}
+
 int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D, const void* x_dev, int64_t ldx,
                                        const void* weight_dev, int64_t ldw, const void* bias_dev, const int64_t* target_dev,
                                        int64_t ignore_index, float label_smoothing, int reduction, float* loss_dev,
-                                       float* lse_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
+                                       float* lse_dev, void* kept_dev, void* workspace_dev, size_t workspace_bytes, void* stream) {
     const char* who = "pngpd_linear_cross_entropy_forward";
     int rc = check_loss(who, type, T, V, D, x_dev, ldx, weight_dev, ldw, target_dev, label_smoothing, reduction);
     if (rc) return rc;
     if ((T > 0 || reduction != PNGPD_REDUCE_NONE) && !loss_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL loss", who);
+    if (((uintptr_t)kept_dev & 15) != 0) return fail(PNGPD_ERR_INVALID, "%s: kept must be aligned to 16 bytes", who);
     if (T > 0 && !lse_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL lse", who);
     hipStream_t s = (hipStream_t)stream;
     LossWs ws(workspace_dev, type, T, V, D, false, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
@@ -311,6 +331,7 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
         const Rows w = direct_rows(type, V, D, weight_dev, ldw, ws.w, &job_w, &lay_w);
         HIP_TRY(pngpd::head_set_up(type, lay_x ? &job_x : nullptr, lay_w ? &job_w : nullptr, nullptr, s));
         float* row_loss = reduction == PNGPD_REDUCE_NONE ? loss_dev : ws.row_loss;
+        float* kept = kept_bytes(type, T, V, D) ? (float*)kept_dev : nullptr;
         for (int64_t t = 0; t < T; t += ws.rows_at_once) {
             const int64_t n = T - t < ws.rows_at_once ? T - t : ws.rows_at_once;
             const bool whole = n == T;
@@ -322,8 +343,8 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
             e.target_logit = ws.target_logit;
             e.want_logit_sum = label_smoothing > 0.f;
             HIP_TRY(pngpd::head_product(type, n, V, D, HeadOperand{at(x.p, t * x.ld, type), x.ld, true}, HeadOperand{w.p, w.ld, true}, e,
-                                        ws.partial, s));
-            const int blocks = pngpd::head_plan(type, n, V, D, pngpd::HEAD_EPI_STATS).stats_blocks;
+                                        kept ? kept : ws.partial, kept != nullptr, s));
+            const int blocks = kept ? 1 : pngpd::head_plan(type, n, V, D, pngpd::HEAD_EPI_STATS).stats_blocks;
             HIP_TRY(pngpd::head_row_loss(n, V, blocks, ws.stats, ws.target_logit, target_dev + t, ignore_index, label_smoothing,
                                          row_loss + t, lse_dev + t, reduction,
                                          whole && reduction != PNGPD_REDUCE_NONE ? loss_dev : nullptr, s));
@@ -337,7 +358,7 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
 int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t D, const void* x_dev, int64_t ldx,
                                         const void* weight_dev, int64_t ldw, const void* bias_dev, const int64_t* target_dev,
                                         int64_t ignore_index, float label_smoothing, int reduction, const float* lse_dev,
-                                        const float* dloss_dev, void* dx_dev, void* dweight_dev, void* dbias_dev,
+                                        const void* kept_dev, const float* dloss_dev, void* dx_dev, void* dweight_dev, void* dbias_dev,
                                         void* workspace_dev, size_t workspace_bytes, void* stream) {
     const char* who = "pngpd_linear_cross_entropy_backward";
     int rc = check_loss(who, type, T, V, D, x_dev, ldx, weight_dev, ldw, target_dev, label_smoothing, reduction);
@@ -349,6 +370,8 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         return PNGPD_OK;
     }
     if (!lse_dev || !dloss_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL argument", who);
+    if (((uintptr_t)kept_dev & 15) != 0) return fail(PNGPD_ERR_INVALID, "%s: kept must be aligned to 16 bytes", who);
+    const float* kept = kept_bytes(type, T, V, D) ? (const float*)kept_dev : nullptr;
     LossWs ws(workspace_dev, type, T, V, D, true, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
     const HeadOperand x{ws.x, padded(D, type), true}, xt{ws.x, padded(D, type), false};
@@ -372,7 +395,8 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         e.one_minus_eps = 1.f - label_smoothing;
         e.out = ws.tile;
         e.ld_out = np;
-        HIP_TRY(pngpd::head_product(type, T, n, D, x, HeadOperand{w, whole.ld, true}, e, ws.partial, s));
+        if (kept) HIP_TRY(pngpd::head_kept(type, T, V, D, e, kept, s));
+        else HIP_TRY(pngpd::head_product(type, T, n, D, x, HeadOperand{w, whole.ld, true}, e, ws.partial, false, s));
         if (dbias_dev)
             HIP_TRY(pngpd::head_grad_rows(type, T, n, ws.tile, np, nullptr, PNGPD_ACT_NONE, nullptr, 0, ws.part, ws.scale,
                                           at(dbias_dev, v, type), s));
@@ -382,7 +406,7 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         if (dweight_dev) {
             g.out = at(dweight_dev, v * D, type);
             g.scale = ws.scale;
-            HIP_TRY(pngpd::head_product(type, n, D, T, HeadOperand{ws.tile, np, false}, xt, g, ws.partial, s));
+            HIP_TRY(pngpd::head_product(type, n, D, T, HeadOperand{ws.tile, np, false}, xt, g, ws.partial, false, s));
         }
         if (dx_dev) {
             const bool last = v + n == V;
@@ -390,7 +414,7 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
             g.out_f32 = !last;
             g.scale = last ? ws.scale : nullptr;
             g.out = last ? dx_dev : (void*)ws.dx_sum;
-            HIP_TRY(pngpd::head_product(type, T, D, n, HeadOperand{ws.tile, np, true}, HeadOperand{w, whole.ld, false}, g, ws.partial, s));
+            HIP_TRY(pngpd::head_product(type, T, D, n, HeadOperand{ws.tile, np, true}, HeadOperand{w, whole.ld, false}, g, ws.partial, false, s));
         }
     }
     return PNGPD_OK;

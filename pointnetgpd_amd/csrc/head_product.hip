@@ -12,7 +12,7 @@ namespace {
 // 8 neighbouring columns of a row a thread: the cuts of the contraction added in order, then the epilogue
 template <typename E, int KIND, int THREADS>
 __global__ __launch_bounds__(THREADS) void join_kernel(int64_t M, int64_t N, int64_t groups, int splits, const float* partial, HeadEpilogue e,
-                                                   bool vec, bool partial_vec) {
+                                                   bool vec) {
     const int64_t total = M * groups;
     for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * THREADS) {
         const int64_t m = i / groups, n = (i - m * groups) * 8;
@@ -20,14 +20,15 @@ __global__ __launch_bounds__(THREADS) void join_kernel(int64_t M, int64_t N, int
         const int valid = (int)(have < 0 ? 0 : have < 8 ? have : 8);
         Eight v = {};
 #pragma unroll 4
-        for (int s = 0; s < splits; ++s) add8(v, load8(partial + ((int64_t)s * M + m) * N + n, valid, partial_vec));
+        for (int s = 0; s < splits; ++s) add8(v, load8(partial + ((int64_t)s * M + m) * head_partial_ld(N) + n, valid, true));
         const int64_t room = (KIND == TILE_DZ ? e.ld_out : N) - n;
         const int real = (int)(room < 8 ? room : 8);
         finish8<E, KIND>(e, N, m, n, real, vec, load_columns<E, KIND>(e, N, n, vec), load_ahead<E, KIND>(e, N, m, n, real, vec), v);
     }
 }
 
-// a row a workgroup: statistics of its logits, formed from the cuts of the contraction
+// a row a workgroup: statistics of its logits, formed from the cuts of the contraction.  Eight logits at a time share one
+// rescaling of the sum; 1023 rows of 10007 sums (41 MB) take 12 us, 29 with one at a time.
 template <typename E>
 __global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, int splits, const float* partial, HeadEpilogue e) {
     __shared__ float4 share[4];
@@ -35,14 +36,24 @@ __global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, i
     const int64_t y = e.target[m];
     const E* bias = (const E*)e.bias;
     float mx = -__builtin_inff(), sum = 0.f, zs = 0.f;
-    for (int64_t n = threadIdx.x; n < N; n += 256) {
-        float z = 0.f;
-        for (int s = 0; s < splits; ++s) z += partial[((int64_t)s * M + m) * N + n];
-        if (bias) z += to_f32(bias[n]);
-        if (n == y) e.target_logit[m] = z;
-        zs += z;
-        const float top = __builtin_fmaxf(mx, z);
-        sum = sum * (mx == top ? 1.f : __expf(mx - top)) + (z == -__builtin_inff() ? 0.f : __expf(z - top));
+    const bool bias_vec = ((uintptr_t)bias & 15) == 0;
+    for (int64_t n = (int64_t)threadIdx.x * 8; n < N; n += 2048) {
+        const int valid = N - n < 8 ? (int)(N - n) : 8;
+        Eight z = {};
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s) add8(z, load8(partial + ((int64_t)s * M + m) * head_partial_ld(N) + n, valid, true));
+        if (bias) add8(z, load8(bias + n, valid, bias_vec));
+        float top = mx, part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i >= valid) z.v[i] = -__builtin_inff();
+            else zs += z.v[i];
+            if (n + i == y) e.target_logit[m] = z.v[i];
+            top = __builtin_fmaxf(top, z.v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) part += z.v[i] == -__builtin_inff() ? 0.f : __expf(z.v[i] - top);
+        sum = sum * (mx == top ? 1.f : __expf(mx - top)) + part;
         mx = top;
     }
     const float top = wave_max(mx);
@@ -65,15 +76,15 @@ __global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, i
 
 template <typename E>
 hipError_t join(int64_t M, int64_t N, int splits, const float* partial, const HeadEpilogue& e, hipStream_t s) {
-    const bool vec = epilogue_vec(e, N, sizeof(E)), pv = N % 4 == 0;
+    const bool vec = epilogue_vec(e, N, sizeof(E));
     const int64_t groups = ((e.kind == HEAD_EPI_DZ ? e.ld_out : N) + 7) / 8;
     // little to join: small workgroups, so that its loads leave from many compute units
     const bool few = M * groups < 65536;
     const int64_t threads = few ? 64 : 256, blocks = (M * groups + threads - 1) / threads;
     const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
 #define PNGPD_JOIN(KIND)                                                                                          \
-    if (few) join_kernel<E, KIND, 64><<<grid, 64, 0, s>>>(M, N, groups, splits, partial, e, vec, pv);              \
-    else join_kernel<E, KIND, 256><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e, vec, pv)
+    if (few) join_kernel<E, KIND, 64><<<grid, 64, 0, s>>>(M, N, groups, splits, partial, e, vec);              \
+    else join_kernel<E, KIND, 256><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e, vec)
     switch (e.kind) {
         case HEAD_EPI_LINEAR: PNGPD_JOIN(TILE_LINEAR); break;
         case HEAD_EPI_DZ: PNGPD_JOIN(TILE_DZ); break;
@@ -168,7 +179,7 @@ hipError_t rows(int M, int64_t N, int64_t K, const HeadOperand& a, const HeadOpe
 
 template <typename E>
 hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b, const HeadEpilogue& e,
-                   float* partial, hipStream_t s) {
+                   float* partial, bool keep, hipStream_t s) {
     if (M <= FEW_M && e.kind == HEAD_EPI_LINEAR) {
         if (M == 1) return rows<E, 1>((int)M, N, K, a, b, e, s);
         if (M == 2) return rows<E, 2>((int)M, N, K, a, b, e, s);
@@ -190,17 +201,18 @@ hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand&
     g.k_split = p.k_split;
     g.partial = partial;
     g.e = e;
-    const int kind = p.splits > 1 ? TILE_PARTIAL
+    const bool parts = p.splits > 1 || keep;
+    const int kind = parts ? TILE_PARTIAL
                      : e.kind == HEAD_EPI_LINEAR ? TILE_LINEAR
                      : e.kind == HEAD_EPI_DZ     ? TILE_DZ
                      : e.kind == HEAD_EPI_STATS  ? TILE_STATS
                                                  : TILE_SCALED;
-    const bool vec = p.splits > 1 ? N % 4 == 0 : epilogue_vec(e, N, sizeof(E));
+    const bool vec = parts || epilogue_vec(e, N, sizeof(E));
     hipError_t err;
     if constexpr (__is_same(E, float)) err = launch_tile_f32(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
     else if constexpr (__is_same(E, bf16_t)) err = launch_tile_bf16(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
     else err = launch_tile_f16(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
-    if (err != hipSuccess || p.splits == 1) return err;
+    if (err != hipSuccess || !parts) return err;
     return join<E>(M, N, p.splits, partial, e, s);
 }
 
@@ -490,7 +502,7 @@ HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
         }
     }
     p.stats_blocks = p.splits > 1 ? 1 : p.tiles_n;
-    p.partial_bytes = p.splits > 1 ? (size_t)p.splits * M * N * 4 : 0;
+    p.partial_bytes = p.splits > 1 ? (size_t)p.splits * M * head_partial_ld(N) * 4 : 0;
     return p;
 }
 
@@ -503,8 +515,15 @@ HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
     }
 
 hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b,
-                        const HeadEpilogue& e, float* partial, hipStream_t s) {
-    PNGPD_BY_TYPE((product<T>(type, M, N, K, a, b, e, partial, s)))
+                        const HeadEpilogue& e, float* partial, bool keep, hipStream_t s) {
+    PNGPD_BY_TYPE((product<T>(type, M, N, K, a, b, e, partial, keep, s)))
+}
+size_t head_kept_bytes(int type, int64_t M, int64_t N, int64_t K) {
+    return (size_t)head_plan(type, M, N, K, HEAD_EPI_STATS).splits * M * head_partial_ld(N) * 4;
+}
+hipError_t head_kept(int type, int64_t M, int64_t N, int64_t K, const HeadEpilogue& e, const float* kept, hipStream_t s) {
+    const int splits = head_plan(type, M, N, K, HEAD_EPI_STATS).splits;
+    PNGPD_BY_TYPE((join<T>(M, N, splits, kept, e, s)))
 }
 hipError_t head_set_up(int type, const HeadLayOut* a, const HeadLayOut* b, const HeadRowWeights* w, hipStream_t s) {
     PNGPD_BY_TYPE((set_up<T>(a, b, w, s)))

@@ -33,7 +33,7 @@ struct TileArgs {
     int64_t lda, ldb;           // bytes between rows (k_contiguous) or between contraction steps
     int tiles_m, tiles_n, splits;
     int64_t k_split;            // contraction elements a split takes (a multiple of a step)
-    float* partial;             // [split][M][N] when splits > 1
+    float* partial;             // [split][M][head_partial_ld(N)] when splits > 1 or the sums are kept
     HeadEpilogue e;
 };
 
@@ -599,7 +599,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
                     const f32x4 lo = *(const f32x4*)(smem + r * (BN * 4) + (c ^ (r & MIX)) * 16);
                     const f32x4 hi = *(const f32x4*)(smem + r * (BN * 4) + ((c + 1) ^ (r & MIX)) * 16);
                     Eight a = {{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
-                    if constexpr (KIND == TILE_PARTIAL) store8(g.partial + ((int64_t)split * g.M + m) * g.N + n, a, valid, vec);
+                    if constexpr (KIND == TILE_PARTIAL) store8(g.partial + ((int64_t)split * g.M + m) * head_partial_ld(g.N) + n, a, valid, vec);
                     else finish8<E, KIND>(g.e, g.N, m, n, valid, vec, col, ahead[k], a);
                 }
             }

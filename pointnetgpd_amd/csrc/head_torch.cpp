@@ -219,7 +219,7 @@ struct LossArgs {
 };
 
 at::Tensor loss_forward(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, const Maybe& bias, const LossArgs& a,
-                        at::Tensor* lse) {
+                        at::Tensor* lse, at::Tensor* kept) {
     const c10::OptionalDeviceGuard guard(x.device());
     const int64_t V = w.size(0), D = w.size(1), T = x.numel() / D;
     const int type = type_of(x);
@@ -228,20 +228,21 @@ at::Tensor loss_forward(const at::Tensor& x, const at::Tensor& w, const at::Tens
     const auto f32 = x.options().dtype(at::kFloat);
     at::Tensor loss = at::empty(a.reduction == PNGPD_REDUCE_NONE ? x.sizes().slice(0, x.dim() - 1) : at::IntArrayRef(), f32);
     *lse = at::empty({T}, f32);
+    if (kept) *kept = workspace(pngpd_linear_cross_entropy_kept_bytes(type, T, V, D), x);
     const size_t bytes = pngpd_linear_cross_entropy_workspace_bytes(type, T, V, D, 0, xr.aligned() && wr.aligned());
     const at::Tensor ws = workspace(bytes, x);
     check(pngpd_linear_cross_entropy_forward(type, T, V, D, xr.p(), xr.ld, wr.p(), wr.ld, data(b), target.const_data_ptr<int64_t>(),
                                              a.ignore_index, (float)a.label_smoothing, (int)a.reduction, (float*)out(loss),
-                                             (float*)out(*lse), out(ws), bytes, stream_of(x)));
+                                             (float*)out(*lse), kept ? out(*kept) : nullptr, out(ws), bytes, stream_of(x)));
     return loss;
 }
 
 struct LinearCrossEntropyFunction : torch::autograd::Function<LinearCrossEntropyFunction> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const Maybe& bias, const at::Tensor& target,
                               int64_t ignore_index, double label_smoothing, int64_t reduction) {
-        at::Tensor lse;
-        at::Tensor loss = loss_forward(x, w, target, bias, {ignore_index, label_smoothing, reduction}, &lse);
-        ctx->save_for_backward({x, w, dense(bias), target, lse});
+        at::Tensor lse, kept;
+        at::Tensor loss = loss_forward(x, w, target, bias, {ignore_index, label_smoothing, reduction}, &lse, &kept);
+        ctx->save_for_backward({x, w, dense(bias), target, lse, kept});
         ctx->saved_data["ignore_index"] = ignore_index;
         ctx->saved_data["label_smoothing"] = label_smoothing;
         ctx->saved_data["reduction"] = reduction;
@@ -265,7 +266,7 @@ struct LinearCrossEntropyFunction : torch::autograd::Function<LinearCrossEntropy
         const at::Tensor ws = workspace(bytes, x);
         check(pngpd_linear_cross_entropy_backward(
             type, T, V, D, xr.p(), xr.ld, wr.p(), wr.ld, data(b), target.const_data_ptr<int64_t>(), ctx->saved_data["ignore_index"].toInt(),
-            (float)ctx->saved_data["label_smoothing"].toDouble(), (int)ctx->saved_data["reduction"].toInt(), (const float*)data(lse),
+            (float)ctx->saved_data["label_smoothing"].toDouble(), (int)ctx->saved_data["reduction"].toInt(), (const float*)data(lse), data(saved[5]),
             (const float*)data(dloss), out(result[0]), out(result[1]), out(result[2]), out(ws), bytes, stream_of(x)));
         return once(std::move(result));
     }
@@ -276,7 +277,7 @@ at::Tensor linear_cross_entropy(const at::Tensor& x, const at::Tensor& w, const 
     if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(bias)))
         return LinearCrossEntropyFunction::apply(x, w, bias, target, ignore_index, label_smoothing, reduction);
     at::Tensor lse;
-    return loss_forward(x, w, target, bias, {ignore_index, label_smoothing, reduction}, &lse);
+    return loss_forward(x, w, target, bias, {ignore_index, label_smoothing, reduction}, &lse, nullptr);
 }
 
 }  // namespace

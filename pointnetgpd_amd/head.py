@@ -6,7 +6,7 @@ regularised, with many classes - there are
 
 * `linear`                 y = act(x W^T + b) + residual,
 * `dropout`                counter-based, its mask a function of (seed, offset, position) that is never stored,
-* `linear_cross_entropy`   the loss of softmax(x W^T + b) without the logits ever being stored whole,
+* `linear_cross_entropy`   the loss of softmax(x W^T + b) without the logits having to be stored whole,
 
 each differentiable once through torch.autograd, in float32, bfloat16 and float16.  Every tensor of a call has one type
 and lies on one GPU; sums and row statistics are 32-bit.  Calls run on the current stream of the tensors' device and can be
@@ -114,7 +114,10 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, label_
     [...] for "none".
 
     Rows with target == ignore_index have loss 0 and no gradient, whatever values they hold.  Another target outside [0, V)
-    makes the loss NaN and gives its row no gradient, as `training.nll_loss` does.  A class is masked by a bias of -inf."""
+    makes the loss NaN and gives its row no gradient, as `training.nll_loss` does.  A class is masked by a bias of -inf.
+
+    The logits are formed in pieces, in the backward pass again.  Only float32 logits of at most 256 MiB (or as much as x and
+    weight take) are kept for the backward pass, where that is quicker."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction: expected one of {list(_REDUCTIONS)}, got {reduction!r}")
     _require(x, "x")

@@ -78,15 +78,15 @@ def test_dropout_refuses(change, code):
     (dict(type=-2), ERR_INVALID), (dict(T=-1), ERR_SHAPE), (dict(V=0), ERR_SHAPE), (dict(D=0), ERR_SHAPE),
     (dict(x=None), ERR_INVALID), (dict(w=None), ERR_INVALID), (dict(target=None), ERR_INVALID), (dict(eps=1.5), ERR_INVALID),
     (dict(eps=float("nan")), ERR_INVALID), (dict(reduction=3), ERR_INVALID), (dict(ldw=3), ERR_SHAPE),
-    (dict(lse=None), ERR_INVALID), (dict(out=None), ERR_INVALID), (dict(V=2 ** 24 + 1), ERR_SHAPE), (dict(D=2 ** 21 + 1, ldw=2 ** 22), ERR_SHAPE), (dict(ws=None), ERR_INVALID), (dict(nbytes=64), ERR_WORKSPACE)])
+    (dict(lse=None), ERR_INVALID), (dict(out=None), ERR_INVALID), (dict(V=2 ** 24 + 1), ERR_SHAPE), (dict(D=2 ** 21 + 1, ldw=2 ** 22), ERR_SHAPE), (dict(ws=None), ERR_INVALID), (dict(nbytes=64), ERR_WORKSPACE), (dict(kept=24), ERR_INVALID)])
 def test_linear_cross_entropy_refuses(change, code):
     lib = _lib.load()
-    a = dict(type=0, T=2, V=5, D=4, x=16, w=16, ldw=4, target=16, eps=0.0, reduction=1, lse=16, out=16, ws=4096, nbytes=1 << 20)
+    a = dict(type=0, T=2, V=5, D=4, x=16, w=16, ldw=4, target=16, eps=0.0, reduction=1, lse=16, out=16, kept=None, ws=4096, nbytes=1 << 20)
     a.update(change)
     args = (a["type"], a["T"], a["V"], a["D"], a["x"], 4, a["w"], a["ldw"], None, a["target"], -100, a["eps"], a["reduction"])
-    assert lib.pngpd_linear_cross_entropy_forward(*args, a["out"], a["lse"], a["ws"], a["nbytes"], None) == code
+    assert lib.pngpd_linear_cross_entropy_forward(*args, a["out"], a["lse"], a["kept"], a["ws"], a["nbytes"], None) == code
     assert b"pngpd_linear_cross_entropy_forward" in lib.pngpd_last_error()
-    assert lib.pngpd_linear_cross_entropy_backward(*args, a["lse"], a["out"], 16, 16, 16, a["ws"], a["nbytes"], None) == code
+    assert lib.pngpd_linear_cross_entropy_backward(*args, a["lse"], a["kept"], a["out"], 16, 16, 16, a["ws"], a["nbytes"], None) == code
     assert b"pngpd_linear_cross_entropy_backward" in lib.pngpd_last_error()
 
 
@@ -96,6 +96,10 @@ def test_workspace_sizes_are_bounded_and_grow_with_no_logits():
     assert 0 < lib.pngpd_linear_cross_entropy_workspace_bytes(1, 8192, 131072, 1024, 0, 1) < whole // 8
     assert 0 < lib.pngpd_linear_cross_entropy_workspace_bytes(1, 8192, 131072, 1024, 1, 1) < whole // 8
     assert lib.pngpd_linear_workspace_bytes(5, 1, 1, 1, 0, 1) == 0
+    kept = lib.pngpd_linear_cross_entropy_kept_bytes
+    assert kept(0, 1023, 10007, 1000) == 1023 * 10008 * 4      # rows of whole 16-byte chunks
+    assert kept(1, 8192, 131072, 1024) == kept(2, 1024, 8192, 1024) == kept(0, 4096, 131072, 1024) == 0
+    assert kept(0, 256, 3, 256) == kept(0, 1024, 8192, 100) == kept(0, 0, 8192, 1024) == kept(7, 1024, 8192, 1024) == 0
 
 
 def test_a_missing_binding_is_an_error(monkeypatch, tmp_path):

@@ -681,3 +681,45 @@ def test_limits_raise_the_librarys_error():
     with pytest.raises(PngpdError) as e:
         head.linear(torch.zeros(2, 4, device="cuda"), w)
     assert e.value.code != 0 and "pngpd_linear_forward" in str(e.value)
+
+
+KEPT = [(333, 5003, 200), (1023, 1000, 300), (5, 30011, 2000), (40, 2002, 4096)]      # many tiles, few rows, a cut contraction
+
+
+@pytest.mark.parametrize("T,V,D", KEPT)
+def test_logits_kept_for_the_backward_pass(T, V, D):
+    """float32 sizes whose logits are kept: padding rows that hold NaN, a bad label, a masked class, odd sizes."""
+    from pointnetgpd_amd import _lib
+    assert _lib.load().pngpd_linear_cross_entropy_kept_bytes(0, T, V, D) > 0
+    i = KEPT.index((T, V, D))
+    reduction = ("mean", "sum", "none", "mean")[i]
+    x, w, b, target = loss_case(T + V, T, V, D, torch.float32, bias=i != 1)
+    target[0], target[1] = 3, -100
+    x[target == -100] = float("nan")
+    if b is not None:
+        b[7] = float("-inf")
+        target[target == 7] = 8
+    if reduction == "none":
+        target[2] = V
+    dloss = torch.rand(T, generator=torch.Generator().manual_seed(i)) / T if reduction == "none" else \
+        torch.tensor(1.0 if reduction == "mean" else 1.0 / T)
+    clean = torch.where(torch.isnan(x), torch.zeros(()), x)
+    got = run_loss(x, w, target, b, 0.0, reduction, dloss)
+    check(got, ho.cross_entropy(clean, w, target, b, -100, 0.0, reduction, dloss))
+
+
+def test_kept_logits_serve_two_backward_passes():
+    x, w, b = (t.cuda().requires_grad_() for t in make(95, (300, 320), (3001, 320), (3001,)))
+    target = torch.randint(0, 3001, (300,), generator=torch.Generator().manual_seed(9)).cuda()
+    loss = head.linear_cross_entropy(x, w, target, b, label_smoothing=0.1)
+    first = torch.autograd.grad(loss, (x, w, b), retain_graph=True)
+    other = torch.autograd.grad(head.linear_cross_entropy(x * 2, w, target, b), (x, w, b))      # another call in between
+    again = torch.autograd.grad(loss, (x, w, b))
+    assert all(torch.equal(p, q) for p, q in zip(first, again)) and not torch.equal(first[0], other[0])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, (x, w, b))
+    loss = head.linear_cross_entropy(x, w, target, b)
+    with torch.no_grad():
+        b.add_(1)                                              # the kept logits are of the bias as it was
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, (x, w, b))
