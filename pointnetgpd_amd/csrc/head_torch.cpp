@@ -65,8 +65,12 @@ at::Tensor workspace(size_t bytes, const at::Tensor& like) {
 }
 
 // In a capture the engine would make a stream outside it wait for a gradient, or it for the stream, which ends the process.
-// That happens where what the gradients go to belongs to another stream: a leaf whose eager graph is still alive, or an eager
+// That happens where what the gradients go to belongs to such a stream: a leaf whose eager graph is still alive, or an eager
 // result.  Called by a backward pass before it launches anything; costs a comparison for each gradient outside a capture.
+bool capturing(hipStream_t s) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(s, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+}
 void refuse_mixed_capture(const at::Tensor& like) {
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
@@ -75,10 +79,12 @@ void refuse_mixed_capture(const at::Tensor& like) {
         if (!edge.is_valid()) continue;
         const auto theirs = edge.function->stream();
         if (!theirs.has_value() || *theirs == current.unwrap()) continue;
-        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing(current.stream(), &status) == hipSuccess && status == hipStreamCaptureStatusNone) return;
-        throw std::runtime_error("a captured backward pass reaches a tensor whose eager graph is still alive on another stream: let go "
-                                 "of the eager results (a kept loss or output) before the capture");
+        if (!capturing(current.stream())) return;
+        // the default stream captures nothing, and may not even be asked meanwhile
+        const hipStream_t other = c10::hip::HIPStreamMasqueradingAsCUDA(*theirs).stream();
+        if (!other || !capturing(other))
+            throw std::runtime_error("a captured backward pass reaches a tensor whose eager graph is still alive on another stream: let "
+                                     "go of the eager results (a kept loss or output) before the capture");
     }
 }
 

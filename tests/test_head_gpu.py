@@ -723,3 +723,75 @@ def test_kept_logits_serve_two_backward_passes():
         b.add_(1)                                              # the kept logits are of the bias as it was
     with pytest.raises(RuntimeError):
         torch.autograd.grad(loss, (x, w, b))
+
+
+def test_a_step_captured_over_two_streams():
+    """A capture that forks: the loss on a stream of its own, with float32 logits that are kept; replayed between eager work."""
+    x, w, v, b = (t.cuda().requires_grad_() for t in make(96, (300, 64), (320, 64), (3001, 320), (3001,)))
+    target = torch.randint(0, 3001, (300,), generator=torch.Generator().manual_seed(9)).cuda()
+
+    def step(main, side):
+        h = head.linear(x, w, activation="relu")
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            loss = head.linear_cross_entropy(h, v, target, b)
+        main.wait_stream(side)
+        return [loss.detach(), *torch.autograd.grad(loss, (x, w, v, b))]
+
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    main.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(main):
+        step(main, side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=main):
+        got = step(main, side)
+    for i in range(3):
+        with torch.no_grad():
+            x.mul_(1.25)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(main):
+            want = step(main, side)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), i
+
+
+def test_one_tensor_in_two_places():
+    """The same tensor as input, weight and residual: its gradients add up."""
+    x, = make(97, (40, 40))
+    a = x.cuda().requires_grad_()
+    dx, = torch.autograd.grad(head.linear(a, a, residual=a).sum(), a)
+    parts = [x.clone().cuda().requires_grad_() for _ in range(3)]
+    want = torch.autograd.grad(head.linear(parts[0], parts[1], residual=parts[2]).sum(), parts)
+    assert (dx - sum(t.double() for t in want)).abs().max().item() <= 2 * 2 ** -23 * sum(t.abs() for t in want).max().item()
+    target = torch.arange(40, device="cuda")
+    dx, = torch.autograd.grad(head.linear_cross_entropy(a, a, target, a[0]), a)
+    assert torch.isfinite(dx).all()
+
+
+def test_threads_call_at_once():
+    """Threads of one process, each on a stream of its own, forward and backward at the same time."""
+    import threading
+    cases = []
+    for i in range(4):
+        x, w, b = (t.cuda().requires_grad_() for t in make(100 + i, (200 + i, 64), (500, 64), (500,)))
+        cases.append((x, w, b, torch.randint(0, 500, (200 + i,), generator=torch.Generator().manual_seed(i)).cuda()))
+    want = [torch.autograd.grad(head.linear_cross_entropy(head.dropout(x, 0.2, 3), w, t, b), (x, w, b)) for x, w, b, t in cases]
+    torch.cuda.synchronize()
+    got, streams = [None] * 4, [torch.cuda.Stream() for _ in range(4)]
+
+    def run(i):
+        x, w, b, t = cases[i]
+        with torch.cuda.stream(streams[i]):
+            for _ in range(10):
+                got[i] = torch.autograd.grad(head.linear_cross_entropy(head.dropout(x, 0.2, 3), w, t, b), (x, w, b))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for a, c in zip(got, want) for p, q in zip(a, c))
