@@ -41,6 +41,7 @@ LIB_SOURCES = [
     "head_tile_f16.hip",
     "head_dropout.hip",
     "head_loss.hip",
+    "head_few.hip",
     "head_api.cpp",
 ]
 

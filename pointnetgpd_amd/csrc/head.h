@@ -113,6 +113,29 @@ hipError_t head_dropout(int type, int64_t rows, int64_t cols, const void* x, int
 bool head_loss_at_once(int64_t T, int blocks);
 hipError_t head_row_loss(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit, const int64_t* target,
                          int64_t ignore_index, float eps, float* row_loss, float* lse, int reduction, float* batch, hipStream_t s);
+// used (may be NULL) receives the number of rows that are not ignored
 hipError_t head_batch_loss(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore_index, int reduction, float* loss,
-                           hipStream_t s);
+                           float* used, hipStream_t s);
+
+// The loss over at most HEAD_FEW classes, operands with any strides.  logits: what is kept for the backward pass, head_few_room
+// floats a row (NULL: forward only).
+constexpr int64_t HEAD_FEW = 8;
+inline int64_t head_few_room(int64_t V) { return V <= 4 ? 4 : 8; }
+struct HeadFew {
+    int64_t T, V, D;
+    const void* x;
+    int64_t ldx;
+    const void* w;
+    int64_t ldw;
+    const void* bias;           // may be NULL
+    const int64_t* target;
+    int64_t ignore_index;
+    float eps;
+    float* logits;
+};
+hipError_t head_few_loss(int type, const HeadFew& g, float* row_loss, float* lse, hipStream_t s);
+// part: head_few_part_bytes; used: what head_batch_loss left (for the mean)
+size_t head_few_part_bytes(int type, int64_t T, int64_t V, int64_t D);
+hipError_t head_few_grad(int type, const HeadFew& g, const float* lse, const float* used, const float* dloss, int reduction, void* dx,
+                         void* dw, void* db, float* part, hipStream_t s);
 }  // namespace pngpd

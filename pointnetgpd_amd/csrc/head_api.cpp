@@ -115,6 +115,7 @@ struct LossWs {
     void *x, *w, *tile;        // laid out; gradients of a piece's logits, [T][padded(piece)]
     float4* stats;
     float *target_logit, *row_loss, *row_weight, *scale, *part, *dx_sum, *partial;
+    float* few;                // partial sums of few classes' gradients
     size_t bytes;
     LossWs(void* base, int type, int64_t T, int64_t V, int64_t D, bool backward, bool copy_x, bool copy_w) {
         Bump b(base);
@@ -124,7 +125,7 @@ struct LossWs {
         w = copy_w ? b.take((size_t)V * dp * e) : nullptr;
         tile = nullptr;
         stats = nullptr;
-        target_logit = row_loss = row_weight = scale = part = dx_sum = partial = nullptr;
+        target_logit = row_loss = row_weight = scale = part = dx_sum = partial = few = nullptr;
         piece = V;
         rows_at_once = rows;
         if (!backward) {
@@ -155,6 +156,7 @@ struct LossWs {
             row_weight = (float*)b.take((size_t)rows * 4);
             scale = (float*)b.take(4);
             part = (float*)b.take((size_t)max2(pngpd::head_col_parts(type, rows, piece) * piece, pngpd::head_col_parts(type, rows, last) * last) * 4);
+            if (V <= pngpd::HEAD_FEW) few = (float*)b.take(pngpd::head_few_part_bytes(type, rows, V, D));
             if (piece < V) dx_sum = (float*)b.take((size_t)rows * D * 4);
             size_t cut = 0;
             for (int64_t n : {piece, last}) {
@@ -181,12 +183,18 @@ int check_loss(const char* who, int type, int64_t T, int64_t V, int64_t D, const
     return PNGPD_OK;
 }
 
-// What the forward pass keeps for the backward pass, or 0: float32 logits (without the bias) where they are one piece of the
+constexpr size_t FEW_HEAD = 256;       // bytes in front of few classes' kept logits: the number of rows that count
+
+// What the forward pass keeps for the backward pass, or 0.  Few classes: their logits, at most 32 bytes a row.  More: float32 logits (without the bias) where they are one piece of the
 // gradients' and forming them again takes longer than writing them once and reading them twice.  That is 2 D operations a
 // logit at 0.13 PFLOP/s against 12 bytes at 5 TB/s, equal at D = 160; the pass over them is a launch more, so 2^28 products
 // at least.  16-bit operands are multiplied ten times as fast and form their logits again.  Training 1023 x 1000 -> 10007
 // takes 581 us with its 41 MB kept, 684 without.
 size_t kept_bytes(int type, int64_t T, int64_t V, int64_t D) {
+    if (V <= pngpd::HEAD_FEW) {
+        const size_t bytes = FEW_HEAD + (size_t)T * pngpd::head_few_room(V) * 4;
+        return T > 0 && bytes <= loss_budget(type, T, V, D) ? bytes : 0;
+    }
     if (type != PNGPD_TYPE_F32 || T < 1 || D < 160 || (double)T * (double)V * (double)D < 268435456.0) return 0;
     if (LossWs(nullptr, type, T, V, D, false, false, false).rows_at_once < T || LossWs(nullptr, type, T, V, D, true, false, false).piece < V) return 0;
     const size_t bytes = pngpd::head_kept_bytes(type, T, V, D);
@@ -325,6 +333,15 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
     LossWs ws(workspace_dev, type, T, V, D, false, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
     if (T > 0) {
         if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
+        if (V <= pngpd::HEAD_FEW) {
+            char* few = kept_bytes(type, T, V, D) ? (char*)kept_dev : nullptr;
+            const pngpd::HeadFew g{T, V, D, x_dev, ldx, weight_dev, ldw, bias_dev, target_dev, ignore_index, label_smoothing,
+                                   few ? (float*)(few + FEW_HEAD) : nullptr};
+            HIP_TRY(pngpd::head_few_loss(type, g, reduction == PNGPD_REDUCE_NONE ? loss_dev : ws.row_loss, lse_dev, s));
+            if (reduction != PNGPD_REDUCE_NONE)
+                HIP_TRY(pngpd::head_batch_loss(T, ws.row_loss, target_dev, ignore_index, reduction, loss_dev, (float*)few, s));
+            return PNGPD_OK;
+        }
         pngpd::HeadLayOut job_x, job_w;
         bool lay_x, lay_w;
         const Rows x = direct_rows(type, T, D, x_dev, ldx, ws.x, &job_x, &lay_x);
@@ -351,7 +368,7 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
             if (whole && reduction != PNGPD_REDUCE_NONE && pngpd::head_loss_at_once(n, blocks)) return PNGPD_OK;
         }
     }
-    if (reduction != PNGPD_REDUCE_NONE) HIP_TRY(pngpd::head_batch_loss(T, ws.row_loss, target_dev, ignore_index, reduction, loss_dev, s));
+    if (reduction != PNGPD_REDUCE_NONE) HIP_TRY(pngpd::head_batch_loss(T, ws.row_loss, target_dev, ignore_index, reduction, loss_dev, nullptr, s));
     return PNGPD_OK;
 }
 
@@ -374,6 +391,12 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
     const float* kept = kept_bytes(type, T, V, D) ? (const float*)kept_dev : nullptr;
     LossWs ws(workspace_dev, type, T, V, D, true, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
+    if (kept && V <= pngpd::HEAD_FEW) {
+        const pngpd::HeadFew g{T, V, D, x_dev, ldx, weight_dev, ldw, bias_dev, target_dev, ignore_index, label_smoothing,
+                               const_cast<float*>(kept) + FEW_HEAD / 4};
+        HIP_TRY(pngpd::head_few_grad(type, g, lse_dev, kept, dloss_dev, reduction, dx_dev, dweight_dev, dbias_dev, ws.few, s));
+        return PNGPD_OK;
+    }
     const HeadOperand x{ws.x, padded(D, type), true}, xt{ws.x, padded(D, type), false};
     const pngpd::HeadRowWeights weights{target_dev, T, V, ignore_index, reduction, dloss_dev, ws.row_weight, ws.scale};
     const pngpd::HeadLayOut job_x{x_dev, T, D, ldx, ws.x, x.ld, true};      // what padding rows hold stays out of the sums

@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void row_loss_kernel(int64_t T, int64_t V, int
 }
 
 // the batch's loss: one workgroup, sums over the rows in 64 bits
-__device__ __forceinline__ void batch_sum(double sum, double used, int reduction, float* loss) {
+__device__ __forceinline__ void batch_sum(double sum, double used, int reduction, float* loss, float* count_out) {
     __shared__ double part[16], count[16];
     for (int o = 32; o; o >>= 1) {
         sum += __shfl_xor(sum, o);
@@ -63,18 +63,19 @@ __device__ __forceinline__ void batch_sum(double sum, double used, int reduction
             used += count[i];
         }
         loss[0] = (float)(reduction == PNGPD_REDUCE_MEAN ? sum / used : sum);
+        if (count_out) count_out[0] = (float)used;
     }
 }
 
 __global__ __launch_bounds__(1024) void batch_loss_kernel(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore,
-                                                          int reduction, float* loss) {
+                                                          int reduction, float* loss, float* count) {
     double sum = 0, used = 0;
 #pragma unroll 8
     for (int64_t t = threadIdx.x; t < T; t += 1024) {
         sum += row_loss[t];
         used += target[t] != ignore;
     }
-    batch_sum(sum, used, reduction, loss);
+    batch_sum(sum, used, reduction, loss, count);
 }
 
 // rows' losses and the batch's for a small batch: a thread a row
@@ -89,7 +90,7 @@ __global__ __launch_bounds__(1024) void small_loss_kernel(int T, int64_t V, int 
         sum = loss_of_row(v, t, V, target_logit, target, ignore, eps, lse);
         used = target[t] != ignore;
     }
-    batch_sum(sum, used, reduction, loss);
+    batch_sum(sum, used, reduction, loss, nullptr);
 }
 
 // bytes: an even number (every element type has at least two)
@@ -122,8 +123,8 @@ hipError_t head_row_loss(int64_t T, int64_t V, int blocks, const float4* stats, 
 }
 
 hipError_t head_batch_loss(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore, int reduction, float* loss,
-                           hipStream_t s) {
-    batch_loss_kernel<<<1, 1024, 0, s>>>(T, row_loss, target, ignore, reduction, loss);
+                           float* used, hipStream_t s) {
+    batch_loss_kernel<<<1, 1024, 0, s>>>(T, row_loss, target, ignore, reduction, loss, used);
     return hipGetLastError();
 }
 

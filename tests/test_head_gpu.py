@@ -795,3 +795,71 @@ def test_threads_call_at_once():
         t.join(60)
     torch.cuda.synchronize()
     assert all(torch.equal(p, q) for a, c in zip(got, want) for p, q in zip(a, c))
+
+
+FEW = [(1, 1, 7), (1000, 8, 513), (70, 7, 1001), (5000, 2, 64), (33, 4, 4096), (256, 3, 256), (2049, 5, 2056), (17, 8, 30000)]
+
+
+@pytest.mark.parametrize("T,V,D", FEW)
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_few_classes(kind, T, V, D):
+    """At most eight classes: padding rows that hold NaN, a bad label, masked classes, label smoothing, odd sizes."""
+    dt = TYPES[kind]
+    i = FEW.index((T, V, D))
+    reduction, eps = ("mean", "sum", "none")[i % 3], 0.1 if i % 2 else 0.0
+    x, w, b, target = loss_case(T + V + D, T, V, D, dt, bias=i != 4)
+    scale = 256.0 if kind == "f16" else 1.0
+    if T > 20:
+        target[:2], target[3] = 0, -100
+        x[target == -100] = float("nan")
+        if reduction == "none":
+            target[2] = V
+        if i == 2:
+            eps, b[3] = 0.0, float("-inf")
+            target[target == 3] = 2
+    dloss = torch.rand(T, generator=torch.Generator().manual_seed(i)) * scale / T if reduction == "none" else \
+        torch.tensor(scale if reduction == "mean" else scale / T)
+    clean = torch.where(torch.isnan(x), torch.zeros((), dtype=dt), x)
+    got = run_loss(x, w, target, b, eps, reduction, dloss)
+    check(got, ho.cross_entropy(clean, w, target, b, -100, eps, reduction, dloss))
+    assert (got["dx"][(target < 0) | (target >= V)] == 0).all()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_few_classes_of_any_strides(kind):
+    dt = TYPES[kind]
+    x, w, b, target = loss_case(41, 60, 6, 72, dt, True)
+    dloss = torch.tensor(64.0 if kind == "f16" else 1.0)
+    want = run_loss(x, w, target, b, 0.05, "mean", dloss)
+    X, W = torch.zeros(60, 101, dtype=dt).cuda(), torch.zeros(72, 6, dtype=dt).cuda()
+    X[:, 3:75], W[:] = x.cuda(), w.t().cuda()
+    B = torch.zeros(12, dtype=dt).cuda()
+    B[::2] = b.cuda()
+    leaves = [X[:, 3:75].requires_grad_(), W.t().requires_grad_(), B[::2].requires_grad_()]
+    loss = head.linear_cross_entropy(leaves[0], leaves[1], target.cuda(), leaves[2], label_smoothing=0.05)
+    grads = torch.autograd.grad(loss, leaves, dloss.cuda())
+    check({"loss": loss, **dict(zip(("dx", "dw", "db"), grads))}, ho.cross_entropy(x, w, target, b, -100, 0.05, "mean", dloss))
+    assert torch.equal(loss, want["loss"]) and all(torch.equal(p, want[k]) for k, p in zip(("dx", "dw", "db"), grads))
+    some = torch.autograd.grad(head.linear_cross_entropy(x.cuda(), w.cuda(), target.cuda(), leaves[2], label_smoothing=0.05), leaves[2],
+                               dloss.cuda())
+    assert torch.equal(some[0], grads[2])
+
+
+def test_few_classes_without_kept_logits():
+    """The C entries without the memory that carries the logits: the general products' gradients."""
+    from pointnetgpd_amd import _lib
+    lib = _lib.load()
+    T, V, D = 300, 3, 128
+    x, w, b, target = loss_case(43, T, V, D, torch.float32, True)
+    dev = [t.cuda() for t in (x, w, b, target)]
+    loss, lse = torch.empty(1, device="cuda"), torch.empty(T, device="cuda")
+    out = [torch.empty(s, device="cuda") for s in ((T, D), (V, D), (V,))]
+    ws = torch.empty(max(lib.pngpd_linear_cross_entropy_workspace_bytes(0, T, V, D, k, 1) for k in (0, 1)), dtype=torch.uint8, device="cuda")
+    dloss = torch.ones(1, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    args = (0, T, V, D, dev[0].data_ptr(), D, dev[1].data_ptr(), D, dev[2].data_ptr(), dev[3].data_ptr(), -100, 0.1, 1)
+    assert lib.pngpd_linear_cross_entropy_forward(*args, loss.data_ptr(), lse.data_ptr(), None, ws.data_ptr(), ws.numel(), stream) == 0
+    assert lib.pngpd_linear_cross_entropy_backward(*args, lse.data_ptr(), None, dloss.data_ptr(), *(t.data_ptr() for t in out),
+                                                   ws.data_ptr(), ws.numel(), stream) == 0
+    want = ho.cross_entropy(x, w, target, b, -100, 0.1, "mean", torch.tensor(1.0))
+    check({"loss": loss[0], "dx": out[0], "dw": out[1], "db": out[2]}, want)
