@@ -64,6 +64,7 @@ struct HeadPlan {
     int64_t k_split;
     size_t partial_bytes;
     int stats_blocks;           // blocks of columns a STATS epilogue writes
+    double us;                  // what it should take
 };
 HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind);
 

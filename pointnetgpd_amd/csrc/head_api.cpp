@@ -185,17 +185,17 @@ int check_loss(const char* who, int type, int64_t T, int64_t V, int64_t D, const
 
 constexpr size_t FEW_HEAD = 256;       // bytes in front of few classes' kept logits: the number of rows that count
 
-// What the forward pass keeps for the backward pass, or 0.  Few classes: their logits, at most 32 bytes a row.  More: float32 logits (without the bias) where they are one piece of the
-// gradients' and forming them again takes longer than writing them once and reading them twice.  That is 2 D operations a
-// logit at 0.13 PFLOP/s against 12 bytes at 5 TB/s, equal at D = 160; the pass over them is a launch more, so 2^28 products
-// at least.  16-bit operands are multiplied ten times as fast and form their logits again.  Training 1023 x 1000 -> 10007
-// takes 581 us with its 41 MB kept, 684 without.
+// What the forward pass keeps for the backward pass, or 0.  Few classes: their logits, at most 32 bytes a row.  More: the
+// 32-bit logits (without the bias) where they are one piece of the gradients' and forming them again should take longer than
+// writing them once and reading them twice, at 4.5 TB/s and with a launch more.  Training 1023 x 1000 -> 10007 in float32 takes
+// 581 us with its 41 MB kept, 684 without; 4096 x 4096 -> 8192 in bfloat16 774 and 913, 8192 x 4096 -> 16 (where x is what
+// costs) 121 and 138; 2048 x 1024 -> 4096 in bfloat16 as long either way (108), and is not kept.
 size_t kept_bytes(int type, int64_t T, int64_t V, int64_t D) {
     if (V <= pngpd::HEAD_FEW) {
         const size_t bytes = FEW_HEAD + (size_t)T * pngpd::head_few_room(V) * 4;
         return T > 0 && bytes <= loss_budget(type, T, V, D) ? bytes : 0;
     }
-    if (type != PNGPD_TYPE_F32 || T < 1 || D < 160 || (double)T * (double)V * (double)D < 268435456.0) return 0;
+    if (T < 1 || pngpd::head_plan(type, T, V, D, pngpd::HEAD_EPI_DZ).us < 10.0 + 12.0 * (double)T * (double)V / 4.5e6) return 0;
     if (LossWs(nullptr, type, T, V, D, false, false, false).rows_at_once < T || LossWs(nullptr, type, T, V, D, true, false, false).piece < V) return 0;
     const size_t bytes = pngpd::head_kept_bytes(type, T, V, D);
     return bytes <= loss_budget(type, T, V, D) ? bytes : 0;

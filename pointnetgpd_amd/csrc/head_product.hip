@@ -27,17 +27,18 @@ __global__ __launch_bounds__(THREADS) void join_kernel(int64_t M, int64_t N, int
     }
 }
 
-// a row a workgroup: statistics of its logits, formed from the cuts of the contraction.  Eight logits at a time share one
+// a row a workgroup, or a wave where rows are short (LANES): statistics of its logits, formed from the cuts of the contraction.  Eight logits at a time share one
 // rescaling of the sum; 1023 rows of 10007 sums (41 MB) take 12 us, 29 with one at a time.
-template <typename E>
+template <typename E, int LANES>
 __global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, int splits, const float* partial, HeadEpilogue e) {
     __shared__ float4 share[4];
-    const int64_t m = blockIdx.x;
+    const int64_t m = LANES == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    if (m >= M) return;
     const int64_t y = e.target[m];
     const E* bias = (const E*)e.bias;
     float mx = -__builtin_inff(), sum = 0.f, zs = 0.f;
     const bool bias_vec = ((uintptr_t)bias & 15) == 0;
-    for (int64_t n = (int64_t)threadIdx.x * 8; n < N; n += 2048) {
+    for (int64_t n = (threadIdx.x & (LANES - 1)) * 8; n < N; n += LANES * 8) {
         const int valid = N - n < 8 ? (int)(N - n) : 8;
         Eight z = {};
 #pragma unroll 4
@@ -59,6 +60,10 @@ __global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, i
     const float top = wave_max(mx);
     sum = wave_sum(sum * (mx == top ? 1.f : __expf(mx - top)));
     zs = wave_sum(zs);
+    if (LANES == 64) {
+        if ((threadIdx.x & 63) == 0) e.stats[m] = make_float4(top, sum, zs, 0.f);
+        return;
+    }
     if ((threadIdx.x & 63) == 0) share[threadIdx.x >> 6] = make_float4(top, sum, zs, 0.f);
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -89,7 +94,9 @@ hipError_t join(int64_t M, int64_t N, int splits, const float* partial, const He
         case HEAD_EPI_LINEAR: PNGPD_JOIN(TILE_LINEAR); break;
         case HEAD_EPI_DZ: PNGPD_JOIN(TILE_DZ); break;
         case HEAD_EPI_SCALED: PNGPD_JOIN(TILE_SCALED); break;
-        default: join_stats_kernel<E><<<(unsigned)M, 256, 0, s>>>(M, N, splits, partial, e);
+        default:
+            if (N <= 512) join_stats_kernel<E, 64><<<(unsigned)((M + 3) / 4), 256, 0, s>>>(M, N, splits, partial, e);
+            else join_stats_kernel<E, 256><<<(unsigned)M, 256, 0, s>>>(M, N, splits, partial, e);
     }
 #undef PNGPD_JOIN
     return hipGetLastError();
@@ -492,7 +499,7 @@ HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
             double us = (double)per * step_us(f32, shape, k) + tile_us(shape) * (shape == SHAPE_256 ? (double)k : 1.0);
             if (cuts > 1) us += 4.0 + (double)cuts * (double)M * (double)N * 8e-6 / 4.0;
             if (us < best * 0.999) {
-                best = us;
+                best = p.us = us;
                 p.shape = shape;
                 p.splits = (int)cuts;
                 p.tiles_m = (int)tm;

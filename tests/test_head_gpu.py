@@ -683,17 +683,20 @@ def test_limits_raise_the_librarys_error():
     assert e.value.code != 0 and "pngpd_linear_forward" in str(e.value)
 
 
-KEPT = [(333, 5003, 200), (1023, 1000, 300), (5, 30011, 2000), (40, 2002, 4096)]      # many tiles, few rows, a cut contraction
+# many tiles, few rows, a cut contraction, few columns
+KEPT = [("f32", 333, 5003, 700), ("f32", 1023, 1000, 1000), ("f32", 5, 30011, 2000), ("f32", 40, 2002, 4096), ("bf16", 8000, 40, 4104),
+        ("f16", 2000, 2001, 4104), ("bf16", 517, 8001, 4100)]
 
 
-@pytest.mark.parametrize("T,V,D", KEPT)
-def test_logits_kept_for_the_backward_pass(T, V, D):
-    """float32 sizes whose logits are kept: padding rows that hold NaN, a bad label, a masked class, odd sizes."""
+@pytest.mark.parametrize("kind,T,V,D", KEPT)
+def test_logits_kept_for_the_backward_pass(kind, T, V, D):
+    """Sizes whose logits are kept: padding rows that hold NaN, a bad label, a masked class, odd sizes."""
     from pointnetgpd_amd import _lib
-    assert _lib.load().pngpd_linear_cross_entropy_kept_bytes(0, T, V, D) > 0
-    i = KEPT.index((T, V, D))
-    reduction = ("mean", "sum", "none", "mean")[i]
-    x, w, b, target = loss_case(T + V, T, V, D, torch.float32, bias=i != 1)
+    dt = TYPES[kind]
+    assert _lib.load().pngpd_linear_cross_entropy_kept_bytes(list(TYPES).index(kind), T, V, D) > 0
+    i = KEPT.index((kind, T, V, D))
+    reduction = ("mean", "sum", "none")[i % 3]
+    x, w, b, target = loss_case(T + V, T, V, D, dt, bias=i % 4 != 1)
     target[0], target[1] = 3, -100
     x[target == -100] = float("nan")
     if b is not None:
@@ -701,15 +704,16 @@ def test_logits_kept_for_the_backward_pass(T, V, D):
         target[target == 7] = 8
     if reduction == "none":
         target[2] = V
-    dloss = torch.rand(T, generator=torch.Generator().manual_seed(i)) / T if reduction == "none" else \
-        torch.tensor(1.0 if reduction == "mean" else 1.0 / T)
-    clean = torch.where(torch.isnan(x), torch.zeros(()), x)
+    scale = 256.0 if kind == "f16" else 1.0
+    dloss = torch.rand(T, generator=torch.Generator().manual_seed(i)) * scale / T if reduction == "none" else \
+        torch.tensor(scale if reduction == "mean" else scale / T)
+    clean = torch.where(torch.isnan(x), torch.zeros((), dtype=dt), x)
     got = run_loss(x, w, target, b, 0.0, reduction, dloss)
     check(got, ho.cross_entropy(clean, w, target, b, -100, 0.0, reduction, dloss))
 
 
 def test_kept_logits_serve_two_backward_passes():
-    x, w, b = (t.cuda().requires_grad_() for t in make(95, (300, 320), (3001, 320), (3001,)))
+    x, w, b = (t.cuda().requires_grad_() for t in make(95, (300, 1024), (3001, 1024), (3001,)))
     target = torch.randint(0, 3001, (300,), generator=torch.Generator().manual_seed(9)).cuda()
     loss = head.linear_cross_entropy(x, w, target, b, label_smoothing=0.1)
     first = torch.autograd.grad(loss, (x, w, b), retain_graph=True)
@@ -727,7 +731,7 @@ def test_kept_logits_serve_two_backward_passes():
 
 def test_a_step_captured_over_two_streams():
     """A capture that forks: the loss on a stream of its own, with float32 logits that are kept; replayed between eager work."""
-    x, w, v, b = (t.cuda().requires_grad_() for t in make(96, (300, 64), (320, 64), (3001, 320), (3001,)))
+    x, w, v, b = (t.cuda().requires_grad_() for t in make(96, (300, 64), (1024, 64), (3001, 1024), (3001,)))
     target = torch.randint(0, 3001, (300,), generator=torch.Generator().manual_seed(9)).cuda()
 
     def step(main, side):
