@@ -428,8 +428,8 @@ int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64
  * loss_dev: float [T] for PNGPD_REDUCE_NONE, else float [1] (the mean is over the rows that are not ignored: NaN when
  * there are none).  lse_dev float [T]: log sum exp of every row's logits, what the backward pass needs.
  * kept_dev: NULL, or pngpd_linear_cross_entropy_kept_bytes of memory (16-byte aligned) that carries what the backward
- * pass of the same call would otherwise compute again: 32-bit logits, where that is quicker and they take at most 256 MiB or as
- * much as x and weight.  Its size is 0 where nothing is kept.
+ * pass of the same call would otherwise compute again: 32-bit logits, where that is quicker and, rounded to `type`, they take
+ * at most 256 MiB or as much as x and weight.  Its size is 0 where nothing is kept.
  */
 size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V, int64_t D, int backward, int aligned);
 size_t pngpd_linear_cross_entropy_kept_bytes(int type, int64_t T, int64_t V, int64_t D);

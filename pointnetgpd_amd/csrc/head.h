@@ -68,7 +68,7 @@ struct HeadPlan {
 };
 HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind);
 
-// partial: head_plan(...).partial_bytes.  keep: the sums are left in partial (head_kept_bytes) and the statistics are one block
+// partial: head_plan(...).partial_bytes.  keep: the sums are left in partial (head_kept_bytes)
 hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b,
                         const HeadEpilogue& e, float* partial, bool keep, hipStream_t s);
 // Kept sums of a STATS product, and another epilogue from them.

@@ -187,18 +187,19 @@ constexpr size_t FEW_HEAD = 256;       // bytes in front of few classes' kept lo
 
 // What the forward pass keeps for the backward pass, or 0.  Few classes: their logits, at most 32 bytes a row.  More: the
 // 32-bit logits (without the bias) where they are one piece of the gradients' and forming them again should take longer than
-// writing them once and reading them twice, at 4.5 TB/s and with a launch more.  Training 1023 x 1000 -> 10007 in float32 takes
-// 581 us with its 41 MB kept, 684 without; 4096 x 4096 -> 8192 in bfloat16 774 and 913, 8192 x 4096 -> 16 (where x is what
-// costs) 121 and 138; 2048 x 1024 -> 4096 in bfloat16 as long either way (108), and is not kept.
+// writing and reading them at 4.5 TB/s, with a launch that costs a little more.  Training, kept and formed again, in us:
+// 4096 x 2048 -> 32768 in bfloat16 1620 and 1822, 4096 x 4096 -> 32768 2718 and 3332, 4096 x 1024 -> 32768 1103 and 1146,
+// 1023 x 1000 -> 10007 in float32 581 and 684, 8192 x 4096 -> 16 in bfloat16 (where x is what costs) 121 and 138; the worst
+// found is 2048 x 1024 -> 32768 in bfloat16, 573 and 559.
 size_t kept_bytes(int type, int64_t T, int64_t V, int64_t D) {
     if (V <= pngpd::HEAD_FEW) {
         const size_t bytes = FEW_HEAD + (size_t)T * pngpd::head_few_room(V) * 4;
         return T > 0 && bytes <= loss_budget(type, T, V, D) ? bytes : 0;
     }
-    if (T < 1 || pngpd::head_plan(type, T, V, D, pngpd::HEAD_EPI_DZ).us < 10.0 + 12.0 * (double)T * (double)V / 4.5e6) return 0;
+    if (T < 1 || pngpd::head_plan(type, T, V, D, pngpd::HEAD_EPI_DZ).us < 8.0 + 8.0 * (double)T * (double)V / 4.5e6) return 0;
     if (LossWs(nullptr, type, T, V, D, false, false, false).rows_at_once < T || LossWs(nullptr, type, T, V, D, true, false, false).piece < V) return 0;
     const size_t bytes = pngpd::head_kept_bytes(type, T, V, D);
-    return bytes <= loss_budget(type, T, V, D) ? bytes : 0;
+    return bytes <= loss_budget(type, T, V, D) / esize(type) * 4 ? bytes : 0;
 }
 
 inline const void* at(const void* p, int64_t elements, int type) { return p ? (const char*)p + (size_t)elements * esize(type) : nullptr; }
@@ -361,7 +362,7 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
             e.want_logit_sum = label_smoothing > 0.f;
             HIP_TRY(pngpd::head_product(type, n, V, D, HeadOperand{at(x.p, t * x.ld, type), x.ld, true}, HeadOperand{w.p, w.ld, true}, e,
                                         kept ? kept : ws.partial, kept != nullptr, s));
-            const int blocks = kept ? 1 : pngpd::head_plan(type, n, V, D, pngpd::HEAD_EPI_STATS).stats_blocks;
+            const int blocks = pngpd::head_plan(type, n, V, D, pngpd::HEAD_EPI_STATS).stats_blocks;
             HIP_TRY(pngpd::head_row_loss(n, V, blocks, ws.stats, ws.target_logit, target_dev + t, ignore_index, label_smoothing,
                                          row_loss + t, lse_dev + t, reduction,
                                          whole && reduction != PNGPD_REDUCE_NONE ? loss_dev : nullptr, s));

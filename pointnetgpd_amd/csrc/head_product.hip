@@ -206,15 +206,15 @@ hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand&
     g.tiles_n = p.tiles_n;
     g.splits = p.splits;
     g.k_split = p.k_split;
-    g.partial = partial;
+    g.partial = p.splits > 1 || keep ? partial : nullptr;
     g.e = e;
-    const bool parts = p.splits > 1 || keep;
+    const bool parts = p.splits > 1;
     const int kind = parts ? TILE_PARTIAL
                      : e.kind == HEAD_EPI_LINEAR ? TILE_LINEAR
                      : e.kind == HEAD_EPI_DZ     ? TILE_DZ
                      : e.kind == HEAD_EPI_STATS  ? TILE_STATS
                                                  : TILE_SCALED;
-    const bool vec = parts || epilogue_vec(e, N, sizeof(E));
+    const bool vec = parts || keep || epilogue_vec(e, N, sizeof(E));
     hipError_t err;
     if constexpr (__is_same(E, float)) err = launch_tile_f32(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
     else if constexpr (__is_same(E, bf16_t)) err = launch_tile_bf16(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);

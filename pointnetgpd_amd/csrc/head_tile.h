@@ -33,7 +33,7 @@ struct TileArgs {
     int64_t lda, ldb;           // bytes between rows (k_contiguous) or between contraction steps
     int tiles_m, tiles_n, splits;
     int64_t k_split;            // contraction elements a split takes (a multiple of a step)
-    float* partial;             // [split][M][head_partial_ld(N)] when splits > 1 or the sums are kept
+    float* partial;             // [split][M][head_partial_ld(N)] when splits > 1; of a STATS product whose sums are kept; else NULL
     HeadEpilogue e;
 };
 
@@ -481,6 +481,54 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
     if (AHEAD > 0) asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
 
     const int t = lane & 15, q = lane >> 4;
+    if (KIND != TILE_STATS || g.partial) {
+        // The sums go through LDS, as many rows as it holds at a time, and come back as 8 neighbouring columns a thread: whole
+        // lines of memory for the epilogue's loads and stores.  16-byte chunk c of staged row r at slot c ^ (r & 15).
+        constexpr int HOLD = RING * STAGE / (BN * 4), ROWS = HOLD < BM ? HOLD : BM, PASSES = BM / ROWS, JP = FM / PASSES;
+        constexpr int MIX = (BN / 4 < 16 ? BN / 4 : 16) - 1, GROUPS = BN / 8;
+        constexpr int RSTEP = WAVES * 64 / GROUPS, BATCH = ROWS / RSTEP < 4 ? ROWS / RSTEP : 4;
+        static_assert(ROWS * PASSES == BM && JP * PASSES == FM && (WAVES * 64) % GROUPS == 0 && ROWS % (RSTEP * BATCH) == 0, "rows of a pass");
+        const int c = (threadIdx.x % GROUPS) * 2;
+        const int64_t n = n0 + c * 4, have = (KIND == TILE_DZ ? g.e.ld_out : g.N) - n;
+        const int valid = (int)(have < 0 ? 0 : have < 8 ? have : 8);
+        const Columns col = load_columns<E, KIND>(g.e, g.N, n, vec);
+#pragma unroll
+        for (int pass = 0; pass < PASSES; ++pass) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < JP; ++j) {
+                const int r = (wm * JP + j) * 16 + t;
+#pragma unroll
+                for (int i = 0; i < FN; ++i) {
+                    const int c = (wn * FN + i) * 4 + q;
+                    *(f32x4*)(smem + r * (BN * 4) + (c ^ (r & MIX)) * 16) = acc[i][pass * JP + j];
+                }
+            }
+            __syncthreads();
+            // a thread keeps its columns; its rows are THREADS / GROUPS apart
+#pragma unroll 1
+            for (int r0 = threadIdx.x / GROUPS; r0 < ROWS; r0 += RSTEP * BATCH) {
+                Ahead ahead[BATCH];
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    const int r = r0 + k * RSTEP, in = r / (JP * 16);      // which wave row staged it
+                    const int64_t m = m0 + (in * FM + pass * JP) * 16 + (r - in * JP * 16);
+                    if (r < ROWS && m < g.M && valid > 0) ahead[k] = load_ahead<E, KIND>(g.e, g.N, m, n, valid, vec);
+                }
+#pragma unroll
+                for (int k = 0; k < BATCH; ++k) {
+                    const int r = r0 + k * RSTEP, in = r / (JP * 16);
+                    const int64_t m = m0 + (in * FM + pass * JP) * 16 + (r - in * JP * 16);
+                    if (r >= ROWS || m >= g.M || valid <= 0) continue;
+                    const f32x4 lo = *(const f32x4*)(smem + r * (BN * 4) + (c ^ (r & MIX)) * 16);
+                    const f32x4 hi = *(const f32x4*)(smem + r * (BN * 4) + ((c + 1) ^ (r & MIX)) * 16);
+                    Eight a = {{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
+                    if constexpr (KIND == TILE_PARTIAL || KIND == TILE_STATS) store8(g.partial + ((int64_t)split * g.M + m) * head_partial_ld(g.N) + n, a, valid, vec);
+                    else finish8<E, KIND>(g.e, g.N, m, n, valid, vec, col, ahead[k], a);
+                }
+            }
+        }
+    }
     if constexpr (KIND == TILE_STATS) {
         // a row's maximum, sum and target over this tile's columns: lane, then the 4 lanes of the row, then the waves
         __syncthreads();
@@ -556,53 +604,6 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
                 v.z += u.z;
             }
             g.e.stats[(int64_t)tn * g.M + m0 + r] = v;
-        }
-    } else {
-        // The sums go through LDS, as many rows as it holds at a time, and come back as 8 neighbouring columns a thread: whole
-        // lines of memory for the epilogue's loads and stores.  16-byte chunk c of staged row r at slot c ^ (r & 15).
-        constexpr int HOLD = RING * STAGE / (BN * 4), ROWS = HOLD < BM ? HOLD : BM, PASSES = BM / ROWS, JP = FM / PASSES;
-        constexpr int MIX = (BN / 4 < 16 ? BN / 4 : 16) - 1, GROUPS = BN / 8;
-        constexpr int RSTEP = WAVES * 64 / GROUPS, BATCH = ROWS / RSTEP < 4 ? ROWS / RSTEP : 4;
-        static_assert(ROWS * PASSES == BM && JP * PASSES == FM && (WAVES * 64) % GROUPS == 0 && ROWS % (RSTEP * BATCH) == 0, "rows of a pass");
-        const int c = (threadIdx.x % GROUPS) * 2;
-        const int64_t n = n0 + c * 4, have = (KIND == TILE_DZ ? g.e.ld_out : g.N) - n;
-        const int valid = (int)(have < 0 ? 0 : have < 8 ? have : 8);
-        const Columns col = load_columns<E, KIND>(g.e, g.N, n, vec);
-#pragma unroll
-        for (int pass = 0; pass < PASSES; ++pass) {
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < JP; ++j) {
-                const int r = (wm * JP + j) * 16 + t;
-#pragma unroll
-                for (int i = 0; i < FN; ++i) {
-                    const int c = (wn * FN + i) * 4 + q;
-                    *(f32x4*)(smem + r * (BN * 4) + (c ^ (r & MIX)) * 16) = acc[i][pass * JP + j];
-                }
-            }
-            __syncthreads();
-            // a thread keeps its columns; its rows are THREADS / GROUPS apart
-#pragma unroll 1
-            for (int r0 = threadIdx.x / GROUPS; r0 < ROWS; r0 += RSTEP * BATCH) {
-                Ahead ahead[BATCH];
-#pragma unroll
-                for (int k = 0; k < BATCH; ++k) {
-                    const int r = r0 + k * RSTEP, in = r / (JP * 16);      // which wave row staged it
-                    const int64_t m = m0 + (in * FM + pass * JP) * 16 + (r - in * JP * 16);
-                    if (r < ROWS && m < g.M && valid > 0) ahead[k] = load_ahead<E, KIND>(g.e, g.N, m, n, valid, vec);
-                }
-#pragma unroll
-                for (int k = 0; k < BATCH; ++k) {
-                    const int r = r0 + k * RSTEP, in = r / (JP * 16);
-                    const int64_t m = m0 + (in * FM + pass * JP) * 16 + (r - in * JP * 16);
-                    if (r >= ROWS || m >= g.M || valid <= 0) continue;
-                    const f32x4 lo = *(const f32x4*)(smem + r * (BN * 4) + (c ^ (r & MIX)) * 16);
-                    const f32x4 hi = *(const f32x4*)(smem + r * (BN * 4) + ((c + 1) ^ (r & MIX)) * 16);
-                    Eight a = {{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
-                    if constexpr (KIND == TILE_PARTIAL) store8(g.partial + ((int64_t)split * g.M + m) * head_partial_ld(g.N) + n, a, valid, vec);
-                    else finish8<E, KIND>(g.e, g.N, m, n, valid, vec, col, ahead[k], a);
-                }
-            }
         }
     }
 }

@@ -116,8 +116,8 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, label_
     Rows with target == ignore_index have loss 0 and no gradient, whatever values they hold.  Another target outside [0, V)
     makes the loss NaN and gives its row no gradient, as `training.nll_loss` does.  A class is masked by a bias of -inf.
 
-    The logits are formed in pieces, in the backward pass again.  Where that is quicker, and they take
-    at most 256 MiB (or as much as x and weight), the backward pass finds them kept in 32 bits instead."""
+    The logits are formed in pieces, in the backward pass again.  Where that is quicker, and one
+    piece holds them all (256 MiB in x's type, or as much as x and weight take), they are kept in 32 bits instead."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction: expected one of {list(_REDUCTIONS)}, got {reduction!r}")
     _require(x, "x")

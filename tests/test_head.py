@@ -98,10 +98,10 @@ def test_workspace_sizes_are_bounded_and_grow_with_no_logits():
     assert lib.pngpd_linear_workspace_bytes(5, 1, 1, 1, 0, 1) == 0
     kept = lib.pngpd_linear_cross_entropy_kept_bytes
     assert kept(0, 1023, 10007, 1000) == 1023 * 10008 * 4      # rows of whole 16-byte chunks
-    assert kept(1, 8192, 131072, 1024) == kept(2, 1024, 8192, 1024) == kept(0, 4096, 131072, 1024) == 0
+    assert kept(1, 8192, 131072, 1024) == kept(2, 1024, 8192, 128) == kept(0, 4096, 131072, 1024) == 0
     assert kept(0, 256, 3, 256) == 256 + 256 * 4 * 4 and kept(1, 77, 8, 99) == 256 + 77 * 8 * 4      # few classes
     assert kept(0, 2 ** 30, 8, 2) == kept(2, 256, 9, 256) == 0
-    assert kept(0, 1024, 8192, 100) == kept(0, 0, 8192, 1024) == kept(7, 1024, 8192, 1024) == 0
+    assert kept(0, 1024, 8192, 16) == kept(0, 0, 8192, 1024) == kept(7, 1024, 8192, 1024) == 0
 
 
 def test_a_missing_binding_is_an_error(monkeypatch, tmp_path):
