@@ -381,12 +381,14 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, co
             if constexpr (ACT != PNGPD_ACT_NONE) {
                 const typename Chunk<T>::V v = Chunk<T>::load(z + m * N + col, N - col, z_aligned);
 #pragma unroll
-                for (int i = 0; i < C; ++i) o[i] = (T)((float)g[i] * act_slope<ACT>((float)v[i]));
-            }
+                for (int i = 0; i < C; ++i) {
+                    const float d = (float)g[i] * act_slope<ACT>((float)v[i]);
+                    sum[i] += d;                          // before it is rounded
+                    o[i] = col + i < N ? (T)d : (T)0.f;
+                }
+            } else {
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                if (ACT != PNGPD_ACT_NONE && col + i >= N) o[i] = (T)0.f;
-                sum[i] += (float)o[i];
+                for (int i = 0; i < C; ++i) sum[i] += (float)g[i];
             }
             if constexpr (WRITE) *(typename Chunk<T>::V*)(dz + m * ld_dz + col) = o;
         }
