@@ -71,6 +71,14 @@ HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind);
 // partial: head_plan(...).partial_bytes.  keep: the sums are left in partial (head_kept_bytes)
 hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b,
                         const HeadEpilogue& e, float* partial, bool keep, hipStream_t s);
+// Both gradients of a product, dx = dz W and dW = dz^T x (SCALED epilogues), in one launch where they are small.
+struct HeadGradient {
+    int64_t M, N, K;
+    HeadOperand a, b;
+    HeadEpilogue e;
+    float* partial;             // of its own
+};
+hipError_t head_gradients(int type, const HeadGradient& x, const HeadGradient& w, hipStream_t s);
 // Kept sums of a STATS product, and another epilogue from them.
 size_t head_kept_bytes(int type, int64_t M, int64_t N, int64_t K);
 hipError_t head_kept(int type, int64_t M, int64_t N, int64_t K, const HeadEpilogue& e, const float* kept, hipStream_t s);

@@ -84,12 +84,13 @@ inline size_t max2(size_t a, size_t b) { return a > b ? a : b; }
 struct LinearWs {
     void *x, *w, *dz;           // laid out, if they have to be
     float *part, *partial;
+    float* partial_w;           // the weight's gradient's own
     size_t bytes;
     // copy_*: x, weight or dz (dy where there is no activation) is not as the products take it
     LinearWs(void* base, int type, int64_t M, int64_t N, int64_t K, bool backward, bool copy_x, bool copy_w, bool copy_dz) {
         Bump b(base);
         dz = nullptr;
-        part = partial = nullptr;
+        part = partial = partial_w = nullptr;
         x = w = nullptr;
         if (M > 0) {
             if (copy_x) x = b.take((size_t)M * padded(K, type) * esize(type));
@@ -98,8 +99,8 @@ struct LinearWs {
             if (backward) {
                 if (copy_dz) dz = b.take((size_t)M * padded(N, type) * esize(type));
                 part = (float*)b.take((size_t)pngpd::head_col_parts(type, M, N) * N * 4);
-                cut = max2(pngpd::head_plan(type, M, K, N, pngpd::HEAD_EPI_SCALED).partial_bytes,
-                           pngpd::head_plan(type, N, K, M, pngpd::HEAD_EPI_SCALED).partial_bytes);
+                cut = pngpd::head_plan(type, M, K, N, pngpd::HEAD_EPI_SCALED).partial_bytes;
+                partial_w = (float*)b.take(pngpd::head_plan(type, N, K, M, pngpd::HEAD_EPI_SCALED).partial_bytes);
             }
             partial = (float*)b.take(cut);
         }
@@ -115,6 +116,7 @@ struct LossWs {
     void *x, *w, *tile;        // laid out; gradients of a piece's logits, [T][padded(piece)]
     float4* stats;
     float *target_logit, *row_loss, *row_weight, *scale, *part, *dx_sum, *partial;
+    float* partial_w;          // the weight's gradient's own
     float* few;                // partial sums of few classes' gradients
     size_t bytes;
     LossWs(void* base, int type, int64_t T, int64_t V, int64_t D, bool backward, bool copy_x, bool copy_w) {
@@ -125,7 +127,7 @@ struct LossWs {
         w = copy_w ? b.take((size_t)V * dp * e) : nullptr;
         tile = nullptr;
         stats = nullptr;
-        target_logit = row_loss = row_weight = scale = part = dx_sum = partial = few = nullptr;
+        target_logit = row_loss = row_weight = scale = part = dx_sum = partial = partial_w = few = nullptr;
         piece = V;
         rows_at_once = rows;
         if (!backward) {
@@ -158,13 +160,14 @@ struct LossWs {
             part = (float*)b.take((size_t)max2(pngpd::head_col_parts(type, rows, piece) * piece, pngpd::head_col_parts(type, rows, last) * last) * 4);
             if (V <= pngpd::HEAD_FEW) few = (float*)b.take(pngpd::head_few_part_bytes(type, rows, V, D));
             if (piece < V) dx_sum = (float*)b.take((size_t)rows * D * 4);
-            size_t cut = 0;
+            size_t cut = 0, cut_w = 0;
             for (int64_t n : {piece, last}) {
                 cut = max2(cut, pngpd::head_plan(type, rows, n, D, pngpd::HEAD_EPI_DZ).partial_bytes);
-                cut = max2(cut, pngpd::head_plan(type, n, D, rows, pngpd::HEAD_EPI_SCALED).partial_bytes);
+                cut_w = max2(cut_w, pngpd::head_plan(type, n, D, rows, pngpd::HEAD_EPI_SCALED).partial_bytes);
                 cut = max2(cut, pngpd::head_plan(type, rows, D, n, pngpd::HEAD_EPI_SCALED).partial_bytes);
             }
             partial = (float*)b.take(cut);
+            partial_w = (float*)b.take(cut_w);
         }
         bytes = b.off;
     }
@@ -200,6 +203,14 @@ size_t kept_bytes(int type, int64_t T, int64_t V, int64_t D) {
     if (LossWs(nullptr, type, T, V, D, false, false, false).rows_at_once < T || LossWs(nullptr, type, T, V, D, true, false, false).piece < V) return 0;
     const size_t bytes = pngpd::head_kept_bytes(type, T, V, D);
     return bytes <= loss_budget(type, T, V, D) / esize(type) * 4 ? bytes : 0;
+}
+
+// those that are asked for
+hipError_t gradients(int type, const pngpd::HeadGradient& x, const pngpd::HeadGradient& w, hipStream_t s) {
+    if (x.e.out && w.e.out) return pngpd::head_gradients(type, x, w, s);
+    if (!x.e.out && !w.e.out) return hipSuccess;
+    const pngpd::HeadGradient& g = x.e.out ? x : w;
+    return pngpd::head_product(type, g.M, g.N, g.K, g.a, g.b, g.e, g.partial, false, s);
 }
 
 inline const void* at(const void* p, int64_t elements, int type) { return p ? (const char*)p + (size_t)elements * esize(type) : nullptr; }
@@ -278,17 +289,12 @@ int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void*
     if (dx_dev) w = direct_rows(type, N, K, weight_dev, ldw, ws.w, &job_w, &lay_w);
     if (dweight_dev) x = direct_rows(type, M, K, x_dev, ldx, ws.x, &job_x, &lay_x);
     HIP_TRY(pngpd::head_set_up(type, lay_x ? &job_x : nullptr, lay_w ? &job_w : nullptr, nullptr, s));
-    HeadEpilogue e;
-    e.kind = pngpd::HEAD_EPI_SCALED;
-    e.ld_out = K;
-    if (dx_dev) {
-        e.out = dx_dev;
-        HIP_TRY(pngpd::head_product(type, M, K, N, HeadOperand{dz.p, dz.ld, true}, HeadOperand{w.p, w.ld, false}, e, ws.partial, false, s));
-    }
-    if (dweight_dev) {
-        e.out = dweight_dev;
-        HIP_TRY(pngpd::head_product(type, N, K, M, HeadOperand{dz.p, dz.ld, false}, HeadOperand{x.p, x.ld, false}, e, ws.partial, false, s));
-    }
+    pngpd::HeadGradient gx{M, K, N, HeadOperand{dz.p, dz.ld, true}, HeadOperand{w.p, w.ld, false}, HeadEpilogue{}, ws.partial};
+    pngpd::HeadGradient gw{N, K, M, HeadOperand{dz.p, dz.ld, false}, HeadOperand{x.p, x.ld, false}, HeadEpilogue{}, ws.partial_w};
+    gx.e.ld_out = gw.e.ld_out = K;
+    gx.e.out = dx_dev;
+    gw.e.out = dweight_dev;
+    HIP_TRY(gradients(type, gx, gw, s));
     return PNGPD_OK;
 }
 
@@ -424,22 +430,17 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         if (dbias_dev)
             HIP_TRY(pngpd::head_grad_rows(type, T, n, ws.tile, np, nullptr, PNGPD_ACT_NONE, nullptr, 0, ws.part, ws.scale,
                                           at(dbias_dev, v, type), s));
-        HeadEpilogue g;
-        g.kind = pngpd::HEAD_EPI_SCALED;
-        g.ld_out = D;
-        if (dweight_dev) {
-            g.out = at(dweight_dev, v * D, type);
-            g.scale = ws.scale;
-            HIP_TRY(pngpd::head_product(type, n, D, T, HeadOperand{ws.tile, np, false}, xt, g, ws.partial, false, s));
-        }
-        if (dx_dev) {
-            const bool last = v + n == V;
-            g.add = v > 0 ? ws.dx_sum : nullptr;
-            g.out_f32 = !last;
-            g.scale = last ? ws.scale : nullptr;
-            g.out = last ? dx_dev : (void*)ws.dx_sum;
-            HIP_TRY(pngpd::head_product(type, T, D, n, HeadOperand{ws.tile, np, true}, HeadOperand{w, whole.ld, false}, g, ws.partial, false, s));
-        }
+        const bool last = v + n == V;
+        pngpd::HeadGradient gx{T, D, n, HeadOperand{ws.tile, np, true}, HeadOperand{w, whole.ld, false}, HeadEpilogue{}, ws.partial};
+        pngpd::HeadGradient gw{n, D, T, HeadOperand{ws.tile, np, false}, xt, HeadEpilogue{}, ws.partial_w};
+        gx.e.ld_out = gw.e.ld_out = D;
+        gx.e.add = v > 0 ? ws.dx_sum : nullptr;
+        gx.e.out_f32 = !last;
+        gx.e.scale = last ? ws.scale : nullptr;
+        gx.e.out = !dx_dev || last ? dx_dev : (void*)ws.dx_sum;
+        gw.e.scale = ws.scale;
+        gw.e.out = at(dweight_dev, v * D, type);
+        HIP_TRY(gradients(type, gx, gw, s));
     }
     return PNGPD_OK;
 }

@@ -185,15 +185,8 @@ hipError_t rows(int M, int64_t N, int64_t K, const HeadOperand& a, const HeadOpe
 }
 
 template <typename E>
-hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b, const HeadEpilogue& e,
-                   float* partial, bool keep, hipStream_t s) {
-    if (M <= FEW_M && e.kind == HEAD_EPI_LINEAR) {
-        if (M == 1) return rows<E, 1>((int)M, N, K, a, b, e, s);
-        if (M == 2) return rows<E, 2>((int)M, N, K, a, b, e, s);
-        return rows<E, 4>((int)M, N, K, a, b, e, s);
-    }
-    const HeadPlan p = head_plan(type, M, N, K, e.kind);
-    if (p.tiles_m == 0) return hipErrorInvalidValue;
+TileArgs tile_args(const HeadPlan& p, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b, const HeadEpilogue& e,
+                   float* partial) {
     TileArgs g{};
     g.M = M;
     g.N = N;
@@ -206,8 +199,22 @@ hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand&
     g.tiles_n = p.tiles_n;
     g.splits = p.splits;
     g.k_split = p.k_split;
-    g.partial = p.splits > 1 || keep ? partial : nullptr;
+    g.partial = partial;
     g.e = e;
+    return g;
+}
+
+template <typename E>
+hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b, const HeadEpilogue& e,
+                   float* partial, bool keep, hipStream_t s) {
+    if (M <= FEW_M && e.kind == HEAD_EPI_LINEAR) {
+        if (M == 1) return rows<E, 1>((int)M, N, K, a, b, e, s);
+        if (M == 2) return rows<E, 2>((int)M, N, K, a, b, e, s);
+        return rows<E, 4>((int)M, N, K, a, b, e, s);
+    }
+    const HeadPlan p = head_plan(type, M, N, K, e.kind);
+    if (p.tiles_m == 0) return hipErrorInvalidValue;
+    const TileArgs g = tile_args<E>(p, M, N, K, a, b, e, p.splits > 1 || keep ? partial : nullptr);
     const bool parts = p.splits > 1;
     const int kind = parts ? TILE_PARTIAL
                      : e.kind == HEAD_EPI_LINEAR ? TILE_LINEAR
@@ -221,6 +228,26 @@ hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand&
     else err = launch_tile_f16(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
     if (err != hipSuccess || !parts) return err;
     return join<E>(M, N, p.splits, partial, e, s);
+}
+
+// A(m,k) of x's gradient is dense in its contraction, the other three operands are not.
+template <typename E>
+hipError_t gradients(int type, const HeadGradient& x, const HeadGradient& w, hipStream_t s) {
+    const HeadPlan px = head_plan(type, x.M, x.N, x.K, HEAD_EPI_SCALED), pw = head_plan(type, w.M, w.N, w.K, HEAD_EPI_SCALED);
+    const int64_t grid = (int64_t)px.tiles_m * px.tiles_n * px.splits + (int64_t)pw.tiles_m * pw.tiles_n * pw.splits;
+    if (px.shape != SHAPE_64 || pw.shape != SHAPE_64 || grid >= (int64_t)1 << 23) {
+        const hipError_t err = product<E>(type, w.M, w.N, w.K, w.a, w.b, w.e, w.partial, false, s);
+        return err != hipSuccess ? err : product<E>(type, x.M, x.N, x.K, x.a, x.b, x.e, x.partial, false, s);
+    }
+    const TileArgs gx = tile_args<E>(px, x.M, x.N, x.K, x.a, x.b, x.e, x.partial), gw = tile_args<E>(pw, w.M, w.N, w.K, w.a, w.b, w.e, w.partial);
+    const bool vx = px.splits > 1 || epilogue_vec(x.e, x.N, sizeof(E)), vw = pw.splits > 1 || epilogue_vec(w.e, w.N, sizeof(E));
+    hipError_t err;
+    if constexpr (__is_same(E, float)) err = launch_pair_f32(gx, gw, vx, vw, s);
+    else if constexpr (__is_same(E, bf16_t)) err = launch_pair_bf16(gx, gw, vx, vw, s);
+    else err = launch_pair_f16(gx, gw, vx, vw, s);
+    if (err == hipSuccess && pw.splits > 1) err = join<E>(w.M, w.N, pw.splits, w.partial, w.e, s);
+    if (err == hipSuccess && px.splits > 1) err = join<E>(x.M, x.N, px.splits, x.partial, x.e, s);
+    return err;
 }
 
 // ---- passes over whole matrices -----------------------------------------------------------------------------------------------------
@@ -526,6 +553,9 @@ HeadPlan head_plan(int type, int64_t M, int64_t N, int64_t K, int kind) {
 hipError_t head_product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b,
                         const HeadEpilogue& e, float* partial, bool keep, hipStream_t s) {
     PNGPD_BY_TYPE((product<T>(type, M, N, K, a, b, e, partial, keep, s)))
+}
+hipError_t head_gradients(int type, const HeadGradient& x, const HeadGradient& w, hipStream_t s) {
+    PNGPD_BY_TYPE((gradients<T>(type, x, w, s)))
 }
 size_t head_kept_bytes(int type, int64_t M, int64_t N, int64_t K) {
     return (size_t)head_plan(type, M, N, K, HEAD_EPI_STATS).splits * M * head_partial_ld(N) * 4;

@@ -334,7 +334,7 @@ inline bool epilogue_vec(const HeadEpilogue& e, int64_t N, size_t sz) {
 
 // BM x BN outputs by WM x WN waves; AK / BK: the contraction is dense in the m / n operand
 template <typename E, int BM, int BN, int WM, int WN, bool AK, bool BK, int KIND, int RING>
-__global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs g, bool vec) {
+__device__ __forceinline__ void product_tile(const TileArgs& g, bool vec, int block) {
     constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, STEP = 128 / (int)sizeof(E);
     constexpr int STAGE = (BM + BN) * 128;
     typedef TileOperand<E, BM, AK, WAVES> OpA;
@@ -348,8 +348,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
     // Workgroups go round the 8 XCDs: each XCD takes a run of neighbouring tiles, in groups of 8 rows of tiles, so that
     // the operands' tiles in its L2 serve as many products as they can.
     const int tiles = g.tiles_m * g.tiles_n;
-    const int split = blockIdx.x / tiles;
-    int id = blockIdx.x - split * tiles;
+    const int split = block / tiles;
+    int id = block - split * tiles;
     {
         const int per = tiles / 8, rest = tiles % 8, x = id % 8, i = id / 8;
         id = x * per + (x < rest ? x : rest) + i;
@@ -608,6 +608,22 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs 
     }
 }
 
+template <typename E, int BM, int BN, int WM, int WN, bool AK, bool BK, int KIND, int RING>
+__global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs g, bool vec) {
+    product_tile<E, BM, BN, WM, WN, AK, BK, KIND, RING>(g, vec, blockIdx.x);
+}
+
+// Both gradients of a product in one launch, 64 x 64 tiles: the first `first` workgroups are x's (or the weight's, where
+// `weight_first`).  A launch less, and the second product's tiles run while the first one's last ones do: training 1024 x 1024 ->
+// 1024 takes 33 us instead of 38 in bfloat16, 77 instead of 85 in float32.
+template <typename E, int KIND_X, int KIND_W>
+__global__ __launch_bounds__(256, 2) void gradient_pair_kernel(TileArgs x, TileArgs w, bool x_vec, bool w_vec, int first, bool weight_first) {
+    const int block = blockIdx.x;
+    const bool early = block < first;
+    if (early != weight_first) product_tile<E, 64, 64, 2, 2, true, false, KIND_X, 3>(x, x_vec, early ? block : block - first);
+    else product_tile<E, 64, 64, 2, 2, false, false, KIND_W, 3>(w, w_vec, early ? block : block - first);
+}
+
 // ---- launch -----------------------------------------------------------------------------------------------------------------
 
 // tile shapes: 256 x 256 by 8 waves, 128 x 128, 64 x 64, 32 x 128 (few rows) and 128 x 32 (few columns) by 4
@@ -671,6 +687,28 @@ hipError_t launch_tile(int shape, int kind, bool ak, bool bk, const TileArgs& g,
     return hipErrorInvalidValue;
 }
 
+// x's and the weight's gradient, both in 64 x 64 tiles; the one whose tiles take more steps first
+template <typename E>
+hipError_t launch_pair(const TileArgs& x, const TileArgs& w, bool x_vec, bool w_vec, hipStream_t s) {
+    constexpr int lds = 3 * 128 * 128;
+    const int nx = x.tiles_m * x.tiles_n * x.splits, nw = w.tiles_m * w.tiles_n * w.splits;
+    const bool weight_first = w.k_split > x.k_split;
+    const int first = weight_first ? nw : nx;
+#define PNGPD_PAIR(KX, KW) gradient_pair_kernel<E, KX, KW><<<(unsigned)(nx + nw), 256, lds, s>>>(x, w, x_vec, w_vec, first, weight_first)
+    if (x.splits > 1) {
+        if (w.splits > 1) PNGPD_PAIR(TILE_PARTIAL, TILE_PARTIAL);
+        else PNGPD_PAIR(TILE_PARTIAL, TILE_SCALED);
+    } else {
+        if (w.splits > 1) PNGPD_PAIR(TILE_SCALED, TILE_PARTIAL);
+        else PNGPD_PAIR(TILE_SCALED, TILE_SCALED);
+    }
+#undef PNGPD_PAIR
+    return hipGetLastError();
+}
+
+hipError_t launch_pair_f32(const TileArgs& x, const TileArgs& w, bool x_vec, bool w_vec, hipStream_t s);
+hipError_t launch_pair_bf16(const TileArgs& x, const TileArgs& w, bool x_vec, bool w_vec, hipStream_t s);
+hipError_t launch_pair_f16(const TileArgs& x, const TileArgs& w, bool x_vec, bool w_vec, hipStream_t s);
 hipError_t launch_tile_f32(int shape, int kind, bool ak, bool bk, const TileArgs& g, bool vec, hipStream_t s);
 hipError_t launch_tile_bf16(int shape, int kind, bool ak, bool bk, const TileArgs& g, bool vec, hipStream_t s);
 hipError_t launch_tile_f16(int shape, int kind, bool ak, bool bk, const TileArgs& g, bool vec, hipStream_t s);
