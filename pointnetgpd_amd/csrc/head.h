@@ -27,6 +27,9 @@ inline bool head_direct(const void* p, int64_t ld, int64_t extent, size_t size) 
 // Partial sums lie in rows of whole 16-byte chunks.
 __host__ __device__ inline int64_t head_partial_ld(int64_t N) { return (N + 3) & ~(int64_t)3; }
 
+// A LINEAR product of so few rows takes them, and the weight's, as they lie.
+constexpr int64_t HEAD_FEW_ROWS = 4;
+
 // What becomes of a product's 32-bit sums.
 enum { HEAD_EPI_LINEAR = 0, HEAD_EPI_DZ = 1, HEAD_EPI_SCALED = 2, HEAD_EPI_STATS = 3 };
 struct HeadEpilogue {

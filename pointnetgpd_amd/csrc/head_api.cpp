@@ -222,7 +222,7 @@ extern "C" {
 
 size_t pngpd_linear_workspace_bytes(int type, int64_t M, int64_t N, int64_t K, int backward, int aligned) {
     if (check_linear("pngpd_linear_workspace_bytes", type, M, N, K, PNGPD_ACT_NONE)) return 0;
-    const bool k = !aligned || padded(K, type) != K;
+    const bool k = (!aligned || padded(K, type) != K) && (backward || M > pngpd::HEAD_FEW_ROWS);
     return LinearWs(nullptr, type, M, N, K, backward != 0, k, k, true).bytes;
 }
 
@@ -236,7 +236,8 @@ int pngpd_linear_forward(int type, int64_t M, int64_t N, int64_t K, const void* 
     if (!x_dev || !weight_dev || !y_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL argument", who);
     if ((rc = check_ld(who, "ldx", ldx, K)) || (rc = check_ld(who, "ldw", ldw, K))) return rc;
     if (residual_dev && (rc = check_ld(who, "ldr", ldr, N))) return rc;
-    LinearWs ws(workspace_dev, type, M, N, K, false, !direct(x_dev, ldx, K, type), !direct(weight_dev, ldw, K, type), false);
+    const bool few = M <= pngpd::HEAD_FEW_ROWS;
+    LinearWs ws(workspace_dev, type, M, N, K, false, !few && !direct(x_dev, ldx, K, type), !few && !direct(weight_dev, ldw, K, type), false);
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
     HeadEpilogue e;
     e.kind = pngpd::HEAD_EPI_LINEAR;
@@ -249,9 +250,9 @@ int pngpd_linear_forward(int type, int64_t M, int64_t N, int64_t K, const void* 
     e.ld_out = N;
     hipStream_t s = (hipStream_t)stream;
     pngpd::HeadLayOut job_x, job_w;
-    bool lay_x, lay_w;
-    const Rows x = direct_rows(type, M, K, x_dev, ldx, ws.x, &job_x, &lay_x);
-    const Rows w = direct_rows(type, N, K, weight_dev, ldw, ws.w, &job_w, &lay_w);
+    bool lay_x = false, lay_w = false;
+    const Rows x = few ? Rows{x_dev, ldx} : direct_rows(type, M, K, x_dev, ldx, ws.x, &job_x, &lay_x);
+    const Rows w = few ? Rows{weight_dev, ldw} : direct_rows(type, N, K, weight_dev, ldw, ws.w, &job_w, &lay_w);
     HIP_TRY(pngpd::head_set_up(type, lay_x ? &job_x : nullptr, lay_w ? &job_w : nullptr, nullptr, s));
     HIP_TRY(pngpd::head_product(type, M, N, K, HeadOperand{x.p, x.ld, true}, HeadOperand{w.p, w.ld, true}, e, ws.partial, false, s));
     return PNGPD_OK;

@@ -22,7 +22,8 @@ struct Eight {
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
         for (int k = 0; k < PER_THREAD / C; ++k) {
-            const chunk c = ((const chunk*)p)[k];
+            chunk c;
+            __builtin_memcpy(&c, p + k * C, 16);      // at any element: the hardware takes it
 #pragma unroll
             for (int i = 0; i < C; ++i) v[k * C + i] = c[i];
         }
@@ -33,22 +34,22 @@ struct Eight {
             chunk c;
 #pragma unroll
             for (int i = 0; i < C; ++i) c[i] = v[k * C + i];
-            ((chunk*)p)[k] = c;
+            __builtin_memcpy(p + k * C, &c, 16);
         }
     }
 };
 
-// DENSE: x and the residual are one run of memory as y is, all 16-byte aligned
+// DENSE: x and the residual are one run of memory as y is
 template <typename T, bool DENSE, bool RESIDUAL>
 __device__ __forceinline__ void dropout_eight(int64_t i0, int64_t total, int64_t cols, const T* x, int64_t ldx, const T* r, int64_t ldr,
-                                              T* y, unsigned long long border, float scale, unsigned long long key, bool y_aligned) {
+                                              T* y, unsigned long long border, float scale, unsigned long long key) {
     Eight<T> a, b;
-    const bool whole = DENSE && i0 + PER_THREAD <= total;
-    if (whole) {
-        a.load(x + i0);
-        if (RESIDUAL) b.load(r + i0);
+    int64_t m = DENSE ? 0 : i0 / cols, n = i0 - m * cols;
+    const bool whole = i0 + PER_THREAD <= total;
+    if (whole && (DENSE || n + PER_THREAD <= cols)) {
+        a.load(x + m * ldx + n);
+        if (RESIDUAL) b.load(r + m * ldr + n);
     } else {
-        int64_t m = DENSE ? 0 : i0 / cols, n = i0 - m * cols;
 #pragma unroll
         for (int k = 0; k < PER_THREAD; ++k) {
             const bool there = i0 + k < total;
@@ -72,7 +73,7 @@ __device__ __forceinline__ void dropout_eight(int64_t i0, int64_t total, int64_t
             a.v[k + h] = from_f32<T>(v);
         }
     }
-    if (y_aligned && i0 + PER_THREAD <= total) {
+    if (whole) {
         a.store(y + i0);
     } else {
 #pragma unroll
@@ -84,7 +85,7 @@ __device__ __forceinline__ void dropout_eight(int64_t i0, int64_t total, int64_t
 template <typename T, bool DENSE, bool RESIDUAL>
 __global__ __launch_bounds__(256) void dropout_kernel(int64_t total, int64_t cols, const T* x, int64_t ldx, const T* r, int64_t ldr,
                                                       T* y, unsigned long long border, float scale, unsigned long long seed,
-                                                      unsigned long long offset, const int64_t* rng, bool y_aligned) {
+                                                      unsigned long long offset, const int64_t* rng) {
     if (rng) {
         seed = (unsigned long long)rng[0];
         offset = (unsigned long long)rng[1];
@@ -93,7 +94,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(int64_t total, int64_t col
     // one turn, unless the grid's 2^32 threads are not enough
     for (int64_t i0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * PER_THREAD; i0 < total;
          i0 += (int64_t)gridDim.x * 256 * PER_THREAD)
-        dropout_eight<T, DENSE, RESIDUAL>(i0, total, cols, x, ldx, r, ldr, y, border, scale, key, y_aligned);
+        dropout_eight<T, DENSE, RESIDUAL>(i0, total, cols, x, ldx, r, ldr, y, border, scale, key);
 }
 
 template <typename T>
@@ -104,10 +105,10 @@ hipError_t launch(int64_t rows, int64_t cols, const void* x, int64_t ldx, const 
     const unsigned grid = (unsigned)(blocks < (1 << 23) ? blocks : 1 << 23);
     const unsigned long long border = (unsigned long long)__builtin_rint(p * 4294967296.0);
     const float scale = p < 1.0 ? (float)(1.0 / (1.0 - p)) : 0.f;
-    auto run_of = [&](const void* q, int64_t ld) { return ((uintptr_t)q & 15) == 0 && (ld == cols || rows == 1); };
-    const bool dense = run_of(x, ldx) && (!r || run_of(r, ldr));
+    auto run_of = [&](int64_t ld) { return ld == cols || rows == 1; };
+    const bool dense = run_of(ldx) && (!r || run_of(ldr));
 #define PNGPD_DROPOUT(D, R) \
-    dropout_kernel<T, D, R><<<grid, 256, 0, s>>>(total, cols, (const T*)x, ldx, (const T*)r, ldr, (T*)y, border, scale, seed, offset, rng, ((uintptr_t)y & 15) == 0)
+    dropout_kernel<T, D, R><<<grid, 256, 0, s>>>(total, cols, (const T*)x, ldx, (const T*)r, ldr, (T*)y, border, scale, seed, offset, rng)
     if (dense && r) PNGPD_DROPOUT(true, true);
     else if (dense) PNGPD_DROPOUT(true, false);
     else if (r) PNGPD_DROPOUT(false, true);

@@ -19,11 +19,14 @@ constexpr int BLOCK = 256;      // rows whose dz a backward workgroup has at a t
 
 // 16 bytes from p, `valid` elements of them there, zeros behind
 template <typename E>
-__device__ __forceinline__ i32x4 chunk_of(const E* p, int64_t valid, bool vec) {
+__device__ __forceinline__ i32x4 chunk_of(const E* p, int64_t valid) {
     constexpr int C = 16 / sizeof(E);
     typedef __attribute__((ext_vector_type(16 / sizeof(E)))) E V;
-    if (vec && valid >= C) return *(const i32x4*)p;
     V v;
+    if (valid >= C) {
+        __builtin_memcpy(&v, p, 16);
+        return __builtin_bit_cast(i32x4, v);
+    }
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] = i < valid ? p[i] : (E)0.f;
     return __builtin_bit_cast(i32x4, v);
@@ -31,13 +34,13 @@ __device__ __forceinline__ i32x4 chunk_of(const E* p, int64_t valid, bool vec) {
 
 // VP: classes a row has room for, 4 or 8
 template <typename E, int VP>
-__global__ __launch_bounds__(256) void few_loss_kernel(HeadFew g, bool x_vec, bool w_vec, float* row_loss, float* lse) {
+__global__ __launch_bounds__(256) void few_loss_kernel(HeadFew g, float* row_loss, float* lse) {
     constexpr int C = 16 / sizeof(E);
     __shared__ f32x4 share[4][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = lane & 15, q = lane >> 4;
     const int V = (int)g.V;
     const E* bias = (const E*)g.bias;
-    const int64_t steps = (g.D + 4 * C - 1) / (4 * C), whole = x_vec && w_vec ? g.D / (4 * C) : 0;
+    const int64_t steps = (g.D + 4 * C - 1) / (4 * C), whole = g.D / (4 * C);
     // rows and classes beyond the last repeat it: what comes of them is not used
     const E* w = (const E*)g.w + (t < V ? t : V - 1) * g.ldw;
     for (int64_t m0 = (int64_t)blockIdx.x * TILE; m0 < g.T; m0 += (int64_t)gridDim.x * TILE) {
@@ -50,8 +53,8 @@ __global__ __launch_bounds__(256) void few_loss_kernel(HeadFew g, bool x_vec, bo
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const int64_t at = s + 4 * j < whole ? s + 4 * j : whole - 1, d = (at * 4 + q) * C;
-                fw[j] = *(const i32x4*)(w + d);
-                fx[j] = *(const i32x4*)(x + d);
+                fw[j] = chunk_of<E>(w + d, C);
+                fx[j] = chunk_of<E>(x + d, C);
             }
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
@@ -61,7 +64,7 @@ __global__ __launch_bounds__(256) void few_loss_kernel(HeadFew g, bool x_vec, bo
         }
         for (int64_t s = whole + (wave - whole & 3); s < steps; s += 4) {
             const int64_t d = (s * 4 + q) * C;
-            acc = mma16<E>(chunk_of<E>(w + d, g.D - d, w_vec), chunk_of<E>(x + d, g.D - d, x_vec), acc);
+            acc = mma16<E>(chunk_of<E>(w + d, g.D - d), chunk_of<E>(x + d, g.D - d), acc);
         }
         share[wave][lane] = acc;
         __syncthreads();
@@ -113,7 +116,6 @@ struct FewGrad {
     float* part;                // [parts][V][D] and [parts][V], unless there is one part
     int lanes;                  // 2^lanes threads side by side over chunks of columns
     int64_t rows;               // of a part
-    bool x_vec, w_vec, dx_vec;
 };
 
 template <typename E, int VP>
@@ -132,7 +134,7 @@ __global__ __launch_bounds__(256) void few_grad_kernel(HeadFew g, FewGrad o) {
     Vec w[VP];
     if (o.dx) {
 #pragma unroll
-        for (int n = 0; n < VP; ++n) w[n] = __builtin_bit_cast(Vec, chunk_of<E>((const E*)g.w + n * g.ldw + col, n < V ? g.D - col : 0, o.w_vec));
+        for (int n = 0; n < VP; ++n) w[n] = __builtin_bit_cast(Vec, chunk_of<E>((const E*)g.w + n * g.ldw + col, n < V ? g.D - col : 0));
     }
     float acc[VP][C] = {}, db[VP] = {};
     for (int64_t base = m0; base < m1; base += BLOCK) {
@@ -175,7 +177,7 @@ __global__ __launch_bounds__(256) void few_grad_kernel(HeadFew g, FewGrad o) {
                     Vec out;
 #pragma unroll
                     for (int i = 0; i < C; ++i) out[i] = (E)(on ? v.v[i] : 0.f);
-                    if (o.dx_vec) *(Vec*)dx = out;
+                    if (col + C <= g.D) __builtin_memcpy(dx, &out, 16);
                     else
 #pragma unroll
                         for (int i = 0; i < C; ++i)
@@ -183,11 +185,11 @@ __global__ __launch_bounds__(256) void few_grad_kernel(HeadFew g, FewGrad o) {
                 }
             };
             const E* x = (const E*)g.x + base * g.ldx + col;
-            if (o.x_vec && col + C <= g.D) {
+            if (col + C <= g.D) {
 #pragma unroll 4
-                for (int r = row; r < rows; r += side) one(r, *(const Vec*)(x + r * g.ldx));
+                for (int r = row; r < rows; r += side) one(r, __builtin_bit_cast(Vec, chunk_of<E>(x + r * g.ldx, C)));
             } else {
-                for (int r = row; r < rows; r += side) one(r, __builtin_bit_cast(Vec, chunk_of<E>(x + r * g.ldx, g.D - col, false)));
+                for (int r = row; r < rows; r += side) one(r, __builtin_bit_cast(Vec, chunk_of<E>(x + r * g.ldx, g.D - col)));
             }
         }
     }
@@ -271,15 +273,12 @@ FewCut few_cut(int64_t T, int64_t D, int chunk) {
     return c;
 }
 
-bool rows_aligned(const void* p, int64_t ld, size_t size) { return ((uintptr_t)p & 15) == 0 && ld * (int64_t)size % 16 == 0; }
-
 template <typename E>
 hipError_t few_loss(const HeadFew& g, float* row_loss, float* lse, hipStream_t s) {
     const int64_t tiles = (g.T + TILE - 1) / TILE;
     const unsigned grid = (unsigned)(tiles < 65536 ? tiles : 65536);
-    const bool xv = rows_aligned(g.x, g.ldx, sizeof(E)), wv = rows_aligned(g.w, g.ldw, sizeof(E));
-    if (g.V <= 4) few_loss_kernel<E, 4><<<grid, 256, 0, s>>>(g, xv, wv, row_loss, lse);
-    else few_loss_kernel<E, 8><<<grid, 256, 0, s>>>(g, xv, wv, row_loss, lse);
+    if (g.V <= 4) few_loss_kernel<E, 4><<<grid, 256, 0, s>>>(g, row_loss, lse);
+    else few_loss_kernel<E, 8><<<grid, 256, 0, s>>>(g, row_loss, lse);
     return hipGetLastError();
 }
 
@@ -287,8 +286,7 @@ template <typename E>
 hipError_t few_grad(const HeadFew& g, const float* lse, const float* used, const float* dloss, int reduction, void* dx, void* dw,
                     void* db, float* part, hipStream_t s) {
     const FewCut c = few_cut(g.T, g.D, 16 / sizeof(E));
-    const FewGrad o{lse, dloss, used, reduction, dx, dw, db, part, c.lanes, c.rows, rows_aligned(g.x, g.ldx, sizeof(E)),
-                    rows_aligned(g.w, g.ldw, sizeof(E)), rows_aligned(dx, g.D, sizeof(E))};
+    const FewGrad o{lse, dloss, used, reduction, dx, dw, db, part, c.lanes, c.rows};
     const dim3 grid(c.blocks, (unsigned)c.parts);
     if (g.V <= 4) few_grad_kernel<E, 4><<<grid, 256, 0, s>>>(g, o);
     else few_grad_kernel<E, 8><<<grid, 256, 0, s>>>(g, o);

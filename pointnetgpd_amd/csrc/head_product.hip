@@ -11,8 +11,7 @@ namespace {
 
 // 8 neighbouring columns of a row a thread: the cuts of the contraction added in order, then the epilogue
 template <typename E, int KIND, int THREADS>
-__global__ __launch_bounds__(THREADS) void join_kernel(int64_t M, int64_t N, int64_t groups, int splits, const float* partial, HeadEpilogue e,
-                                                   bool vec) {
+__global__ __launch_bounds__(THREADS) void join_kernel(int64_t M, int64_t N, int64_t groups, int splits, const float* partial, HeadEpilogue e) {
     const int64_t total = M * groups;
     for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < total; i += (int64_t)gridDim.x * THREADS) {
         const int64_t m = i / groups, n = (i - m * groups) * 8;
@@ -20,10 +19,10 @@ __global__ __launch_bounds__(THREADS) void join_kernel(int64_t M, int64_t N, int
         const int valid = (int)(have < 0 ? 0 : have < 8 ? have : 8);
         Eight v = {};
 #pragma unroll 4
-        for (int s = 0; s < splits; ++s) add8(v, load8(partial + ((int64_t)s * M + m) * head_partial_ld(N) + n, valid, true));
+        for (int s = 0; s < splits; ++s) add8(v, load8(partial + ((int64_t)s * M + m) * head_partial_ld(N) + n, valid));
         const int64_t room = (KIND == TILE_DZ ? e.ld_out : N) - n;
         const int real = (int)(room < 8 ? room : 8);
-        finish8<E, KIND>(e, N, m, n, real, vec, load_columns<E, KIND>(e, N, n, vec), load_ahead<E, KIND>(e, N, m, n, real, vec), v);
+        finish8<E, KIND>(e, N, m, n, real, load_columns<E, KIND>(e, N, n), load_ahead<E, KIND>(e, N, m, n, real), v);
     }
 }
 
@@ -37,13 +36,12 @@ __global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, i
     const int64_t y = e.target[m];
     const E* bias = (const E*)e.bias;
     float mx = -__builtin_inff(), sum = 0.f, zs = 0.f;
-    const bool bias_vec = ((uintptr_t)bias & 15) == 0;
     for (int64_t n = (threadIdx.x & (LANES - 1)) * 8; n < N; n += LANES * 8) {
         const int valid = N - n < 8 ? (int)(N - n) : 8;
         Eight z = {};
 #pragma unroll 4
-        for (int s = 0; s < splits; ++s) add8(z, load8(partial + ((int64_t)s * M + m) * head_partial_ld(N) + n, valid, true));
-        if (bias) add8(z, load8(bias + n, valid, bias_vec));
+        for (int s = 0; s < splits; ++s) add8(z, load8(partial + ((int64_t)s * M + m) * head_partial_ld(N) + n, valid));
+        if (bias) add8(z, load8(bias + n, valid));
         float top = mx, part = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -81,15 +79,14 @@ __global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, i
 
 template <typename E>
 hipError_t join(int64_t M, int64_t N, int splits, const float* partial, const HeadEpilogue& e, hipStream_t s) {
-    const bool vec = epilogue_vec(e, N, sizeof(E));
     const int64_t groups = ((e.kind == HEAD_EPI_DZ ? e.ld_out : N) + 7) / 8;
     // little to join: small workgroups, so that its loads leave from many compute units
     const bool few = M * groups < 65536;
     const int64_t threads = few ? 64 : 256, blocks = (M * groups + threads - 1) / threads;
     const unsigned grid = (unsigned)(blocks < 65536 ? blocks : 65536);
 #define PNGPD_JOIN(KIND)                                                                                          \
-    if (few) join_kernel<E, KIND, 64><<<grid, 64, 0, s>>>(M, N, groups, splits, partial, e, vec);              \
-    else join_kernel<E, KIND, 256><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e, vec)
+    if (few) join_kernel<E, KIND, 64><<<grid, 64, 0, s>>>(M, N, groups, splits, partial, e);              \
+    else join_kernel<E, KIND, 256><<<grid, 256, 0, s>>>(M, N, groups, splits, partial, e)
     switch (e.kind) {
         case HEAD_EPI_LINEAR: PNGPD_JOIN(TILE_LINEAR); break;
         case HEAD_EPI_DZ: PNGPD_JOIN(TILE_DZ); break;
@@ -105,11 +102,12 @@ hipError_t join(int64_t M, int64_t N, int splits, const float* partial, const He
 // ---- one to four rows -----------------------------------------------------------------------------------------------------------
 
 // y[m][n] for up to MR rows m: a wave takes NR rows of the weight, its lanes 16-byte chunks of them side by side, and adds its
-// lanes' 32-bit fma chains at the end.  Bound by reading the weight once: 4096 x 4096 bf16 (33.5 MB) for one row.
-constexpr int FEW_M = 4;
+// lanes' 32-bit fma chains at the end.  Rows may start at any element.  Bound by reading the weight once: 4096 x 4096 bf16
+// (33.5 MB) for one row, 9 us.
+constexpr int64_t FEW_M = HEAD_FEW_ROWS;
 
 template <typename E, int MR, int NR>
-__global__ __launch_bounds__(256) void rows_kernel(int M, int64_t N, int64_t chunks, const E* x, int64_t ldx, const E* w, int64_t ldw,
+__global__ __launch_bounds__(256) void rows_kernel(int M, int64_t N, int64_t K, const E* x, int64_t ldx, const E* w, int64_t ldw,
                                                    HeadEpilogue e) {
     constexpr int C = 16 / sizeof(E), U = MR * NR > 8 ? 2 : 4;
     typedef __attribute__((ext_vector_type(16 / sizeof(E)))) E chunk;
@@ -122,15 +120,16 @@ __global__ __launch_bounds__(256) void rows_kernel(int M, int64_t N, int64_t chu
 #pragma unroll
     for (int r = 0; r < NR; ++r) pw[r] = w + (n0 + r < N ? n0 + r : n0) * ldw;
     float acc[MR][NR] = {};
+    const int64_t chunks = K / C;
     int64_t c = lane;
     for (; c + (U - 1) * 64 < chunks; c += U * 64) {
         chunk a[U][MR], b[U][NR];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
 #pragma unroll
-            for (int r = 0; r < NR; ++r) b[u][r] = ((const chunk*)pw[r])[c + u * 64];
+            for (int r = 0; r < NR; ++r) __builtin_memcpy(&b[u][r], pw[r] + (c + u * 64) * C, 16);
 #pragma unroll
-            for (int m = 0; m < MR; ++m) a[u][m] = ((const chunk*)px[m])[c + u * 64];
+            for (int m = 0; m < MR; ++m) __builtin_memcpy(&a[u][m], px[m] + (c + u * 64) * C, 16);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -144,15 +143,21 @@ __global__ __launch_bounds__(256) void rows_kernel(int M, int64_t N, int64_t chu
     for (; c < chunks; c += 64) {
         chunk a[MR], b[NR];
 #pragma unroll
-        for (int r = 0; r < NR; ++r) b[r] = ((const chunk*)pw[r])[c];
+        for (int r = 0; r < NR; ++r) __builtin_memcpy(&b[r], pw[r] + c * C, 16);
 #pragma unroll
-        for (int m = 0; m < MR; ++m) a[m] = ((const chunk*)px[m])[c];
+        for (int m = 0; m < MR; ++m) __builtin_memcpy(&a[m], px[m] + c * C, 16);
 #pragma unroll
         for (int i = 0; i < C; ++i)
 #pragma unroll
             for (int m = 0; m < MR; ++m)
 #pragma unroll
                 for (int r = 0; r < NR; ++r) acc[m][r] = __builtin_fmaf((float)a[m][i], (float)b[r][i], acc[m][r]);
+    }
+    for (int64_t k = chunks * C + lane; k < K; k += 64) {
+#pragma unroll
+        for (int m = 0; m < MR; ++m)
+#pragma unroll
+            for (int r = 0; r < NR; ++r) acc[m][r] = __builtin_fmaf((float)px[m][k], (float)pw[r][k], acc[m][r]);
     }
     float mine = 0.f;
 #pragma unroll
@@ -165,18 +170,16 @@ __global__ __launch_bounds__(256) void rows_kernel(int M, int64_t N, int64_t chu
     const int m = lane / NR;
     const int64_t n = n0 + lane % NR;
     if (lane >= MR * NR || m >= M || n >= N) return;
-    const Columns col = load_columns<E, TILE_LINEAR>(e, n + 1, n, false);
+    const Columns col = load_columns<E, TILE_LINEAR>(e, n + 1, n);
     Eight v = {{mine}};
-    finish8<E, TILE_LINEAR>(e, N, m, n, 1, false, col, load_ahead<E, TILE_LINEAR>(e, N, m, n, 1, false), v);
+    finish8<E, TILE_LINEAR>(e, N, m, n, 1, col, load_ahead<E, TILE_LINEAR>(e, N, m, n, 1), v);
 }
 
 template <typename E, int MR>
 hipError_t rows(int M, int64_t N, int64_t K, const HeadOperand& a, const HeadOperand& b, const HeadEpilogue& e, hipStream_t s) {
-    constexpr int C = 16 / sizeof(E);
-    const int64_t chunks = (K + C - 1) / C;
     // four rows of the weight a wave once that leaves a wave for every SIMD
 #define PNGPD_ROWS(NR) \
-    rows_kernel<E, MR, NR><<<(unsigned)((N + 4 * NR - 1) / (4 * NR)), 256, 0, s>>>(M, N, chunks, (const E*)a.p, a.ld, (const E*)b.p, b.ld, e)
+    rows_kernel<E, MR, NR><<<(unsigned)((N + 4 * NR - 1) / (4 * NR)), 256, 0, s>>>(M, N, K, (const E*)a.p, a.ld, (const E*)b.p, b.ld, e)
     if (N >= 4096) PNGPD_ROWS(4);
     else if (N >= 2048) PNGPD_ROWS(2);
     else PNGPD_ROWS(1);
@@ -221,11 +224,10 @@ hipError_t product(int type, int64_t M, int64_t N, int64_t K, const HeadOperand&
                      : e.kind == HEAD_EPI_DZ     ? TILE_DZ
                      : e.kind == HEAD_EPI_STATS  ? TILE_STATS
                                                  : TILE_SCALED;
-    const bool vec = parts || keep || epilogue_vec(e, N, sizeof(E));
     hipError_t err;
-    if constexpr (__is_same(E, float)) err = launch_tile_f32(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
-    else if constexpr (__is_same(E, bf16_t)) err = launch_tile_bf16(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
-    else err = launch_tile_f16(p.shape, kind, a.k_contiguous, b.k_contiguous, g, vec, s);
+    if constexpr (__is_same(E, float)) err = launch_tile_f32(p.shape, kind, a.k_contiguous, b.k_contiguous, g, s);
+    else if constexpr (__is_same(E, bf16_t)) err = launch_tile_bf16(p.shape, kind, a.k_contiguous, b.k_contiguous, g, s);
+    else err = launch_tile_f16(p.shape, kind, a.k_contiguous, b.k_contiguous, g, s);
     if (err != hipSuccess || !parts) return err;
     return join<E>(M, N, p.splits, partial, e, s);
 }
@@ -240,11 +242,10 @@ hipError_t gradients(int type, const HeadGradient& x, const HeadGradient& w, hip
         return err != hipSuccess ? err : product<E>(type, x.M, x.N, x.K, x.a, x.b, x.e, x.partial, false, s);
     }
     const TileArgs gx = tile_args<E>(px, x.M, x.N, x.K, x.a, x.b, x.e, x.partial), gw = tile_args<E>(pw, w.M, w.N, w.K, w.a, w.b, w.e, w.partial);
-    const bool vx = px.splits > 1 || epilogue_vec(x.e, x.N, sizeof(E)), vw = pw.splits > 1 || epilogue_vec(w.e, w.N, sizeof(E));
     hipError_t err;
-    if constexpr (__is_same(E, float)) err = launch_pair_f32(gx, gw, vx, vw, s);
-    else if constexpr (__is_same(E, bf16_t)) err = launch_pair_bf16(gx, gw, vx, vw, s);
-    else err = launch_pair_f16(gx, gw, vx, vw, s);
+    if constexpr (__is_same(E, float)) err = launch_pair_f32(gx, gw, s);
+    else if constexpr (__is_same(E, bf16_t)) err = launch_pair_bf16(gx, gw, s);
+    else err = launch_pair_f16(gx, gw, s);
     if (err == hipSuccess && pw.splits > 1) err = join<E>(w.M, w.N, pw.splits, w.partial, w.e, s);
     if (err == hipSuccess && px.splits > 1) err = join<E>(x.M, x.N, px.splits, x.partial, x.e, s);
     return err;
@@ -257,9 +258,12 @@ struct Chunk {
     static constexpr int C = 16 / sizeof(T);
     typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T V;
     // up to C values from p, `valid` of them there, zeros behind
-    __device__ static __forceinline__ V load(const T* p, int64_t valid, bool aligned) {
+    __device__ static __forceinline__ V load(const T* p, int64_t valid) {
         V v;
-        if (aligned && valid >= C) return *(const V*)p;
+        if (valid >= C) {
+            __builtin_memcpy(&v, p, 16);
+            return v;
+        }
 #pragma unroll
         for (int i = 0; i < C; ++i) v[i] = i < valid ? p[i] : (T)0.f;
         return v;
@@ -311,7 +315,6 @@ __device__ __forceinline__ void row_weights(const HeadRowWeights& w, bool scaled
 
 struct LayOutRun {
     HeadLayOut m;
-    bool aligned;
     int64_t blocks;        // of 256 chunks
     unsigned grid;
 };
@@ -339,7 +342,7 @@ __global__ __launch_bounds__(256) void set_up_kernel(LayOutRun a, LayOutRun b, H
             live = y != w.ignore_index && y >= 0 && y < w.V;
         }
         typename Chunk<T>::V v = {};
-        if (live) v = Chunk<T>::load((const T*)u.m.src + r * u.m.ld_src + c, u.m.cols - c, u.aligned);
+        if (live) v = Chunk<T>::load((const T*)u.m.src + r * u.m.ld_src + c, u.m.cols - c);
         *(typename Chunk<T>::V*)((T*)u.m.dst + r * u.m.ld + c) = v;
     }
 }
@@ -351,7 +354,6 @@ hipError_t set_up(const HeadLayOut* a, const HeadLayOut* b, const HeadRowWeights
         LayOutRun r{};
         if (!m) return r;
         r.m = *m;
-        r.aligned = ((uintptr_t)m->src & 15) == 0 && m->ld_src % C == 0;
         r.blocks = (m->rows * (m->ld / C) + 255) / 256;
         r.grid = (unsigned)(r.blocks < (1 << 22) ? r.blocks : 1 << 22);
         return r;
@@ -390,8 +392,8 @@ ColumnCut column_cut(int64_t M, int64_t N, int chunk) {
 
 // One pass over dy and z: bound by memory, so the sums of the columns ride along.
 template <typename T, int ACT, bool WRITE>
-__global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, const T* dy, int64_t ld, bool dy_aligned, const T* z,
-                                                        bool z_aligned, T* dz, int64_t ld_dz, float* part, int lanes, int64_t rows,
+__global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, const T* dy, int64_t ld, const T* z, T* dz,
+                                                        int64_t ld_dz, float* part, int lanes, int64_t rows,
                                                         const float* scale, T* sums) {
     constexpr int C = Chunk<T>::C;
     __shared__ float share[256][C + 1];
@@ -403,10 +405,10 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, co
     if (col < N) {
 #pragma unroll 2
         for (int64_t m = m0 + row; m < m1; m += side) {
-            const typename Chunk<T>::V g = Chunk<T>::load(dy + m * ld + col, N - col, dy_aligned);
+            const typename Chunk<T>::V g = Chunk<T>::load(dy + m * ld + col, N - col);
             typename Chunk<T>::V o = g;
             if constexpr (ACT != PNGPD_ACT_NONE) {
-                const typename Chunk<T>::V v = Chunk<T>::load(z + m * N + col, N - col, z_aligned);
+                const typename Chunk<T>::V v = Chunk<T>::load(z + m * N + col, N - col);
 #pragma unroll
                 for (int i = 0; i < C; ++i) {
                     const float d = (float)g[i] * act_slope<ACT>((float)v[i]);
@@ -458,9 +460,8 @@ hipError_t grad_rows(int64_t M, int64_t N, const void* dy, int64_t ld, const voi
     constexpr int C = Chunk<T>::C;
     const ColumnCut c = column_cut(M, N, C);
     const dim3 grid(c.blocks, (unsigned)c.parts);
-    const bool da = ((uintptr_t)dy & 15) == 0 && ld % C == 0, za = ((uintptr_t)z & 15) == 0 && N % C == 0;
 #define PNGPD_GRAD_ROWS(A, W) \
-    grad_rows_kernel<T, A, W><<<grid, 256, 0, s>>>(M, N, (const T*)dy, ld, da, (const T*)z, za, (T*)dz, ld_dz, part, c.lanes, c.rows, scale, (T*)sums)
+    grad_rows_kernel<T, A, W><<<grid, 256, 0, s>>>(M, N, (const T*)dy, ld, (const T*)z, (T*)dz, ld_dz, part, c.lanes, c.rows, scale, (T*)sums)
     switch (act) {
         case PNGPD_ACT_NONE:
             if (dz) PNGPD_GRAD_ROWS(PNGPD_ACT_NONE, true);

@@ -179,19 +179,21 @@ struct TileOperand {
     }
 };
 
-// Eight neighbouring values of a row, as 16-byte accesses where `vec` says that every row starts suitably aligned.
+// Eight neighbouring values of a row, as 16-byte accesses wherever they start: the hardware takes
+// them at any element (4001 x 2001 -> 1999 bfloat16 training 171 us, 220 with an access an element in such rows).
 struct Eight {
     float v[8];
 };
 template <typename T>
-__device__ __forceinline__ Eight load8(const T* p, int valid, bool vec) {
+__device__ __forceinline__ Eight load8(const T* p, int valid) {
     constexpr int C = 16 / sizeof(T);
     typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T chunk;
     Eight r;
-    if (vec && valid >= 8) {
+    if (valid >= 8) {
 #pragma unroll
         for (int k = 0; k < 8 / C; ++k) {
-            const chunk c = ((const chunk*)p)[k];
+            chunk c;
+            __builtin_memcpy(&c, p + k * C, 16);
 #pragma unroll
             for (int i = 0; i < C; ++i) r.v[k * C + i] = (float)c[i];
         }
@@ -202,16 +204,16 @@ __device__ __forceinline__ Eight load8(const T* p, int valid, bool vec) {
     return r;
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const Eight& r, int valid, bool vec) {
+__device__ __forceinline__ void store8(T* p, const Eight& r, int valid) {
     constexpr int C = 16 / sizeof(T);
     typedef __attribute__((ext_vector_type(16 / sizeof(T)))) T chunk;
-    if (vec && valid >= 8) {
+    if (valid >= 8) {
 #pragma unroll
         for (int k = 0; k < 8 / C; ++k) {
             chunk c;
 #pragma unroll
             for (int i = 0; i < C; ++i) c[i] = (T)r.v[k * C + i];
-            ((chunk*)p)[k] = c;
+            __builtin_memcpy(p + k * C, &c, 16);
         }
     } else {
 #pragma unroll
@@ -244,11 +246,11 @@ struct Columns {
     float scale;
 };
 template <typename E, int KIND>
-__device__ __forceinline__ Columns load_columns(const HeadEpilogue& e, int64_t N, int64_t n, bool vec) {
+__device__ __forceinline__ Columns load_columns(const HeadEpilogue& e, int64_t N, int64_t n) {
     Columns c = {};
     c.scale = 1.f;
     if constexpr (KIND == TILE_LINEAR || KIND == TILE_DZ) {
-        if (e.bias) c.bias = load8((const E*)e.bias + n, (int)(N - n < 0 ? 0 : N - n < 8 ? N - n : 8), vec);
+        if (e.bias) c.bias = load8((const E*)e.bias + n, (int)(N - n < 0 ? 0 : N - n < 8 ? N - n : 8));
     }
     if constexpr (KIND == TILE_SCALED) {
         if (e.scale) c.scale = e.scale[0];
@@ -261,22 +263,22 @@ struct Ahead {
     int label;
 };
 template <typename E, int KIND>
-__device__ __forceinline__ Ahead load_ahead(const HeadEpilogue& e, int64_t N, int64_t m, int64_t n, int valid, bool vec) {
+__device__ __forceinline__ Ahead load_ahead(const HeadEpilogue& e, int64_t N, int64_t m, int64_t n, int valid) {
     Ahead h = {};
     if constexpr (KIND == TILE_LINEAR) {
-        if (e.residual) h.more = load8((const E*)e.residual + m * e.ld_residual + n, valid, vec);
+        if (e.residual) h.more = load8((const E*)e.residual + m * e.ld_residual + n, valid);
     } else if constexpr (KIND == TILE_DZ) {
         h.weight = e.row_weight[m];
         h.lse = e.lse[m];
         const int64_t y = e.target[m] - e.first_n - n;
         h.label = y >= 0 && y < 8 ? (int)y : -1;
     } else if constexpr (KIND == TILE_SCALED) {
-        if (e.add) h.more = load8(e.add + m * N + n, valid, vec);
+        if (e.add) h.more = load8(e.add + m * N + n, valid);
     }
     return h;
 }
 template <typename E, int KIND>
-__device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_t m, int64_t n, int valid, bool vec, const Columns& col,
+__device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_t m, int64_t n, int valid, const Columns& col,
                                         const Ahead& h, Eight& a) {
     if constexpr (KIND == TILE_LINEAR) {
         add8(a, col.bias);
@@ -286,9 +288,9 @@ __device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_
                 Eight k;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) k.v[i] = (float)keep_z<E, PNGPD_ACT_RELU>(a.v[i]);
-                store8(z, k, valid, vec);
+                store8(z, k, valid);
             } else {
-                store8(z, a, valid, vec);
+                store8(z, a, valid);
             }
         }
         switch (e.act) {
@@ -298,7 +300,7 @@ __device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_
             case PNGPD_ACT_SILU: act8<PNGPD_ACT_SILU>(a); break;
         }
         if (e.residual) add8(a, h.more);
-        store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
+        store8((E*)e.out + m * e.ld_out + n, a, valid);
     } else if constexpr (KIND == TILE_DZ) {
         // What only some rows or columns have stands in branches of its own: an instruction on every element costs half a
         // microsecond a tile.
@@ -314,27 +316,21 @@ __device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_
 #pragma unroll
             for (int i = 0; i < 8; ++i) a.v[i] = h.weight == 0.f || n + i >= N ? 0.f : a.v[i];
         }
-        store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
+        store8((E*)e.out + m * e.ld_out + n, a, valid);
     } else {
         if (e.add) add8(a, h.more);
 #pragma unroll
         for (int i = 0; i < 8; ++i) a.v[i] *= col.scale;
-        if (e.out_f32) store8((float*)e.out + m * e.ld_out + n, a, valid, vec);
-        else store8((E*)e.out + m * e.ld_out + n, a, valid, vec);
+        if (e.out_f32) store8((float*)e.out + m * e.ld_out + n, a, valid);
+        else store8((E*)e.out + m * e.ld_out + n, a, valid);
     }
-}
-
-// rows of every matrix the epilogue touches start at 16-byte addresses, so does every eighth of their columns
-inline bool epilogue_vec(const HeadEpilogue& e, int64_t N, size_t sz) {
-    auto ok = [](const void* p, int64_t ld, size_t size) { return !p || (((uintptr_t)p & 15) == 0 && ld % (16 / (int64_t)size) == 0); };
-    return ok(e.out, e.ld_out, e.out_f32 ? 4 : sz) && ok(e.bias, 0, sz) && ok(e.residual, e.ld_residual, sz) && ok(e.z, N, sz) && ok(e.add, N, 4);
 }
 
 // ---- the kernel -------------------------------------------------------------------------------------------------------------
 
 // BM x BN outputs by WM x WN waves; AK / BK: the contraction is dense in the m / n operand
 template <typename E, int BM, int BN, int WM, int WN, bool AK, bool BK, int KIND, int RING>
-__device__ __forceinline__ void product_tile(const TileArgs& g, bool vec, int block) {
+__device__ __forceinline__ void product_tile(const TileArgs& g, int block) {
     constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16, STEP = 128 / (int)sizeof(E);
     constexpr int STAGE = (BM + BN) * 128;
     typedef TileOperand<E, BM, AK, WAVES> OpA;
@@ -491,7 +487,7 @@ __device__ __forceinline__ void product_tile(const TileArgs& g, bool vec, int bl
         const int c = (threadIdx.x % GROUPS) * 2;
         const int64_t n = n0 + c * 4, have = (KIND == TILE_DZ ? g.e.ld_out : g.N) - n;
         const int valid = (int)(have < 0 ? 0 : have < 8 ? have : 8);
-        const Columns col = load_columns<E, KIND>(g.e, g.N, n, vec);
+        const Columns col = load_columns<E, KIND>(g.e, g.N, n);
 #pragma unroll
         for (int pass = 0; pass < PASSES; ++pass) {
             __syncthreads();
@@ -513,7 +509,7 @@ __device__ __forceinline__ void product_tile(const TileArgs& g, bool vec, int bl
                 for (int k = 0; k < BATCH; ++k) {
                     const int r = r0 + k * RSTEP, in = r / (JP * 16);      // which wave row staged it
                     const int64_t m = m0 + (in * FM + pass * JP) * 16 + (r - in * JP * 16);
-                    if (r < ROWS && m < g.M && valid > 0) ahead[k] = load_ahead<E, KIND>(g.e, g.N, m, n, valid, vec);
+                    if (r < ROWS && m < g.M && valid > 0) ahead[k] = load_ahead<E, KIND>(g.e, g.N, m, n, valid);
                 }
 #pragma unroll
                 for (int k = 0; k < BATCH; ++k) {
@@ -523,8 +519,8 @@ __device__ __forceinline__ void product_tile(const TileArgs& g, bool vec, int bl
                     const f32x4 lo = *(const f32x4*)(smem + r * (BN * 4) + (c ^ (r & MIX)) * 16);
                     const f32x4 hi = *(const f32x4*)(smem + r * (BN * 4) + ((c + 1) ^ (r & MIX)) * 16);
                     Eight a = {{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
-                    if constexpr (KIND == TILE_PARTIAL || KIND == TILE_STATS) store8(g.partial + ((int64_t)split * g.M + m) * head_partial_ld(g.N) + n, a, valid, vec);
-                    else finish8<E, KIND>(g.e, g.N, m, n, valid, vec, col, ahead[k], a);
+                    if constexpr (KIND == TILE_PARTIAL || KIND == TILE_STATS) store8(g.partial + ((int64_t)split * g.M + m) * head_partial_ld(g.N) + n, a, valid);
+                    else finish8<E, KIND>(g.e, g.N, m, n, valid, col, ahead[k], a);
                 }
             }
         }
@@ -609,19 +605,19 @@ __device__ __forceinline__ void product_tile(const TileArgs& g, bool vec, int bl
 }
 
 template <typename E, int BM, int BN, int WM, int WN, bool AK, bool BK, int KIND, int RING>
-__global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs g, bool vec) {
-    product_tile<E, BM, BN, WM, WN, AK, BK, KIND, RING>(g, vec, blockIdx.x);
+__global__ __launch_bounds__(WM * WN * 64, 2) void product_tile_kernel(TileArgs g) {
+    product_tile<E, BM, BN, WM, WN, AK, BK, KIND, RING>(g, blockIdx.x);
 }
 
 // Both gradients of a product in one launch, 64 x 64 tiles: the first `first` workgroups are x's (or the weight's, where
 // `weight_first`).  A launch less, and the second product's tiles run while the first one's last ones do: training 1024 x 1024 ->
 // 1024 takes 33 us instead of 38 in bfloat16, 77 instead of 85 in float32.
 template <typename E, int KIND_X, int KIND_W>
-__global__ __launch_bounds__(256, 2) void gradient_pair_kernel(TileArgs x, TileArgs w, bool x_vec, bool w_vec, int first, bool weight_first) {
+__global__ __launch_bounds__(256, 2) void gradient_pair_kernel(TileArgs x, TileArgs w, int first, bool weight_first) {
     const int block = blockIdx.x;
     const bool early = block < first;
-    if (early != weight_first) product_tile<E, 64, 64, 2, 2, true, false, KIND_X, 3>(x, x_vec, early ? block : block - first);
-    else product_tile<E, 64, 64, 2, 2, false, false, KIND_W, 3>(w, w_vec, early ? block : block - first);
+    if (early != weight_first) product_tile<E, 64, 64, 2, 2, true, false, KIND_X, 3>(x, early ? block : block - first);
+    else product_tile<E, 64, 64, 2, 2, false, false, KIND_W, 3>(w, early ? block : block - first);
 }
 
 // ---- launch -----------------------------------------------------------------------------------------------------------------
@@ -634,54 +630,54 @@ inline void shape_size(int shape, int* bm, int* bn) {
 }
 
 template <typename E, int BM, int BN, int WM, int WN, bool AK, bool BK, int KIND, int RING>
-hipError_t launch_one(const TileArgs& g, bool vec, hipStream_t s) {
+hipError_t launch_one(const TileArgs& g, hipStream_t s) {
     constexpr int lds = RING * (BM + BN) * 128;
     const auto kern = product_tile_kernel<E, BM, BN, WM, WN, AK, BK, KIND, RING>;
     if (lds > 65536) {
         const hipError_t e = set_max_lds_once((const void*)kern, lds);
         if (e != hipSuccess) return e;
     }
-    kern<<<(unsigned)(g.tiles_m * g.tiles_n * g.splits), WM * WN * 64, lds, s>>>(g, vec);
+    kern<<<(unsigned)(g.tiles_m * g.tiles_n * g.splits), WM * WN * 64, lds, s>>>(g);
     return hipGetLastError();
 }
 
 template <typename E, bool AK, bool BK, int KIND>
-hipError_t launch_shape(int shape, const TileArgs& g, bool vec, hipStream_t s) {
+hipError_t launch_shape(int shape, const TileArgs& g, hipStream_t s) {
     switch (shape) {
         case SHAPE_256:
             // floats need no larger tile than 128: their matrix instructions take eight times as long over what LDS delivers
-            if constexpr (sizeof(E) == 2) return launch_one<E, 256, 256, 2, 4, AK, BK, KIND, 2>(g, vec, s);
+            if constexpr (sizeof(E) == 2) return launch_one<E, 256, 256, 2, 4, AK, BK, KIND, 2>(g, s);
             return hipErrorInvalidValue;
         case SHAPE_128:
             // alone on its compute unit a tile waits for its loads: one more stage (0.65 instead of 0.90 us a step); two to a
             // unit cover each other and would not fit with three stages
-            if (sizeof(E) == 2 && g.tiles_m * g.tiles_n * g.splits <= 256) return launch_one<E, 128, 128, 2, 2, AK, BK, KIND, 3>(g, vec, s);
-            return launch_one<E, 128, 128, 2, 2, AK, BK, KIND, 2>(g, vec, s);
-        case SHAPE_64: return launch_one<E, 64, 64, 2, 2, AK, BK, KIND, 3>(g, vec, s);
-        case SHAPE_FEW_ROWS: return launch_one<E, 32, 128, 1, 4, AK, BK, KIND, 3>(g, vec, s);
-        default: return launch_one<E, 128, 32, 4, 1, AK, BK, KIND, 3>(g, vec, s);
+            if (sizeof(E) == 2 && g.tiles_m * g.tiles_n * g.splits <= 256) return launch_one<E, 128, 128, 2, 2, AK, BK, KIND, 3>(g, s);
+            return launch_one<E, 128, 128, 2, 2, AK, BK, KIND, 2>(g, s);
+        case SHAPE_64: return launch_one<E, 64, 64, 2, 2, AK, BK, KIND, 3>(g, s);
+        case SHAPE_FEW_ROWS: return launch_one<E, 32, 128, 1, 4, AK, BK, KIND, 3>(g, s);
+        default: return launch_one<E, 128, 32, 4, 1, AK, BK, KIND, 3>(g, s);
     }
 }
 
 // forward products and logits: both operands dense in the contraction; dx: the second one transposed; dW: both
 template <typename E>
-hipError_t launch_tile(int shape, int kind, bool ak, bool bk, const TileArgs& g, bool vec, hipStream_t s) {
+hipError_t launch_tile(int shape, int kind, bool ak, bool bk, const TileArgs& g, hipStream_t s) {
     if (ak && bk) {
         switch (kind) {
-            case TILE_LINEAR: return launch_shape<E, true, true, TILE_LINEAR>(shape, g, vec, s);
-            case TILE_DZ: return launch_shape<E, true, true, TILE_DZ>(shape, g, vec, s);
-            case TILE_STATS: return launch_shape<E, true, true, TILE_STATS>(shape, g, vec, s);
-            case TILE_PARTIAL: return launch_shape<E, true, true, TILE_PARTIAL>(shape, g, vec, s);
+            case TILE_LINEAR: return launch_shape<E, true, true, TILE_LINEAR>(shape, g, s);
+            case TILE_DZ: return launch_shape<E, true, true, TILE_DZ>(shape, g, s);
+            case TILE_STATS: return launch_shape<E, true, true, TILE_STATS>(shape, g, s);
+            case TILE_PARTIAL: return launch_shape<E, true, true, TILE_PARTIAL>(shape, g, s);
         }
     } else if (ak && !bk) {
         switch (kind) {
-            case TILE_SCALED: return launch_shape<E, true, false, TILE_SCALED>(shape, g, vec, s);
-            case TILE_PARTIAL: return launch_shape<E, true, false, TILE_PARTIAL>(shape, g, vec, s);
+            case TILE_SCALED: return launch_shape<E, true, false, TILE_SCALED>(shape, g, s);
+            case TILE_PARTIAL: return launch_shape<E, true, false, TILE_PARTIAL>(shape, g, s);
         }
     } else if (!ak && !bk) {
         switch (kind) {
-            case TILE_SCALED: return launch_shape<E, false, false, TILE_SCALED>(shape, g, vec, s);
-            case TILE_PARTIAL: return launch_shape<E, false, false, TILE_PARTIAL>(shape, g, vec, s);
+            case TILE_SCALED: return launch_shape<E, false, false, TILE_SCALED>(shape, g, s);
+            case TILE_PARTIAL: return launch_shape<E, false, false, TILE_PARTIAL>(shape, g, s);
         }
     }
     return hipErrorInvalidValue;
@@ -689,12 +685,12 @@ hipError_t launch_tile(int shape, int kind, bool ak, bool bk, const TileArgs& g,
 
 // x's and the weight's gradient, both in 64 x 64 tiles; the one whose tiles take more steps first
 template <typename E>
-hipError_t launch_pair(const TileArgs& x, const TileArgs& w, bool x_vec, bool w_vec, hipStream_t s) {
+hipError_t launch_pair(const TileArgs& x, const TileArgs& w, hipStream_t s) {
     constexpr int lds = 3 * 128 * 128;
     const int nx = x.tiles_m * x.tiles_n * x.splits, nw = w.tiles_m * w.tiles_n * w.splits;
     const bool weight_first = w.k_split > x.k_split;
     const int first = weight_first ? nw : nx;
-#define PNGPD_PAIR(KX, KW) gradient_pair_kernel<E, KX, KW><<<(unsigned)(nx + nw), 256, lds, s>>>(x, w, x_vec, w_vec, first, weight_first)
+#define PNGPD_PAIR(KX, KW) gradient_pair_kernel<E, KX, KW><<<(unsigned)(nx + nw), 256, lds, s>>>(x, w, first, weight_first)
     if (x.splits > 1) {
         if (w.splits > 1) PNGPD_PAIR(TILE_PARTIAL, TILE_PARTIAL);
         else PNGPD_PAIR(TILE_PARTIAL, TILE_SCALED);
@@ -706,11 +702,11 @@ hipError_t launch_pair(const TileArgs& x, const TileArgs& w, bool x_vec, bool w_
     return hipGetLastError();
 }
 
-hipError_t launch_pair_f32(const TileArgs& x, const TileArgs& w, bool x_vec, bool w_vec, hipStream_t s);
-hipError_t launch_pair_bf16(const TileArgs& x, const TileArgs& w, bool x_vec, bool w_vec, hipStream_t s);
-hipError_t launch_pair_f16(const TileArgs& x, const TileArgs& w, bool x_vec, bool w_vec, hipStream_t s);
-hipError_t launch_tile_f32(int shape, int kind, bool ak, bool bk, const TileArgs& g, bool vec, hipStream_t s);
-hipError_t launch_tile_bf16(int shape, int kind, bool ak, bool bk, const TileArgs& g, bool vec, hipStream_t s);
-hipError_t launch_tile_f16(int shape, int kind, bool ak, bool bk, const TileArgs& g, bool vec, hipStream_t s);
+hipError_t launch_pair_f32(const TileArgs& x, const TileArgs& w, hipStream_t s);
+hipError_t launch_pair_bf16(const TileArgs& x, const TileArgs& w, hipStream_t s);
+hipError_t launch_pair_f16(const TileArgs& x, const TileArgs& w, hipStream_t s);
+hipError_t launch_tile_f32(int shape, int kind, bool ak, bool bk, const TileArgs& g, hipStream_t s);
+hipError_t launch_tile_bf16(int shape, int kind, bool ak, bool bk, const TileArgs& g, hipStream_t s);
+hipError_t launch_tile_f16(int shape, int kind, bool ak, bool bk, const TileArgs& g, hipStream_t s);
 
 }  // namespace pngpd

@@ -42,7 +42,7 @@ def _linear(lib, type=0, M=2, N=3, K=4, x=16, ldx=4, w=16, ldw=4, act=0, r=0, ld
     (dict(K=0), ERR_SHAPE), (dict(M=2 ** 31), ERR_SHAPE), (dict(x=None), ERR_INVALID), (dict(w=None), ERR_INVALID),
     (dict(y=None), ERR_INVALID), (dict(act=5), ERR_INVALID), (dict(ldx=3), ERR_SHAPE), (dict(ldw=3), ERR_SHAPE),
     (dict(r=16, ldr=2), ERR_SHAPE), (dict(K=2 ** 21 + 1, ldx=2 ** 22, ldw=2 ** 22), ERR_SHAPE), (dict(N=2 ** 21 + 1), ERR_SHAPE),
-    (dict(K=5, ldx=5, ldw=5), ERR_INVALID)])      # rows that have to be copied, and no workspace
+    (dict(M=6, K=5, ldx=5, ldw=5), ERR_INVALID)])      # rows that have to be copied, and no workspace
 def test_linear_forward_refuses(change, code):
     lib = _lib.load()
     assert _linear(lib, **change) == code

@@ -867,3 +867,39 @@ def test_few_classes_without_kept_logits():
                                                    ws.data_ptr(), ws.numel(), stream) == 0
     want = ho.cross_entropy(x, w, target, b, -100, 0.1, "mean", torch.tensor(1.0))
     check({"loss": loss[0], "dx": out[0], "dw": out[1], "db": out[2]}, want)
+
+
+def shifted(t, by, gap):
+    """The same values `by` elements behind an aligned address, rows `gap` elements apart behind their end."""
+    flat = torch.zeros(by + t.shape[0] * (t.shape[1] + gap), dtype=t.dtype, device="cuda")
+    view = flat[by:].view(t.shape[0], t.shape[1] + gap)[:, :t.shape[1]]
+    view.copy_(t.cuda())
+    return view
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("M", [1, 3, 70])
+@pytest.mark.parametrize("by,gap", [(1, 0), (3, 1), (0, 5), (2, 6)])
+def test_rows_that_start_at_any_element(kind, M, by, gap):
+    """Inputs, weight, residual, bias and incoming gradient away from 16-byte addresses: the same results, bit for bit."""
+    dt = TYPES[kind]
+    x, w, b, r, dy = linear_case(7, M, 88, 120, dt, "silu", True, True)
+    bias = torch.zeros(88 + by, dtype=dt, device="cuda")
+    bias[by:] = b.cuda()
+    target = torch.arange(M, device="cuda") % 88
+
+    def run(x, w, b, r, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        y = head.linear(leaves[0], leaves[1], leaves[2], "silu", leaves[3])
+        d = head.dropout(leaves[3], 0.3, 5, 1, residual=dy)
+        loss = head.linear_cross_entropy(leaves[0], leaves[1], target, leaves[2], reduction="sum")
+        few = head.linear_cross_entropy(leaves[0], leaves[1][:5], target % 5, leaves[2][:5], reduction="sum")
+        with torch.no_grad():
+            plain = head.linear(x, w, b, "silu", r)
+        return [y, d, plain, *torch.autograd.grad(y, leaves, dy), *torch.autograd.grad(d, leaves[3], dy),
+                *torch.autograd.grad(loss, leaves[:3]), *torch.autograd.grad(few, leaves[:3])]
+
+    want = run(*(t.cuda() for t in (x, w, b, r, dy)))
+    got = run(shifted(x, by, gap), shifted(w, by, gap), bias[by:], shifted(r, by, gap), shifted(dy, by, gap))
+    for i, (p, q) in enumerate(zip(got, want)):
+        assert torch.equal(p, q), i
