@@ -56,6 +56,7 @@ __global__ __launch_bounds__(256) void few_loss_kernel(HeadFew g, float* row_los
                 fw[j] = chunk_of<E>(w + d, C);
                 fx[j] = chunk_of<E>(x + d, C);
             }
+            fence();      // or the compiler takes them one by one
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const bool real = s + 4 * j < whole;
