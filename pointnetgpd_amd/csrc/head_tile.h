@@ -12,6 +12,10 @@
 //                      touches spread over the banks.  16-bit fragments come out of ds_read_b64_tr_b16, which hands
 //                      lane t of 16 the column t of a 4 x 16 block.
 // The n side is the matrix instruction's first operand, so a lane ends up with 4 neighbouring n of one m.
+//
+// 16-bit: 256 x 256 tiles reach 1.24 PFLOP/s (8192 x 4096 x 8192 in 445 us, 488 with gelu_tanh and a residual) and are bound by
+// power: the same instructions on zeros run 1.4 times as fast.  Floats: 64 x 64 tiles, three to a compute unit, reach 0.14
+// PFLOP/s of the matrix unit's 0.157 inside the loop, 0.13 over 4096 x 2048 x 2048.
 #pragma once
 #include "head.h"
 #include "head_math.h"
