@@ -27,8 +27,8 @@ __global__ __launch_bounds__(THREADS) void join_kernel(int64_t M, int64_t N, int
     }
 }
 
-// a row a workgroup, or a wave where rows are short (LANES): statistics of its logits, formed from the cuts of the contraction.  Eight logits at a time share one
-// rescaling of the sum; 1023 rows of 10007 sums (41 MB) take 12 us, 29 with one at a time.
+// a row a workgroup, or a wave where rows are short (LANES): statistics of its logits, formed from the cuts of the contraction.
+// Eight logits at a time share one rescaling of the sum; 1023 rows of 10007 sums (41 MB) take 12 us, 29 with one at a time.
 template <typename E, int LANES>
 __global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, int splits, const float* partial, HeadEpilogue e) {
     __shared__ float4 share[4];

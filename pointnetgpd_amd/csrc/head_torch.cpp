@@ -75,8 +75,9 @@ void refuse_mixed_capture(const at::Tensor& like) {
     const auto node = torch::autograd::get_current_node();
     if (!node) return;
     const auto current = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(like.get_device());
-    for (const auto& edge : node->next_edges()) {
-        if (!edge.is_valid()) continue;
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+        const auto& edge = node->next_edge(i);
+        if (!edge.is_valid() || !node->task_should_compute_output(i)) continue;
         const auto theirs = edge.function->stream();
         if (!theirs.has_value() || *theirs == current.unwrap()) continue;
         if (!capturing(current.stream())) return;

@@ -903,3 +903,19 @@ def test_rows_that_start_at_any_element(kind, M, by, gap):
     got = run(shifted(x, by, gap), shifted(w, by, gap), bias[by:], shifted(r, by, gap), shifted(dy, by, gap))
     for i, (p, q) in enumerate(zip(got, want)):
         assert torch.equal(p, q), i
+
+
+def test_a_captured_head_on_an_eager_feature():
+    """Gradients of the head's own parameters alone: the eager graph behind the feature is not reached, and not refused."""
+    x, w0, w, b = (t.cuda().requires_grad_() for t in make(98, (32, 24), (40, 24), (50, 40), (50,)))
+    target = torch.randint(0, 50, (32,), generator=torch.Generator().manual_seed(9)).cuda()
+    feature = head.linear(x, w0)
+    want = torch.autograd.grad(head.linear_cross_entropy(feature, w, target, b), (w, b))
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = torch.autograd.grad(head.linear_cross_entropy(feature, w, target, b), (w, b))
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
