@@ -235,13 +235,9 @@ __device__ __forceinline__ void act8(Eight& a) {
     for (int i = 0; i < 8; ++i) a.v[i] = act_f<ACT>(a.v[i]);
 }
 
-// exp(z - base).  16-bit operands: in one fma, whose rounded LOG2E base is off by 2^-24 of itself (a relative 1e-6 of the result
-// for |base| = 10, far below the operands' 2^-9); floats: the difference first, which is exact for z near base.
-template <typename E>
-__device__ __forceinline__ float exp_of(float z, float base) {
-    if constexpr (sizeof(E) == 2) return exp2_f(__builtin_fmaf(LOG2E, z, -LOG2E * base));
-    return exp2_f(LOG2E * (z - base));
-}
+// exp(z - base), the difference first: it is exact for z near base, however large both are (a class masked by a bias of -1e30
+// has a maximum of that size in its tile).
+__device__ __forceinline__ float exp_of(float z, float base) { return exp2_f(LOG2E * (z - base)); }
 
 // The epilogue of 8 neighbouring sums of a row, in the order a latency-bound loop wants it: what depends on the columns is
 // loaded once (Columns), what depends on the row for several rows ahead (Ahead), then the sums are finished.
@@ -311,7 +307,7 @@ __device__ __forceinline__ void finish8(const HeadEpilogue& e, int64_t N, int64_
         if (e.bias) add8(a, col.bias);
         const float gone = e.smooth * h.weight;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a.v[i] = __builtin_fmaf(exp_of<E>(a.v[i], h.lse), h.weight, -gone);
+        for (int i = 0; i < 8; ++i) a.v[i] = __builtin_fmaf(exp_of(a.v[i], h.lse), h.weight, -gone);
         if (h.label >= 0) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) a.v[i] = h.label == i ? __builtin_fmaf(-e.one_minus_eps, h.weight, a.v[i]) : a.v[i];
@@ -588,7 +584,7 @@ __device__ __forceinline__ void product_tile(const TileArgs& g, int block) {
 #pragma unroll
             for (int i = 0; i < FN; ++i)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s += exp_of<E>(acc[i][j][c], base);
+                for (int c = 0; c < 4; ++c) s += exp_of(acc[i][j][c], base);
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
             if (q == 0) share[wn * BM + r] = make_float4(mx, s, zs, 0.f);

@@ -919,3 +919,40 @@ def test_a_captured_head_on_an_eager_feature():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("T,V,D", [(300, 2048, 64), (40, 1100, 4096), (600, 2100, 2048)])      # a whole, a cut contraction, kept logits
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_runs_of_classes_masked_by_finite_values(kind, T, V, D):
+    """Aligned runs of 64, 128 and 512 classes under a large finite bias: nothing of them is left in 32 bits (exp(-8000) = 0), so
+    the results are those of a bias of -inf."""
+    dt = TYPES[kind]
+    x, w, b, target = loss_case(T + V, T, V, D, dt, True)
+    masked = torch.zeros(V, dtype=torch.bool)
+    masked[:64] = masked[192:320] = masked[512:1024] = True
+    free = (~masked).nonzero()[:, 0]
+    target = torch.where(target == -100, target, free[target % len(free)])
+    dloss = torch.tensor(64.0 if kind == "f16" else 1.0)
+    want = ho.cross_entropy(x, w, target, b.masked_fill(masked, -math.inf), -100, 0.0, "mean", dloss)
+    for low in (-1e4, torch.finfo(dt).min) if kind == "f16" else (-1e4, -1e10, -1e30, torch.finfo(dt).min):
+        got = run_loss(x, w, target, b.masked_fill(masked, low), 0.0, "mean", dloss)
+        check(got, want)
+        assert not got["dw"][masked.cuda()].any() and not got["db"][masked.cuda()].any()
+
+
+@pytest.mark.parametrize("shift", [3e4, -3e4, 1e10, -1e10, 1e30, -1e30])
+@pytest.mark.parametrize("T,V,D", [(300, 2048, 64), (40, 1100, 4096), (600, 2100, 2048)])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_rows_whose_log_sum_is_large(kind, T, V, D, shift):
+    """Every class under the same large bias: what 32 bits leave of the probabilities stays in [0, 1], and nothing overflows."""
+    dt = TYPES[kind]
+    if abs(shift) > torch.finfo(dt).max:
+        return
+    x, w, _, target = loss_case(T + V, T, V, D, dt, False)
+    b = torch.full((V,), shift, dtype=dt)
+    got = run_loss(x, w, target, b, 0.0, "sum", torch.tensor(1.0))
+    check(got, ho.cross_entropy(x, w, target, b, -100, 0.0, "sum", torch.tensor(1.0)))
+    count = torch.bincount(target[target >= 0], minlength=V).double()
+    db, h = got["db"].double().cpu(), ho.half_step(dt)
+    # sum of p - [label] over the rows that count, p in [0, 1], each rounded once, the sum once (its 32-bit errors are smaller)
+    assert ((db >= -count * (1 + h) ** 2 * 1.001) & (db <= (count.sum() - count) * (1 + h) ** 2 * 1.001 + 1e-30)).all()
