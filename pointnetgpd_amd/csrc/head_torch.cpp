@@ -54,9 +54,21 @@ Rows rows_of(const at::Tensor& t, int64_t cols) {
 const void* data(const at::Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* out(const at::Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 at::Tensor dense(const Maybe& t) { return t.has_value() && t->defined() ? t->contiguous() : at::Tensor(); }
-// Whether autograd follows a tensor: backwards, or forwards (which the nodes refuse).
-bool wants(const at::Tensor& t) { return t.requires_grad() || t._fw_grad(0).defined(); }
+bool wants(const at::Tensor& t) { return t.requires_grad(); }
 bool wants(const Maybe& t) { return t.has_value() && wants(*t); }
+
+// Forward-mode differentiation: no_grad leaves it on, and a result without its tangent would read as a derivative of zero.
+void refuse_tangent(const at::Tensor& t) {
+    if (t._fw_grad(0).defined())
+        throw std::runtime_error("forward-mode differentiation of this operator is not supported (an input is a dual tensor)");
+}
+void refuse_tangent(const Maybe& t) {
+    if (t.has_value()) refuse_tangent(*t);
+}
+template <typename... Tensors>
+void refuse_tangents(const Tensors&... t) {
+    (refuse_tangent(t), ...);
+}
 
 void* stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.get_device()).stream(); }
 
@@ -165,6 +177,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
 };
 
 at::Tensor linear(const at::Tensor& x, const at::Tensor& w, const Maybe& bias, const Maybe& residual, int64_t act) {
+    refuse_tangents(x, w, bias, residual);
     if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(bias) || wants(residual)))
         return LinearFunction::apply(x, w, bias, residual, act);
     at::Tensor z;
@@ -212,6 +225,7 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
 };
 
 at::Tensor dropout(const at::Tensor& x, const Maybe& residual, double p, uint64_t seed, uint64_t offset, const Maybe& rng) {
+    refuse_tangents(x, residual);
     if (at::GradMode::is_enabled() && (wants(x) || wants(residual)))
         return DropoutFunction::apply(x, residual, p, (int64_t)seed, (int64_t)offset, rng);
     return dropout_call(x, residual, p, seed, offset, rng.has_value() ? *rng : at::Tensor());
@@ -281,6 +295,7 @@ struct LinearCrossEntropyFunction : torch::autograd::Function<LinearCrossEntropy
 
 at::Tensor linear_cross_entropy(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, const Maybe& bias,
                                 int64_t ignore_index, double label_smoothing, int64_t reduction) {
+    refuse_tangents(x, w, bias);
     if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(bias)))
         return LinearCrossEntropyFunction::apply(x, w, bias, target, ignore_index, label_smoothing, reduction);
     at::Tensor lse;

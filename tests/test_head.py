@@ -164,3 +164,25 @@ def test_a_planted_mistake_exceeds_the_bounds():
     loss, lb = ho.cross_entropy(x, w, t, None, -100, 0.0, "none", None)["loss"]
     other = ho.cross_entropy(x, w, (t + 1) % 21, None, -100, 0.0, "none", None)["loss"][0]
     assert ho.worst(loss.float(), loss, lb) <= 1.0 and ho.worst(other.float(), loss, lb) > 10.0
+
+
+def test_forward_mode_is_refused_before_anything_is_launched():
+    """A tangent raises in the binding itself, with gradients enabled or not (no_grad leaves forward-mode on in torch)."""
+    m, fw = _lib.load_head(), torch.autograd.forward_ad
+    x, w, b, t = torch.ones(2, 4), torch.ones(3, 4), torch.ones(3), torch.zeros(2, dtype=torch.int64)
+    with fw.dual_level():
+        for mode in (torch.no_grad, torch.enable_grad):
+            with mode():
+                dual = [fw.make_dual(v, torch.ones_like(v)) for v in (x, w, b)]
+                for i in range(3):
+                    a = [dual[j] if j == i else v for j, v in enumerate((x, w, b))]
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        m.linear(a[0], a[1], a[2], None, 0)
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        m.linear_cross_entropy(a[0], a[1], t, a[2], -100, 0.0, 1)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    m.linear(x, w, None, fw.make_dual(torch.ones(2, 3), torch.ones(2, 3)), 0)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    m.dropout(dual[0], None, 0.5, 1, 0, None)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    m.dropout(x, dual[0], 0.5, 1, 0, None)

@@ -956,3 +956,29 @@ def test_rows_whose_log_sum_is_large(kind, T, V, D, shift):
     db, h = got["db"].double().cpu(), ho.half_step(dt)
     # sum of p - [label] over the rows that count, p in [0, 1], each rounded once, the sum once (its 32-bit errors are smaller)
     assert ((db >= -count * (1 + h) ** 2 * 1.001) & (db <= (count.sum() - count) * (1 + h) ** 2 * 1.001 + 1e-30)).all()
+
+
+def test_forward_mode_is_refused_whatever_the_gradient_mode():
+    """no_grad leaves forward-mode differentiation on: a result without its tangent would read as a derivative of zero."""
+    x, w, b = (t.cuda() for t in make(92, (4, 24), (40, 24), (40,)))
+    target = torch.zeros(4, dtype=torch.int64, device="cuda")
+    fw = torch.autograd.forward_ad
+    with fw.dual_level():
+        duals = [fw.make_dual(t, torch.ones_like(t)) for t in (x, w, b)]
+        dual_r = fw.make_dual(torch.zeros(4, 40, device="cuda"), torch.ones(4, 40, device="cuda"))
+        for mode in (torch.no_grad, torch.enable_grad):
+            with mode():
+                for i in range(3):
+                    args = [duals[j] if j == i else t for j, t in enumerate((x, w, b))]
+                    for call in (lambda: head.linear(*args), lambda: head.linear_cross_entropy(args[0], args[1], target, args[2])):
+                        with pytest.raises(RuntimeError, match="forward-mode"):
+                            call()
+                for call in (lambda: head.dropout(duals[0], 0.25, 5), lambda: head.dropout(x, 0.25, 5, residual=duals[0]),
+                             lambda: head.linear(x, w, residual=dual_r)):
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        call()
+        with torch.inference_mode():                          # torch itself has no tangents there
+            assert head.linear(duals[0], w).shape == (4, 40)
+        x2 = fw.unpack_dual(duals[0]).primal
+        assert head.linear(x2, w).shape == (4, 40)
+    assert head.linear(x, w).shape == (4, 40)
