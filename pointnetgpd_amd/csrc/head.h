@@ -95,8 +95,8 @@ struct HeadLayOut {
     int64_t ld;
     bool live_rows_only;
 };
-// row_weight[t] = weight of row t in the loss's gradient divided by out_scale[0], a power of two (half precision) or the one
-// weight of all rows
+// row_weight[t] = weight of row t in the loss's gradient divided by out_scale[0]: the one weight of all rows, the largest of
+// them (16-bit types), or 1
 struct HeadRowWeights {
     const int64_t* target;
     int64_t T, V, ignore_index;

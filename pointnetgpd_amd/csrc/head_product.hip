@@ -274,46 +274,48 @@ struct Chunk {
 };
 
 // Gradient weights of the loss's rows, by one workgroup of 256 beside those that lay operands out, which take longer.
-__device__ __forceinline__ void row_weights(const HeadRowWeights& w, bool scaled) {
-    __shared__ float count[4], top[4];
-    float used = 0.f, g = 0.f;
+__device__ __forceinline__ void row_weights(const HeadRowWeights& w, bool bits16, bool half) {
+    __shared__ float count[4], most[4], least[4];
+    float used = 0.f, up = 0.f, down = 0.f;
 #pragma unroll 8
     for (int64_t t = threadIdx.x; t < w.T; t += 256) {
         const int64_t y = w.target[t];
         used += y != w.ignore_index ? 1.f : 0.f;
-        if (w.reduction == PNGPD_REDUCE_NONE)
-            g = __builtin_fmaxf(g, y != w.ignore_index && y >= 0 && y < w.V ? __builtin_fabsf(w.dloss[t]) : 0.f);
+        if (w.reduction == PNGPD_REDUCE_NONE && y != w.ignore_index && y >= 0 && y < w.V) {
+            up = __builtin_fmaxf(up, w.dloss[t]);
+            down = __builtin_fmaxf(down, -w.dloss[t]);
+        }
     }
     used = wave_sum(used);
-    g = wave_max(g);
+    up = wave_max(up);
+    down = wave_max(down);
     if ((threadIdx.x & 63) == 0) {
         count[threadIdx.x >> 6] = used;
-        top[threadIdx.x >> 6] = g;
+        most[threadIdx.x >> 6] = up;
+        least[threadIdx.x >> 6] = down;
     }
     __syncthreads();
     used = count[0] + count[1] + count[2] + count[3];
-    g = __builtin_fmaxf(__builtin_fmaxf(top[0], top[1]), __builtin_fmaxf(top[2], top[3]));
-    // Half precision: the largest weight becomes 2^13 .. 2^14, |dz| <= 2 times that is inside its range, and a probability of
-    // 2^-37 still is a number.
-    // One weight for all rows stays out of dz and goes into the products' 32-bit sums: p - 1 of the labels would be rounded
-    // the same way in every row otherwise (off by up to 2^-9 in one direction in bfloat16).
-    const bool one = w.reduction != PNGPD_REDUCE_NONE;
-    float scale = 1.f;
-    if (one) {
-        scale = scaled ? 16384.f : 1.f;
-    } else if (scaled && g > 0.f && g < __builtin_inff()) {
-        int e;
-        (void)frexpf(g, &e);
-        scale = ldexpf(1.f, e - 14);
-    }
+    up = __builtin_fmaxf(__builtin_fmaxf(most[0], most[1]), __builtin_fmaxf(most[2], most[3]));
+    down = __builtin_fmaxf(__builtin_fmaxf(least[0], least[1]), __builtin_fmaxf(least[2], least[3]));
+    const float g = up >= down ? up : -down;      // the largest in size, with its sign
+    // Operands of 16 bits: one weight for all rows stays out of dz and goes into the products' 32-bit sums, or p - 1 of the labels
+    // would be rounded the same way in every row (off by up to 2^-9 in one direction in bfloat16).  Rows' own weights are divided
+    // by the largest for the same reason, so that equal ones, the usual case, become 1; a row's quotient with another is rounded
+    // with its dz.  Half precision: the largest weight becomes 2^14, |dz| <= 2 times that is inside its range, and a probability
+    // of 2^-37 still is a number.
+    const bool one = w.reduction != PNGPD_REDUCE_NONE, shared = bits16 && g != 0.f && __builtin_fabsf(g) < __builtin_inff();
+    const float top_weight = half ? 16384.f : 1.f;
 #pragma unroll 8
     for (int64_t t = threadIdx.x; t < w.T; t += 256) {
         const int64_t y = w.target[t];
         const bool live = y != w.ignore_index && y >= 0 && y < w.V;
-        w.row_weight[t] = !live ? 0.f : one ? scale : w.dloss[t] / scale;
+        w.row_weight[t] = !live ? 0.f : one ? top_weight : shared ? w.dloss[t] / g * top_weight : w.dloss[t];
     }
-    if (threadIdx.x == 0)
-        w.out_scale[0] = one ? w.dloss[0] * (w.reduction == PNGPD_REDUCE_MEAN ? 1.f / __builtin_fmaxf(used, 1.f) : 1.f) / scale : scale;
+    if (threadIdx.x == 0) {
+        const float all = w.reduction == PNGPD_REDUCE_MEAN ? w.dloss[0] * (1.f / __builtin_fmaxf(used, 1.f)) : w.dloss[0];
+        w.out_scale[0] = one ? all / top_weight : shared ? g / top_weight : 1.f;
+    }
 }
 
 struct LayOutRun {
@@ -328,7 +330,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void set_up_kernel(LayOutRun a, LayOutRun b, HeadRowWeights w) {
     constexpr int C = Chunk<T>::C;
     if (blockIdx.x >= a.grid + b.grid) {
-        row_weights(w, __is_same(T, f16_t));
+        row_weights(w, sizeof(T) == 2, __is_same(T, f16_t));
         return;
     }
     const bool second = blockIdx.x >= a.grid;

@@ -982,3 +982,39 @@ def test_forward_mode_is_refused_whatever_the_gradient_mode():
         x2 = fw.unpack_dual(duals[0]).primal
         assert head.linear(x2, w).shape == (4, 40)
     assert head.linear(x, w).shape == (4, 40)
+
+
+# a whole and a cut contraction, kept logits, several pieces of the vocabulary
+WEIGHTED = [(1500, 700, 80), (40, 1100, 4096), (600, 2100, 2048), (2100, 70000, 16)]
+
+
+@pytest.mark.parametrize("T,V,D", WEIGHTED)
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_rows_of_one_weight_are_the_sum_of_that_weight(kind, T, V, D):
+    """(loss * mask).sum() / n over the losses of the rows: the same gradients as the sum's, bit for bit.  The weight (not a power of
+    two) stays out of the 16-bit logits' gradients, where it would round the labels' p - 1 the same way in every row."""
+    dt = TYPES[kind]
+    x, w, b, target = loss_case(T + V, T, V, D, dt, True)
+    for g in (1.0 / 3891, 0.75, -1.0 / 3, 300.0):
+        want = run_loss(x, w, target, b, 0.1, "sum", torch.tensor(g))
+        got = run_loss(x, w, target, b, 0.1, "none", torch.full((T,), g))
+        for k in ("dx", "dw", "db"):
+            assert torch.equal(got[k], want[k]), (g, k)
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_weights_of_rows_far_apart(kind):
+    """Rows whose incoming gradients differ by up to 2^30, zeros, infinities and NaN among them."""
+    dt = TYPES[kind]
+    x, w, b, target = loss_case(21, 90, 150, 40, dt, True, pad=False)
+    dloss = torch.rand(90, generator=torch.Generator().manual_seed(2)) * 2.0 ** -(torch.arange(90) % 31).float()
+    dloss[::7] = 0.0
+    dloss[5] = -dloss[5]
+    got = run_loss(x, w, target, b, 0.0, "none", dloss)
+    check(got, ho.cross_entropy(x, w, target, b, -100, 0.0, "none", dloss))
+    assert not got["dx"][::7].any()
+    dloss[3], dloss[4], target[6], dloss[6] = math.inf, math.nan, -100, math.nan
+    got = run_loss(x, w, target, b, 0.0, "none", dloss)
+    rest = [i for i in range(90) if i not in (3, 4)]
+    assert torch.isnan(got["dx"][4]).all() and not torch.isfinite(got["dx"][3]).any() and torch.isfinite(got["dx"][rest]).all()
+    assert not got["dx"][6].any()
