@@ -4,6 +4,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <cmath>
+
 namespace pngpd {
 
 constexpr int64_t HEAD_MAX_LD = (int64_t)1 << 23;            // bytes between rows: 256 rows stay below 2^31
@@ -103,7 +105,14 @@ struct HeadRowWeights {
     int reduction;
     const float* dloss;
     float *row_weight, *out_scale;
+    float label_factor;         // 16-bit types: of all weights (head_label_factor)
 };
+// c in (1/2, 1] with c (1 - eps) a power of two (1 where eps is)
+inline float head_label_factor(float eps) {
+    int e;
+    const float m = std::frexp(1.f - eps, &e);
+    return m > 0.5f ? 0.5f / m : 1.f;
+}
 // Up to two matrices laid out and the rows' weights, in one launch; each may be NULL, all NULL launches nothing.
 hipError_t head_set_up(int type, const HeadLayOut* a, const HeadLayOut* b, const HeadRowWeights* w, hipStream_t s);
 // dz[m][n] = dy[m][n] * act'(z[m][n]) (z dense; act NONE: dy itself) into dz (may be NULL; rows of ld_dz, whole chunks, zeros

@@ -406,7 +406,8 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         return PNGPD_OK;
     }
     const HeadOperand x{ws.x, padded(D, type), true}, xt{ws.x, padded(D, type), false};
-    const pngpd::HeadRowWeights weights{target_dev, T, V, ignore_index, reduction, dloss_dev, ws.row_weight, ws.scale};
+    const pngpd::HeadRowWeights weights{target_dev, T, V, ignore_index, reduction, dloss_dev, ws.row_weight, ws.scale,
+                                        pngpd::head_label_factor(label_smoothing)};
     const pngpd::HeadLayOut job_x{x_dev, T, D, ldx, ws.x, x.ld, true};      // what padding rows hold stays out of the sums
     pngpd::HeadLayOut job_w;
     bool lay_w;

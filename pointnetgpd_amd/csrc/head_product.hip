@@ -302,10 +302,11 @@ __device__ __forceinline__ void row_weights(const HeadRowWeights& w, bool bits16
     // Operands of 16 bits: one weight for all rows stays out of dz and goes into the products' 32-bit sums, or p - 1 of the labels
     // would be rounded the same way in every row (off by up to 2^-9 in one direction in bfloat16).  Rows' own weights are divided
     // by the largest for the same reason, so that equal ones, the usual case, become 1; a row's quotient with another is rounded
-    // with its dz.  Half precision: the largest weight becomes 2^14, |dz| <= 2 times that is inside its range, and a probability
-    // of 2^-37 still is a number.
+    // with its dz.  Smoothed labels hold p - (1 - eps): dz is formed times the factor in (1/2, 1] that makes 1 - eps a power of two
+    // (eps = 0.1 in bfloat16: 0.9 is off by 0.0017 of itself, in every row).  Half precision: the largest weight becomes at most
+    // 2^14, |dz| <= 2 times that is inside its range, and a probability of 2^-37 still is a number.
     const bool one = w.reduction != PNGPD_REDUCE_NONE, shared = bits16 && g != 0.f && __builtin_fabsf(g) < __builtin_inff();
-    const float top_weight = half ? 16384.f : 1.f;
+    const float top_weight = (half ? 16384.f : 1.f) * (bits16 ? w.label_factor : 1.f);
 #pragma unroll 8
     for (int64_t t = threadIdx.x; t < w.T; t += 256) {
         const int64_t y = w.target[t];

@@ -1018,3 +1018,34 @@ def test_weights_of_rows_far_apart(kind):
     rest = [i for i in range(90) if i not in (3, 4)]
     assert torch.isnan(got["dx"][4]).all() and not torch.isfinite(got["dx"][3]).any() and torch.isfinite(got["dx"][rest]).all()
     assert not got["dx"][6].any()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("eps", [0.1, 0.3])
+def test_labels_of_smoothed_targets_are_not_rounded_one_way(eps, reduction):
+    """1 - eps has no exact bfloat16: were it in every row's gradient, the weight's gradient would be off by one factor (0.0017 for
+    0.1, 0.0011 for 0.3), which the projection on the exact gradient shows.  Its elements carry two roundings of at most h each,
+    random in sign: the projection of N = 65536 of them deviates by at most 2 h / sqrt N (Gaussian values: sqrt(3) for their fourth
+    moment, 1 / sqrt(3) for a rounding's deviation), taken six times; the label's p - (1 - eps) may lose p besides, below 2^-11."""
+    T, V, D = 8192, 4096, 16
+    g = torch.Generator().manual_seed(33)
+    x, w = torch.randn(T, D, generator=g).bfloat16(), (torch.randn(V, D, generator=g) * 0.02).bfloat16()
+    target = torch.arange(T) % V
+    dloss = torch.tensor(1.0) if reduction == "mean" else torch.full((T,), 1.0 / T)
+    got = run_loss(x, w, target, None, eps, reduction, dloss)["dw"].double()
+    X, W, y = x.cuda().double(), w.cuda().double(), target.cuda()
+    p = torch.softmax(X @ W.t(), 1)
+    assert p.max() < 2.0 ** -11
+    p -= eps / V
+    p[torch.arange(T, device="cuda"), y] -= 1 - eps
+    want = p.t() @ X / T
+    off = ((got - want) * want).sum() / want.square().sum()
+    assert abs(off.item()) <= 6 * 2 * ho.half_step(torch.bfloat16) / (V * D) ** 0.5 + 2.0 ** -11
+
+
+@pytest.mark.parametrize("eps", [0.5, 0.999, 1.0])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_strong_smoothing(kind, eps):
+    x, w, b, target = loss_case(37, 70, 90, 40, TYPES[kind], True)
+    dloss = torch.tensor(64.0 if kind == "f16" else 1.0)
+    check(run_loss(x, w, target, b, eps, "mean", dloss), ho.cross_entropy(x, w, target, b, -100, eps, "mean", dloss))
