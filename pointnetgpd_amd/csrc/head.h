@@ -49,6 +49,7 @@ struct HeadEpilogue {
     const int64_t* target = nullptr;
     int64_t first_n = 0;
     float smooth = 0.f, one_minus_eps = 1.f;
+    float* col_part = nullptr;  // may be NULL; [head_dz_parts][N]: sums of blocks of rows, of the values before they are rounded
     // SCALED: out = scale[0] * (acc + add[m][n]); scale NULL: 1; add NULL: 0 (32-bit, dense [M][N])
     const float* scale = nullptr;
     const float* add = nullptr;
@@ -84,9 +85,12 @@ struct HeadGradient {
     float* partial;             // of its own
 };
 hipError_t head_gradients(int type, const HeadGradient& x, const HeadGradient& w, hipStream_t s);
-// Kept sums of a STATS product, and another epilogue from them.
+// Kept sums of a STATS product, and the DZ epilogue from them.
 size_t head_kept_bytes(int type, int64_t M, int64_t N, int64_t K);
 hipError_t head_kept(int type, int64_t M, int64_t N, int64_t K, const HeadEpilogue& e, const float* kept, hipStream_t s);
+// Blocks of rows whose column sums a DZ product of this plan (kept: head_kept) leaves in col_part, and their sum times scale[0].
+int64_t head_dz_parts(int type, int64_t M, int64_t N, const HeadPlan& plan, bool kept);
+hipError_t head_col_sums(int type, int64_t parts, int64_t N, const float* part, const float* scale, void* out, hipStream_t s);
 
 // dst[r][0 .. ld) = src[r][0 .. cols) and zeros behind them.  dst is 16-byte aligned, ld whole chunks.  With a target, rows
 // whose target is ignored or no class become zeros whatever they hold.
@@ -116,11 +120,10 @@ inline float head_label_factor(float eps) {
 // Up to two matrices laid out and the rows' weights, in one launch; each may be NULL, all NULL launches nothing.
 hipError_t head_set_up(int type, const HeadLayOut* a, const HeadLayOut* b, const HeadRowWeights* w, hipStream_t s);
 // dz[m][n] = dy[m][n] * act'(z[m][n]) (z dense; act NONE: dy itself) into dz (may be NULL; rows of ld_dz, whole chunks, zeros
-// behind column N), and into sums (may be NULL) scale[0] (NULL: 1) times the columns' sums, by way of
-// part: 32-bit [head_col_parts][N]
+// behind column N), and into sums (may be NULL) the columns' sums, by way of part: 32-bit [head_col_parts][N]
 size_t head_col_parts(int type, int64_t M, int64_t N);
 hipError_t head_grad_rows(int type, int64_t M, int64_t N, const void* dy, int64_t ld_dy, const void* z, int act, void* dz,
-                          int64_t ld_dz, float* part, const float* scale, void* sums, hipStream_t s);
+                          int64_t ld_dz, float* part, void* sums, hipStream_t s);
 
 // a fill kernel, not a memset: the call may be captured
 hipError_t head_zero(void* p, size_t bytes, hipStream_t s);

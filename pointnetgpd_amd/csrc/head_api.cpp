@@ -118,6 +118,7 @@ struct LossWs {
     float *target_logit, *row_loss, *row_weight, *scale, *part, *dx_sum, *partial;
     float* partial_w;          // the weight's gradient's own
     float* few;                // partial sums of few classes' gradients
+    pngpd::HeadPlan dz, dz_last;      // of a piece's logits, and of the last piece's where that is smaller
     size_t bytes;
     LossWs(void* base, int type, int64_t T, int64_t V, int64_t D, bool backward, bool copy_x, bool copy_w) {
         Bump b(base);
@@ -157,15 +158,18 @@ struct LossWs {
             tile = b.take((size_t)rows * padded(piece, type) * e);
             row_weight = (float*)b.take((size_t)rows * 4);
             scale = (float*)b.take(4);
-            part = (float*)b.take((size_t)max2(pngpd::head_col_parts(type, rows, piece) * piece, pngpd::head_col_parts(type, rows, last) * last) * 4);
             if (V <= pngpd::HEAD_FEW) few = (float*)b.take(pngpd::head_few_part_bytes(type, rows, V, D));
             if (piece < V) dx_sum = (float*)b.take((size_t)rows * D * 4);
-            size_t cut = 0, cut_w = 0;
+            size_t cut = 0, cut_w = 0, sums = 0;
             for (int64_t n : {piece, last}) {
-                cut = max2(cut, pngpd::head_plan(type, rows, n, D, pngpd::HEAD_EPI_DZ).partial_bytes);
+                pngpd::HeadPlan& p = n == piece ? dz : dz_last;
+                p = pngpd::head_plan(type, rows, n, D, pngpd::HEAD_EPI_DZ);
+                for (bool kept : {false, true}) sums = max2(sums, (size_t)pngpd::head_dz_parts(type, rows, n, p, kept) * n * 4);
+                cut = max2(cut, p.partial_bytes);
                 cut_w = max2(cut_w, pngpd::head_plan(type, n, D, rows, pngpd::HEAD_EPI_SCALED).partial_bytes);
                 cut = max2(cut, pngpd::head_plan(type, rows, D, n, pngpd::HEAD_EPI_SCALED).partial_bytes);
             }
+            part = (float*)b.take(sums);
             partial = (float*)b.take(cut);
             partial_w = (float*)b.take(cut_w);
         }
@@ -283,7 +287,7 @@ int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void*
     const Rows dz = same ? Rows{dy_dev, ld_dy} : Rows{ws.dz, padded(N, type)};
     if (!same || dbias_dev)
         HIP_TRY(pngpd::head_grad_rows(type, M, N, dy_dev, ld_dy, z_dev, act, same ? nullptr : ws.dz, dz.ld,
-                                      ws.part, nullptr, dbias_dev, s));
+                                      ws.part, dbias_dev, s));
     pngpd::HeadLayOut job_x, job_w;
     bool lay_x = false, lay_w = false;
     Rows x{}, w{};
@@ -427,11 +431,12 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         e.one_minus_eps = 1.f - label_smoothing;
         e.out = ws.tile;
         e.ld_out = np;
+        e.col_part = dbias_dev ? ws.part : nullptr;
         if (kept) HIP_TRY(pngpd::head_kept(type, T, V, D, e, kept, s));
         else HIP_TRY(pngpd::head_product(type, T, n, D, x, HeadOperand{w, whole.ld, true}, e, ws.partial, false, s));
         if (dbias_dev)
-            HIP_TRY(pngpd::head_grad_rows(type, T, n, ws.tile, np, nullptr, PNGPD_ACT_NONE, nullptr, 0, ws.part, ws.scale,
-                                          at(dbias_dev, v, type), s));
+            HIP_TRY(pngpd::head_col_sums(type, pngpd::head_dz_parts(type, T, n, n == ws.piece ? ws.dz : ws.dz_last, kept != nullptr), n, ws.part, ws.scale,
+                                         at(dbias_dev, v, type), s));
         const bool last = v + n == V;
         pngpd::HeadGradient gx{T, D, n, HeadOperand{ws.tile, np, true}, HeadOperand{w, whole.ld, false}, HeadEpilogue{}, ws.partial};
         pngpd::HeadGradient gw{n, D, T, HeadOperand{ws.tile, np, false}, xt, HeadEpilogue{}, ws.partial_w};

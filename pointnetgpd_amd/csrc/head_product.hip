@@ -78,8 +78,76 @@ __global__ __launch_bounds__(256) void join_stats_kernel(int64_t M, int64_t N, i
     }
 }
 
+// How a pass over [M, N] is cut when it also sums columns: 2^lanes threads of a workgroup side by side over chunks of
+// columns, the others over rows, `parts` blocks of `rows` rows, `turns` turns of the threads at least.
+struct ColumnCut {
+    int lanes;
+    unsigned blocks;
+    int64_t parts, rows;
+};
+ColumnCut column_cut(int64_t M, int64_t N, int chunk, int turns, int most_lanes) {
+    if (M < 1) M = 1;
+    ColumnCut c;
+    const int64_t chunks = (N + chunk - 1) / chunk;
+    c.lanes = 0;
+    while (c.lanes < most_lanes && (1 << c.lanes) < chunks) ++c.lanes;
+    c.blocks = (unsigned)((chunks + (1 << c.lanes) - 1) >> c.lanes);
+    const int64_t side = 256 >> c.lanes;                        // rows at a time
+    int64_t parts = 2048 / c.blocks;                            // enough workgroups to fill the chip
+    const int64_t most = (M + turns * side - 1) / (turns * side);
+    if (parts > most) parts = most;
+    if (parts > 256) parts = 256;
+    if (parts < 1) parts = 1;
+    c.rows = ((M + parts - 1) / parts + side - 1) / side * side;
+    c.parts = (M + c.rows - 1) / c.rows;
+    return c;
+}
+
+// The logits' gradients from partial sums together with their columns' sums before they are rounded, a part of col_part a block
+// of rows.  Bound by memory: 4096 x 32768 from kept sums in bfloat16 (805 MB) takes 202 us, 4.0 TB/s (210 with at most 64 groups
+// of columns side by side); join_kernel and a pass over its rounded output took 149 + 56.  One turn a thread is enough where rows
+// are few: each reads every cut of the contraction (300 x 4096 -> 40: 6 us; with four the training step took 7 us more).
+ColumnCut dz_cut(int64_t M, int64_t ld_out) { return column_cut(M, ld_out, 8, 1, 8); }
+
+template <typename E>
+__global__ __launch_bounds__(256) void join_dz_kernel(int64_t M, int64_t N, int splits, const float* partial, HeadEpilogue e, int lanes,
+                                                      int64_t rows) {
+    __shared__ float share[256][9];
+    const int wide = 1 << lanes, side = 256 >> lanes;
+    const int64_t n = ((int64_t)blockIdx.x * wide + (threadIdx.x & (wide - 1))) * 8;
+    const int64_t m0 = (int64_t)blockIdx.y * rows, m1 = m0 + rows < M ? m0 + rows : M;
+    const int64_t have = N - n, room = e.ld_out - n;
+    const int valid = (int)(have < 0 ? 0 : have < 8 ? have : 8), real = (int)(room < 8 ? room : 8);
+    Eight sums = {};
+    if (real > 0) {
+        const Columns col = load_columns<E, TILE_DZ>(e, N, n);
+        for (int64_t m = m0 + (threadIdx.x >> lanes); m < m1; m += side) {
+            Eight v = {};
+#pragma unroll 4
+            for (int s = 0; s < splits; ++s) add8(v, load8(partial + ((int64_t)s * M + m) * head_partial_ld(N) + n, valid));
+            finish8<E, TILE_DZ>(e, N, m, n, real, col, load_ahead<E, TILE_DZ>(e, N, m, n, real), v);
+            add8(sums, v);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) share[threadIdx.x][i] = sums.v[i];
+    __syncthreads();
+    for (int c = threadIdx.x; c < wide * 8; c += 256) {
+        const int64_t k = (int64_t)blockIdx.x * wide * 8 + c;
+        if (k >= N) continue;
+        float v = 0.f;
+        for (int r = 0; r < side; ++r) v += share[(r << lanes) + c / 8][c % 8];
+        e.col_part[(int64_t)blockIdx.y * N + k] = v;
+    }
+}
+
 template <typename E>
 hipError_t join(int64_t M, int64_t N, int splits, const float* partial, const HeadEpilogue& e, hipStream_t s) {
+    if (e.kind == HEAD_EPI_DZ && e.col_part) {
+        const ColumnCut c = dz_cut(M, e.ld_out);
+        join_dz_kernel<E><<<dim3(c.blocks, (unsigned)c.parts), 256, 0, s>>>(M, N, splits, partial, e, c.lanes, c.rows);
+        return hipGetLastError();
+    }
     const int64_t groups = ((e.kind == HEAD_EPI_DZ ? e.ld_out : N) + 7) / 8;
     // little to join: small workgroups, so that its loads leave from many compute units
     const bool few = M * groups < 65536;
@@ -371,37 +439,11 @@ hipError_t set_up(const HeadLayOut* a, const HeadLayOut* b, const HeadRowWeights
     return hipGetLastError();
 }
 
-// How a pass over [M, N] is cut when it also sums columns: 2^lanes threads of a workgroup side by side over chunks of
-// columns, the others over rows, `parts` blocks of `rows` rows.
-struct ColumnCut {
-    int lanes;
-    unsigned blocks;
-    int64_t parts, rows;
-};
-ColumnCut column_cut(int64_t M, int64_t N, int chunk) {
-    if (M < 1) M = 1;
-    ColumnCut c;
-    const int64_t chunks = (N + chunk - 1) / chunk;
-    c.lanes = 0;
-    while (c.lanes < 6 && (1 << c.lanes) < chunks) ++c.lanes;
-    c.blocks = (unsigned)((chunks + (1 << c.lanes) - 1) >> c.lanes);
-    const int64_t side = 256 >> c.lanes;                        // rows at a time
-    int64_t parts = 2048 / c.blocks;                            // enough workgroups to fill the chip
-    const int64_t most = (M + 4 * side - 1) / (4 * side);       // but four turns of each at least
-    if (parts > most) parts = most;
-    if (parts > 256) parts = 256;
-    if (parts < 1) parts = 1;
-    c.rows = ((M + parts - 1) / parts + side - 1) / side * side;
-    c.parts = (M + c.rows - 1) / c.rows;
-    return c;
-}
-
 // One pass over dy and z, bound by memory, so the sums of the columns ride along: 8192 x 8192 in bfloat16 with gelu's slope
 // (402 MB) takes 95 us, 4.2 TB/s (its exponential and reciprocal take about two thirds of that by themselves).
 template <typename T, int ACT, bool WRITE>
 __global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, const T* dy, int64_t ld, const T* z, T* dz,
-                                                        int64_t ld_dz, float* part, int lanes, int64_t rows,
-                                                        const float* scale, T* sums) {
+                                                        int64_t ld_dz, float* part, int lanes, int64_t rows, T* sums) {
     constexpr int C = Chunk<T>::C;
     __shared__ float share[256][C + 1];
     const int wide = 1 << lanes, side = 256 >> lanes;
@@ -438,21 +480,21 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, co
         if (n >= N) continue;
         float s = 0.f;
         for (int r = 0; r < side; ++r) s += share[(r << lanes) + c / C][c % C];
-        if (gridDim.y == 1) sums[n] = from_f32<T>(scale ? s * scale[0] : s);
+        if (gridDim.y == 1) sums[n] = from_f32<T>(s);
         else part[(int64_t)blockIdx.y * N + n] = s;
     }
 }
 
 // 32 columns by 8 shares of the parts a workgroup
 template <typename T>
-__global__ __launch_bounds__(256) void col_join_kernel(int parts, int64_t N, const float* part, const float* scale, T* out) {
+__global__ __launch_bounds__(256) void col_join_kernel(int64_t parts, int64_t N, const float* part, const float* scale, T* out) {
     __shared__ float share[8][32];
     const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t n = (int64_t)blockIdx.x * 32 + c;
     float s = 0.f;
     if (n < N) {
 #pragma unroll 8
-        for (int i = w; i < parts; i += 8) s += part[(int64_t)i * N + n];
+        for (int64_t i = w; i < parts; i += 8) s += part[i * N + n];
     }
     share[w][c] = s;
     __syncthreads();
@@ -462,13 +504,19 @@ __global__ __launch_bounds__(256) void col_join_kernel(int parts, int64_t N, con
 }
 
 template <typename T>
+hipError_t col_sums(int64_t parts, int64_t N, const float* part, const float* scale, void* out, hipStream_t s) {
+    col_join_kernel<T><<<(unsigned)((N + 31) / 32), 256, 0, s>>>(parts, N, part, scale, (T*)out);
+    return hipGetLastError();
+}
+
+template <typename T>
 hipError_t grad_rows(int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz, int64_t ld_dz, float* part,
-                     const float* scale, void* sums, hipStream_t s) {
+                     void* sums, hipStream_t s) {
     constexpr int C = Chunk<T>::C;
-    const ColumnCut c = column_cut(M, N, C);
+    const ColumnCut c = column_cut(M, N, C, 4, 6);
     const dim3 grid(c.blocks, (unsigned)c.parts);
 #define PNGPD_GRAD_ROWS(A, W) \
-    grad_rows_kernel<T, A, W><<<grid, 256, 0, s>>>(M, N, (const T*)dy, ld, (const T*)z, (T*)dz, ld_dz, part, c.lanes, c.rows, scale, (T*)sums)
+    grad_rows_kernel<T, A, W><<<grid, 256, 0, s>>>(M, N, (const T*)dy, ld, (const T*)z, (T*)dz, ld_dz, part, c.lanes, c.rows, (T*)sums)
     switch (act) {
         case PNGPD_ACT_NONE:
             if (dz) PNGPD_GRAD_ROWS(PNGPD_ACT_NONE, true);
@@ -483,13 +531,12 @@ hipError_t grad_rows(int64_t M, int64_t N, const void* dy, int64_t ld, const voi
 #undef PNGPD_GRAD_ROWS
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !sums || c.parts == 1) return e;
-    col_join_kernel<T><<<(unsigned)((N + 31) / 32), 256, 0, s>>>((int)c.parts, N, part, scale, (T*)sums);
-    return hipGetLastError();
+    return col_sums<T>(c.parts, N, part, nullptr, sums, s);
 }
 
 }  // namespace
 
-size_t head_col_parts(int type, int64_t M, int64_t N) { return (size_t)column_cut(M, N, type == PNGPD_TYPE_F32 ? 4 : 8).parts; }
+size_t head_col_parts(int type, int64_t M, int64_t N) { return (size_t)column_cut(M, N, type == PNGPD_TYPE_F32 ? 4 : 8, 4, 6).parts; }
 
 namespace {
 
@@ -572,12 +619,19 @@ hipError_t head_kept(int type, int64_t M, int64_t N, int64_t K, const HeadEpilog
     const int splits = head_plan(type, M, N, K, HEAD_EPI_STATS).splits;
     PNGPD_BY_TYPE((join<T>(M, N, splits, kept, e, s)))
 }
+int64_t head_dz_parts(int type, int64_t M, int64_t N, const HeadPlan& p, bool kept) {
+    const int64_t chunk = type == PNGPD_TYPE_F32 ? 4 : 8;
+    return kept || p.splits > 1 ? dz_cut(M, (N + chunk - 1) / chunk * chunk).parts : p.tiles_m;
+}
+hipError_t head_col_sums(int type, int64_t parts, int64_t N, const float* part, const float* scale, void* out, hipStream_t s) {
+    PNGPD_BY_TYPE((col_sums<T>(parts, N, part, scale, out, s)))
+}
 hipError_t head_set_up(int type, const HeadLayOut* a, const HeadLayOut* b, const HeadRowWeights* w, hipStream_t s) {
     PNGPD_BY_TYPE((set_up<T>(a, b, w, s)))
 }
 hipError_t head_grad_rows(int type, int64_t M, int64_t N, const void* dy, int64_t ld, const void* z, int act, void* dz,
-                          int64_t ld_dz, float* part, const float* scale, void* sums, hipStream_t s) {
-    PNGPD_BY_TYPE((grad_rows<T>(M, N, dy, ld, z, act, dz, ld_dz, part, scale, sums, s)))
+                          int64_t ld_dz, float* part, void* sums, hipStream_t s) {
+    PNGPD_BY_TYPE((grad_rows<T>(M, N, dy, ld, z, act, dz, ld_dz, part, sums, s)))
 }
 
 }  // namespace pngpd

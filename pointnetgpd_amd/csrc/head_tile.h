@@ -488,6 +488,7 @@ __device__ __forceinline__ void product_tile(const TileArgs& g, int block) {
         const int64_t n = n0 + c * 4, have = (KIND == TILE_DZ ? g.e.ld_out : g.N) - n;
         const int valid = (int)(have < 0 ? 0 : have < 8 ? have : 8);
         const Columns col = load_columns<E, KIND>(g.e, g.N, n);
+        Eight sums = {};
 #pragma unroll
         for (int pass = 0; pass < PASSES; ++pass) {
             __syncthreads();
@@ -521,6 +522,24 @@ __device__ __forceinline__ void product_tile(const TileArgs& g, int block) {
                     Eight a = {{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}};
                     if constexpr (KIND == TILE_PARTIAL || KIND == TILE_STATS) store8(g.partial + ((int64_t)split * g.M + m) * head_partial_ld(g.N) + n, a, valid);
                     else finish8<E, KIND>(g.e, g.N, m, n, valid, col, ahead[k], a);
+                    if constexpr (KIND == TILE_DZ) {
+                        if (g.e.col_part) add8(sums, a);
+                    }
+                }
+            }
+        }
+        if constexpr (KIND == TILE_DZ) {
+            // the tile's column sums: the threads of a column in order
+            if (g.e.col_part) {
+                __syncthreads();
+                float* share = (float*)smem;      // [RSTEP][BN]
+#pragma unroll
+                for (int i = 0; i < 8; ++i) share[threadIdx.x / GROUPS * BN + c * 4 + i] = sums.v[i];
+                __syncthreads();
+                for (int k = threadIdx.x; k < BN && n0 + k < g.N; k += WAVES * 64) {
+                    float v = 0.f;
+                    for (int r = 0; r < RSTEP; ++r) v += share[r * BN + k];
+                    g.e.col_part[(int64_t)tm * g.N + n0 + k] = v;
                 }
             }
         }

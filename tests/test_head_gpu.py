@@ -1049,3 +1049,23 @@ def test_strong_smoothing(kind, eps):
     x, w, b, target = loss_case(37, 70, 90, 40, TYPES[kind], True)
     dloss = torch.tensor(64.0 if kind == "f16" else 1.0)
     check(run_loss(x, w, target, b, eps, "mean", dloss), ho.cross_entropy(x, w, target, b, -100, eps, "mean", dloss))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("T,V,D", WEIGHTED[:3] + [(77, 9, 40), (4, 3000, 4096), (5000, 40, 24)])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_bias_gradient_of_the_loss_is_rounded_once(kind, T, V, D, reduction):
+    """Sums of the logits' gradients before these are rounded: off by what 32 bits leave, as for float32 operands, and one rounding
+    of the result."""
+    dt = TYPES[kind]
+    x, w, b, target = loss_case(T + V, T, V, D, dt, True)
+    scale = 256.0 if kind == "f16" else 1.0
+    dloss = torch.tensor(scale) if reduction == "mean" else torch.rand(T, generator=torch.Generator().manual_seed(T)) * scale / T
+    got = run_loss(x, w, target, b, 0.1, reduction, dloss)
+    v, e = ho.cross_entropy(x.float(), w.float(), target, b.float(), -100, 0.1, reduction, dloss)["db"]
+    check({"db": got["db"]}, {"db": (v, e + ho.half_step(dt) * (v.abs() + e) + ho.tiny(dt))})
+    # alone, without the other two
+    bs = b.cuda().requires_grad_()
+    loss = head.linear_cross_entropy(x.cuda(), w.cuda(), target.cuda(), bs, label_smoothing=0.1, reduction=reduction)
+    alone, = torch.autograd.grad(loss, bs, dloss.cuda())
+    assert torch.equal(alone, got["db"])
