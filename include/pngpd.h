@@ -430,6 +430,8 @@ int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64
  * kept_dev: NULL, or pngpd_linear_cross_entropy_kept_bytes of memory (16-byte aligned) that carries what the backward
  * pass of the same call would otherwise compute again: 32-bit logits, where that is quicker and, rounded to `type`, they take
  * at most 256 MiB or as much as x and weight.  Its size is 0 where nothing is kept.
+ * workspace_bytes: backward is 0 for the forward pass, 1 for the backward pass, 2 for a backward pass that is given kept_dev
+ * (at most 8 classes then need little; 1 covers both).
  */
 size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V, int64_t D, int backward, int aligned);
 size_t pngpd_linear_cross_entropy_kept_bytes(int type, int64_t T, int64_t V, int64_t D);

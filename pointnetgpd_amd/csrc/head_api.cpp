@@ -117,7 +117,6 @@ struct LossWs {
     float4* stats;
     float *target_logit, *row_loss, *row_weight, *scale, *part, *dx_sum, *partial;
     float* partial_w;          // the weight's gradient's own
-    float* few;                // partial sums of few classes' gradients
     pngpd::HeadPlan dz, dz_last;      // of a piece's logits, and of the last piece's where that is smaller
     size_t bytes;
     LossWs(void* base, int type, int64_t T, int64_t V, int64_t D, bool backward, bool copy_x, bool copy_w) {
@@ -128,7 +127,7 @@ struct LossWs {
         w = copy_w ? b.take((size_t)V * dp * e) : nullptr;
         tile = nullptr;
         stats = nullptr;
-        target_logit = row_loss = row_weight = scale = part = dx_sum = partial = partial_w = few = nullptr;
+        target_logit = row_loss = row_weight = scale = part = dx_sum = partial = partial_w = nullptr;
         piece = V;
         rows_at_once = rows;
         if (!backward) {
@@ -158,7 +157,6 @@ struct LossWs {
             tile = b.take((size_t)rows * padded(piece, type) * e);
             row_weight = (float*)b.take((size_t)rows * 4);
             scale = (float*)b.take(4);
-            if (V <= pngpd::HEAD_FEW) few = (float*)b.take(pngpd::head_few_part_bytes(type, rows, V, D));
             if (piece < V) dx_sum = (float*)b.take((size_t)rows * D * 4);
             size_t cut = 0, cut_w = 0, sums = 0;
             for (int64_t n : {piece, last}) {
@@ -188,6 +186,19 @@ int check_loss(const char* who, int type, int64_t T, int64_t V, int64_t D, const
     if (!(eps >= 0.f && eps <= 1.f)) return fail(PNGPD_ERR_INVALID, "%s: label_smoothing %g", who, (double)eps);
     if (reduction < PNGPD_REDUCE_NONE || reduction > PNGPD_REDUCE_SUM) return fail(PNGPD_ERR_INVALID, "%s: unknown reduction %d", who, reduction);
     return PNGPD_OK;
+}
+
+// Few classes have kernels of their own, which take x and the weight as they lie: the rows' losses, and the parts of the gradients
+// where the logits were kept (the general products serve those that were not).
+size_t few_forward_bytes(int64_t T) {
+    Bump b(nullptr);
+    b.take((size_t)T * 4);
+    return b.off;
+}
+size_t few_backward_bytes(int type, int64_t T, int64_t V, int64_t D) {
+    Bump b(nullptr);
+    b.take(pngpd::head_few_part_bytes(type, T, V, D));
+    return b.off;
 }
 
 constexpr size_t FEW_HEAD = 256;       // bytes in front of few classes' kept logits: the number of rows that count
@@ -321,6 +332,8 @@ int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64
 size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V, int64_t D, int backward, int aligned) {
     const void* some = &type;      // the sizes alone are checked
     if (check_loss("pngpd_linear_cross_entropy_workspace_bytes", type, T, V, D, some, D, some, D, (const int64_t*)some, 0.f, 0)) return 0;
+    if (V <= pngpd::HEAD_FEW && !backward) return few_forward_bytes(T);
+    if (V <= pngpd::HEAD_FEW && backward == 2 && kept_bytes(type, T, V, D)) return few_backward_bytes(type, T, V, D);
     const bool d = !aligned || padded(D, type) != D;
     return LossWs(nullptr, type, T, V, D, backward != 0, d, d).bytes;
 }
@@ -342,18 +355,20 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
     if (((uintptr_t)kept_dev & 15) != 0) return fail(PNGPD_ERR_INVALID, "%s: kept must be aligned to 16 bytes", who);
     if (T > 0 && !lse_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL lse", who);
     hipStream_t s = (hipStream_t)stream;
+    if (T > 0 && V <= pngpd::HEAD_FEW) {
+        const bool rows = reduction == PNGPD_REDUCE_NONE;
+        if ((rc = check_ws(who, workspace_dev, workspace_bytes, rows ? 0 : few_forward_bytes(T)))) return rc;
+        char* few = kept_bytes(type, T, V, D) ? (char*)kept_dev : nullptr;
+        float* row_loss = rows ? loss_dev : (float*)workspace_dev;
+        const pngpd::HeadFew g{T, V, D, x_dev, ldx, weight_dev, ldw, bias_dev, target_dev, ignore_index, label_smoothing,
+                               few ? (float*)(few + FEW_HEAD) : nullptr};
+        HIP_TRY(pngpd::head_few_loss(type, g, row_loss, lse_dev, s));
+        if (!rows) HIP_TRY(pngpd::head_batch_loss(T, row_loss, target_dev, ignore_index, reduction, loss_dev, (float*)few, s));
+        return PNGPD_OK;
+    }
     LossWs ws(workspace_dev, type, T, V, D, false, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
     if (T > 0) {
         if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
-        if (V <= pngpd::HEAD_FEW) {
-            char* few = kept_bytes(type, T, V, D) ? (char*)kept_dev : nullptr;
-            const pngpd::HeadFew g{T, V, D, x_dev, ldx, weight_dev, ldw, bias_dev, target_dev, ignore_index, label_smoothing,
-                                   few ? (float*)(few + FEW_HEAD) : nullptr};
-            HIP_TRY(pngpd::head_few_loss(type, g, reduction == PNGPD_REDUCE_NONE ? loss_dev : ws.row_loss, lse_dev, s));
-            if (reduction != PNGPD_REDUCE_NONE)
-                HIP_TRY(pngpd::head_batch_loss(T, ws.row_loss, target_dev, ignore_index, reduction, loss_dev, (float*)few, s));
-            return PNGPD_OK;
-        }
         pngpd::HeadLayOut job_x, job_w;
         bool lay_x, lay_w;
         const Rows x = direct_rows(type, T, D, x_dev, ldx, ws.x, &job_x, &lay_x);
@@ -401,14 +416,15 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
     if (!lse_dev || !dloss_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL argument", who);
     if (((uintptr_t)kept_dev & 15) != 0) return fail(PNGPD_ERR_INVALID, "%s: kept must be aligned to 16 bytes", who);
     const float* kept = kept_bytes(type, T, V, D) ? (const float*)kept_dev : nullptr;
-    LossWs ws(workspace_dev, type, T, V, D, true, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
-    if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
     if (kept && V <= pngpd::HEAD_FEW) {
+        if ((rc = check_ws(who, workspace_dev, workspace_bytes, few_backward_bytes(type, T, V, D)))) return rc;
         const pngpd::HeadFew g{T, V, D, x_dev, ldx, weight_dev, ldw, bias_dev, target_dev, ignore_index, label_smoothing,
                                const_cast<float*>(kept) + FEW_HEAD / 4};
-        HIP_TRY(pngpd::head_few_grad(type, g, lse_dev, kept, dloss_dev, reduction, dx_dev, dweight_dev, dbias_dev, ws.few, s));
+        HIP_TRY(pngpd::head_few_grad(type, g, lse_dev, kept, dloss_dev, reduction, dx_dev, dweight_dev, dbias_dev, (float*)workspace_dev, s));
         return PNGPD_OK;
     }
+    LossWs ws(workspace_dev, type, T, V, D, true, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
+    if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
     const HeadOperand x{ws.x, padded(D, type), true}, xt{ws.x, padded(D, type), false};
     const pngpd::HeadRowWeights weights{target_dev, T, V, ignore_index, reduction, dloss_dev, ws.row_weight, ws.scale,
                                         pngpd::head_label_factor(label_smoothing)};

@@ -283,7 +283,7 @@ struct LinearCrossEntropyFunction : torch::autograd::Function<LinearCrossEntropy
         if (ctx->needs_input_grad(0)) result[0] = at::empty(x.sizes(), x.options());
         if (ctx->needs_input_grad(1)) result[1] = at::empty({V, D}, x.options());
         if (b.defined() && ctx->needs_input_grad(2)) result[2] = at::empty({V}, x.options());
-        const size_t bytes = pngpd_linear_cross_entropy_workspace_bytes(type, T, V, D, 1, xr.aligned() && wr.aligned());
+        const size_t bytes = pngpd_linear_cross_entropy_workspace_bytes(type, T, V, D, saved[5].defined() ? 2 : 1, xr.aligned() && wr.aligned());
         const at::Tensor ws = workspace(bytes, x);
         check(pngpd_linear_cross_entropy_backward(
             type, T, V, D, xr.p(), xr.ld, wr.p(), wr.ld, data(b), target.const_data_ptr<int64_t>(), ctx->saved_data["ignore_index"].toInt(),

@@ -186,3 +186,22 @@ def test_forward_mode_is_refused_before_anything_is_launched():
                     m.dropout(dual[0], None, 0.5, 1, 0, None)
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     m.dropout(x, dual[0], 0.5, 1, 0, None)
+
+
+@pytest.mark.parametrize("type", [0, 1, 2])
+def test_few_classes_ask_for_the_memory_they_use(type):
+    """At most eight classes: the rows' losses forward, parts of the gradients backward; no copy of x, aligned or not."""
+    lib = _lib.load()
+    size = lib.pngpd_linear_cross_entropy_workspace_bytes
+    for T, V, D in ((192000, 3, 1024), (2 ** 20, 8, 1024), (8192, 3, 4096), (1, 1, 1)):
+        parts = 256 * V * (D + 1) * 4 + 255
+        for aligned in (0, 1):
+            assert size(type, T, V, D, 0, aligned) == (T * 4 + 255) // 256 * 256
+            assert size(type, T, V, D, 2, aligned) <= parts < size(type, T, V, D, 1, aligned) + parts
+    assert size(type, 192000, 3, 1024, 1, 1) > 192000 * 1024 * 2          # without kept logits the general products run
+    assert size(type, 1024, 9, 64, 2, 1) == size(type, 1024, 9, 64, 1, 1)
+    # the entries ask for as much
+    need = size(type, 8192, 3, 4096, 2, 1)
+    args = (type, 8192, 3, 4096, 16, 4096, 16, 4096, None, 16, -100, 0.0, 1)
+    assert lib.pngpd_linear_cross_entropy_backward(*args, 16, 16, 16, 16, 16, 16, 4096, need - 1, None) == ERR_WORKSPACE
+    assert lib.pngpd_linear_cross_entropy_forward(*args, 16, 16, 16, 4096, size(type, 8192, 3, 4096, 0, 1) - 1, None) == ERR_WORKSPACE

@@ -1069,3 +1069,43 @@ def test_bias_gradient_of_the_loss_is_rounded_once(kind, T, V, D, reduction):
     loss = head.linear_cross_entropy(x.cuda(), w.cuda(), target.cuda(), bs, label_smoothing=0.1, reduction=reduction)
     alone, = torch.autograd.grad(loss, bs, dloss.cuda())
     assert torch.equal(alone, got["db"])
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("T,V,D", [(5000, 3, 200), (5000, 8, 513), (20, 4, 2056)])
+def test_few_classes_stay_inside_the_workspace_they_ask_for(kind, T, V, D):
+    """The C entries with exactly the memory that the size functions name, marks behind it; x away from 16-byte addresses."""
+    from pointnetgpd_amd import _lib
+    lib, dt, t = _lib.load(), TYPES[kind], list(TYPES).index(kind)
+    x, w, b, target = loss_case(T + V, T, V, D, dt, True)
+    X, W, B, Y = shifted(x, 1, 3), shifted(w, 3, 0), b.cuda(), target.cuda()
+    loss, lse = torch.empty(1, device="cuda"), torch.empty(T, device="cuda")
+    out = [torch.empty(s, dtype=dt, device="cuda") for s in ((T, D), (V, D), (V,))]
+    dloss = torch.full((1,), 64.0 if kind == "f16" else 1.0, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def room(n):
+        return torch.full((n + 4096,), 0xA5, dtype=torch.uint8, device="cuda")
+
+    size = lib.pngpd_linear_cross_entropy_workspace_bytes
+    nk, nf, nb = lib.pngpd_linear_cross_entropy_kept_bytes(t, T, V, D), size(t, T, V, D, 0, 0), size(t, T, V, D, 2, 0)
+    kept, ws, wsb = room(nk), room(nf), room(nb)
+    args = (t, T, V, D, X.data_ptr(), X.stride(0), W.data_ptr(), W.stride(0), B.data_ptr(), Y.data_ptr(), -100, 0.1, 1)
+    assert lib.pngpd_linear_cross_entropy_forward(*args, loss.data_ptr(), lse.data_ptr(), kept.data_ptr(), ws.data_ptr(), nf, stream) == 0
+    assert lib.pngpd_linear_cross_entropy_backward(*args, lse.data_ptr(), kept.data_ptr(), dloss.data_ptr(), *(o.data_ptr() for o in out),
+                                                   wsb.data_ptr(), nb, stream) == 0
+    check({"loss": loss[0], "dx": out[0], "dw": out[1], "db": out[2]},
+          ho.cross_entropy(x, w, target, b, -100, 0.1, "mean", dloss.cpu()[0]))
+    for buffer, n in ((kept, nk), (ws, nf), (wsb, nb)):
+        assert (buffer[n:] == 0xA5).all()
+
+
+def test_few_classes_take_no_copy_of_a_large_input():
+    x = torch.randn(100000, 1025, device="cuda")[:, 1:].requires_grad_()      # rows away from 16-byte addresses
+    w, y = torch.randn(3, 1024, device="cuda").requires_grad_(), torch.arange(100000, device="cuda") % 3
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    loss = head.linear_cross_entropy(x, w, y)
+    torch.autograd.grad(loss, (x, w))
+    assert torch.cuda.max_memory_allocated() - before < 100000 * 1024 * 4 + (32 << 20)      # x's gradient, and little else
