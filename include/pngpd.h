@@ -378,9 +378,9 @@ int pngpd_adam_step(float* params_dev, const float* grads_dev, float* exp_avg_de
  * Matrices are row-major; ld* is the distance of two rows in elements (at least the row's length), and a matrix
  * without an ld argument is dense.  `type` is the element type of every matrix and bias; sums and statistics are
  * 32-bit (64-bit over a batch's losses).  Outputs must not overlap inputs or each other.  Sizes: 0 <= rows < 2^31,
- * 1 <= N, K, D <= 2^21, 1 <= V <= 2^24.  A call with no rows still writes the outputs that do not depend on
- * rows (zero gradients).  All calls are stream-ordered, allocate nothing and can be captured into a graph; two calls
- * that may run at the same time need workspaces of their own.
+ * 1 <= N, K, D <= 2^21, 1 <= V <= 2^24 (dropout has its own).  A call with no rows still writes the outputs that do
+ * not depend on rows (zero gradients).  All calls are stream-ordered, allocate nothing and can be captured into a graph;
+ * two calls that may run at the same time need workspaces of their own.
  *
  * Matrices may start anywhere and have any ld, but rows that are not whole 16-byte chunks are copied into the workspace
  * first.  pngpd_*_workspace_bytes(..., aligned): aligned != 0 if x, weight and dy start at 16-byte addresses and their
@@ -415,6 +415,7 @@ int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void*
  * = splitmix64's step.  The mask depends on seed, offset and position alone and is never stored; the backward pass is
  * the same call on dy without the residual.  rng_dev, optional: int64 [2] = {seed, offset} read on the device when the
  * kernel runs, in place of the two arguments (a captured graph draws a new mask whenever they change).
+ * At most 2^42 elements, 2^40 a row.
  */
 int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64_t ldx, const void* residual_dev, int64_t ldr,
                   void* y_dev, double p, uint64_t seed, uint64_t offset, const int64_t* rng_dev, void* stream);

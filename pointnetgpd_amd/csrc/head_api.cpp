@@ -317,9 +317,10 @@ int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void*
 int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64_t ldx, const void* residual_dev, int64_t ldr,
                   void* y_dev, double p, uint64_t seed, uint64_t offset, const int64_t* rng_dev, void* stream) {
     const char* who = "pngpd_dropout";
-    int rc = check_sizes(who, type, rows, cols, 1);
-    if (rc) return rc;
-    if ((double)rows * (double)cols > 4398046511104.0) return fail(PNGPD_ERR_SHAPE, "%s: more than 2^42 elements", who);
+    int rc = PNGPD_OK;
+    if (!type_ok(type)) return fail(PNGPD_ERR_INVALID, "%s: unknown type %d", who, type);
+    if (rows < 0 || cols < 1 || (double)rows * (double)cols > 4398046511104.0 || cols > ((int64_t)1 << 40))
+        return fail(PNGPD_ERR_SHAPE, "%s: %lld x %lld, at most 2^42 elements, 2^40 a row", who, (long long)rows, (long long)cols);
     if (!(p >= 0.0 && p <= 1.0)) return fail(PNGPD_ERR_INVALID, "%s: p = %g", who, p);
     if (rows == 0) return PNGPD_OK;
     if (!x_dev || !y_dev) return fail(PNGPD_ERR_INVALID, "%s: NULL argument", who);

@@ -205,3 +205,19 @@ def test_few_classes_ask_for_the_memory_they_use(type):
     args = (type, 8192, 3, 4096, 16, 4096, 16, 4096, None, 16, -100, 0.0, 1)
     assert lib.pngpd_linear_cross_entropy_backward(*args, 16, 16, 16, 16, 16, 16, 4096, need - 1, None) == ERR_WORKSPACE
     assert lib.pngpd_linear_cross_entropy_forward(*args, 16, 16, 16, 4096, size(type, 8192, 3, 4096, 0, 1) - 1, None) == ERR_WORKSPACE
+
+
+@pytest.mark.parametrize("rows,cols", [(2 ** 21, 2 ** 21 + 1), (1, 2 ** 40 + 1), (2 ** 42 + 1, 1), (2 ** 62, 4)])
+def test_dropout_refuses_what_passes_its_own_limits(rows, cols):
+    """2^42 elements, 2^40 a row: neither the rows nor a row end at 2^31."""
+    lib = _lib.load()
+    assert lib.pngpd_dropout(0, rows, cols, 16, cols, None, cols, 16, 0.5, 1, 0, None, None) == ERR_SHAPE
+    assert b"2^42" in lib.pngpd_last_error()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 2 ** 31 + 9), (2 ** 31 + 9, 1), (2 ** 32, 2 ** 10)])
+def test_dropout_takes_more_than_31_bits_of_rows_or_columns(rows, cols):
+    """The sizes pass; what is refused is the missing pointer, which is looked at behind them."""
+    lib = _lib.load()
+    assert lib.pngpd_dropout(0, rows, cols, None, cols, None, cols, None, 0.5, 1, 0, None, None) == ERR_INVALID
+    assert b"NULL" in lib.pngpd_last_error()

@@ -1109,3 +1109,16 @@ def test_few_classes_take_no_copy_of_a_large_input():
     loss = head.linear_cross_entropy(x, w, y)
     torch.autograd.grad(loss, (x, w))
     assert torch.cuda.max_memory_allocated() - before < 100000 * 1024 * 4 + (32 << 20)      # x's gradient, and little else
+
+
+def test_dropout_of_one_dimension_beyond_31_bits():
+    """A one-dimensional tensor, and a column, of 2^31 + 9 elements drop what the same elements of another shape do."""
+    n, tail = 2 ** 31 + 9, 5001
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    keep = torch.cat([torch.from_numpy(ho.keep_mask(tail, 0.25, 3, 1)), torch.from_numpy(ho.keep_mask_at(n - tail, tail, 0.25, 3, 1))])
+    for view in (x, x.view(n, 1), x.view(1, n)):
+        y = head.dropout(view, 0.25, 3, 1)
+        assert y.shape == view.shape
+        y = y.view(-1)
+        assert torch.equal(torch.cat([y[:tail], y[-tail:]]).cpu() != 0, keep)
+        del y
