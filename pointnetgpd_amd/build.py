@@ -146,10 +146,10 @@ def build_example(force: bool = False) -> str:
 
 def build_all(force: bool = False) -> None:
     build_library(force)
-    build_head(force)
     build_example(force)
     build_probe(force)
     build_oracle_c(force)
+    build_head(force)        # last: a host without torch's C++ headers still gets the rest
 
 
 if __name__ == "__main__":

@@ -221,3 +221,18 @@ def test_dropout_takes_more_than_31_bits_of_rows_or_columns(rows, cols):
     lib = _lib.load()
     assert lib.pngpd_dropout(0, rows, cols, None, cols, None, cols, None, 0.5, 1, 0, None, None) == ERR_INVALID
     assert b"NULL" in lib.pngpd_last_error()
+
+
+def test_a_host_without_torchs_headers_builds_the_rest(monkeypatch):
+    from pointnetgpd_amd import build
+    done = []
+    for name in ("build_library", "build_example", "build_probe", "build_oracle_c"):
+        monkeypatch.setattr(build, name, lambda force=False, name=name: done.append(name))
+
+    def no_headers(force=False):
+        raise OSError("torch/extension.h")
+
+    monkeypatch.setattr(build, "build_head", no_headers)
+    with pytest.raises(OSError):
+        build.build_all()
+    assert sorted(done) == ["build_example", "build_library", "build_oracle_c", "build_probe"]
