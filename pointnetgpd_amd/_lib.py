@@ -127,6 +127,12 @@ def load_head():
         if not os.path.exists(HEAD_PATH):
             raise ImportError(f"{HEAD_PATH} not found: it has not been built "
                               "(python -c 'import __graft_entry__ as g; g.build()'); there is no other path")
+        import torch
+
+        from .build import built_for
+        if not built_for(HEAD_PATH, torch.__version__):
+            raise ImportError(f"{HEAD_PATH} was not built for this torch ({torch.__version__}): build it again "
+                              "(python -c 'import __graft_entry__ as g; g.build()')")
         from . import _head as module
         _head = module
     return _head

@@ -9,6 +9,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "pointnetgpd_amd", "csrc")
@@ -72,7 +73,7 @@ def build_library(force: bool = False, verbose_resources: bool = False) -> str:
     hdrs.append(os.path.abspath(__file__))        # the flags
     if not force and not _newer(LIB_PATH, srcs + hdrs):
         return LIB_PATH
-    objs = []
+    objs, jobs = [], []
     for s in srcs:
         o = os.path.splitext(s)[0] + ".o"
         if force or _newer(o, [s] + hdrs):
@@ -81,13 +82,25 @@ def build_library(force: bool = False, verbose_resources: bool = False) -> str:
                 cmd += ["-x", "hip"]
             if verbose_resources:
                 cmd += ["-Rpass-analysis=kernel-resource-usage"]
-            _run(cmd + ["-c", s, "-o", o])
+            jobs.append(cmd + ["-c", s, "-o", o])
         objs.append(o)
+    with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        list(pool.map(_run, jobs))
     _run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", LIB_PATH] + objs)
     return LIB_PATH
 
 
 HEAD_PATH = os.path.join(ROOT, "pointnetgpd_amd", "_head.so")
+
+
+def _mark(version: str) -> str:
+    return f"built for torch {version};"
+
+
+def built_for(path: str, version: str) -> bool:
+    """Whether the binding was compiled against this version of torch, whose C++ interface is no other version's."""
+    with open(path, "rb") as f:
+        return _mark(version).encode() in f.read()
 
 
 def build_head(force: bool = False) -> str:
@@ -97,11 +110,12 @@ def build_head(force: bool = False) -> str:
     import torch
 
     src = os.path.join(CSRC, "head_torch.cpp")
-    if force or _newer(HEAD_PATH, [src, os.path.join(ROOT, "include", "pngpd.h"), os.path.abspath(__file__)]):
+    if force or _newer(HEAD_PATH, [src, os.path.join(ROOT, "include", "pngpd.h"), os.path.abspath(__file__)]) or \
+            not built_for(HEAD_PATH, torch.__version__):
         base = os.path.dirname(torch.__file__)
         rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
         _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
-              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", os.path.join(ROOT, "include"),
+              f'-DPNGPD_TORCH="{_mark(torch.__version__)}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I", os.path.join(ROOT, "include"),
               "-isystem", os.path.join(base, "include"), "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
               "-isystem", sysconfig.get_paths()["include"], "-isystem", os.path.join(rocm, "include"), src, "-o", HEAD_PATH,
               "-L", os.path.join(base, "lib"), "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lamdhip64",

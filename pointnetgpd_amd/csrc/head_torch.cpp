@@ -306,6 +306,7 @@ at::Tensor linear_cross_entropy(const at::Tensor& x, const at::Tensor& w, const 
 
 PYBIND11_MODULE(_head, m) {
     m.doc() = "autograd nodes of pointnetgpd_amd.head";
+    m.attr("built_for") = PNGPD_TORCH;      // "built for torch <version>;"
     pybind11::register_local_exception_translator([](std::exception_ptr e) {
         try {
             if (e) std::rethrow_exception(e);

@@ -223,6 +223,28 @@ def test_dropout_takes_more_than_31_bits_of_rows_or_columns(rows, cols):
     assert b"NULL" in lib.pngpd_last_error()
 
 
+def test_a_binding_for_another_torch_is_an_error(monkeypatch, tmp_path):
+    """The binding is compiled against one version of torch's C++ interface; another's is built again, and not loaded."""
+    from pointnetgpd_amd import build
+    assert build.built_for(_lib.HEAD_PATH, torch.__version__) and not build.built_for(_lib.HEAD_PATH, torch.__version__ + "1")
+    other = tmp_path / "_head.so"
+    other.write_bytes(open(_lib.HEAD_PATH, "rb").read().replace(build._mark(torch.__version__).encode(), b"x" * len(build._mark(torch.__version__))))
+    monkeypatch.setattr(_lib, "_head", None)
+    monkeypatch.setattr(_lib, "HEAD_PATH", str(other))
+    with pytest.raises(ImportError, match="not built for this torch"):
+        _lib.load_head()
+    commands = []
+    monkeypatch.setattr(build, "HEAD_PATH", str(other))
+    monkeypatch.setattr(build, "_run", commands.append)
+    build.build_head()
+    assert len(commands) == 1 and any(build._mark(torch.__version__) in word for word in commands[0])
+    monkeypatch.setattr(build, "HEAD_PATH", _lib.__file__.replace("_lib.py", "_head.so"))
+    commands.clear()
+    monkeypatch.setattr(build, "_newer", lambda target, deps: False)
+    build.build_head()
+    assert not commands
+
+
 def test_a_host_without_torchs_headers_builds_the_rest(monkeypatch):
     from pointnetgpd_amd import build
     done = []
