@@ -378,9 +378,10 @@ int pngpd_adam_step(float* params_dev, const float* grads_dev, float* exp_avg_de
  * Matrices are row-major; ld* is the distance of two rows in elements (at least the row's length), and a matrix
  * without an ld argument is dense.  `type` is the element type of every matrix and bias; sums and statistics are
  * 32-bit (64-bit over a batch's losses).  Outputs must not overlap inputs or each other.  Sizes: 0 <= rows < 2^31,
- * 1 <= N, K, D <= 2^21, 1 <= V <= 2^24 (dropout has its own).  A call with no rows still writes the outputs that do
- * not depend on rows (zero gradients).  All calls are stream-ordered, allocate nothing and can be captured into a graph;
- * two calls that may run at the same time need workspaces of their own.
+ * 1 <= N, K, D <= 2^21, 1 <= V <= 2^24 (dropout has its own), and what a product writes has fewer than 2^23 tiles of
+ * 256 x 256 (float32: 128 x 128, so rows end at 2^30 there, but for few classes).  A call with no rows still writes the
+ * outputs that do not depend on rows (zero gradients).  All calls are stream-ordered, allocate nothing and can be
+ * captured into a graph; two calls that may run at the same time need workspaces of their own.
  *
  * Matrices may start anywhere and have any ld, but rows that are not whole 16-byte chunks are copied into the workspace
  * first.  pngpd_*_workspace_bytes(..., aligned): aligned != 0 if x, weight and dy start at 16-byte addresses and their

@@ -46,6 +46,13 @@ int check_linear(const char* who, int type, int64_t M, int64_t N, int64_t K, int
     return PNGPD_OK;
 }
 
+// A launch holds fewer than 2^23 tiles of a product's output, 256 x 256 (16 bits) or 128 x 128 (float32) at most.
+int check_tiles(const char* who, int type, int64_t M, int64_t N) {
+    const int64_t side = type == PNGPD_TYPE_F32 ? 128 : 256;
+    if ((double)((M + side - 1) / side) * (double)((N + side - 1) / side) < 8388608.0) return PNGPD_OK;
+    return fail(PNGPD_ERR_SHAPE, "%s: a product of %lld x %lld has more than 2^23 tiles", who, (long long)M, (long long)N);
+}
+
 int check_ld(const char* who, const char* name, int64_t ld, int64_t least) {
     if (ld < least || ld > ((int64_t)1 << 40)) return fail(PNGPD_ERR_SHAPE, "%s: %s = %lld for rows of %lld", who, name, (long long)ld, (long long)least);
     return PNGPD_OK;
@@ -252,6 +259,7 @@ int pngpd_linear_forward(int type, int64_t M, int64_t N, int64_t K, const void* 
     if ((rc = check_ld(who, "ldx", ldx, K)) || (rc = check_ld(who, "ldw", ldw, K))) return rc;
     if (residual_dev && (rc = check_ld(who, "ldr", ldr, N))) return rc;
     const bool few = M <= pngpd::HEAD_FEW_ROWS;
+    if (!few && (rc = check_tiles(who, type, M, N))) return rc;
     LinearWs ws(workspace_dev, type, M, N, K, false, !few && !direct(x_dev, ldx, K, type), !few && !direct(weight_dev, ldw, K, type), false);
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
     HeadEpilogue e;
@@ -290,6 +298,7 @@ int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void*
     if ((rc = check_ld(who, "ld_dy", ld_dy, N))) return rc;
     if (dweight_dev && (rc = check_ld(who, "ldx", ldx, K))) return rc;
     if (dx_dev && (rc = check_ld(who, "ldw", ldw, K))) return rc;
+    if ((dx_dev && (rc = check_tiles(who, type, M, K))) || (dweight_dev && (rc = check_tiles(who, type, N, K)))) return rc;
     LinearWs ws(workspace_dev, type, M, N, K, true, dweight_dev && !direct(x_dev, ldx, K, type),
                 dx_dev && !direct(weight_dev, ldw, K, type), act != PNGPD_ACT_NONE || !direct(dy_dev, ld_dy, N, type));
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
@@ -425,6 +434,7 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
         return PNGPD_OK;
     }
     LossWs ws(workspace_dev, type, T, V, D, true, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
+    if ((rc = check_tiles(who, type, T, ws.piece)) || (rc = check_tiles(who, type, T, D)) || (rc = check_tiles(who, type, ws.piece, D))) return rc;
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
     const HeadOperand x{ws.x, padded(D, type), true}, xt{ws.x, padded(D, type), false};
     const pngpd::HeadRowWeights weights{target_dev, T, V, ignore_index, reduction, dloss_dev, ws.row_weight, ws.scale,

@@ -258,3 +258,20 @@ def test_a_host_without_torchs_headers_builds_the_rest(monkeypatch):
     with pytest.raises(OSError):
         build.build_all()
     assert sorted(done) == ["build_example", "build_library", "build_oracle_c", "build_probe"]
+
+
+def test_more_tiles_than_a_launch_holds_are_refused():
+    """2^23 tiles of 128 x 128 (float32) or 256 x 256: an error that says so, not the runtime's."""
+    lib = _lib.load()
+    for type, M, N in ((0, 2 ** 30, 1), (0, 2 ** 20, 2 ** 17), (1, 2 ** 31 - 1, 1), (2, 2 ** 22, 2 ** 17)):
+        assert _linear(lib, type=type, M=M, N=N, ldr=N) == ERR_SHAPE
+        assert b"tiles" in lib.pngpd_last_error()
+        rc = lib.pngpd_linear_backward(type, M, 4, N, 16, 4, None, 16, N, 16, N, 0, 16, None, None, None, 0, None)
+        assert rc == ERR_SHAPE and b"tiles" in lib.pngpd_last_error()
+    # one row less passes the sizes: the missing workspace is refused next
+    assert _linear(lib, M=2 ** 30 - 128, N=1, K=5, ldx=5, ldw=5) == ERR_INVALID
+    rc = lib.pngpd_linear_backward(0, 8, 2 ** 21, 2 ** 21, 16, 2 ** 21, None, 16, 2 ** 21, 16, 2 ** 21, 0, None, 16, None, None, 0, None)
+    assert rc == ERR_SHAPE and b"tiles" in lib.pngpd_last_error()
+    args = (0, 2 ** 30, 9, 4, 16, 4, 16, 4, None, 16, -100, 0.0, 1)
+    assert lib.pngpd_linear_cross_entropy_backward(*args, 16, None, 16, 16, 16, None, 4096, 1 << 60, None) == ERR_SHAPE
+    assert b"tiles" in lib.pngpd_last_error()
