@@ -1122,3 +1122,49 @@ def test_dropout_of_one_dimension_beyond_31_bits():
         y = y.view(-1)
         assert torch.equal(torch.cat([y[:tail], y[-tail:]]).cpu() != 0, keep)
         del y
+
+
+def test_a_head_behind_the_trunk():
+    """PointNetfeat in training mode, then linear, dropout and linear_cross_entropy, one backward pass through both: the head's
+    gradients against 64 bits on the feature as it is, the trunk's against the trunk's own backward pass of the feature's gradient."""
+    from pointnetgpd_amd import synth
+    from pointnetgpd_amd.pointnet import PointNetfeat
+    B, P, H, V = 12, 64, 96, 5
+    sd = {k[len("feat."):]: v for k, v in synth.torch_state_dict(3, 2, 0.02).items() if k.startswith("feat.")}
+    points = torch.from_numpy(synth.candidate_points(5, B, P, "gripper")).cuda()
+    target = (torch.arange(B) % V).cuda()
+
+    def trunk():
+        m = PointNetfeat(P, 3)
+        m.load_state_dict(sd)
+        return m.cuda().train()
+
+    params = [t.cuda().requires_grad_() for t in make(6, (H, 1024), (H,), (H, H), (H,), (V, H), (V,), scale=0.05)]
+    m = trunk()
+    feat, trans = m(points)
+    feat.retain_grad()
+    h0 = head.linear(feat, params[0], params[1])
+    h1 = head.linear(h0, params[2], params[3], activation="gelu")
+    h = head.dropout(h1, 0.3, 11, 2, residual=h0)
+    loss = head.linear_cross_entropy(h, params[4], target, params[5], label_smoothing=0.1)
+    (loss + 0.001 * trans.square().sum()).backward()
+
+    P64 = [p.detach().cpu().double().requires_grad_() for p in params]
+    F64 = feat.detach().cpu().double().requires_grad_()
+    keep = torch.from_numpy(ho.keep_mask(B * H, 0.3, 11, 2)).view(B, H).double()
+    a0 = F64 @ P64[0].t() + P64[1]
+    a1 = torch.nn.functional.gelu(a0 @ P64[2].t() + P64[3])
+    want = torch.nn.functional.cross_entropy((a0 + keep * a1 / 0.7) @ P64[4].t() + P64[5], target.cpu(), label_smoothing=0.1)
+    want.backward()
+    # three layers of 32-bit sums over at most 1024 terms, random in sign: 64 units a layer, and their functions
+    tol = 4 * 64 * ho.U * 3
+    assert abs(loss.item() - want.item()) <= tol * abs(want.item())
+    for got, ref in zip(params + [feat], P64 + [F64]):
+        assert (got.grad.cpu().double() - ref.grad).norm() <= tol * ref.grad.norm()
+
+    twin = trunk()
+    again, trans2 = twin(points)
+    assert torch.equal(again, feat)
+    torch.autograd.backward([again, trans2], [feat.grad, 0.002 * trans2.detach()])
+    for (name, p), q in zip(m.named_parameters(), twin.parameters()):
+        assert torch.equal(p.grad, q.grad), name
