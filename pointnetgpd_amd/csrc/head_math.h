@@ -33,8 +33,9 @@ __device__ __forceinline__ float gelu_gate(float z) {
 constexpr float GELU_C = 0.7978845608028654f;      // sqrt(2 / pi)
 
 // Phi(z), and exp(-z^2 / 2) on the way.  Phi(-|z|) = exp(-z^2 / 2) Q(t), t = 1 / (1 + 0.297 |z|): Q is a least-squares fit of
-// erfcx's scaled form in t, reweighted towards equal relative error over |z| <= 14 (4e-8 in exact arithmetic, 2.7e-7 in
-// 32 bits); one exponential and one reciprocal, where the library's erfcf takes some 60 instructions.
+// erfcx's scaled form in t, reweighted towards equal relative error over |z| <= 14 (4e-8 in exact arithmetic, 3e-7 in 32 bits);
+// one exponential and one reciprocal, where the library's erfcf takes some 60 instructions.  The exponential's argument is
+// rounded to 32 bits, which Phi sees as an error growing with z^2: 1e-6 of its value at z = -3, 7e-6 at -12.
 __device__ __forceinline__ float normal_cdf(float z, float* bell) {
     const float e = exp2_f(-0.5f * LOG2E * z * z);
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.2969848480983499f, __builtin_fabsf(z), 1.f));

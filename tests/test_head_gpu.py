@@ -1168,3 +1168,23 @@ def test_a_head_behind_the_trunk():
     torch.autograd.backward([again, trans2], [feat.grad, 0.002 * trans2.detach()])
     for (name, p), q in zip(m.named_parameters(), twin.parameters()):
         assert torch.equal(p.grad, q.grad), name
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_negative_tails_of_the_activations(act):
+    """Relative to the value, down to z = -12, in units of 2^-24.  The exponential's argument a is rounded three times (its constant
+    and two products; gelu_tanh's fma besides), which the result sees as 4 |a| ln 2 <= 4 |ln of the factor|; besides at most 12 for
+    the fit, the instructions' own steps and the last products.  Factors below 2^-126 may be 0."""
+    z = -torch.linspace(0.0, 12.0, 4801)[1:, None]
+    Z = z.double()
+    if act == "gelu":
+        gate, expo = 0.5 * torch.special.erfc(-Z / math.sqrt(2)), Z * Z / 2
+    elif act == "silu":
+        gate, expo = torch.sigmoid(Z), Z.abs()
+    else:
+        u = math.sqrt(2 / math.pi) * (Z + 0.044715 * Z ** 3)
+        gate, expo = torch.sigmoid(2 * u), 2 * u.abs()
+    want = Z * gate
+    bound = (12 + 4 * expo) * ho.U * want.abs() + 2 * 2.0 ** -126 * Z.abs()
+    one = torch.ones(1, 1, device="cuda")
+    assert ho.worst(head.linear(z.cuda(), one, activation=act), want, bound) <= 1.0
