@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(int64_t total, int64_t col
         offset = (unsigned long long)rng[1];
     }
     const unsigned long long key = mix64(seed ^ mix64(offset));
-    // one turn, unless the grid's 2^32 threads are not enough
+    // one turn, unless the grid's 2^31 threads are not enough
     for (int64_t i0 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * PER_THREAD; i0 < total;
          i0 += (int64_t)gridDim.x * 256 * PER_THREAD)
         dropout_eight<T, DENSE, RESIDUAL>(i0, total, cols, x, ldx, r, ldr, y, border, scale, key);
