@@ -110,7 +110,11 @@ struct HeadRowWeights {
     const float* dloss;
     float *row_weight, *out_scale;
     float label_factor;         // 16-bit types: of all weights (head_label_factor)
+    float* parts;               // head_row_parts(T) times three floats
 };
+// Many rows: their count, and the largest of their weights, come from this many workgroups in a launch in front (0: from one,
+// beside those that lay operands out).
+int64_t head_row_parts(int64_t T);
 // c in (1/2, 1] with c (1 - eps) a power of two (1 where eps is)
 inline float head_label_factor(float eps) {
     int e;
@@ -137,9 +141,10 @@ hipError_t head_dropout(int type, int64_t rows, int64_t cols, const void* x, int
 bool head_loss_at_once(int64_t T, int blocks);
 hipError_t head_row_loss(int64_t T, int64_t V, int blocks, const float4* stats, const float* target_logit, const int64_t* target,
                          int64_t ignore_index, float eps, float* row_loss, float* lse, int reduction, float* batch, hipStream_t s);
-// used (may be NULL) receives the number of rows that are not ignored
+// used (may be NULL) receives the number of rows that are not ignored; parts: head_batch_parts(T) pairs of doubles
+int64_t head_batch_parts(int64_t T);
 hipError_t head_batch_loss(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore_index, int reduction, float* loss,
-                           float* used, hipStream_t s);
+                           float* used, double2* parts, hipStream_t s);
 
 // The loss over at most HEAD_FEW classes, operands with any strides.  logits: what is kept for the backward pass, head_few_room
 // floats a row (NULL: forward only).

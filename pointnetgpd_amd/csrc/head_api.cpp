@@ -123,6 +123,8 @@ struct LossWs {
     void *x, *w, *tile;        // laid out; gradients of a piece's logits, [T][padded(piece)]
     float4* stats;
     float *target_logit, *row_loss, *row_weight, *scale, *part, *dx_sum, *partial;
+    double2* loss_parts;
+    float* row_parts;
     float* partial_w;          // the weight's gradient's own
     pngpd::HeadPlan dz, dz_last;      // of a piece's logits, and of the last piece's where that is smaller
     size_t bytes;
@@ -134,7 +136,8 @@ struct LossWs {
         w = copy_w ? b.take((size_t)V * dp * e) : nullptr;
         tile = nullptr;
         stats = nullptr;
-        target_logit = row_loss = row_weight = scale = part = dx_sum = partial = partial_w = nullptr;
+        target_logit = row_loss = row_weight = scale = part = dx_sum = partial = partial_w = row_parts = nullptr;
+        loss_parts = nullptr;
         piece = V;
         rows_at_once = rows;
         if (!backward) {
@@ -154,6 +157,7 @@ struct LossWs {
             stats = (float4*)b.take(blocks * sizeof(float4));
             target_logit = (float*)b.take((size_t)rows * 4);
             row_loss = (float*)b.take((size_t)rows * 4);
+            loss_parts = (double2*)b.take((size_t)pngpd::head_batch_parts(rows) * sizeof(double2));
             partial = (float*)b.take(cut);
         } else {
             piece = (int64_t)(loss_budget(type, rows, V, D) / ((size_t)rows * e)) / 256 * 256;
@@ -164,6 +168,7 @@ struct LossWs {
             tile = b.take((size_t)rows * padded(piece, type) * e);
             row_weight = (float*)b.take((size_t)rows * 4);
             scale = (float*)b.take(4);
+            row_parts = (float*)b.take((size_t)pngpd::head_row_parts(rows) * 12);
             if (piece < V) dx_sum = (float*)b.take((size_t)rows * D * 4);
             size_t cut = 0, cut_w = 0, sums = 0;
             for (int64_t n : {piece, last}) {
@@ -197,11 +202,17 @@ int check_loss(const char* who, int type, int64_t T, int64_t V, int64_t D, const
 
 // Few classes have kernels of their own, which take x and the weight as they lie: the rows' losses, and the parts of the gradients
 // where the logits were kept (the general products serve those that were not).
-size_t few_forward_bytes(int64_t T) {
-    Bump b(nullptr);
-    b.take((size_t)T * 4);
-    return b.off;
-}
+struct FewForwardWs {
+    float* row_loss;
+    double2* loss_parts;
+    size_t bytes;
+    FewForwardWs(void* base, int64_t T) {
+        Bump b(base);
+        row_loss = (float*)b.take((size_t)T * 4);
+        loss_parts = (double2*)b.take((size_t)pngpd::head_batch_parts(T) * sizeof(double2));
+        bytes = b.off;
+    }
+};
 size_t few_backward_bytes(int type, int64_t T, int64_t V, int64_t D) {
     Bump b(nullptr);
     b.take(pngpd::head_few_part_bytes(type, T, V, D));
@@ -342,7 +353,7 @@ int pngpd_dropout(int type, int64_t rows, int64_t cols, const void* x_dev, int64
 size_t pngpd_linear_cross_entropy_workspace_bytes(int type, int64_t T, int64_t V, int64_t D, int backward, int aligned) {
     const void* some = &type;      // the sizes alone are checked
     if (check_loss("pngpd_linear_cross_entropy_workspace_bytes", type, T, V, D, some, D, some, D, (const int64_t*)some, 0.f, 0)) return 0;
-    if (V <= pngpd::HEAD_FEW && !backward) return few_forward_bytes(T);
+    if (V <= pngpd::HEAD_FEW && !backward) return FewForwardWs(nullptr, T).bytes;
     if (V <= pngpd::HEAD_FEW && backward == 2 && kept_bytes(type, T, V, D)) return few_backward_bytes(type, T, V, D);
     const bool d = !aligned || padded(D, type) != D;
     return LossWs(nullptr, type, T, V, D, backward != 0, d, d).bytes;
@@ -367,13 +378,14 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
     hipStream_t s = (hipStream_t)stream;
     if (T > 0 && V <= pngpd::HEAD_FEW) {
         const bool rows = reduction == PNGPD_REDUCE_NONE;
-        if ((rc = check_ws(who, workspace_dev, workspace_bytes, rows ? 0 : few_forward_bytes(T)))) return rc;
+        const FewForwardWs ws(workspace_dev, T);
+        if ((rc = check_ws(who, workspace_dev, workspace_bytes, rows ? 0 : ws.bytes))) return rc;
         char* few = kept_bytes(type, T, V, D) ? (char*)kept_dev : nullptr;
-        float* row_loss = rows ? loss_dev : (float*)workspace_dev;
+        float* row_loss = rows ? loss_dev : ws.row_loss;
         const pngpd::HeadFew g{T, V, D, x_dev, ldx, weight_dev, ldw, bias_dev, target_dev, ignore_index, label_smoothing,
                                few ? (float*)(few + FEW_HEAD) : nullptr};
         HIP_TRY(pngpd::head_few_loss(type, g, row_loss, lse_dev, s));
-        if (!rows) HIP_TRY(pngpd::head_batch_loss(T, row_loss, target_dev, ignore_index, reduction, loss_dev, (float*)few, s));
+        if (!rows) HIP_TRY(pngpd::head_batch_loss(T, row_loss, target_dev, ignore_index, reduction, loss_dev, (float*)few, ws.loss_parts, s));
         return PNGPD_OK;
     }
     LossWs ws(workspace_dev, type, T, V, D, false, !direct(x_dev, ldx, D, type), !direct(weight_dev, ldw, D, type));
@@ -405,7 +417,7 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
             if (whole && reduction != PNGPD_REDUCE_NONE && pngpd::head_loss_at_once(n, blocks)) return PNGPD_OK;
         }
     }
-    if (reduction != PNGPD_REDUCE_NONE) HIP_TRY(pngpd::head_batch_loss(T, ws.row_loss, target_dev, ignore_index, reduction, loss_dev, nullptr, s));
+    if (reduction != PNGPD_REDUCE_NONE) HIP_TRY(pngpd::head_batch_loss(T, ws.row_loss, target_dev, ignore_index, reduction, loss_dev, nullptr, ws.loss_parts, s));
     return PNGPD_OK;
 }
 
@@ -438,7 +450,7 @@ int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t 
     if ((rc = check_ws(who, workspace_dev, workspace_bytes, ws.bytes))) return rc;
     const HeadOperand x{ws.x, padded(D, type), true}, xt{ws.x, padded(D, type), false};
     const pngpd::HeadRowWeights weights{target_dev, T, V, ignore_index, reduction, dloss_dev, ws.row_weight, ws.scale,
-                                        pngpd::head_label_factor(label_smoothing)};
+                                        pngpd::head_label_factor(label_smoothing), ws.row_parts};
     const pngpd::HeadLayOut job_x{x_dev, T, D, ldx, ws.x, x.ld, true};      // what padding rows hold stays out of the sums
     pngpd::HeadLayOut job_w;
     bool lay_w;

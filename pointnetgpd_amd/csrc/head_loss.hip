@@ -2,7 +2,7 @@
 //
 // A block of columns leaves a row's maximum m, sum s of exp(z - m) and sum of z; blocks join by
 // s = s1 exp(m1 - m) + s2 exp(m2 - m) under m = max(m1, m2).  Bound by their launches: 4096 rows of 128 blocks (8 MB) take
-// 12 us, the batch's sum over them 5 us (65536 rows: 12 us).
+// 12 us, the batch's sum over them 5 us.
 #include "head.h"
 #include "head_math.h"
 
@@ -79,6 +79,35 @@ __global__ __launch_bounds__(1024) void batch_loss_kernel(int64_t T, const float
     batch_sum(sum, used, reduction, loss, count);
 }
 
+// Many rows: runs of them by a workgroup each, then their sums by one (65536 x 64 -> 3 training in bfloat16 44 -> 38 us, scoring
+// 2^20 x 16 -> 3 280 -> 129 us).
+constexpr int64_t BATCH_ALONE = 16384, BATCH_PARTS = 256;
+inline int64_t rows_of_part(int64_t T) { return T <= 4096 * BATCH_PARTS ? 4096 : (T + BATCH_PARTS - 1) / BATCH_PARTS; }
+
+__global__ __launch_bounds__(256) void loss_parts_kernel(int64_t T, int64_t rows, const float* row_loss, const int64_t* target,
+                                                         int64_t ignore, double2* parts) {
+    __shared__ double2 share[4];
+    const int64_t first = blockIdx.x * rows, last = first + rows < T ? first + rows : T;
+    double sum = 0, used = 0;
+#pragma unroll 8
+    for (int64_t t = first + threadIdx.x; t < last; t += 256) {
+        sum += row_loss[t];
+        used += target[t] != ignore;
+    }
+    for (int o = 32; o; o >>= 1) {
+        sum += __shfl_xor(sum, o);
+        used += __shfl_xor(used, o);
+    }
+    if ((threadIdx.x & 63) == 0) share[threadIdx.x >> 6] = make_double2(sum, used);
+    __syncthreads();
+    if (threadIdx.x == 0)
+        parts[blockIdx.x] = make_double2(share[0].x + share[1].x + share[2].x + share[3].x, share[0].y + share[1].y + share[2].y + share[3].y);
+}
+__global__ __launch_bounds__(1024) void join_loss_kernel(int n, const double2* parts, int reduction, float* loss, float* count) {
+    const double2 v = (int)threadIdx.x < n ? parts[threadIdx.x] : make_double2(0, 0);
+    batch_sum(v.x, v.y, reduction, loss, count);
+}
+
 // rows' losses and the batch's for a small batch: a thread a row
 __global__ __launch_bounds__(1024) void small_loss_kernel(int T, int64_t V, int blocks, const float4* stats, const float* target_logit,
                                                           const int64_t* target, int64_t ignore, float eps, int reduction, float* loss,
@@ -123,8 +152,17 @@ hipError_t head_row_loss(int64_t T, int64_t V, int blocks, const float4* stats, 
     return hipGetLastError();
 }
 
+int64_t head_batch_parts(int64_t T) { return T <= BATCH_ALONE ? 0 : (T + rows_of_part(T) - 1) / rows_of_part(T); }
+
 hipError_t head_batch_loss(int64_t T, const float* row_loss, const int64_t* target, int64_t ignore, int reduction, float* loss,
-                           float* used, hipStream_t s) {
+                           float* used, double2* parts, hipStream_t s) {
+    if (const int64_t n = head_batch_parts(T)) {
+        loss_parts_kernel<<<(unsigned)n, 256, 0, s>>>(T, rows_of_part(T), row_loss, target, ignore, parts);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        join_loss_kernel<<<1, 1024, 0, s>>>((int)n, parts, reduction, loss, used);
+        return hipGetLastError();
+    }
     batch_loss_kernel<<<1, 1024, 0, s>>>(T, row_loss, target, ignore, reduction, loss, used);
     return hipGetLastError();
 }

@@ -341,32 +341,59 @@ struct Chunk {
     }
 };
 
-// Gradient weights of the loss's rows, by one workgroup of 256 beside those that lay operands out, which take longer.
-__device__ __forceinline__ void row_weights(const HeadRowWeights& w, bool bits16, bool half) {
-    __shared__ float count[4], most[4], least[4];
-    float used = 0.f, up = 0.f, down = 0.f;
+// How many of the loss's rows count, and the largest gradient up and down among those that have one.
+struct RowSums {
+    float used, up, down;
+};
+__device__ __forceinline__ RowSums row_sums(const HeadRowWeights& w, int64_t first, int64_t last) {
+    RowSums r = {};
 #pragma unroll 8
-    for (int64_t t = threadIdx.x; t < w.T; t += 256) {
+    for (int64_t t = first + threadIdx.x; t < last; t += 256) {
         const int64_t y = w.target[t];
-        used += y != w.ignore_index ? 1.f : 0.f;
+        r.used += y != w.ignore_index ? 1.f : 0.f;
         if (w.reduction == PNGPD_REDUCE_NONE && y != w.ignore_index && y >= 0 && y < w.V) {
-            up = __builtin_fmaxf(up, w.dloss[t]);
-            down = __builtin_fmaxf(down, -w.dloss[t]);
+            r.up = __builtin_fmaxf(r.up, w.dloss[t]);
+            r.down = __builtin_fmaxf(r.down, -w.dloss[t]);
         }
     }
-    used = wave_sum(used);
-    up = wave_max(up);
-    down = wave_max(down);
-    if ((threadIdx.x & 63) == 0) {
-        count[threadIdx.x >> 6] = used;
-        most[threadIdx.x >> 6] = up;
-        least[threadIdx.x >> 6] = down;
-    }
+    return r;
+}
+// over a workgroup of 256
+__device__ __forceinline__ RowSums join_rows(RowSums r) {
+    __shared__ RowSums share[4];
+    r.used = wave_sum(r.used);
+    r.up = wave_max(r.up);
+    r.down = wave_max(r.down);
+    if ((threadIdx.x & 63) == 0) share[threadIdx.x >> 6] = r;
     __syncthreads();
-    used = count[0] + count[1] + count[2] + count[3];
-    up = __builtin_fmaxf(__builtin_fmaxf(most[0], most[1]), __builtin_fmaxf(most[2], most[3]));
-    down = __builtin_fmaxf(__builtin_fmaxf(least[0], least[1]), __builtin_fmaxf(least[2], least[3]));
-    const float g = up >= down ? up : -down;      // the largest in size, with its sign
+    r = share[0];
+    for (int i = 1; i < 4; ++i) {
+        r.used += share[i].used;
+        r.up = __builtin_fmaxf(r.up, share[i].up);
+        r.down = __builtin_fmaxf(r.down, share[i].down);
+    }
+    return r;
+}
+
+// Up to 4096 rows one workgroup counts them and writes their weights, beside those that lay operands out; more are counted by up
+// to 256 workgroups in a launch of their own, and written by as many.  Training in bfloat16, one workgroup and many, in us: 8192 x
+// 2048 -> 64 with rows' own weights 88 and 71, 8192 x 1024 -> 16 66 and 60, 8192 x 16 -> 16 41 and 41, 2^20 x 16 -> 64 2810 and 400.
+constexpr int64_t ROWS_ALONE = 4096, ROW_PARTS = 256;
+inline int64_t rows_of_part(int64_t T) { return T <= 1024 * ROW_PARTS ? 1024 : (T + ROW_PARTS - 1) / ROW_PARTS; }
+
+__global__ __launch_bounds__(256) void row_parts_kernel(HeadRowWeights w, int64_t rows) {
+    const int64_t first = blockIdx.x * rows;
+    const RowSums r = join_rows(row_sums(w, first, first + rows < w.T ? first + rows : w.T));
+    if (threadIdx.x == 0) ((RowSums*)w.parts)[blockIdx.x] = r;
+}
+
+// Gradient weights of the loss's rows: workgroup `block` of those that write them, `rows` each
+__device__ __forceinline__ void row_weights(const HeadRowWeights& w, int block, int64_t rows, int parts, bool bits16, bool half) {
+    RowSums r = {};
+    if (!parts) r = row_sums(w, 0, w.T);
+    else if (threadIdx.x < parts) r = ((const RowSums*)w.parts)[threadIdx.x];
+    r = join_rows(r);
+    const float g = r.up >= r.down ? r.up : -r.down;      // the largest in size, with its sign
     // Operands of 16 bits: one weight for all rows stays out of dz and goes into the products' 32-bit sums, or p - 1 of the labels
     // would be rounded the same way in every row (off by up to 2^-9 in one direction in bfloat16).  Rows' own weights are divided
     // by the largest for the same reason, so that equal ones, the usual case, become 1; a row's quotient with another is rounded
@@ -375,14 +402,15 @@ __device__ __forceinline__ void row_weights(const HeadRowWeights& w, bool bits16
     // 2^14, |dz| <= 2 times that is inside its range, and a probability of 2^-37 still is a number.
     const bool one = w.reduction != PNGPD_REDUCE_NONE, shared = bits16 && g != 0.f && __builtin_fabsf(g) < __builtin_inff();
     const float top_weight = (half ? 16384.f : 1.f) * (bits16 ? w.label_factor : 1.f);
+    const int64_t first = block * rows, last = first + rows < w.T ? first + rows : w.T;
 #pragma unroll 8
-    for (int64_t t = threadIdx.x; t < w.T; t += 256) {
+    for (int64_t t = first + threadIdx.x; t < last; t += 256) {
         const int64_t y = w.target[t];
         const bool live = y != w.ignore_index && y >= 0 && y < w.V;
         w.row_weight[t] = !live ? 0.f : one ? top_weight : shared ? w.dloss[t] / g * top_weight : w.dloss[t];
     }
-    if (threadIdx.x == 0) {
-        const float all = w.reduction == PNGPD_REDUCE_MEAN ? w.dloss[0] * (1.f / __builtin_fmaxf(used, 1.f)) : w.dloss[0];
+    if (block == 0 && threadIdx.x == 0) {
+        const float all = w.reduction == PNGPD_REDUCE_MEAN ? w.dloss[0] * (1.f / __builtin_fmaxf(r.used, 1.f)) : w.dloss[0];
         w.out_scale[0] = one ? all / top_weight : shared ? g / top_weight : 1.f;
     }
 }
@@ -393,13 +421,13 @@ struct LayOutRun {
     unsigned grid;
 };
 
-// Workgroups 0 .. a.grid lay out a, the next b.grid b, the last one the rows' weights: a thread a 16-byte chunk of the
+// Workgroups 0 .. a.grid lay out a, the next b.grid b, the last ones the rows' weights: a thread a 16-byte chunk of the
 // destination; at most HEAD_MAX_LD / 16 chunks a row.  Bound by memory: 8192 x 4096 in bfloat16 (134 MB both ways) 33 us, 4.1 TB/s.
 template <typename T>
-__global__ __launch_bounds__(256) void set_up_kernel(LayOutRun a, LayOutRun b, HeadRowWeights w) {
+__global__ __launch_bounds__(256) void set_up_kernel(LayOutRun a, LayOutRun b, HeadRowWeights w, int64_t rows, int parts) {
     constexpr int C = Chunk<T>::C;
     if (blockIdx.x >= a.grid + b.grid) {
-        row_weights(w, sizeof(T) == 2, __is_same(T, f16_t));
+        row_weights(w, blockIdx.x - a.grid - b.grid, rows, parts, sizeof(T) == 2, __is_same(T, f16_t));
         return;
     }
     const bool second = blockIdx.x >= a.grid;
@@ -433,9 +461,16 @@ hipError_t set_up(const HeadLayOut* a, const HeadLayOut* b, const HeadRowWeights
         return r;
     };
     const LayOutRun ra = run(a), rb = run(b);
-    const unsigned grid = ra.grid + rb.grid + (w ? 1 : 0);
+    const int parts = w ? (int)head_row_parts(w->T) : 0;
+    const int64_t rows = !w ? 0 : parts ? rows_of_part(w->T) : w->T;
+    if (parts) {
+        row_parts_kernel<<<(unsigned)parts, 256, 0, s>>>(*w, rows);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    const unsigned grid = ra.grid + rb.grid + (w ? parts ? parts : 1 : 0);
     if (grid == 0) return hipSuccess;
-    set_up_kernel<T><<<grid, 256, 0, s>>>(ra, rb, w ? *w : HeadRowWeights{});
+    set_up_kernel<T><<<grid, 256, 0, s>>>(ra, rb, w ? *w : HeadRowWeights{}, rows, parts);
     return hipGetLastError();
 }
 
@@ -619,6 +654,7 @@ hipError_t head_kept(int type, int64_t M, int64_t N, int64_t K, const HeadEpilog
     const int splits = head_plan(type, M, N, K, HEAD_EPI_STATS).splits;
     PNGPD_BY_TYPE((join<T>(M, N, splits, kept, e, s)))
 }
+int64_t head_row_parts(int64_t T) { return T <= ROWS_ALONE ? 0 : (T + rows_of_part(T) - 1) / rows_of_part(T); }
 int64_t head_dz_parts(int type, int64_t M, int64_t N, const HeadPlan& p, bool kept) {
     const int64_t chunk = type == PNGPD_TYPE_F32 ? 4 : 8;
     return kept || p.splits > 1 ? dz_cut(M, (N + chunk - 1) / chunk * chunk).parts : p.tiles_m;

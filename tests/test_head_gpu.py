@@ -1188,3 +1188,20 @@ def test_negative_tails_of_the_activations(act):
     bound = (12 + 4 * expo) * ho.U * want.abs() + 2 * 2.0 ** -126 * Z.abs()
     one = torch.ones(1, 1, device="cuda")
     assert ho.worst(head.linear(z.cuda(), one, activation=act), want, bound) <= 1.0
+
+
+@pytest.mark.parametrize("T,V,D", [(4096, 12, 24), (4097, 12, 24), (16384, 12, 16), (16385, 12, 16), (300001, 9, 8), (300001, 3, 8)])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_losses_and_weights_of_many_rows(kind, reduction, T, V, D):
+    """Rows whose count, weights and losses are formed by one workgroup and by many; labels and weights that differ from run to
+    run of the rows, the largest weight in the last one."""
+    dt = TYPES[kind]
+    x, w, b, target = loss_case(T, T, V, D, dt, True)
+    target[T // 2:T // 2 + 1500] = -100
+    scale = 2.0 ** 14 if kind == "f16" else 1.0
+    dloss = torch.tensor(scale) if reduction == "mean" else torch.rand(T, generator=torch.Generator().manual_seed(T)) * scale / T
+    if reduction == "none":
+        dloss[T - 1], target[T - 1] = 3 * scale / T, 1
+    got = run_loss(x, w, target, b, 0.1, reduction, dloss)
+    check(got, ho.cross_entropy(x, w, target, b, -100, 0.1, reduction, dloss))
