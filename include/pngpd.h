@@ -404,7 +404,9 @@ int pngpd_linear_forward(int type, int64_t M, int64_t N, int64_t K, const void* 
 /*
  * Gradients of pngpd_linear_forward from dy_dev [M,N]: dz = dy act'(z), dx_dev [M,K] = dz weight, dweight_dev [N,K] =
  * dz^T x, dbias_dev [N] = column sums of dz; each output is optional.  (The residual's gradient is dy itself.)
- * For 16-bit types dz is rounded to `type` between the two products, as the operands of the matrix unit are.
+ * For 16-bit types dz is rounded to `type` between the two products, as the operands of the matrix unit are, and z is
+ * kept in it: dx and dweight are then off by 1.45 times what rounding the results alone costs (bfloat16: 0.0024 of their
+ * norm instead of 0.0017).
  */
 int pngpd_linear_backward(int type, int64_t M, int64_t N, int64_t K, const void* dy_dev, int64_t ld_dy, const void* z_dev,
                           const void* x_dev, int64_t ldx, const void* weight_dev, int64_t ldw, int act, void* dx_dev,
@@ -445,6 +447,9 @@ int pngpd_linear_cross_entropy_forward(int type, int64_t T, int64_t V, int64_t D
 /*
  * Gradients of the forward call with the same arguments: dloss_dev float [T] (PNGPD_REDUCE_NONE) or [1] -> dx_dev
  * [T,D], dweight_dev [V,D], dbias_dev [V], each optional.  Without kept_dev the logits are formed again piece by piece.
+ * Of more than 8 classes, and without kept_dev, 16-bit types round the logits' gradients to `type` in front of the products
+ * that give dx and dweight.  What all rows share stays out of that rounding: the mean's or the sum's weight, or the largest
+ * of the rows' own, and 1 - label_smoothing.  dbias sums before it.
  */
 int pngpd_linear_cross_entropy_backward(int type, int64_t T, int64_t V, int64_t D, const void* x_dev, int64_t ldx,
                                         const void* weight_dev, int64_t ldw, const void* bias_dev, const int64_t* target_dev,

@@ -7,8 +7,8 @@
 // selected away, not multiplied: infinities and NaN in dropped places do not reach the result.
 //
 // Bound by memory, with eight neighbouring elements a thread: their four hashes hide behind its 16-byte accesses (an element
-// a thread: 294 us).  16384 x 4096 in bfloat16 with its residual, forward and backward (671 MB): 120 us, 5.6 TB/s; without
-// one, forward, 47 us (268 MB).
+// a thread: 294 us).  16384 x 4096 in bfloat16: forward with its residual (403 MB) 73 us, backward without one (268 MB)
+// 47 us, together 5.6 TB/s; 51 us for the latter where the input changes from call to call.
 #include "crop_select.h"
 #include "head.h"
 #include "head_math.h"

@@ -172,7 +172,8 @@ hipError_t join(int64_t M, int64_t N, int splits, const float* partial, const He
 
 // y[m][n] for up to MR rows m: a wave takes NR rows of the weight, its lanes 16-byte chunks of them side by side, and adds its
 // lanes' 32-bit fma chains at the end.  Rows may start at any element.  Bound by reading the weight once: 4096 x 4096 bf16
-// (33.5 MB) for one row, 5.2 us (6.5 TB/s; 8.5 us before its loads were kept together).
+// (33.5 MB) for one row, 5.1 us a launch where the caches hold the weight, 7.6 us from the last-level cache (four weights in turn),
+// 8.6 us (3.9 TB/s) from memory; 8.5 instead of 5.1 before its loads were kept together.
 constexpr int64_t FEW_M = HEAD_FEW_ROWS;
 
 template <typename E, int MR, int NR>

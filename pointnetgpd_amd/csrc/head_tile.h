@@ -13,8 +13,10 @@
 //                      lane t of 16 the column t of a 4 x 16 block.
 // The n side is the matrix instruction's first operand, so a lane ends up with 4 neighbouring n of one m.
 //
-// 16-bit: 256 x 256 tiles reach 1.24 PFLOP/s (8192 x 4096 x 8192 in 445 us, 488 with gelu_tanh and a residual) and are bound by
-// power: the same instructions on zeros run 1.4 times as fast.  Floats: 64 x 64 tiles, three to a compute unit, reach 0.14
+// 16-bit: 256 x 256 tiles reach 1.24 PFLOP/s (8192 x 4096 x 8192 in 445 us, 488 with gelu_tanh and a residual), the library's bare
+// product 1.40 to 1.43 on the same card.  Two things bound them.  The clock: the same product on zeros takes 330 us (library: 256 to
+// 275).  And the tile's ends: one workgroup holds a compute unit (128 KB of LDS), so nothing covers its first loads and its
+// epilogue, 11 us a tile beside 64 steps of 1.7.  Floats: 64 x 64 tiles, three to a compute unit, reach 0.14
 // PFLOP/s of the matrix unit's 0.157 inside the loop, 0.13 over 4096 x 2048 x 2048.
 #pragma once
 #include "head.h"

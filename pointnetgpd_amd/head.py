@@ -63,7 +63,8 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     """act(x W^T + b) + residual: x [..., K], weight [N, K], bias [N], residual and result [..., N].
 
     activation: None, "relu", "gelu" (the error function's), "gelu_tanh" or "silu".  For 16-bit types the sums are 32-bit
-    and the result is rounded once; in training the pre-activation is kept in the tensors' type."""
+    and the result is rounded once; in training the pre-activation is kept, and its gradient handed to the products, in the
+    tensors' type (dx and dW are off as those of torch's own 16-bit autograd are: 0.0024 of their norm in bfloat16)."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"activation: expected one of {list(_ACTIVATIONS)}, got {activation!r}")
     _require(x, "x")
@@ -114,7 +115,8 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, label_
     [...] for "none".
 
     Rows with target == ignore_index have loss 0 and no gradient, whatever values they hold.  Another target outside [0, V)
-    makes the loss NaN and gives its row no gradient, as `training.nll_loss` does.  A class is masked by a bias of -inf.
+    makes the loss NaN and gives its row no gradient, as `training.nll_loss` does.  A class is masked by a bias of -inf, or a
+    large negative one.
 
     The logits are formed in pieces, in the backward pass again.  Where that is quicker, and one
     piece holds them all (256 MiB in x's type, or as much as x and weight take), they are kept in 32 bits instead."""
