@@ -260,9 +260,9 @@ at::Tensor loss_forward(const at::Tensor& x, const at::Tensor& w, const at::Tens
 
 struct LinearCrossEntropyFunction : torch::autograd::Function<LinearCrossEntropyFunction> {
     static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const Maybe& bias, const at::Tensor& target,
-                              int64_t ignore_index, double label_smoothing, int64_t reduction) {
+                              int64_t ignore_index, double label_smoothing, int64_t reduction, bool keep) {
         at::Tensor lse, kept;
-        at::Tensor loss = loss_forward(x, w, target, bias, {ignore_index, label_smoothing, reduction}, &lse, &kept);
+        at::Tensor loss = loss_forward(x, w, target, bias, {ignore_index, label_smoothing, reduction}, &lse, keep ? &kept : nullptr);
         ctx->save_for_backward({x, w, dense(bias), target, lse, kept});
         ctx->saved_data["ignore_index"] = ignore_index;
         ctx->saved_data["label_smoothing"] = label_smoothing;
@@ -272,7 +272,7 @@ struct LinearCrossEntropyFunction : torch::autograd::Function<LinearCrossEntropy
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const at::Tensor &x = saved[0], &w = saved[1], &b = saved[2], &target = saved[3], &lse = saved[4];
-        variable_list result(7);
+        variable_list result(8);
         if (!grads[0].defined()) return result;
         refuse_mixed_capture(grads[0]);
         const c10::OptionalDeviceGuard guard(x.device());
@@ -294,10 +294,10 @@ struct LinearCrossEntropyFunction : torch::autograd::Function<LinearCrossEntropy
 };
 
 at::Tensor linear_cross_entropy(const at::Tensor& x, const at::Tensor& w, const at::Tensor& target, const Maybe& bias,
-                                int64_t ignore_index, double label_smoothing, int64_t reduction) {
+                                int64_t ignore_index, double label_smoothing, int64_t reduction, bool keep) {
     refuse_tangents(x, w, bias);
     if (at::GradMode::is_enabled() && (wants(x) || wants(w) || wants(bias)))
-        return LinearCrossEntropyFunction::apply(x, w, bias, target, ignore_index, label_smoothing, reduction);
+        return LinearCrossEntropyFunction::apply(x, w, bias, target, ignore_index, label_smoothing, reduction, keep);
     at::Tensor lse;
     return loss_forward(x, w, target, bias, {ignore_index, label_smoothing, reduction}, &lse, nullptr);
 }

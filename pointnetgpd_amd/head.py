@@ -109,7 +109,7 @@ def dropout(x, p, seed, offset=0, residual=None):
 
 # ---- linear + cross entropy -----------------------------------------------------------------------------------------------
 
-def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, label_smoothing=0.0, reduction="mean", keep_logits=True):
     """F.cross_entropy(F.linear(x, weight, bias), target) without the logits: x [..., D], weight [V, D], target [...] of
     whole numbers, bias [V] -> float32 loss, a scalar for reduction "mean" (over the rows that are not ignored) and "sum",
     [...] for "none".
@@ -118,8 +118,9 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, label_
     makes the loss NaN and gives its row no gradient, as `training.nll_loss` does.  A class is masked by a bias of -inf, or a
     large negative one.
 
-    The logits are formed in pieces, in the backward pass again.  Where that is quicker, and one
-    piece holds them all (256 MiB in x's type, or as much as x and weight take), they are kept in 32 bits instead."""
+    The logits are formed in pieces, in the backward pass again.  Where that is quicker, and one piece holds them all (256 MiB in
+    x's type, or as much as x and weight take), they are kept in 32 bits instead; keep_logits=False never keeps them (at most
+    eight classes always do: 16 or 32 bytes a row)."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"reduction: expected one of {list(_REDUCTIONS)}, got {reduction!r}")
     _require(x, "x")
@@ -144,4 +145,4 @@ def linear_cross_entropy(x, weight, target, bias=None, ignore_index=-100, label_
     if target.dtype != torch.int64:
         target = target.to(torch.int64)
     return _lib.load_head().linear_cross_entropy(_plain(x), _plain(weight), target.contiguous(), _plain(bias), int(ignore_index),
-                                                 label_smoothing, _REDUCTIONS[reduction])
+                                                 label_smoothing, _REDUCTIONS[reduction], bool(keep_logits) or V <= 8)

@@ -179,7 +179,7 @@ def test_forward_mode_is_refused_before_anything_is_launched():
                     with pytest.raises(RuntimeError, match="forward-mode"):
                         m.linear(a[0], a[1], a[2], None, 0)
                     with pytest.raises(RuntimeError, match="forward-mode"):
-                        m.linear_cross_entropy(a[0], a[1], t, a[2], -100, 0.0, 1)
+                        m.linear_cross_entropy(a[0], a[1], t, a[2], -100, 0.0, 1, True)
                 with pytest.raises(RuntimeError, match="forward-mode"):
                     m.linear(x, w, None, fw.make_dual(torch.ones(2, 3), torch.ones(2, 3)), 0)
                 with pytest.raises(RuntimeError, match="forward-mode"):

@@ -1205,3 +1205,25 @@ def test_losses_and_weights_of_many_rows(kind, reduction, T, V, D):
         dloss[T - 1], target[T - 1] = 3 * scale / T, 1
     got = run_loss(x, w, target, b, 0.1, reduction, dloss)
     check(got, ho.cross_entropy(x, w, target, b, -100, 0.1, reduction, dloss))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_a_caller_may_refuse_kept_logits(kind):
+    """keep_logits=False: nothing of the logits' size lives between the passes, and the gradients are within the same bounds."""
+    dt = TYPES[kind]
+    T, V, D = 1000, 6000, 1536
+    x, w, b, target = loss_case(61, T, V, D, dt, True)
+    dloss = torch.tensor(64.0 if kind == "f16" else 1.0)
+    want = ho.cross_entropy(x, w, target, b, -100, 0.1, "mean", dloss)
+    held = {}
+    for keep in (True, False):
+        leaves = [t.cuda().requires_grad_() for t in (x, w, b)]
+        y = target.cuda()
+        before = torch.cuda.memory_allocated()
+        loss = head.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], label_smoothing=0.1, keep_logits=keep)
+        held[keep] = torch.cuda.memory_allocated() - before
+        check({"loss": loss, **dict(zip(("dx", "dw", "db"), torch.autograd.grad(loss, leaves, dloss.cuda())))}, want)
+    assert held[True] >= T * V * 4 and held[False] < 1 << 20
+    few = [t.cuda().requires_grad_() for t in (x, w[:5], b[:5])]
+    grads = [torch.autograd.grad(head.linear_cross_entropy(*few[:2], target.cuda() % 5, few[2], keep_logits=keep), few) for keep in (True, False)]
+    assert all(torch.equal(p, q) for p, q in zip(*grads))
