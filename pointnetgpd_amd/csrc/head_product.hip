@@ -521,27 +521,30 @@ __global__ __launch_bounds__(256) void grad_rows_kernel(int64_t M, int64_t N, co
     }
 }
 
-// 32 columns by 8 shares of the parts a workgroup
-template <typename T>
+// COLS columns by 256 / COLS shares of the parts a workgroup
+template <typename T, int COLS>
 __global__ __launch_bounds__(256) void col_join_kernel(int64_t parts, int64_t N, const float* part, const float* scale, T* out) {
-    __shared__ float share[8][32];
-    const int c = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int64_t n = (int64_t)blockIdx.x * 32 + c;
+    constexpr int SHARES = 256 / COLS;
+    __shared__ float share[SHARES][COLS];
+    const int c = threadIdx.x % COLS, w = threadIdx.x / COLS;
+    const int64_t n = (int64_t)blockIdx.x * COLS + c;
     float s = 0.f;
     if (n < N) {
 #pragma unroll 8
-        for (int64_t i = w; i < parts; i += 8) s += part[i * N + n];
+        for (int64_t i = w; i < parts; i += SHARES) s += part[i * N + n];
     }
     share[w][c] = s;
     __syncthreads();
     if (w || n >= N) return;
-    for (int i = 1; i < 8; ++i) s += share[i][c];
+    for (int i = 1; i < SHARES; ++i) s += share[i][c];
     out[n] = from_f32<T>(scale ? s * scale[0] : s);
 }
 
+// A tile's rows are a part: 2^20 rows are 16384 of them, which 32 shares join in 25 us and 8 in 91.
 template <typename T>
 hipError_t col_sums(int64_t parts, int64_t N, const float* part, const float* scale, void* out, hipStream_t s) {
-    col_join_kernel<T><<<(unsigned)((N + 31) / 32), 256, 0, s>>>(parts, N, part, scale, (T*)out);
+    if (parts <= 256) col_join_kernel<T, 32><<<(unsigned)((N + 31) / 32), 256, 0, s>>>(parts, N, part, scale, (T*)out);
+    else col_join_kernel<T, 8><<<(unsigned)((N + 7) / 8), 256, 0, s>>>(parts, N, part, scale, (T*)out);
     return hipGetLastError();
 }
 
