@@ -403,17 +403,18 @@ __device__ __forceinline__ void row_weights(const HeadRowWeights& w, int block, 
     // 2^14, |dz| <= 2 times that is inside its range, and a probability of 2^-37 still is a number.
     const bool one = w.reduction != PNGPD_REDUCE_NONE, shared = bits16 && g != 0.f && __builtin_fabsf(g) < __builtin_inff();
     const float top_weight = (half ? 16384.f : 1.f) * (bits16 ? w.label_factor : 1.f);
+    float all = one ? w.dloss[0] : 0.f;
+    if (w.reduction == PNGPD_REDUCE_MEAN) all *= 1.f / __builtin_fmaxf(r.used, 1.f);
+    // an infinite gradient goes into dz, so that rows that have none keep their zeros
+    const bool apart = one && __builtin_fabsf(all) < __builtin_inff();
     const int64_t first = block * rows, last = first + rows < w.T ? first + rows : w.T;
 #pragma unroll 8
     for (int64_t t = first + threadIdx.x; t < last; t += 256) {
         const int64_t y = w.target[t];
         const bool live = y != w.ignore_index && y >= 0 && y < w.V;
-        w.row_weight[t] = !live ? 0.f : one ? top_weight : shared ? w.dloss[t] / g * top_weight : w.dloss[t];
+        w.row_weight[t] = !live ? 0.f : apart ? top_weight : one ? all : shared ? w.dloss[t] / g * top_weight : w.dloss[t];
     }
-    if (block == 0 && threadIdx.x == 0) {
-        const float all = w.reduction == PNGPD_REDUCE_MEAN ? w.dloss[0] * (1.f / __builtin_fmaxf(r.used, 1.f)) : w.dloss[0];
-        w.out_scale[0] = one ? all / top_weight : shared ? g / top_weight : 1.f;
-    }
+    if (block == 0 && threadIdx.x == 0) w.out_scale[0] = apart ? all / top_weight : shared ? g / top_weight : 1.f;
 }
 
 struct LayOutRun {

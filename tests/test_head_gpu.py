@@ -1227,3 +1227,17 @@ def test_a_caller_may_refuse_kept_logits(kind):
     few = [t.cuda().requires_grad_() for t in (x, w[:5], b[:5])]
     grads = [torch.autograd.grad(head.linear_cross_entropy(*few[:2], target.cuda() % 5, few[2], keep_logits=keep), few) for keep in (True, False)]
     assert all(torch.equal(p, q) for p, q in zip(*grads))
+
+
+@pytest.mark.parametrize("grad", [math.inf, math.nan])
+@pytest.mark.parametrize("T,V", [(70, 50), (70, 5), (5000, 50)])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_ignored_rows_under_an_infinite_gradient(kind, T, V, grad):
+    """A loss scale that overflowed: every gradient shows it but those of the rows that have none."""
+    x, w, b, target = loss_case(71, T, V, 24, TYPES[kind], True)
+    target[1], target[2], target[3] = -100, 2, V
+    for reduction in ("mean", "sum"):
+        got = run_loss(x, w, target, b, 0.0, reduction, torch.tensor(grad))
+        none = ((target < 0) | (target >= V)).cuda()
+        assert not got["dx"][none].any() and not torch.isfinite(got["dx"][~none]).any(1).all()
+        assert not torch.isfinite(got["dw"]).all() and not torch.isfinite(got["db"]).all()
